@@ -472,6 +472,132 @@ exl3_verdict exl3_resident(const exl3_weight *ws, int32_t count, uint64_t room, 
 /* The bytes exl3_resident admitted and no prefill call has filled yet (QuantTable.resident_pending). */
 uint64_t exl3_resident_pending(void);
 
+/* ------------------------------------------------------------------ a layer's attention side
+ *
+ * Between a layer's q|k|v linears and its o linear (no counterpart in the reference's EXL3 path, whose host keeps its
+ * own attention): a paged key/value cache, the norms and rotation that fill it, attention of one token, of a tree of
+ * drafted tokens or of a prompt chunk over it, and the bookkeeping of its pages.  The calls follow the conventions at
+ * the top of this file: they enqueue on `stream`, allocate nothing and do not synchronise; arrays named "device" are
+ * read by the kernels when the call's work runs.  A device value out of range (a page id, a context, a path) is never
+ * followed: the access is skipped and EXL3_ERR_BAD_SHAPE recorded. */
+
+/* The paged cache of every layer.  Token slot `t` of page `p` of kv head `h` of layer `l` is the head_dim contiguous
+ * elements at k (v) + l * layer_stride + p * page_stride + h * head_stride + t * token_stride (elements; the same
+ * strides for k and v).  Pages and heads may be stored in any order; the strides must be multiples of 8 elements and
+ * k, v 16-byte aligned, and no two slots may overlap. */
+typedef struct exl3_kv_cache {
+  uint32_t size;      /* sizeof(exl3_kv_cache) */
+  int32_t device;
+  int32_t dtype;      /* EXL3_F16 or EXL3_BF16 */
+  int32_t layers, pages, page_size, kv_heads, head_dim; /* page_size 16, 32, 64, 128 or 256; head_dim 64, 128 or 256 */
+  void *k, *v;        /* device */
+  int64_t layer_stride, page_stride, head_stride, token_stride;
+} exl3_kv_cache;
+
+/* Checks a cache the host filled in and creates the device workspace (like exl3_weight_view): once per cache, before
+ * the calls below. */
+exl3_verdict exl3_kv_register(const exl3_kv_cache *cache);
+
+/* One step's new tokens: sequence s owns rows row_start[s] .. row_start[s + 1] - 1 (none is allowed), which follow its
+ * context[s] tokens already in the cache; row i of a sequence lives in slot context + i, slot j in page
+ * table[s][j / page_size].  With `tree`, bit j of a row's words (word j / 32, bit j % 32) says whether the row sees row
+ * j of its own sequence -- its ancestors and, normally, itself; rows beyond the words' bits are not seen.  Without it
+ * row i sees rows 0 .. i.  Every row sees the whole context.  `position` (or null: context + i) is what the rotation
+ * turns by.  Rows from row_start[nseq] on are padding (a step of a fixed width in a CUDA graph): nothing is written for
+ * them. */
+typedef struct exl3_tree_batch {
+  uint32_t size;            /* sizeof(exl3_tree_batch) */
+  int32_t nseq;             /* 0 .. 65535 */
+  int32_t rows;             /* all sequences' rows */
+  int32_t max_rows;         /* the most rows of one sequence */
+  int32_t max_context;      /* a bound on context + rows of every sequence (0: the table's width) */
+  int32_t max_pages;        /* the table's width */
+  int32_t tree_words;       /* words per row of `tree` */
+  const int32_t *row_start; /* device, [nseq + 1] */
+  const int32_t *context;   /* device, [nseq] */
+  const int32_t *table;     /* device, [nseq][max_pages] */
+  const uint32_t *tree;     /* device, [rows][tree_words], or null */
+  const int32_t *position;  /* device, [rows], or null */
+} exl3_tree_batch;
+
+/* A device array of rows of heads: head h of row r is `dim` contiguous elements at data + r * row_stride +
+ * h * head_stride (elements). */
+typedef struct exl3_heads {
+  void *data;
+  int32_t dtype;
+  int32_t rows, heads, dim;
+  int64_t row_stride, head_stride;
+} exl3_heads;
+
+/* Norms and rotation of queries and keys.  Each head vector x becomes x / sqrt(mean(x^2) + eps) * (weight +
+ * weight_offset) (skipped where the weight is null), then its first rot_dims elements are turned by position *
+ * inv_freq[i]: pair i is (i, i + rot_dims / 2), or (2i, 2i + 1) with `adjacent`. */
+typedef struct exl3_norm_rope {
+  uint32_t size;          /* sizeof(exl3_norm_rope) */
+  int32_t rot_dims;       /* 0 .. head_dim; even, and a multiple of 16 unless adjacent */
+  int32_t adjacent;
+  int32_t weight_dtype;   /* of both weights */
+  float eps;              /* >= 0 */
+  float weight_offset;    /* 0, or 1 where the pack stores weights around zero */
+  const void *q_weight;   /* device, [head_dim], or null: no norm of the queries */
+  const void *k_weight;   /* device, [head_dim], or null: no norm of the keys */
+  const double *inv_freq; /* device, [rot_dims / 2] radians per position (null with rot_dims 0) */
+} exl3_norm_rope;
+
+/* One pass over a layer's q, k, v rows: q normed and rotated into q_out (may be q itself), k normed and rotated and v
+ * as it is into their slots of `layer`.  f16, bf16 or f32 in one dtype; q_out in that dtype or the cache's; the
+ * arithmetic is f32, the angle exact to 2^-52 turns of position * inv_freq, each output rounded once. */
+exl3_verdict exl3_qk_norm_rope(const exl3_kv_cache *cache, int32_t layer, const exl3_tree_batch *batch,
+                               const exl3_heads *q, const exl3_heads *k, const exl3_heads *v,
+                               const exl3_norm_rope *opts, void *stream, const exl3_heads *q_out);
+
+/* Attention of the batch's rows over `layer`: out[r][h] = sum_j softmax_j(scale q[r][h] . k[j]) v[j] over the slots the
+ * row sees, kv head h / (heads / kv_heads).  q and out in the cache's dtype; scale > 0.  `lse` (device f32
+ * [rows][heads], or null) receives log sum_j exp(scale q . k[j]).  A row that sees nothing gets zeros and -inf.  What
+ * lies in slots a row does not see -- stale pages, other branches of the tree, infinities, NaN -- does not reach it.
+ * Any number of rows per sequence: one (a decode step), a drafted tree, a prompt chunk. */
+exl3_verdict exl3_tree_attention(const exl3_kv_cache *cache, int32_t layer, const exl3_tree_batch *batch,
+                                 const exl3_heads *q, float scale, void *stream, const exl3_heads *out, float *lse);
+
+/* The host's page bookkeeping, on the device: how many rows refer to each page (0: free), each row's page ids (-1 past
+ * its `held` pages), and its tokens. */
+typedef struct exl3_page_state {
+  uint32_t size;      /* sizeof(exl3_page_state) */
+  int32_t nseq;
+  int32_t max_pages;  /* the table's width */
+  int32_t *refs;      /* device, [cache pages] */
+  int32_t *table;     /* device, [nseq][max_pages] */
+  int32_t *held;      /* device, [nseq] */
+  int32_t *lens;      /* device, [nseq] */
+} exl3_page_state;
+
+/* Fork, reorder and free: row i of `out` becomes row parent[i] of `in` (-1: an empty row), sharing its pages; each
+ * page's references follow the rows that hold it, so the pages of rows nobody names become free.  No key or value
+ * moves.  out->nseq rows; out's arrays are not in's. */
+exl3_verdict exl3_cache_fork(const exl3_kv_cache *cache, const exl3_page_state *in, const int32_t *parent, void *stream,
+                             const exl3_page_state *out);
+
+/* Grow: every row gets pages for need[i] tokens, and sole ownership of the page its next token falls in.  A partly
+ * filled last page that others share and the row will write is replaced by a copy (in every layer) -- except that when
+ * all its sharers grow, the first of them keeps it.  Pages are given lowest id first, rows in order, a row's copy
+ * before its new pages.  Rows never shrink; lens stay.  missing[0] (device) receives 0, or, when the free pages or the
+ * table's width do not suffice, how many pages are lacking, and then `out` is `in` unchanged and nothing is copied.
+ * out's arrays are not in's. */
+exl3_verdict exl3_cache_grow(const exl3_kv_cache *cache, const exl3_page_state *in, const int32_t *need, void *stream,
+                             const exl3_page_state *out, int32_t *missing);
+
+/* Keep a verified path: of each sequence's drafted rows, path[s][0 .. kept[s] - 1] (ascending row indices, [nseq][depth])
+ * were accepted; their keys and values move, in every layer, from slots context + path[d] to context + d, and
+ * lens[s] = context[s] + kept[s].  A null path keeps the first kept[s] rows where they are. */
+exl3_verdict exl3_cache_keep(const exl3_kv_cache *cache, const exl3_tree_batch *batch, const int32_t *path,
+                             int32_t depth, const int32_t *kept, void *stream, int32_t *lens);
+
+/* Compact: the live pages (refs > 0), counted c, end up in pages 0 .. c - 1: the live pages from c on move, in
+ * ascending order and in every layer, into the free pages below c; tables and references follow.  out's arrays are not
+ * in's. */
+exl3_verdict exl3_cache_compact(const exl3_kv_cache *cache, const exl3_page_state *in, void *stream,
+                                const exl3_page_state *out);
+
 /* Device error bits the kernels recorded on `device`; `clear` resets them. */
 #define EXL3_ERR_WAIT_TIMEOUT 1u  /* a bounded mbarrier wait gave up (the kernel left its loop and returned) */
 #define EXL3_ERR_BAD_SHAPE 2u     /* a launch saw a shape its host validation should have refused */

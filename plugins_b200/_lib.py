@@ -41,6 +41,8 @@ EXPORTS = (
     "exl3_decode_dense", "exl3_reconstruct_public", "exl3_encode_trellis", "exl3_matmul_noalloc", "exl3_device_error", "exl3_version",
     "exl3_model_claims", "exl3_model_parse", "exl3_model_bill", "exl3_model_load", "exl3_model_unload",
     "exl3_model_weight", "exl3_model_linear", "exl3_model_linears", "exl3_model_mlp", "exl3_model_experts", "exl3_resident", "exl3_resident_pending",
+    "exl3_kv_register", "exl3_qk_norm_rope", "exl3_tree_attention", "exl3_cache_fork", "exl3_cache_grow",
+    "exl3_cache_keep", "exl3_cache_compact",
 )
 
 
@@ -114,6 +116,44 @@ class SharedSwiglu(ctypes.Structure):
     _fields_ = [("size", ctypes.c_uint32), ("limit", ctypes.c_int32), ("gate", ctypes.c_void_p),
                 ("up", ctypes.c_void_p), ("down", ctypes.c_void_p), ("shared", ctypes.c_void_p),
                 ("logit", ctypes.c_void_p), ("gate_vec", ctypes.c_void_p), ("sigtab", ctypes.c_void_p)]
+
+
+class KvCache(ctypes.Structure):
+    """exl3_kv_cache: the paged key/value cache of every layer, strides in elements."""
+    _fields_ = [("size", ctypes.c_uint32), ("device", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("layers", ctypes.c_int32), ("pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("k", ctypes.c_void_p),
+                ("v", ctypes.c_void_p), ("layer_stride", ctypes.c_int64), ("page_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64)]
+
+
+class TreeBatch(ctypes.Structure):
+    """exl3_tree_batch: one step's new tokens by sequence."""
+    _fields_ = [("size", ctypes.c_uint32), ("nseq", ctypes.c_int32), ("rows", ctypes.c_int32),
+                ("max_rows", ctypes.c_int32), ("max_context", ctypes.c_int32), ("max_pages", ctypes.c_int32),
+                ("tree_words", ctypes.c_int32), ("row_start", ctypes.c_void_p), ("context", ctypes.c_void_p),
+                ("table", ctypes.c_void_p), ("tree", ctypes.c_void_p), ("position", ctypes.c_void_p)]
+
+
+class Heads(ctypes.Structure):
+    """exl3_heads: a strided array of rows of heads."""
+    _fields_ = [("data", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("rows", ctypes.c_int32),
+                ("heads", ctypes.c_int32), ("dim", ctypes.c_int32), ("row_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64)]
+
+
+class NormRope(ctypes.Structure):
+    """exl3_norm_rope: the norms' weights and the rotation."""
+    _fields_ = [("size", ctypes.c_uint32), ("rot_dims", ctypes.c_int32), ("adjacent", ctypes.c_int32),
+                ("weight_dtype", ctypes.c_int32), ("eps", ctypes.c_float), ("weight_offset", ctypes.c_float),
+                ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p)]
+
+
+class PageState(ctypes.Structure):
+    """exl3_page_state: reference counts, page tables, held pages and tokens."""
+    _fields_ = [("size", ctypes.c_uint32), ("nseq", ctypes.c_int32), ("max_pages", ctypes.c_int32),
+                ("refs", ctypes.c_void_p), ("table", ctypes.c_void_p), ("held", ctypes.c_void_p),
+                ("lens", ctypes.c_void_p)]
 
 
 _lock = threading.Lock()
@@ -273,6 +313,24 @@ def lib() -> ctypes.CDLL:
             L.exl3_resident.argtypes = [P(Weight), ctypes.c_int32, ctypes.c_uint64, ctypes.c_void_p, P(ctypes.c_uint64)]
             L.exl3_resident_pending.restype = ctypes.c_uint64
             L.exl3_resident_pending.argtypes = []
+            L.exl3_kv_register.restype = Verdict
+            L.exl3_kv_register.argtypes = [P(KvCache)]
+            L.exl3_qk_norm_rope.restype = Verdict
+            L.exl3_qk_norm_rope.argtypes = [P(KvCache), ctypes.c_int32, P(TreeBatch), P(Heads), P(Heads), P(Heads),
+                                            P(NormRope), ctypes.c_void_p, P(Heads)]
+            L.exl3_tree_attention.restype = Verdict
+            L.exl3_tree_attention.argtypes = [P(KvCache), ctypes.c_int32, P(TreeBatch), P(Heads), ctypes.c_float,
+                                              ctypes.c_void_p, P(Heads), ctypes.c_void_p]
+            L.exl3_cache_fork.restype = Verdict
+            L.exl3_cache_fork.argtypes = [P(KvCache), P(PageState), ctypes.c_void_p, ctypes.c_void_p, P(PageState)]
+            L.exl3_cache_grow.restype = Verdict
+            L.exl3_cache_grow.argtypes = [P(KvCache), P(PageState), ctypes.c_void_p, ctypes.c_void_p, P(PageState),
+                                          ctypes.c_void_p]
+            L.exl3_cache_keep.restype = Verdict
+            L.exl3_cache_keep.argtypes = [P(KvCache), P(TreeBatch), ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p,
+                                          ctypes.c_void_p, ctypes.c_void_p]
+            L.exl3_cache_compact.restype = Verdict
+            L.exl3_cache_compact.argtypes = [P(KvCache), P(PageState), ctypes.c_void_p, P(PageState)]
             L.exl3_version.restype = ctypes.c_char_p
             L.exl3_version.argtypes = []
             _lib = L

@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "../../include/exl3_b200.h"
+#include "exl3_attn.h"
 #include "exl3_internal.h"
 #include "exl3_json.h"
 #include "exl3_moe.h"
@@ -147,6 +148,23 @@ DeviceState* device_state(int dev) {
   if (dev < 0 || dev >= kMaxDevices || !g_dev[dev].ready) return nullptr;
   return &g_dev[dev];
 }
+
+}  // namespace
+
+namespace exl3 {
+
+exl3_verdict workspace_create(int device) { return ensure_device(device); }
+
+bool workspace_get(int device, Workspace& ws) {
+  const DeviceState* d = device_state(device);
+  if (!d) return false;
+  ws = {d->partials, d->partial_floats, d->counters, d->err, d->sms};
+  return true;
+}
+
+}  // namespace exl3
+
+namespace {
 
 bool rate_served(int n) { return exl3::rate_served_n(n); }
 

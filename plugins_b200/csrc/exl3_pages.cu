@@ -1,0 +1,415 @@
+// exl3_pages.cu -- the pages of the key/value cache: fork / reorder / free, grow with copy on write, compaction, and
+// keeping a drafted tree's accepted path.
+//
+// The bookkeeping (reference counts, tables) is a few hundred kilobytes of whole numbers with dependent steps -- count,
+// scan, assign -- so one thread-block cluster does it in one launch, its CTAs joined by the cluster barrier between the
+// steps; a single launch of eight CTAs costs less than the launches a grid would need.  Everything is decided by ranks
+// (the n-th lowest free page, the n-th row that asks), never by the order in which threads arrive.  The pages'
+// contents then move in a second launch over the whole GPU, bound by HBM: every moved byte read and written once.
+#include <cuda_runtime.h>
+
+#include "exl3_attn.h"
+#include "exl3_common.cuh"
+#include "exl3_internal.h"
+
+namespace exl3 {
+
+namespace {
+
+constexpr int kCluster = 8;
+constexpr int kThreads = 1024;
+constexpr int kAll = kCluster * kThreads;
+constexpr int kMaxGrowRows = 4096;  // rows of a grow call (their asks are scanned in shared memory)
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// Shared word w of CTA `rank` of the cluster.
+__device__ __forceinline__ int cluster_word(const int* w, int rank) {
+  uint32_t a;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(w)), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+
+// The cluster's pages cut into one run per CTA, a run into one part per thread: [lo, hi).
+struct PageRun {
+  int lo, hi;
+  __device__ __forceinline__ explicit PageRun(int pages) {
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    lo = static_cast<int>(t * pages / kAll), hi = static_cast<int>((t + 1) * pages / kAll);
+  }
+};
+
+// Exclusive rank of this thread's `n` in the cluster (CTA by CTA, thread by thread) and the cluster's total.
+// s_total: one shared word that nothing else writes until the next cluster_sync.
+__device__ __forceinline__ int cluster_scan_excl(int n, int* s_warp, int* s_total, int* total) {
+  int mine;
+  const int r = cta_scan_excl(n, s_warp, &mine);
+  if (threadIdx.x == 0) *s_total = mine;
+  cluster_sync();
+  int before = 0, all = 0;
+  for (int c = 0; c < kCluster; ++c) {
+    const int v = cluster_word(s_total, c);
+    if (c < static_cast<int>(blockIdx.x)) before += v;
+    all += v;
+  }
+  *total = all;
+  return before + r;
+}
+
+// A row's pages, held inside the table whatever the device value is.
+__device__ __forceinline__ int held_of(const PageParams& p, int r) { return max(0, min(p.held_in[r], p.width_in)); }
+
+// ------------------------------------------------------------------ fork / reorder / free
+
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) fork_kernel(const PageParams p) {
+  pdl_wait();
+  const int t = static_cast<int>(blockIdx.x) * kThreads + static_cast<int>(threadIdx.x);
+  const int lane = t & 31, warp = t >> 5;
+  for (int i = t; i < p.pages; i += kAll) p.refs[i] = p.refs_in[i];
+  for (int r = warp; r < p.nseq_out; r += kAll / 32) {
+    int from = p.parent[r];
+    if (from < -1 || from >= p.nseq_in) {
+      if (lane == 0) atomicOr(p.err, kErrBadShape);
+      from = -1;
+    }
+    const int held = from < 0 ? 0 : max(0, min(p.held_in[from], p.width_in));
+    if (lane == 0) p.held[r] = held, p.lens[r] = from < 0 ? 0 : p.lens_in[from];
+    const int64_t src = static_cast<int64_t>(from) * p.width_in, dst = static_cast<int64_t>(r) * p.width_out;
+    for (int j = lane; j < p.width_out; j += 32) p.table[dst + j] = j < held ? p.table_in[src + j] : -1;
+  }
+  cluster_sync();  // the copied counts are in place
+  for (int r = warp; r < p.nseq_in; r += kAll / 32) {
+    int children = 0;
+    for (int j = lane; j < p.nseq_out; j += 32) children += p.parent[j] == r ? 1 : 0;
+    children = __reduce_add_sync(0xFFFFFFFFu, children);
+    if (children == 1) continue;
+    const int held = held_of(p, r);
+    for (int j = lane; j < held; j += 32) {
+      const int id = p.table_in[static_cast<int64_t>(r) * p.width_in + j];
+      if (id >= 0 && id < p.pages) atomicAdd(p.refs + id, children - 1);  // (whole numbers: any order)
+      else atomicOr(p.err, kErrBadShape);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ grow
+
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) grow_kernel(const PageParams p) {
+  extern __shared__ int s_row[];  // [nseq] last pages of growing rows, asks before the row, copies before the row
+  __shared__ int s_warp[32], s_total, s_over;
+  int* s_last = s_row;
+  int* s_ask = s_row + p.nseq_in;
+  int* s_copy = s_ask + p.nseq_in + 1;
+  pdl_wait();
+  const int tid = static_cast<int>(threadIdx.x);
+  const int t = static_cast<int>(blockIdx.x) * kThreads + tid;
+  const int n = p.nseq_in, page = 1 << p.page_shift;
+  for (int i = t; i < p.pages; i += kAll) p.refs[i] = p.refs_in[i];
+  for (int64_t i = t; i < static_cast<int64_t>(n) * p.width_in; i += kAll) p.table[i] = p.table_in[i];
+  // every CTA: what each row asks for
+  for (int r = tid; r < n; r += kThreads) {
+    const int len = p.lens_in[r], held = held_of(p, r);
+    int last = -1;
+    if (p.need[r] > len && len >= 0 && (len & (page - 1)) && (len >> p.page_shift) < held) {
+      last = p.table_in[static_cast<int64_t>(r) * p.width_in + (len >> p.page_shift)];
+      if (last < 0 || last >= p.pages) {
+        last = -1;
+        atomicOr(p.err, kErrBadShape);
+      }
+    }
+    s_last[r] = last;
+  }
+  if (tid == 0) s_over = 0;
+  __syncthreads();
+  int asked = 0, copied = 0;  // rows are scanned in runs of kThreads
+  for (int base = 0; base < n; base += kThreads) {
+    const int r = base + tid;
+    int ask = 0, copy = 0;
+    if (r < n) {
+      const int held = held_of(p, r);
+      const int64_t want = (static_cast<int64_t>(max(p.need[r], 0)) + page - 1) >> p.page_shift;
+      if (want > p.width_in) atomicAdd(&s_over, static_cast<int>(want - p.width_in));
+      ask = static_cast<int>(max(static_cast<int64_t>(0), min(want, static_cast<int64_t>(p.width_in)) - held));
+      const int last = s_last[r];
+      if (last >= 0) {
+        const int refs = p.refs_in[last];
+        if (refs > 1) {  // shared: copied, unless every sharer grows and this row is their first
+          int sharers = 0, first = r;
+          for (int o = 0; o < n; ++o)
+            if (s_last[o] == last) ++sharers, first = min(first, o);
+          copy = sharers == refs && first == r ? 0 : 1;
+        }
+      }
+      ask += copy;
+    }
+    int total;
+    const int a = cta_scan_excl(ask, s_warp, &total);
+    if (r < n) s_ask[r] = asked + a;
+    asked += total;
+    const int c = cta_scan_excl(copy, s_warp, &total);
+    if (r < n) s_copy[r] = copied + c;
+    copied += total;
+  }
+  if (tid == 0) s_ask[n] = asked, s_copy[n] = copied;
+  // the free pages, ranked
+  const PageRun run(p.pages);
+  int mine = 0, free_pages;
+  for (int i = run.lo; i < run.hi; ++i) mine += p.refs_in[i] == 0 ? 1 : 0;
+  int rank = cluster_scan_excl(mine, s_warp, &s_total, &free_pages);  // (its barrier: the copies above are in place)
+  const int missing = max(0, asked - free_pages) + s_over;
+  if (t == 0) {
+    p.missing[0] = missing;
+    p.moves[0] = missing ? 0 : copied;
+  }
+  for (int r = t; r < n; r += kAll) {
+    const int held = held_of(p, r), got = s_ask[r + 1] - s_ask[r] - (s_copy[r + 1] - s_copy[r]);
+    p.held[r] = missing ? held : held + got;
+    p.lens[r] = p.lens_in[r];
+  }
+  if (!missing) {
+    for (int i = run.lo; i < run.hi && rank < asked; ++i) {
+      if (p.refs_in[i] != 0) continue;
+      // the row whose ask holds this rank: the last with s_ask[r] <= rank
+      int lo = 0, hi = n;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_ask[mid] <= rank) lo = mid;
+        else hi = mid;
+      }
+      const int r = lo, copy = s_copy[r + 1] - s_copy[r];
+      const int64_t row = static_cast<int64_t>(r) * p.width_in;
+      const int j = rank - s_ask[r];
+      p.refs[i] = 1;
+      if (copy && j == 0) {
+        p.table[row + (p.lens_in[r] >> p.page_shift)] = i;
+        atomicSub(p.refs + s_last[r], 1);
+        p.moves[1 + 2 * s_copy[r]] = s_last[r];
+        p.moves[2 + 2 * s_copy[r]] = i;
+      } else {
+        p.table[row + held_of(p, r) + j - copy] = i;
+      }
+      ++rank;
+    }
+  }
+  cluster_sync();  // no CTA leaves while another may read its shared words
+}
+
+// ------------------------------------------------------------------ compact
+
+// scratch: [2 * pages] after the moves: the live pages by their rank, then the free pages below the live count by theirs
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) compact_kernel(const PageParams p) {
+  __shared__ int s_warp[32], s_total, s_holes;
+  pdl_wait();
+  int* by_rank = p.moves + 1 + 2 * static_cast<int64_t>(p.pages);
+  int* holes = by_rank + p.pages;
+  const int t = static_cast<int>(blockIdx.x) * kThreads + static_cast<int>(threadIdx.x);
+  const PageRun run(p.pages);
+  int mine = 0, live;
+  for (int i = run.lo; i < run.hi; ++i) mine += p.refs_in[i] > 0 ? 1 : 0;
+  const int before = cluster_scan_excl(mine, s_warp, &s_total, &live);
+  // live page of rank k moves to hole k - (live - holes): the last `holes` live pages are the ones at `live` and above
+  int rank = before, found = 0;
+  for (int i = run.lo; i < run.hi; ++i) {
+    if (p.refs_in[i] > 0) by_rank[rank++] = i;
+    else if (i < live) holes[i - rank] = i, ++found;
+  }
+  int holes_mine;
+  cta_scan_excl(found, s_warp, &holes_mine);
+  if (threadIdx.x == 0) s_holes = holes_mine;
+  cluster_sync();
+  int moves = 0;
+  for (int c = 0; c < kCluster; ++c) moves += cluster_word(&s_holes, c);
+  if (t == 0) p.moves[0] = moves;
+  for (int i = t; i < moves; i += kAll) {
+    p.moves[1 + 2 * i] = __ldcg(by_rank + live - moves + i);
+    p.moves[2 + 2 * i] = __ldcg(holes + i);
+  }
+  for (int i = t; i < p.pages; i += kAll) {
+    int v = 0;
+    if (i < live) v = p.refs_in[i] > 0 ? p.refs_in[i] : -1;
+    if (v >= 0) p.refs[i] = v;
+  }
+  for (int i = t; i < moves; i += kAll) p.refs[__ldcg(holes + i)] = p.refs_in[__ldcg(by_rank + live - moves + i)];
+  for (int r = t; r < p.nseq_in; r += kAll) p.held[r] = p.held_in[r], p.lens[r] = p.lens_in[r];
+  for (int64_t i = t; i < static_cast<int64_t>(p.nseq_in) * p.width_in; i += kAll) {
+    int id = p.table_in[i];
+    if (id >= live && id < p.pages) {
+      // its place among the movers: by_rank[live - moves ..] ascends
+      int lo = live - moves, hi = live;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldcg(by_rank + mid) <= id) lo = mid;
+        else hi = mid;
+      }
+      const bool found_it = moves > 0 && __ldcg(by_rank + lo) == id;
+      if (!found_it) atomicOr(p.err, kErrBadShape);  // a table names a page with no references
+      else id = __ldcg(holes + (lo - (live - moves)));
+    } else if (id >= p.pages) {
+      atomicOr(p.err, kErrBadShape);
+    }
+    p.table[i] = id < 0 ? -1 : id;
+  }
+  cluster_sync();  // no CTA leaves while another may read its shared words
+}
+
+// ------------------------------------------------------------------ page contents
+
+constexpr int kCopyThreads = 256;
+constexpr int kCopyPer = 8;  // 16-byte chunks a thread has in flight
+constexpr int kCopyUnit = kCopyThreads * kCopyPer;
+
+__global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const PagePool pool, const int32_t* moves) {
+  pdl_wait();
+  const int count = moves[0];
+  const int dshift = 31 - __clz(pool.dim / 8), pshift = 31 - __clz(pool.page_size);
+  const int chunks = pool.kv_heads << (pshift + dshift);  // of one page, one layer, k or v
+  const int units = (chunks + kCopyUnit - 1) / kCopyUnit;
+  const int64_t total = static_cast<int64_t>(count) * pool.layers * 2 * units;
+  for (int64_t u = blockIdx.x; u < total; u += gridDim.x) {
+    const int part = static_cast<int>(u % units);
+    int64_t rest = u / units;
+    uint16_t* base = (rest & 1) ? pool.v : pool.k;
+    rest >>= 1;
+    base += (rest % pool.layers) * pool.layer_stride;
+    const int64_t m = rest / pool.layers;
+    const uint16_t* src = base + moves[1 + 2 * m] * pool.page_stride;
+    uint16_t* dst = base + moves[2 + 2 * m] * pool.page_stride;
+    uint4 v[kCopyPer];
+    int64_t off[kCopyPer];
+#pragma unroll
+    for (int i = 0; i < kCopyPer; ++i) {
+      const int c = part * kCopyUnit + i * kCopyThreads + static_cast<int>(threadIdx.x);
+      const int row = c >> dshift;
+      off[i] = c < chunks ? (row >> pshift) * pool.head_stride + (row & (pool.page_size - 1)) * pool.token_stride +
+                                (c & ((1 << dshift) - 1)) * 8
+                          : -1;
+      if (off[i] >= 0) v[i] = *reinterpret_cast<const uint4*>(src + off[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kCopyPer; ++i)
+      if (off[i] >= 0) *reinterpret_cast<uint4*>(dst + off[i]) = v[i];
+  }
+}
+
+// ------------------------------------------------------------------ keep a path
+
+constexpr int kKeepThreads = 256;
+constexpr int kKeepBatch = 8;  // tokens read before any of them is written
+
+// One thread per (16-byte chunk of a head, kv head, k or v, layer) of one sequence (blockIdx.y): it walks the path.  The
+// path ascends, so path[d] >= d, and a slot is never read after a later token was written to it.
+__global__ void __launch_bounds__(kKeepThreads) keep_kernel(const KeepParams p) {
+  pdl_wait();
+  const int s = blockIdx.y;
+  const int ctx = p.b.context[s];
+  const int ntok = max(0, min(p.b.row_start[s + 1], p.b.rows) - max(p.b.row_start[s], 0));
+  int kept = p.kept[s];
+  bool ok = ctx >= 0 && kept >= 0 && kept <= ntok && (!p.path || kept <= p.depth);
+  const int64_t room = static_cast<int64_t>(p.b.max_pages) << p.b.page_shift;
+  if (ok && static_cast<int64_t>(ctx) + ntok > room) ok = false;
+  const int32_t* path = p.path ? p.path + static_cast<int64_t>(s) * p.depth : nullptr;
+  if (ok && path) {
+    for (int d = 0; d < kept; ++d) {
+      const int a = path[d];
+      if (a >= ntok || a < (d ? path[d - 1] + 1 : 0)) ok = false;
+    }
+  }
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * kKeepThreads + threadIdx.x;
+  if (!ok) kept = 0;
+  if (item == 0) {
+    p.lens[s] = max(ctx, 0) + kept;
+    if (!ok) atomicOr(p.b.err, kErrBadShape);
+  }
+  if (!path) return;
+  const int per = p.pool.dim / 8;
+  const int c = static_cast<int>(item % per);
+  int64_t rest = item / per;
+  const int h = static_cast<int>(rest % p.pool.kv_heads);
+  rest /= p.pool.kv_heads;
+  const bool is_v = (rest & 1) != 0;
+  const int64_t layer = rest >> 1;
+  if (layer >= p.pool.layers) return;
+  uint16_t* base = (is_v ? p.pool.v : p.pool.k) + layer * p.pool.layer_stride + h * p.pool.head_stride + c * 8;
+  const int32_t* tab = p.b.table + static_cast<int64_t>(s) * p.b.max_pages;
+  const int mask = (1 << p.b.page_shift) - 1;
+  auto slot = [&](int at) -> int64_t {
+    const int id = tab[at >> p.b.page_shift];
+    if (id < 0 || id >= p.b.pages) {
+      atomicOr(p.b.err, kErrBadShape);
+      return -1;
+    }
+    return id * p.b.page_stride + (at & mask) * p.b.token_stride;
+  };
+  for (int d0 = 0; d0 < kept; d0 += kKeepBatch) {
+    uint4 v[kKeepBatch];
+    int64_t to[kKeepBatch];
+#pragma unroll
+    for (int i = 0; i < kKeepBatch; ++i) {
+      const int d = d0 + i;
+      to[i] = -1;
+      if (d < kept && path[d] != d) {
+        const int64_t from = slot(ctx + path[d]);
+        to[i] = slot(ctx + d);
+        if (from < 0) to[i] = -1;
+        if (to[i] >= 0) v[i] = *reinterpret_cast<const uint4*>(base + from);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kKeepBatch; ++i)
+      if (to[i] >= 0) *reinterpret_cast<uint4*>(base + to[i]) = v[i];
+  }
+}
+
+template <typename Kern>
+cudaError_t launch_cluster(Kern kern, size_t smem, cudaStream_t st, const PageParams& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kCluster);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+}  // namespace
+
+int cache_grow_max_rows() { return kMaxGrowRows; }
+
+cudaError_t launch_cache_fork(const PageParams& p, cudaStream_t st) { return launch_cluster(fork_kernel, 0, st, p); }
+
+cudaError_t launch_cache_grow(const PageParams& p, cudaStream_t st) {
+  static KernelSetup setup;
+  const size_t smem = (static_cast<size_t>(p.nseq_in) * 3 + 2) * sizeof(int);
+  cudaError_t e = kernel_setup(setup, grow_kernel, kThreads, (static_cast<size_t>(kMaxGrowRows) * 3 + 2) * sizeof(int));
+  if (e != cudaSuccess) return e;
+  return launch_cluster(grow_kernel, smem, st, p);
+}
+
+cudaError_t launch_cache_compact(const PageParams& p, cudaStream_t st) {
+  return launch_cluster(compact_kernel, 0, st, p);
+}
+
+cudaError_t launch_page_copy(const PagePool& pool, const int32_t* moves, int64_t max_moves, int sms, cudaStream_t st) {
+  const int64_t units = (static_cast<int64_t>(pool.kv_heads) * pool.page_size * pool.dim / 8 + kCopyUnit - 1) / kCopyUnit;
+  int64_t grid = max_moves * pool.layers * 2 * units;
+  if (grid > static_cast<int64_t>(sms) * 8) grid = static_cast<int64_t>(sms) * 8;
+  if (grid < 1) return cudaSuccess;
+  return launch_pdl_k(page_copy_kernel, dim3(static_cast<unsigned>(grid)), dim3(kCopyThreads), st, pool, moves);
+}
+
+cudaError_t launch_cache_keep(const KeepParams& p, cudaStream_t st) {
+  if (p.b.nseq <= 0) return cudaSuccess;
+  const int64_t items = p.path ? static_cast<int64_t>(p.pool.layers) * 2 * p.pool.kv_heads * (p.pool.dim / 8) : 1;
+  const dim3 grid(static_cast<unsigned>((items + kKeepThreads - 1) / kKeepThreads), static_cast<unsigned>(p.b.nseq));
+  return launch_pdl_k(keep_kernel, grid, dim3(kKeepThreads), st, p);
+}
+
+}  // namespace exl3
