@@ -61,6 +61,10 @@ struct AttnParams {
   float* partials;   // two slots per CTA
   uint32_t* counters;
 };
+// Rows per kv head up to which the few-row kernel runs: its one 16-row tile.
+constexpr int kAttnFewRows = 16;
+// the tensor-core kernel (exl3_attn_tc.cu) and the few-row kernel (exl3_attn_mma.cu)
+cudaError_t launch_attn_tc(const AttnParams& p, int dim, int sms, size_t partial_floats, cudaStream_t st);
 cudaError_t launch_attn_mma(const AttnParams& p, int dim, int sms, size_t partial_floats, cudaStream_t st);
 
 struct PageParams {

@@ -171,9 +171,11 @@ struct WorkLine {
     return p.partials + (static_cast<int64_t>(blockIdx.x) * 2 + (began_before ? 1 : 0)) * floats;
   }
 
-  // After this CTA wrote its slot: the last of the item's CTAs joins them all, in key order.
-  template <int D, bool BF16>
-  __device__ void join(const AttnParams& p, const Item& it, int slot_rows, int rows, int* s_word) const;
+  // After this CTA wrote its slot: the last of the item's CTAs joins them all, in key order.  Called by the CTA's first
+  // `threads` threads; sync() joins them.
+  template <int D, bool BF16, typename Sync>
+  __device__ void join(const AttnParams& p, const Item& it, int slot_rows, int rows, int* s_word, int threads,
+                       Sync&& sync) const;
 };
 
 // Whether new token `tok` of the item's sequence sees slot `key`.
@@ -304,22 +306,23 @@ __device__ __forceinline__ void store_out4(const AttnParams& p, const Item& it, 
     p.lse[static_cast<int64_t>(row) * p.out.heads + h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
 }
 
-template <int D, bool BF16>
-__device__ void WorkLine::join(const AttnParams& p, const Item& it, int slot_rows, int rows, int* s_word) const {
+template <int D, bool BF16, typename Sync>
+__device__ void WorkLine::join(const AttnParams& p, const Item& it, int slot_rows, int rows, int* s_word, int threads,
+                               Sync&& sync) const {
   const int c0 = part_of(it.first), c1 = part_of(it.first + it.tiles - 1), n = c1 - c0 + 1;
   __threadfence();
-  __syncthreads();
+  sync();
   if (threadIdx.x == 0) {
     const uint32_t before = atomicAdd(p.counters + c0, 1u);
     const bool last = before + 1u == static_cast<uint32_t>(n);
     if (last) p.counters[c0] = 0u;
     *s_word = last;
   }
-  __syncthreads();
+  sync();
   if (*s_word) {
     __threadfence();
     const int floats = slot_rows * (D + 2);
-    for (int i = static_cast<int>(threadIdx.x); i < rows * (D / 4); i += blockDim.x) {
+    for (int i = static_cast<int>(threadIdx.x); i < rows * (D / 4); i += threads) {
       const int r = i / (D / 4), d0 = (i % (D / 4)) * 4;
       float mx = -INFINITY, sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
       for (int c = c0; c <= c1; ++c) {
@@ -336,7 +339,7 @@ __device__ void WorkLine::join(const AttnParams& p, const Item& it, int slot_row
       store_out4<BF16>(p, it, slot_rows, r, d0, acc, mx, sum);
     }
   }
-  __syncthreads();
+  sync();
 }
 
 }  // namespace exl3

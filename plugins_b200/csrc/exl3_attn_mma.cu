@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const AttnParams p) 
         if (d0 == 0) *reinterpret_cast<float2*>(slot + S::kRows * D + 2 * r) = make_float2(mx, sum);
       }
     }
-    if (!whole) line.template join<D, BF16>(p, it, S::kRows, rows, s_word);
+    if (!whole) line.template join<D, BF16>(p, it, S::kRows, rows, s_word, kThreads, [] { __syncthreads(); });
     at += tiles;
     if (at < end) line.next(p, it);
   }

@@ -1,0 +1,647 @@
+// exl3_attn_tc.cu -- attention of many rows per kv head over the paged cache (drafted trees, prompt chunks) on the
+// 5th-generation tensor cores.
+//
+// The same one-pass softmax as exl3_attn_mma.cu.  A row block is up to 256 rows (kv head's query heads x new tokens) in
+// one or two 128-row tiles; scores S = Q K^T and outputs O += P V are tcgen05.mma products with the accumulators in
+// TMEM.  P, the probabilities in 16 bits, overwrites its own scores' columns in TMEM and is the A operand of the second
+// product from there.
+//
+// Two S/P buffers keep the tensor pipe and the exponentials busy at once.  With two row tiles, each buffer belongs to
+// one of them (the events of a block: (tile 0, rows 0), (tile 0, rows 1), (tile 1, rows 0), ...); with one, the key
+// tiles alternate between the buffers, for heads up to 128 wide each with its own O and running maximum, joined at the
+// end -- so a small block also has two chains in flight.  256-wide heads (whose O takes half of TMEM) have one O, and
+// 64-key tiles.
+//
+// Roles: NG groups of four softmax warps (a thread per row: tcgen05.ld of its scores, maximum, exponentials, P back by
+// tcgen05.st), then one warp each for the MMAs, K copies, V copies (TMA, one box per page and 64 columns, 128-byte
+// swizzle) and the V tiles' cleaning.  O is rescaled only when a row's maximum has grown by more than 2^8 (P then stays
+// below 2^8, and the f32 sums and the final division take out the difference); the old maximum is kept otherwise.
+//
+// Keys that some row of the block does not see (stale slots, other branches) are masked in S by index; their V rows
+// cannot be masked there (0 x inf = NaN), so in the tiles that hold such keys the cleaning warp zeroes slots past the
+// sequence and infinities and NaN; the latter are added back in the epilogue to the rows that see them.
+//
+// Every mbarrier wait is bounded (role_wait): one that gives up raises an abort flag that all roles poll.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "exl3_attn.h"
+#include "exl3_attn_dev.cuh"
+#include "exl3_common.cuh"
+#include "exl3_internal.h"
+#include "exl3_tc.cuh"
+
+namespace exl3 {
+
+using namespace tc;
+
+namespace {
+
+template <int D>
+struct TcShape {
+  static constexpr int NG = D == 256 ? 1 : 2;             // softmax groups (and O accumulators)
+  static constexpr int KT = D == 256 ? 64 : 128;          // keys per tile
+  static constexpr int kRows = D == 256 ? 128 : 256;      // rows per block
+  static constexpr int kThreads = NG * 128 + 128;
+  static constexpr int kSoft = NG * 128;                  // softmax threads
+  static constexpr int kTile = KT * D * 2;                // bytes of a K or V tile
+  static constexpr int kQBytes = kRows * D * 2;
+  static constexpr int kSlots = 5 * 32768 / kTile;        // K and V tiles in flight: 160 KiB
+  static constexpr int VS = kSlots / 2, KS = kSlots - VS;
+  static constexpr int kOCol = 256;                       // TMEM: S buffers at columns 0 and KT, O of group g at 256 + g * D
+  static constexpr int kTmem = 512;
+  static constexpr int kBars = 2 * KS + 3 * VS + 2 + 2 + 2 + 5;
+  static constexpr int kSmem = kQBytes + kSlots * kTile + 2 * 128 * 8 + kBars * 8 + 64;
+  static_assert(KS * kTile + VS * kTile + kQBytes <= 229376 && kSmem <= 232448, "shared memory");
+  static_assert(VS <= 8, "the odd flags cover eight items");
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A box of the cache: 64 columns from x, the rows from `tok` of one page and head.
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int tok, int head, int page,
+                                        uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
+          "r"(dst),
+      "l"(map), "r"(x), "r"(tok), "r"(head), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// Shared-memory descriptor of an operand whose rows are k (keys) and whose contiguous direction is M or N: 64-element
+// blocks of 128-byte swizzled rows, `block_bytes` apart; 8-key groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t block_bytes) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((block_bytes >> 4) & 0x3FFFu) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+
+// Instruction descriptor of kind::f16 with f32 accumulators; b_mn: B's contiguous direction is N.
+template <bool BF16>
+constexpr uint32_t attn_idesc(int m, int n, bool b_mn) {
+  return umma_idesc(m, n) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u);
+}
+
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Orders uses of registers loaded by tmem_ld32 after an earlier wait (tmem_wait_ld of another load).
+__device__ __forceinline__ void after_wait(uint32_t (&r)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i])::"memory");
+}
+
+// The block as the roles walk it: its key tiles [tile0, tile0 + tiles), one or two row tiles, and its events.
+struct Block {
+  int tile0, tiles, rows, qt, events, full_keys;
+};
+template <int D>
+__device__ __forceinline__ Block block_of(const AttnParams& p, const WorkLine& line, const Item& it, int64_t at) {
+  using S = TcShape<D>;
+  Block b;
+  b.tile0 = static_cast<int>(at - it.first);
+  b.tiles = static_cast<int>(min(line.end - at, static_cast<int64_t>(it.tiles - b.tile0)));
+  b.rows = min(S::kRows, it.nrows - it.row_block * S::kRows);
+  b.qt = b.rows > 128 ? 2 : 1;
+  b.events = b.qt * b.tiles;
+  // the leading keys that every row sees
+  const int all = p.b.tree ? it.context : it.context + it.row_block * S::kRows / p.group + 1;
+  b.full_keys = min(all, it.total_keys);
+  return b;
+}
+
+// Which of the slots key0 .. key0 + 31 new token tok sees.
+__device__ __forceinline__ uint32_t seen32(const PagedBatch& b, const Item& it, int tok, int key0) {
+  if (tok >= it.ntok) return 0u;
+  uint32_t m;
+  const int d = key0 - it.context;  // the first slot's place among the new tokens
+  if (!b.tree) {
+    const int n = tok + 1 - d;
+    m = n >= 32 ? ~0u : (n <= 0 ? 0u : (1u << n) - 1u);
+  } else if (d <= -32) {
+    m = ~0u;
+  } else {
+    const uint32_t* t = b.tree + static_cast<int64_t>(it.row0 + tok) * b.tree_words;
+    if (d < 0) {
+      m = (t[0] << (-d)) | ((1u << (-d)) - 1u);
+    } else {
+      const int w = d >> 5;
+      const uint32_t lo = w < b.tree_words ? t[w] : 0u, hi = w + 1 < b.tree_words ? t[w + 1] : 0u;
+      m = __funnelshift_r(lo, hi, d & 31);
+    }
+  }
+  const int left = it.total_keys - key0;
+  if (left < 32) m &= left <= 0 ? 0u : (1u << left) - 1u;
+  return m;
+}
+
+// The infinities and NaN of V among keys [key_lo, key_hi) that row token `tok` of head `h` sees, which the cleaning
+// warp took out of the product: o[i] += e^(s - m) v for columns d0 .. d0 + 31.  Rare, so plain loads and one thread.
+template <int D, bool BF16>
+__device__ __noinline__ void add_odd(const AttnParams& p, const Item& it, int tok, int h, int key_lo, int key_hi,
+                                     int full_keys, float m, int d0, float* o) {
+  if (tok >= it.ntok) return;
+  const uint16_t* q = static_cast<const uint16_t*>(p.q.data) + static_cast<int64_t>(it.row0 + tok) * p.q.row_stride +
+                      h * p.q.head_stride;
+  // only tiles that reach past full_keys were cleaned
+  constexpr int KT = TcShape<D>::KT;
+  for (int key = max(key_lo, full_keys / KT * KT); key < min(key_hi, it.total_keys); ++key) {
+    if (!sees(p.b, it, tok, key)) continue;
+    const int id = p.b.table[static_cast<int64_t>(it.seq) * p.b.max_pages + (key >> p.b.page_shift)];
+    if (id < 0 || id >= p.b.pages) continue;
+    const int64_t off = id * p.b.page_stride + (key & ((1 << p.b.page_shift) - 1)) * p.b.token_stride +
+                        it.kv_head * p.b.head_stride;
+    bool any = false;
+    for (int i = 0; i < 32; ++i) any |= !isfinite(unpack1<BF16>(p.b.v[off + d0 + i], 0));
+    if (!any) continue;
+    float s = 0.f;
+    for (int d = 0; d < D; ++d) s += unpack1<BF16>(q[d], 0) * unpack1<BF16>(p.b.k[off + d], 0);
+    const float w = ex2(s * p.scale_log2 - (m == -INFINITY ? 0.f : m));
+    for (int i = 0; i < 32; ++i) {
+      const float v = unpack1<BF16>(p.b.v[off + d0 + i], 0);
+      if (!isfinite(v)) o[i] += w * v;
+    }
+  }
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
+    attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap kmap,
+                   const __grid_constant__ CUtensorMap vmap) {
+  using S = TcShape<D>;
+  constexpr int NG = S::NG, KT = S::KT, KS = S::KS, VS = S::VS;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* s_q = smem;                       // [row tile][64-column block][128 rows][128 bytes], swizzled
+  uint8_t* s_k = s_q + S::kQBytes;           // [slot][64-column block][KT rows][128 bytes]
+  uint8_t* s_v = s_k + KS * S::kTile;
+  float2* s_ml = reinterpret_cast<float2*>(s_v + VS * S::kTile);  // [2][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_ml + 256);
+  uint64_t *kfull = bars, *kempty = kfull + KS, *vfull = kempty + KS, *vclean = vfull + VS, *vempty = vclean + VS;
+  uint64_t *sfull = vempty + VS, *pready = sfull + 2, *ofull = pready + 2;
+  uint64_t *qfull = ofull + 2, *ofree = qfull + 1, *xsync = ofree + 1, *pvdone = xsync + 1, *fin = pvdone + 1;
+  uint32_t* words = reinterpret_cast<uint32_t*>(bars + S::kBars);
+  uint32_t* s_tmem = words;
+  volatile uint32_t* abort_flag = words + 1;
+  int* s_last = reinterpret_cast<int*>(words + 2);
+  volatile uint32_t* s_odd = words + 4;  // [8]: serial + 1 of an item whose V held infinities or NaN
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+
+  if (smem_u32(smem) & 1023u) {  // the swizzle goes by address bits: not served
+    if (tid == 0) atomicOr(p.b.err, kErrBadShape);
+    return;
+  }
+  if (warp == NG * 4) {
+    tmem_alloc(smem_u32(s_tmem), S::kTmem);
+    tmem_relinquish();
+  }
+  if (tid == 0) {
+    for (int i = 0; i < KS; ++i) mbar_init(&kfull[i], 1), mbar_init(&kempty[i], 1);
+    for (int i = 0; i < VS; ++i) mbar_init(&vfull[i], 1), mbar_init(&vclean[i], 1), mbar_init(&vempty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&sfull[i], 1), mbar_init(&pready[i], 128), mbar_init(&ofull[i], 1);
+    mbar_init(qfull, S::kSoft), mbar_init(ofree, S::kSoft), mbar_init(xsync, S::kSoft);
+    mbar_init(pvdone, 1), mbar_init(fin, 1);
+    fence_barrier_init();
+    *abort_flag = 0u;
+    for (int i = 0; i < 8; ++i) s_odd[i] = 0u;
+  }
+  pdl_wait();
+  WorkLine line;
+  line.init(p, S::kRows, KT, reinterpret_cast<int64_t*>(s_k));
+  Item it;
+  if (line.begin < line.end) line.locate(p, line.begin, it, reinterpret_cast<int64_t*>(s_k));
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  int64_t at = line.begin;
+
+  if (warp < NG * 4) {
+    // ---------------------------------------------------------------- softmax groups
+    const uint32_t g = warp >> 2, wq = warp & 3u, r128 = wq * 32 + lane;  // row of the 128-row tile = TMEM lane
+    const uint32_t lane_off = (wq * 32u) << 16;
+    uint32_t sphase = 0, ophase = 0, xphase = 0, pvphase = 0;  // sphase: a bit per buffer; ophase: per group
+    bool ok = true;
+    auto group_sync = [&]() {  // all softmax threads
+      mbar_arrive(xsync);
+      ok = __all_sync(0xFFFFFFFFu, ok && role_wait(xsync, xphase, abort_flag, p.b.err));
+      xphase ^= 1u;
+    };
+    for (uint32_t serial = 0; ok && at < line.end; ++serial) {
+      const Block b = block_of<D>(p, line, it, at);
+      // the query rows into their swizzled tiles: with two row tiles a group loads its own, else both share the one
+      {
+        const uint32_t tile = b.qt == 2 ? g : 0u;
+        const int cols0 = b.qt == 2 || NG == 1 ? 0 : static_cast<int>(g) * (D / 2);
+        const int ncols = b.qt == 2 || NG == 1 ? D : D / 2;
+        const int r = static_cast<int>(tile * 128u + r128);
+        const int rr = it.row_block * S::kRows + r, t = rr / p.group, h = it.kv_head * p.group + rr % p.group;
+#pragma unroll 8
+        for (int c = 0; c < ncols / 8; ++c) {
+          const int col = cols0 + c * 8;
+          uint4 u = make_uint4(0u, 0u, 0u, 0u);
+          if (r < b.rows) u = load_q8(p.q, it.row0 + t, h, col);
+          *reinterpret_cast<uint4*>(s_q + tile * (128 * D * 2) + (col >> 6) * (128 * 128) +
+                                    image_offset(r128, static_cast<uint32_t>(col & 63))) = u;
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(qfull);
+
+      const int row = (b.qt == 2 ? static_cast<int>(g) * 128 : 0) + static_cast<int>(r128);
+      const int tok = (it.row_block * S::kRows + row) / p.group;
+      float m = -INFINITY, l = 0.f;  // m in units of log2
+      for (int e = static_cast<int>(g); e < b.events; e += NG) {
+        const uint32_t buf = e & 1;
+        const int tile = b.qt == 2 ? e >> 1 : e;
+        const int key0 = (b.tile0 + tile) * KT;
+        const uint32_t s_addr = tmem + lane_off + buf * KT;
+        ok = __all_sync(0xFFFFFFFFu, ok && role_wait(&sfull[buf], (sphase >> buf) & 1u, abort_flag, p.b.err));
+        sphase ^= 1u << buf;
+        tc_fence_after();
+        uint32_t x[KT / 32][32];
+#pragma unroll
+        for (int c = 0; c < KT / 32; ++c) tmem_ld32(s_addr + c * 32, x[c]);
+        tmem_wait_ld(x[0]);
+#pragma unroll
+        for (int c = 1; c < KT / 32; ++c) after_wait(x[c]);
+        if (key0 + KT > b.full_keys) {
+#pragma unroll
+          for (int c = 0; c < KT / 32; ++c) {
+            const uint32_t mask = seen32(p.b, it, tok, key0 + c * 32);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(mask & (1u << i))) x[c][i] = 0xFF800000u;  // -inf
+          }
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < KT / 32; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(x[c][i]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+        const bool grow = top > m + 8.f;  // (m = -inf: as soon as anything is seen)
+        const bool first = e < NG;
+        if (first) {
+          m = top;
+        } else if (__any_sync(0xFFFFFFFFu, grow)) {
+          if constexpr (NG == 1)
+            ok = __all_sync(0xFFFFFFFFu, ok && role_wait(pvdone, pvphase ^ 1u, abort_flag, p.b.err));
+          tc_fence_after();
+          const float f = grow ? ex2(m - top) : 1.f;
+          if (grow) m = top, l *= f;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            const uint32_t o_addr = tmem + lane_off + S::kOCol + g * D + c * 32;
+            tmem_ld32(o_addr, o);
+            tmem_wait_ld(o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st32(o_addr, o);
+          }
+          tmem_wait_st();
+        }
+        pvphase ^= 1u;
+        const float base = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KT / 64; ++c) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float a = ex2(fmaf(__uint_as_float(x[2 * c + (i >> 4)][(2 * i) & 31]), p.scale_log2, -base));
+            const float d = ex2(fmaf(__uint_as_float(x[2 * c + (i >> 4)][(2 * i + 1) & 31]), p.scale_log2, -base));
+            sum[(2 * i) & 3] += a, sum[(2 * i + 1) & 3] += d;
+            pk[i] = pack2<BF16>(a, d);  // (l keeps the f32 values)
+          }
+          tmem_st32(s_addr + c * 32, pk);
+        }
+        tmem_wait_st();
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tc_fence_before();
+        mbar_arrive(&pready[buf]);
+      }
+
+      // ---- the block's end: o / l, or a partial for the join
+      const bool whole = b.tiles == it.tiles;
+      const bool two = b.qt == 1 && NG == 2;  // two key halves of the same rows
+      const int mine = two ? (b.events > static_cast<int>(g) ? 1 : 0) : 1;  // this group had a tile
+      if (mine) {
+        ok = __all_sync(0xFFFFFFFFu, ok && role_wait(&ofull[g], ophase, abort_flag, p.b.err));
+        ophase ^= 1u;
+      }
+      float f0 = 1.f, f1 = 0.f;
+      if (two) {
+        s_ml[g * 128 + r128] = make_float2(m, l);
+        group_sync();
+        const float2 a = s_ml[r128], c = s_ml[128 + r128];
+        m = fmaxf(a.x, c.x);
+        const float base = m == -INFINITY ? 0.f : m;
+        f0 = ex2(a.x - base), f1 = ex2(c.x - base);
+        l = a.y * f0 + c.y * f1;
+      }
+      tc_fence_after();
+      const bool second = two && b.events > 1;
+      const bool odd = s_odd[serial & 7u] == serial + 1u;
+      const int cols0 = two ? static_cast<int>(g) * (D / 2) : 0, ncols = two ? D / 2 : D;
+      const uint32_t o0 = tmem + lane_off + S::kOCol + (two ? 0u : g * D), o1 = tmem + lane_off + S::kOCol + D;
+      const bool live = row < b.rows;
+      const int rr = it.row_block * S::kRows + row;
+      const int h = it.kv_head * p.group + rr % p.group;
+      const int64_t out_row = it.row0 + tok;
+      float* slot = whole ? nullptr : line.slot(p, S::kRows * (D + 2), at != it.first);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+      for (int c = cols0; c < cols0 + ncols; c += 32) {
+        uint32_t v[32];
+        float o[32];
+        tmem_ld32(o0 + c, v);
+        tmem_wait_ld(v);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(v[i]);
+        if (second) {
+          tmem_ld32(o1 + c, v);
+          tmem_wait_ld(v);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = o[i] * f0 + __uint_as_float(v[i]) * f1;
+        }
+        if (!live) continue;
+        if (odd) {
+          float t[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) t[i] = o[i];
+          add_odd<D, BF16>(p, it, tok, h, b.tile0 * KT, (b.tile0 + b.tiles) * KT, b.full_keys, m, c, t);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = t[i];
+        }
+        if (whole) {
+          uint16_t* dst = static_cast<uint16_t*>(p.out.data) + out_row * p.out.row_stride + h * p.out.head_stride + c;
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            w[i] = l == 0.f ? 0u : pack2<BF16>(o[2 * i] * inv, o[2 * i + 1] * inv);
+          if (p.out.vec) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dst[2 * i] = static_cast<uint16_t>(w[i]), dst[2 * i + 1] = static_cast<uint16_t>(w[i] >> 16);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<float4*>(slot + row * D + c + 4 * i) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+      }
+      if (live && cols0 == 0) {
+        if (whole) {
+          if (p.lse) p.lse[out_row * p.out.heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+        } else {
+          *reinterpret_cast<float2*>(slot + S::kRows * D + 2 * row) = make_float2(m, l);
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(ofree);
+      if (!whole) line.template join<D, BF16>(p, it, S::kRows, b.rows, s_last, S::kSoft, group_sync);
+      group_sync();  // every MMA of the block has finished, and its rows are read: Q may be replaced
+      at += b.tiles;
+      if (at < line.end) line.next(p, it);
+    }
+  } else if (warp == NG * 4) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = attn_idesc<BF16>(128, KT, false), idesc_o = attn_idesc<BF16>(128, D, true);
+      const uint32_t q0 = smem_u32(s_q), k0 = smem_u32(s_k), v0 = smem_u32(s_v);
+      uint32_t kfirst = 0, vfirst = 0;  // tiles of the blocks before
+      uint32_t pphase = 0;
+      bool ok = true;
+      for (uint32_t serial = 0; ok && at < line.end; ++serial) {
+        const Block b = block_of<D>(p, line, it, at);
+        ok = ok && role_wait(qfull, serial & 1u, abort_flag, p.b.err);
+        auto scores = [&](int e) {
+          const int tile = b.qt == 2 ? e >> 1 : e;
+          const uint32_t n = kfirst + static_cast<uint32_t>(tile), slot = n % KS;
+          if (b.qt == 1 || !(e & 1)) ok = ok && role_wait(&kfull[slot], (n / KS) & 1u, abort_flag, p.b.err);
+          if (!ok) return;
+          tc_fence_after();
+          const uint32_t qa = q0 + (b.qt == 2 ? (e & 1) * (128 * D * 2) : 0), ka = k0 + slot * S::kTile;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_f16(tmem + (e & 1) * KT, sw128_desc(qa + (kk >> 2) * (128 * 128) + (kk & 3) * 32),
+                     sw128_desc(ka + (kk >> 2) * (KT * 128) + (kk & 3) * 32), idesc_s, kk != 0 ? 1u : 0u);
+          umma_commit(&sfull[e & 1]);
+          if (b.qt == 1 || (e & 1)) umma_commit(&kempty[slot]);
+        };
+        scores(0);
+        if (b.events > 1) scores(1);
+        if (serial) ok = ok && role_wait(ofree, (serial - 1) & 1u, abort_flag, p.b.err);
+        for (int e = 0; ok && e < b.events; ++e) {
+          const uint32_t buf = e & 1;
+          const int tile = b.qt == 2 ? e >> 1 : e;
+          const uint32_t n = vfirst + static_cast<uint32_t>(tile), slot = n % VS;
+          ok = ok && role_wait(&pready[buf], (pphase >> buf) & 1u, abort_flag, p.b.err);
+          pphase ^= 1u << buf;
+          if (b.qt == 1 || !(e & 1)) ok = ok && role_wait(&vclean[slot], (n / VS) & 1u, abort_flag, p.b.err);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t va = v0 + slot * S::kTile;
+          const uint32_t od = tmem + S::kOCol + (NG == 2 ? buf * D : 0);
+          const bool first = e < NG;
+#pragma unroll
+          for (int kk = 0; kk < KT / 16; ++kk)
+            umma_ts(od, tmem + buf * KT + kk * 8, sw128_mn_desc(va + kk * 2048, KT * 128), idesc_o,
+                    !first || kk != 0 ? 1u : 0u);
+          if constexpr (NG == 1) umma_commit(pvdone);
+          if (b.qt == 1 || (e & 1)) umma_commit(&vempty[slot]);
+          if (e + 2 < b.events) scores(e + 2);
+          if (e + NG >= b.events) umma_commit(&ofull[NG == 2 ? buf : 0]);
+        }
+        kfirst += b.tiles, vfirst += b.tiles;
+        at += b.tiles;
+        if (at < line.end) line.next(p, it);
+      }
+      umma_commit(fin);  // every MMA has finished before TMEM is released
+      if (!mbar_wait_bounded(fin, 0)) atomicOr(p.b.err, kErrWaitTimeout);
+    }
+    __syncwarp();
+  } else if (warp <= NG * 4 + 2) {
+    // ---------------------------------------------------------------- K copies, V copies
+    const bool is_v = warp == NG * 4 + 2;
+    const int slots = is_v ? VS : KS;
+    uint64_t *full = is_v ? vfull : kfull, *empty = is_v ? vempty : kempty;
+    const uint32_t base = smem_u32(is_v ? s_v : s_k);
+    const CUtensorMap* map = is_v ? &vmap : &kmap;
+    const int box_rows = min(1 << p.b.page_shift, KT);
+    const int boxes = KT / box_rows * (D / 64);  // at most 16: a lane each
+    const int blk = static_cast<int>(lane) % (D / 64), part = static_cast<int>(lane) / (D / 64);
+    uint32_t n = 0;
+    bool ok = true;
+    while (ok && at < line.end) {
+      const Block b = block_of<D>(p, line, it, at);
+      const int32_t* tab = p.b.table + static_cast<int64_t>(it.seq) * p.b.max_pages;
+      for (int t = 0; ok && t < b.tiles; ++t, ++n) {
+        const uint32_t slot = n % slots;
+        const int key = (b.tile0 + t) * KT + part * box_rows;
+        int id = -1;
+        if (static_cast<int>(lane) < boxes && key < it.total_keys) {
+          id = tab[key >> p.b.page_shift];
+          if (id < 0 || id >= p.b.pages) {
+            atomicOr(p.b.err, kErrBadShape);
+            id = -1;
+          }
+        }
+        const uint32_t loads = __popc(__ballot_sync(0xFFFFFFFFu, id >= 0));
+        if (n >= static_cast<uint32_t>(slots))
+          ok = role_wait(&empty[slot], (n / slots - 1) & 1u, abort_flag, p.b.err);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&full[slot], loads * box_rows * 128);
+        if (id >= 0)
+          tma_box(base + slot * S::kTile + blk * (KT * 128) + part * box_rows * 128, map, blk * 64,
+                  key & ((1 << p.b.page_shift) - 1), it.kv_head, id, &full[slot]);
+      }
+      at += b.tiles;
+      if (ok && at < line.end) line.next(p, it);
+    }
+    // no copy may outlive the CTA: wait (bounded) for the last fill of every slot
+    const uint32_t last = min(n, static_cast<uint32_t>(slots));
+    for (uint32_t i = 1; i <= last; ++i) {
+      const uint32_t f = n - i;
+      if (!mbar_wait_bounded(&full[f % slots], (f / slots) & 1u)) atomicOr(p.b.err, kErrWaitTimeout);
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- V cleaning
+    uint32_t n = 0;
+    bool ok = true;
+    for (uint32_t serial = 0; ok && at < line.end; ++serial) {
+      const Block b = block_of<D>(p, line, it, at);
+      for (int t = 0; ok && t < b.tiles; ++t, ++n) {
+        const uint32_t slot = n % VS;
+        ok = role_wait(&vfull[slot], (n / VS) & 1u, abort_flag, p.b.err);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+        const int key0 = (b.tile0 + t) * KT;
+        if (key0 + KT > b.full_keys) {
+          uint8_t* tile = s_v + slot * S::kTile;
+          bool odd = false;
+#pragma unroll 4
+          for (int i = static_cast<int>(lane); i < S::kTile / 16; i += 32) {
+            const int key = key0 + (i >> 3) % KT;  // eight 16-byte chunks per row of a block
+            uint4* c = reinterpret_cast<uint4*>(tile) + i;
+            if (key >= it.total_keys) {
+              *c = make_uint4(0u, 0u, 0u, 0u);
+            } else {
+              const uint4 u = *c;
+              if (odd2<BF16>(u.x) || odd2<BF16>(u.y) || odd2<BF16>(u.z) || odd2<BF16>(u.w)) {
+                odd = true;
+                *c = make_uint4(zero_odd2<BF16>(u.x), zero_odd2<BF16>(u.y), zero_odd2<BF16>(u.z), zero_odd2<BF16>(u.w));
+              }
+            }
+          }
+          if (odd) s_odd[serial & 7u] = serial + 1u;
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(&vclean[slot]);
+      }
+      at += b.tiles;
+      if (ok && at < line.end) line.next(p, it);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == NG * 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S::kTmem);
+  }
+}
+
+// ------------------------------------------------------------------ host
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+  static const EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  return fn;
+}
+
+// The layer's K or V as [pages][kv_heads][page_size][dim], in boxes of 64 columns by min(page_size, key tile) rows.
+bool encode(CUtensorMap& map, void* base, const AttnParams& p, int dim, int tile_keys) {
+  const EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t page = 1ull << p.b.page_shift;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(dim), page, static_cast<cuuint64_t>(p.b.kv_heads),
+                              static_cast<cuuint64_t>(p.b.pages)};
+  // (a dimension of one takes no steps: its stride need not mean anything)
+  const cuuint64_t row = static_cast<cuuint64_t>(p.b.token_stride) * 2;
+  const cuuint64_t strides[3] = {row, p.b.kv_heads > 1 ? static_cast<cuuint64_t>(p.b.head_stride) * 2 : row,
+                                 p.b.pages > 1 ? static_cast<cuuint64_t>(p.b.page_stride) * 2 : row};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(page < static_cast<cuuint64_t>(tile_keys) ? page : tile_keys), 1, 1};
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  return fn(&map, p.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims, strides, box,
+            step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D>
+cudaError_t launch_dim(const AttnParams& p, int sms, size_t partial_floats, cudaStream_t st) {
+  using S = TcShape<D>;
+  static KernelSetup setup[2];
+  auto kern = p.bf16 ? attn_tc_kernel<D, true> : attn_tc_kernel<D, false>;
+  cudaError_t e = kernel_setup(setup[p.bf16 ? 1 : 0], kern, S::kThreads, S::kSmem);
+  if (e != cudaSuccess) return e;
+  CUtensorMap kmap, vmap;
+  if (!encode(kmap, p.b.k, p, D, S::KT) || !encode(vmap, p.b.v, p, D, S::KT)) return cudaErrorInvalidValue;
+  const int64_t blocks = (static_cast<int64_t>(p.max_rows) * p.group + S::kRows - 1) / S::kRows;
+  const int64_t tiles = static_cast<int64_t>(p.b.nseq) * p.b.kv_heads * blocks * ((p.max_context + S::KT - 1) / S::KT);
+  int64_t grid = sms;
+  if (grid > tiles) grid = tiles;
+  const int64_t fit = static_cast<int64_t>(partial_floats / (2 * S::kRows * (D + 2)));
+  if (grid > fit) grid = fit;
+  if (grid < 1) grid = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, p, kmap, vmap);
+}
+
+}  // namespace
+
+cudaError_t launch_attn_tc(const AttnParams& p, int dim, int sms, size_t partial_floats, cudaStream_t st) {
+  switch (dim) {
+    case 64: return launch_dim<64>(p, sms, partial_floats, st);
+    case 128: return launch_dim<128>(p, sms, partial_floats, st);
+    default: return launch_dim<256>(p, sms, partial_floats, st);
+  }
+}
+
+}  // namespace exl3

@@ -131,6 +131,9 @@ CASES = [
     ([20], [70], 16, 8, 256, 256),
     ([100], [37], 5, 1, 128, 64),
     ([70, 65], [0, 260], 8, 8, 128, 128),
+    ([17, 1, 31, 0, 64], [129, 700, 0, 3, 255], 8, 2, 128, 16),
+    ([130, 40], [120, 9], 4, 1, 256, 16),
+    ([300], [200], 2, 1, 64, 32),
 ]
 
 
@@ -147,10 +150,11 @@ def test_attention(A, rows, lens, heads, kv_heads, dim, page, kind, dtype):
 
 
 @pytest.mark.parametrize("dim", [64, 128, 256])
-def test_attention_long_keys_split_over_the_gpu(A, dim):
-    st = Step([2], [6001], 2, dim, 64, "bf16", tree=chain, seed=5, layers=1)
-    cache, batch = st.device(A, max_context=6003)
-    q = torch.randn((2, 8, dim), generator=torch.Generator().manual_seed(2)).to(st.dtype) * 2
+@pytest.mark.parametrize("rows", [2, 12, 40, 70])
+def test_attention_long_keys_split_over_the_gpu(A, dim, rows):
+    st = Step([rows], [6001], 2, dim, 64, "bf16", tree=chain, seed=5, layers=1)
+    cache, batch = st.device(A, max_context=6001 + rows)
+    q = torch.randn((rows, 8, dim), generator=torch.Generator().manual_seed(2)).to(st.dtype) * 2
     out, lse = A.tree_attention(cache, 0, batch, q.cuda(), lse=True)
     check_attention(out, lse, *st.want(q, dim ** -0.5), st.dtype)
     for _ in range(3):  # the joins leave their counters clear, and the order of arrival does not show
