@@ -89,6 +89,8 @@ exl3::HeadsView view(const exl3_heads* h) {
   v.data = h->data, v.dtype = h->dtype, v.heads = h->heads, v.row_stride = h->row_stride, v.head_stride = h->head_stride;
   const int64_t per = h->dtype == EXL3_F32 ? 4 : 8;  // elements of 16 bytes
   v.vec = aligned16(h->data) && h->row_stride % per == 0 && h->head_stride % per == 0;
+  if (v.vec && reinterpret_cast<uintptr_t>(h->data) % 32 == 0 && h->row_stride % (2 * per) == 0 && h->head_stride % (2 * per) == 0)
+    v.vec = 2;
   return v;
 }
 
@@ -204,6 +206,7 @@ exl3_verdict exl3_tree_attention(const exl3_kv_cache* cache, int32_t layer, cons
   if (out->heads != q->heads || q->heads % cache->kv_heads)
     return refuse(EXL3_FAILED, "exl3_b200: q and out have a whole number of heads per kv head");
   if (q->heads > 4096) return refuse(EXL3_TOO_LARGE, "exl3_b200: more than 4096 query heads");
+  if (static_cast<int64_t>(rows) * q->heads > (1ll << 30)) return refuse(EXL3_TOO_LARGE, "exl3_b200: more than 2^30 query vectors");
   if (!(scale > 0.f) || std::isinf(scale)) return refuse(EXL3_UNSUPPORTED, "exl3_b200: the scale is a positive number");
   if (batch->max_rows > rows) return refuse(EXL3_FAILED, "exl3_b200: max_rows is above the batch's rows");
   if (batch->nseq == 0 || rows == 0) return kOk;

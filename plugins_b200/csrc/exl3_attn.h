@@ -37,7 +37,7 @@ struct HeadsView {
   void* data;
   int32_t dtype, heads;
   int64_t row_stride, head_stride;
-  int32_t vec;  // 16-byte loads and stores are aligned
+  int32_t vec;  // vectors of this many times 16 bytes are aligned: 0, 1 or 2
 };
 
 struct NormRopeParams {

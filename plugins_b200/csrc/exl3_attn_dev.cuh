@@ -41,22 +41,37 @@ __device__ __forceinline__ void item_seq(const AttnParams& p, int s, Item& it) {
 // The keys a row block can see: all with a tree, up to its last token without.
 __device__ __forceinline__ int block_keys(const AttnParams& p, const Item& it, int rb, int rows_per_block) {
   if (p.b.tree) return it.total_keys;
-  const int last = min(it.ntok - 1, static_cast<int>((static_cast<int64_t>(rb + 1) * rows_per_block - 1) / p.group));
+  // (rb + 1) rows_per_block is below nrows + a block: under 2^31
+  const int last = min(it.ntok - 1, static_cast<int>(((rb + 1u) * rows_per_block - 1u) / static_cast<uint32_t>(p.group)));
   return min(it.total_keys, it.context + last + 1);
 }
 
-// All items' tiles on one line, (sequence, kv head, row block)-major, cut into equal parts: CTA c of `parts` takes
-// [total c / parts, total (c + 1) / parts).
+// a / b for a >= 0, b > 0: nearly always in 32 bits
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  if (static_cast<uint64_t>(a | b) >> 32 == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
+// All items' tiles on one line, (sequence, kv head, row block)-major, cut into equal parts, one per CTA.
 struct WorkLine {
   int64_t total, begin, end;
-  int parts, rows_per_block, tile_keys;
+  int64_t share;  // tiles of a part; the first `extra` parts have one more
+  int extra;
+  int parts, rows_per_block, tile_keys, tile_shift;
 
   // the tiles of one kv head of sequence s
   __device__ __forceinline__ int64_t head_tiles(const AttnParams& p, const Item& it) const {
     const int nb = (it.nrows + rows_per_block - 1) / rows_per_block;
-    if (p.b.tree) return static_cast<int64_t>(nb) * ((it.total_keys + tile_keys - 1) / tile_keys);
+    if (p.b.tree) return static_cast<int64_t>(nb) * ((it.total_keys + tile_keys - 1) >> tile_shift);
+    // block_keys for every block, the last token (rows_per_block (rb + 1) - 1) / group kept as quotient and remainder
+    int q = (rows_per_block - 1) / p.group, r = (rows_per_block - 1) % p.group;
+    const int dq = rows_per_block / p.group, dr = rows_per_block % p.group;
     int64_t t = 0;
-    for (int rb = 0; rb < nb; ++rb) t += (block_keys(p, it, rb, rows_per_block) + tile_keys - 1) / tile_keys;
+    for (int rb = 0; rb < nb; ++rb) {
+      t += (min(it.total_keys, it.context + min(it.ntok - 1, q) + 1) + tile_keys - 1) >> tile_shift;
+      q += dq, r += dr;
+      if (r >= p.group) ++q, r -= p.group;
+    }
     return t;
   }
 
@@ -78,7 +93,7 @@ struct WorkLine {
   int64_t mine_, upto_;  // this thread's sequence of the last scanned chunk
 
   __device__ void init(const AttnParams& p, int rows_per_block_, int tile_keys_, int64_t* scratch) {
-    rows_per_block = rows_per_block_, tile_keys = tile_keys_;
+    rows_per_block = rows_per_block_, tile_keys = tile_keys_, tile_shift = 31 - __clz(tile_keys_);
     int64_t sum = 0;
     for (int base = 0; base < p.b.nseq; base += blockDim.x) {
       const int s = base + static_cast<int>(threadIdx.x);
@@ -98,8 +113,11 @@ struct WorkLine {
     parts = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));
     begin = end = 0;
     if (static_cast<int>(blockIdx.x) < parts) {
-      begin = total * blockIdx.x / parts;
-      end = total * (blockIdx.x + 1) / parts;
+      share = divide(total, parts);
+      extra = static_cast<int>(total - share * parts);
+      const int c = static_cast<int>(blockIdx.x);
+      begin = share * c + min(c, extra);
+      end = begin + share + (c < extra ? 1 : 0);
     }
   }
 
@@ -132,10 +150,15 @@ struct WorkLine {
     item_seq(p, s, it);
     it.nblocks = (it.nrows + rows_per_block - 1) / rows_per_block;
     const int64_t per_head = head_tiles(p, it);
-    it.kv_head = static_cast<int>((at - first) / per_head);
+    it.kv_head = static_cast<int>(divide(at - first, per_head));
     it.first = first + it.kv_head * per_head;
     it.row_block = 0;
     set_block(p, it);
+    if (p.b.tree) {  // blocks of one length
+      it.row_block = static_cast<int>(divide(at - it.first, it.tiles));
+      it.first += static_cast<int64_t>(it.row_block) * it.tiles;
+      set_block(p, it);
+    }
     while (at >= it.first + it.tiles) {
       it.first += it.tiles;
       ++it.row_block;
@@ -144,7 +167,7 @@ struct WorkLine {
   }
   __device__ __forceinline__ void set_block(const AttnParams& p, Item& it) const {
     it.keys = block_keys(p, it, it.row_block, rows_per_block);
-    it.tiles = (it.keys + tile_keys - 1) / tile_keys;
+    it.tiles = (it.keys + tile_keys - 1) >> tile_shift;
   }
   // The item after `it` (there is one).
   __device__ __forceinline__ void next(const AttnParams& p, Item& it) const {
@@ -163,7 +186,10 @@ struct WorkLine {
   }
 
   // The CTA whose part holds tile t.
-  __device__ __forceinline__ int part_of(int64_t t) const { return static_cast<int>(((t + 1) * parts - 1) / total); }
+  __device__ __forceinline__ int part_of(int64_t t) const {
+    const int64_t longer = (share + 1) * extra;  // tiles of the parts with one more
+    return t < longer ? static_cast<int>(divide(t, share + 1)) : extra + static_cast<int>(divide(t - longer, share));
+  }
 
   // This CTA's partial of an item it does not hold whole: slot 1 when the item began in an earlier part, else slot 0.
   // A slot is [rows][D] o, then [rows] (m, l).
@@ -322,21 +348,36 @@ __device__ void WorkLine::join(const AttnParams& p, const Item& it, int slot_row
   if (*s_word) {
     __threadfence();
     const int floats = slot_rows * (D + 2);
-    for (int i = static_cast<int>(threadIdx.x); i < rows * (D / 4); i += threads) {
-      const int r = i / (D / 4), d0 = (i % (D / 4)) * 4;
-      float mx = -INFINITY, sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    constexpr int kBatch = 4;  // elements of a thread in flight, each over all the slots
+    for (int i0 = static_cast<int>(threadIdx.x); i0 < rows * (D / 4); i0 += threads * kBatch) {
+      float mx[kBatch], sum[kBatch], acc[kBatch][4];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) mx[u] = -INFINITY, sum[u] = acc[u][0] = acc[u][1] = acc[u][2] = acc[u][3] = 0.f;
       for (int c = c0; c <= c1; ++c) {
         const float* s = p.partials + (static_cast<int64_t>(c) * 2 + (c == c0 ? 0 : 1)) * floats;
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(s + slot_rows * D + 2 * r));
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(s + r * D + d0));
-        const float m2 = fmaxf(mx, ml.x), base = m2 == -INFINITY ? 0.f : m2;
-        const float fa = exp2f(mx - base), fb = exp2f(ml.x - base);
-        acc[0] = acc[0] * fa + v.x * fb, acc[1] = acc[1] * fa + v.y * fb;
-        acc[2] = acc[2] * fa + v.z * fb, acc[3] = acc[3] * fa + v.w * fb;
-        sum = sum * fa + ml.y * fb;
-        mx = m2;
+        float2 ml[kBatch];
+        float4 v[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int i = min(i0 + u * threads, rows * (D / 4) - 1), r = i / (D / 4), d0 = (i % (D / 4)) * 4;
+          ml[u] = __ldcg(reinterpret_cast<const float2*>(s + slot_rows * D + 2 * r));
+          v[u] = __ldcg(reinterpret_cast<const float4*>(s + r * D + d0));
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const float m2 = fmaxf(mx[u], ml[u].x), base = m2 == -INFINITY ? 0.f : m2;
+          const float fa = exp2f(mx[u] - base), fb = exp2f(ml[u].x - base);
+          acc[u][0] = acc[u][0] * fa + v[u].x * fb, acc[u][1] = acc[u][1] * fa + v[u].y * fb;
+          acc[u][2] = acc[u][2] * fa + v[u].z * fb, acc[u][3] = acc[u][3] * fa + v[u].w * fb;
+          sum[u] = sum[u] * fa + ml[u].y * fb;
+          mx[u] = m2;
+        }
       }
-      store_out4<BF16>(p, it, slot_rows, r, d0, acc, mx, sum);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int i = i0 + u * threads;
+        if (i < rows * (D / 4)) store_out4<BF16>(p, it, slot_rows, i / (D / 4), (i % (D / 4)) * 4, acc[u], mx[u], sum[u]);
+      }
     }
   }
   sync();

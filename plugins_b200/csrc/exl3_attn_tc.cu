@@ -21,9 +21,11 @@
 // cannot be masked there (0 x inf = NaN), so in the tiles that hold such keys the cleaning warp zeroes slots past the
 // sequence and infinities and NaN; the latter are added back in the epilogue to the rows that see them.
 //
-// Every mbarrier wait is bounded (role_wait): one that gives up raises an abort flag that all roles poll.
+// Every mbarrier wait is bounded (wait_bar): one that gives up raises an abort flag that all roles poll.
 #include <cuda.h>
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "exl3_attn.h"
 #include "exl3_attn_dev.cuh"
@@ -37,17 +39,17 @@ using namespace tc;
 
 namespace {
 
-template <int D>
+template <int D, int ROWS>
 struct TcShape {
   static constexpr int NG = D == 256 ? 1 : 2;             // softmax groups (and O accumulators)
   static constexpr int KT = D == 256 ? 64 : 128;          // keys per tile
-  static constexpr int kRows = D == 256 ? 128 : 256;      // rows per block
+  static constexpr int kRows = ROWS;                      // rows per block: 128, or 256 in two row tiles
   static constexpr int kThreads = NG * 128 + 128;
   static constexpr int kSoft = NG * 128;                  // softmax threads
   static constexpr int kTile = KT * D * 2;                // bytes of a K or V tile
   static constexpr int kQBytes = kRows * D * 2;
-  static constexpr int kSlots = 5 * 32768 / kTile;        // K and V tiles in flight: 160 KiB
-  static constexpr int VS = kSlots / 2, KS = kSlots - VS;
+  static constexpr int kSlots = (229376 - kQBytes) / kTile > 12 ? 12 : (229376 - kQBytes) / kTile;
+  static constexpr int VS = kSlots / 2, KS = kSlots - VS; // V and K tiles in flight
   static constexpr int kOCol = 256;                       // TMEM: S buffers at columns 0 and KT, O of group g at 256 + g * D
   static constexpr int kTmem = 512;
   static constexpr int kBars = 2 * KS + 3 * VS + 2 + 2 + 2 + 5;
@@ -56,10 +58,79 @@ struct TcShape {
   static_assert(VS <= 8, "the odd flags cover eight items");
 };
 
+// Two f32 in one 64-bit register pair: one issue slot for both.
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_split(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// the largest of three; NaN if one is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// 2^y of a pair on the FMA pipe, to 2^-18 relative, for finite y <= 8 (below -126: about 2^-126): y = n + f with n the
+// nearest whole number (Cody and Waite's reduction; adding 1.5 x 2^23 leaves n in the low bits), a degree-4 polynomial
+// for 2^f on [-1/2, 1/2] (least relative error by Lawson's iteration), n added to the exponent.  The 16 exponentials a
+// clock of the special-function unit are otherwise what bounds a 256-row block: as many clocks as its two products.
+__device__ __forceinline__ void ex2_fma(uint64_t y, float& a, float& b) {
+  constexpr float kMagic = 12582912.f;
+  float y0, y1;
+  f2_split(y, y0, y1);
+  const uint64_t c = f2(fmaxf(y0, -126.f), fmaxf(y1, -126.f));
+  const uint64_t t = add2(c, f2(kMagic, kMagic));
+  const uint64_t f = fma2(add2(t, f2(-kMagic, -kMagic)), f2(-1.f, -1.f), c);
+  uint64_t r = f2(0.009570096619427204f, 0.009570096619427204f);
+  r = fma2(r, f, f2(0.05591786280274391f, 0.05591786280274391f));
+  r = fma2(r, f, f2(0.240247443318367f, 0.240247443318367f));
+  r = fma2(r, f, f2(0.6931217908859253f, 0.6931217908859253f));
+  r = fma2(r, f, f2(0.9999992847442627f, 0.9999992847442627f));
+  float r0, r1, t0, t1;
+  f2_split(r, r0, r1);
+  f2_split(t, t0, t1);
+  a = __uint_as_float(__float_as_uint(r0) + (__float_as_uint(t0) << 23));
+  b = __uint_as_float(__float_as_uint(r1) + (__float_as_uint(t1) << 23));
+}
+
+// Bounded wait (about two seconds) that also gives up when another role has.  The abort flag and the clock are read once
+// in many polls: a read of the global timer between polls held each wait up, and every tile's chain has three of them
+// (a 256-row prompt block: 568 us with it, see the table of steps in the design notes).
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t* err) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63u) != 0u) continue;
+    if (*abort_flag) return false;
+    if ((i & 1023u) != 0u) continue;
+    const uint64_t now = global_timer_ns();
+    if (t0 == 0) t0 = now;
+    else if (now - t0 > 2000000000ull) {
+      *abort_flag = 1u;
+      atomicOr(err, kErrWaitTimeout);
+      return false;
+    }
+  }
 }
 
 // A box of the cache: 64 columns from x, the rows from `tok` of one page and head.
@@ -85,14 +156,46 @@ constexpr uint32_t attn_idesc(int m, int n, bool b_mn) {
   return umma_idesc(m, n) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u);
 }
 
-// D[tmem] (+)= A[tmem] * B[smem]
-__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                        uint32_t accumulate) {
+// The MMA warp runs converged and one elected lane issues: its operands then stay in uniform registers.  (Issued inside
+// a one-lane branch, each MMA took some 100 clocks to issue, against the 64 it runs for: 4.1k clocks per 256 x 128 tile.)
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t e;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xFFFFFFFF;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e;
+}
+// D[tmem] (+)= A[smem] * B[smem]^T, where `on`
+__device__ __forceinline__ void mma_ss(uint32_t on, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem], where `on`
+__device__ __forceinline__ void mma_ts(uint32_t on, uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on)
+      : "memory");
+}
+// Arrives on `bar` when every tcgen05 operation the elected lane issued before has completed.
+__device__ __forceinline__ void commit(uint32_t on, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(on)
       : "memory");
 }
 
@@ -102,13 +205,22 @@ __device__ __forceinline__ void after_wait(uint32_t (&r)[32]) {
   for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i])::"memory");
 }
 
+constexpr int kFmaPairs = 2;  // of every eight pairs of exponentials, those on the FMA pipe
+
+// Moves registers from the copy and MMA warps to the softmax warps: a row's 128 scores stay in registers.  The shares
+// (8 x 32 x 200 + 4 x 32 x 104 = 64512) are what 384 threads were launched with (168 each).
+template <int R>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int R>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
+
 // The block as the roles walk it: its key tiles [tile0, tile0 + tiles), one or two row tiles, and its events.
 struct Block {
   int tile0, tiles, rows, qt, events, full_keys;
 };
-template <int D>
+template <int D, int ROWS>
 __device__ __forceinline__ Block block_of(const AttnParams& p, const WorkLine& line, const Item& it, int64_t at) {
-  using S = TcShape<D>;
+  using S = TcShape<D, ROWS>;
   Block b;
   b.tile0 = static_cast<int>(at - it.first);
   b.tiles = static_cast<int>(min(line.end - at, static_cast<int64_t>(it.tiles - b.tile0)));
@@ -155,7 +267,7 @@ __device__ __noinline__ void add_odd(const AttnParams& p, const Item& it, int to
   const uint16_t* q = static_cast<const uint16_t*>(p.q.data) + static_cast<int64_t>(it.row0 + tok) * p.q.row_stride +
                       h * p.q.head_stride;
   // only tiles that reach past full_keys were cleaned
-  constexpr int KT = TcShape<D>::KT;
+  constexpr int KT = TcShape<D, 128>::KT;
   for (int key = max(key_lo, full_keys / KT * KT); key < min(key_hi, it.total_keys); ++key) {
     if (!sees(p.b, it, tok, key)) continue;
     const int id = p.b.table[static_cast<int64_t>(it.seq) * p.b.max_pages + (key >> p.b.page_shift)];
@@ -175,11 +287,93 @@ __device__ __noinline__ void add_odd(const AttnParams& p, const Item& it, int to
   }
 }
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
+// The last of the CTAs that an item was cut between joins their slots, in key order: o as [D / 4][ROWS] float4, then
+// (m, l) per row.  A thread takes one row and every n-th pair of column quads, four pairs in flight.
+template <int D, int ROWS, bool BF16, typename Sync>
+__device__ void join_block(const AttnParams& p, const WorkLine& line, const Item& it, int rows, int* s_word, Sync&& sync) {
+  constexpr int kThreads = TcShape<D, ROWS>::kSoft;
+  constexpr int64_t kFloats = static_cast<int64_t>(ROWS) * (D + 2);
+  const int c0 = line.part_of(it.first), c1 = line.part_of(it.first + it.tiles - 1);
+  __threadfence();
+  sync();
+  if (threadIdx.x == 0) {
+    const bool last = atomicAdd(p.counters + c0, 1u) + 1u == static_cast<uint32_t>(c1 - c0 + 1);
+    if (last) p.counters[c0] = 0u;
+    *s_word = last;
+  }
+  sync();
+  if (*s_word) {
+    __threadfence();
+    int pad = 32;
+    while (pad < rows) pad <<= 1;
+    const int r = static_cast<int>(threadIdx.x) & (pad - 1), first = static_cast<int>(threadIdx.x) / pad, step = kThreads / pad;
+    if (r < rows) {
+      auto slot = [&](int c) { return p.partials + (static_cast<int64_t>(c) * 2 + (c == c0 ? 0 : 1)) * kFloats; };
+      float m = -INFINITY, l = 0.f;
+      for (int c = c0; c <= c1; ++c) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(slot(c) + ROWS * D) + r);
+        const float top = fmaxf(m, ml.x), base = top == -INFINITY ? 0.f : top;
+        l = l * ex2(m - base) + ml.y * ex2(ml.x - base);
+        m = top;
+      }
+      const float base = m == -INFINITY ? 0.f : m, inv = l == 0.f ? 0.f : 1.f / l;
+      const int rr = it.row_block * ROWS + r, h = it.kv_head * p.group + rr % p.group;
+      const int64_t row = it.row0 + rr / p.group;
+      uint16_t* dst = static_cast<uint16_t*>(p.out.data) + row * p.out.row_stride + h * p.out.head_stride;
+      constexpr int kBatch = 4;
+      for (int j0 = first; j0 < D / 8; j0 += step * kBatch) {
+        float4 a[kBatch][2];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) a[u][0] = a[u][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+        for (int c = c0; c <= c1; ++c) {
+          const float* s = slot(c);
+          const float f = ex2(__ldcg(reinterpret_cast<const float2*>(s + ROWS * D) + r).x - base);
+          float4 v[kBatch][2];
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            const int j = min(j0 + u * step, D / 8 - 1);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) v[u][e] = __ldcg(reinterpret_cast<const float4*>(s) + (2 * j + e) * ROWS + r);
+          }
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              a[u][e].x += v[u][e].x * f, a[u][e].y += v[u][e].y * f;
+              a[u][e].z += v[u][e].z * f, a[u][e].w += v[u][e].w * f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int j = j0 + u * step;
+          if (j >= D / 8) continue;
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            w[2 * e] = l == 0.f ? 0u : pack2<BF16>(a[u][e].x * inv, a[u][e].y * inv);
+            w[2 * e + 1] = l == 0.f ? 0u : pack2<BF16>(a[u][e].z * inv, a[u][e].w * inv);
+          }
+          if (p.out.vec) {
+            *reinterpret_cast<uint4*>(dst + j * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              dst[j * 8 + 2 * i] = static_cast<uint16_t>(w[i]), dst[j * 8 + 2 * i + 1] = static_cast<uint16_t>(w[i] >> 16);
+          }
+        }
+      }
+      if (p.lse && first == 0) p.lse[row * p.out.heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+    }
+  }
+  sync();
+}
+
+template <int D, int ROWS, bool BF16>
+__global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
     attn_tc_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap kmap,
                    const __grid_constant__ CUtensorMap vmap) {
-  using S = TcShape<D>;
+  using S = TcShape<D, ROWS>;
   constexpr int NG = S::NG, KT = S::KT, KS = S::KS, VS = S::VS;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* s_q = smem;                       // [row tile][64-column block][128 rows][128 bytes], swizzled
@@ -215,6 +409,10 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
     *abort_flag = 0u;
     for (int i = 0; i < 8; ++i) s_odd[i] = 0u;
   }
+  if (tid == 32) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
+  }
   pdl_wait();
   WorkLine line;
   line.init(p, S::kRows, KT, reinterpret_cast<int64_t*>(s_k));
@@ -228,17 +426,18 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
 
   if (warp < NG * 4) {
     // ---------------------------------------------------------------- softmax groups
+    if constexpr (NG == 2) regs_up<200>();
     const uint32_t g = warp >> 2, wq = warp & 3u, r128 = wq * 32 + lane;  // row of the 128-row tile = TMEM lane
     const uint32_t lane_off = (wq * 32u) << 16;
     uint32_t sphase = 0, ophase = 0, xphase = 0, pvphase = 0;  // sphase: a bit per buffer; ophase: per group
     bool ok = true;
     auto group_sync = [&]() {  // all softmax threads
       mbar_arrive(xsync);
-      ok = __all_sync(0xFFFFFFFFu, ok && role_wait(xsync, xphase, abort_flag, p.b.err));
+      ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(xsync, xphase, abort_flag, p.b.err));
       xphase ^= 1u;
     };
     for (uint32_t serial = 0; ok && at < line.end; ++serial) {
-      const Block b = block_of<D>(p, line, it, at);
+      const Block b = block_of<D, ROWS>(p, line, it, at);
       // the query rows into their swizzled tiles: with two row tiles a group loads its own, else both share the one
       {
         const uint32_t tile = b.qt == 2 ? g : 0u;
@@ -246,13 +445,31 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
         const int ncols = b.qt == 2 || NG == 1 ? D : D / 2;
         const int r = static_cast<int>(tile * 128u + r128);
         const int rr = it.row_block * S::kRows + r, t = rr / p.group, h = it.kv_head * p.group + rr % p.group;
-#pragma unroll 8
-        for (int c = 0; c < ncols / 8; ++c) {
-          const int col = cols0 + c * 8;
-          uint4 u = make_uint4(0u, 0u, 0u, 0u);
-          if (r < b.rows) u = load_q8(p.q, it.row0 + t, h, col);
-          *reinterpret_cast<uint4*>(s_q + tile * (128 * D * 2) + (col >> 6) * (128 * 128) +
-                                    image_offset(r128, static_cast<uint32_t>(col & 63))) = u;
+        const int64_t q_row = it.row0 + t;
+        for (int c0 = 0; c0 < ncols; c0 += 64) {  // eight loads in flight
+          uint4 u[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) u[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (r < b.rows) {
+            if (p.q.vec) {
+              const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q.data) +
+                                                                q_row * p.q.row_stride + h * p.q.head_stride + cols0 + c0);
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (c0 + i * 8 < ncols) u[i] = src[i];
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (c0 + i * 8 < ncols) u[i] = load_q8(p.q, q_row, h, cols0 + c0 + i * 8);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int col = cols0 + c0 + i * 8;
+            if (c0 + i * 8 < ncols)
+              *reinterpret_cast<uint4*>(s_q + tile * (128 * D * 2) + (col >> 6) * (128 * 128) +
+                                        image_offset(r128, static_cast<uint32_t>(col & 63))) = u[i];
+          }
         }
       }
       fence_proxy_async_smem();
@@ -260,14 +477,21 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
 
       const int row = (b.qt == 2 ? static_cast<int>(g) * 128 : 0) + static_cast<int>(r128);
       const int tok = (it.row_block * S::kRows + row) / p.group;
+      const bool idle = row - static_cast<int>(lane) >= b.rows;
       float m = -INFINITY, l = 0.f;  // m in units of log2
       for (int e = static_cast<int>(g); e < b.events; e += NG) {
         const uint32_t buf = e & 1;
         const int tile = b.qt == 2 ? e >> 1 : e;
         const int key0 = (b.tile0 + tile) * KT;
+        const uint32_t pv_parity = pvphase ^ 1u;  // the product of the event before (NG = 1)
+        pvphase ^= 1u;
         const uint32_t s_addr = tmem + lane_off + buf * KT;
-        ok = __all_sync(0xFFFFFFFFu, ok && role_wait(&sfull[buf], (sphase >> buf) & 1u, abort_flag, p.b.err));
+        ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(&sfull[buf], (sphase >> buf) & 1u, abort_flag, p.b.err));
         sphase ^= 1u << buf;
+        if (idle) {  // none of the warp's rows is in the block: whatever P holds there is never read back
+          mbar_arrive(&pready[buf]);
+          continue;
+        }
         tc_fence_after();
         uint32_t x[KT / 32][32];
 #pragma unroll
@@ -275,7 +499,8 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
         tmem_wait_ld(x[0]);
 #pragma unroll
         for (int c = 1; c < KT / 32; ++c) after_wait(x[c]);
-        if (key0 + KT > b.full_keys) {
+        const bool partial = key0 + KT > b.full_keys;
+        if (partial) {
 #pragma unroll
           for (int c = 0; c < KT / 32; ++c) {
             const uint32_t mask = seen32(p.b, it, tok, key0 + c * 32);
@@ -284,19 +509,25 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
               if (!(mask & (1u << i))) x[c][i] = 0xFF800000u;  // -inf
           }
         }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float mx[4];
 #pragma unroll
-        for (int c = 0; c < KT / 32; ++c)
+        for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(x[0][i]);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(x[c][i]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+        for (int i = 4; i < KT; i += 8) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int u = i + 2 * j < KT ? i + 2 * j : KT - 2;  // (the last step sees its neighbours again)
+            mx[j] = max3(mx[j], __uint_as_float(x[u >> 5][u & 31]), __uint_as_float(x[(u + 1) >> 5][(u + 1) & 31]));
+          }
+        }
+        const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale_log2;
+        // a visible score of NaN or +inf makes the row NaN; the exponentials below may not show it
+        if (!(top < INFINITY)) l = __uint_as_float(0x7FC00000u);
         const bool grow = top > m + 8.f;  // (m = -inf: as soon as anything is seen)
-        const bool first = e < NG;
-        if (first) {
+        if (e < NG) {
           m = top;
         } else if (__any_sync(0xFFFFFFFFu, grow)) {
-          if constexpr (NG == 1)
-            ok = __all_sync(0xFFFFFFFFu, ok && role_wait(pvdone, pvphase ^ 1u, abort_flag, p.b.err));
+          if constexpr (NG == 1) ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(pvdone, pv_parity, abort_flag, p.b.err));
           tc_fence_after();
           const float f = grow ? ex2(m - top) : 1.f;
           if (grow) m = top, l *= f;
@@ -312,23 +543,39 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
           }
           tmem_wait_st();
         }
-        pvphase ^= 1u;
         const float base = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t scale2 = f2(p.scale_log2, p.scale_log2), base2 = f2(-base, -base);
+        uint64_t sum[2] = {0, 0};
+        // (one straight run of code for each of the two: a branch per pair left every exponential's latency exposed)
+        auto probabilities = [&](auto masked) {
 #pragma unroll
-        for (int c = 0; c < KT / 64; ++c) {
-          uint32_t pk[32];
+          for (int c = 0; c < KT / 64; ++c) {
+            uint32_t pk[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float a = ex2(fmaf(__uint_as_float(x[2 * c + (i >> 4)][(2 * i) & 31]), p.scale_log2, -base));
-            const float d = ex2(fmaf(__uint_as_float(x[2 * c + (i >> 4)][(2 * i + 1) & 31]), p.scale_log2, -base));
-            sum[(2 * i) & 3] += a, sum[(2 * i + 1) & 3] += d;
-            pk[i] = pack2<BF16>(a, d);  // (l keeps the f32 values)
+            for (int i = 0; i < 32; ++i) {
+              const int u = (2 * i) & 31;
+              const uint64_t y = fma2(f2(__uint_as_float(x[2 * c + (i >> 4)][u]), __uint_as_float(x[2 * c + (i >> 4)][u + 1])),
+                                      scale2, base2);
+              float e0, e1;
+              if (i % 8 < kFmaPairs && !decltype(masked)::value) {  // (masked scores need the other form's exact 0)
+                ex2_fma(y, e0, e1);
+              } else {
+                float y0, y1;
+                f2_split(y, y0, y1);
+                e0 = ex2(y0), e1 = ex2(y1);
+              }
+              sum[i & 1] = add2(sum[i & 1], f2(e0, e1));
+              pk[i] = pack2<BF16>(e0, e1);  // (l keeps the f32 values)
+            }
+            tmem_st32(s_addr + c * 32, pk);
           }
-          tmem_st32(s_addr + c * 32, pk);
-        }
+        };
+        if (partial) probabilities(std::true_type{});
+        else probabilities(std::false_type{});
         tmem_wait_st();
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        float s0, s1;
+        f2_split(add2(sum[0], sum[1]), s0, s1);
+        l += s0 + s1;
         tc_fence_before();
         mbar_arrive(&pready[buf]);
       }
@@ -338,7 +585,7 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
       const bool two = b.qt == 1 && NG == 2;  // two key halves of the same rows
       const int mine = two ? (b.events > static_cast<int>(g) ? 1 : 0) : 1;  // this group had a tile
       if (mine) {
-        ok = __all_sync(0xFFFFFFFFu, ok && role_wait(&ofull[g], ophase, abort_flag, p.b.err));
+        ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(&ofull[g], ophase, abort_flag, p.b.err));
         ophase ^= 1u;
       }
       float f0 = 1.f, f1 = 0.f;
@@ -391,7 +638,14 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             w[i] = l == 0.f ? 0u : pack2<BF16>(o[2 * i] * inv, o[2 * i + 1] * inv);
-          if (p.out.vec) {
+          if (p.out.vec == 2) {  // a whole sector per lane and store
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t w8[8] = {w[8 * i],     w[8 * i + 1], w[8 * i + 2], w[8 * i + 3],
+                                      w[8 * i + 4], w[8 * i + 5], w[8 * i + 6], w[8 * i + 7]};
+              st_global_v8(dst + 16 * i, w8);
+            }
+          } else if (p.out.vec) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
@@ -401,8 +655,9 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<float4*>(slot + row * D + c + 4 * i) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (int i = 0; i < 8; ++i)  // [D / 4][rows] float4: a warp's rows are neighbours
+            reinterpret_cast<float4*>(slot)[(c / 4 + i) * S::kRows + row] =
+                make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
       }
       if (live && cols0 == 0) {
@@ -414,67 +669,74 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
       }
       tc_fence_before();
       mbar_arrive(ofree);
-      if (!whole) line.template join<D, BF16>(p, it, S::kRows, b.rows, s_last, S::kSoft, group_sync);
+      if (!whole) join_block<D, ROWS, BF16>(p, line, it, b.rows, s_last, group_sync);
       group_sync();  // every MMA of the block has finished, and its rows are read: Q may be replaced
       at += b.tiles;
       if (at < line.end) line.next(p, it);
     }
-  } else if (warp == NG * 4) {
+  } else {
+   if constexpr (NG == 2) regs_down<104>();
+   if (warp == NG * 4) {
     // ---------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = attn_idesc<BF16>(128, KT, false), idesc_o = attn_idesc<BF16>(128, D, true);
-      const uint32_t q0 = smem_u32(s_q), k0 = smem_u32(s_k), v0 = smem_u32(s_v);
-      uint32_t kfirst = 0, vfirst = 0;  // tiles of the blocks before
-      uint32_t pphase = 0;
-      bool ok = true;
-      for (uint32_t serial = 0; ok && at < line.end; ++serial) {
-        const Block b = block_of<D>(p, line, it, at);
-        ok = ok && role_wait(qfull, serial & 1u, abort_flag, p.b.err);
-        auto scores = [&](int e) {
-          const int tile = b.qt == 2 ? e >> 1 : e;
-          const uint32_t n = kfirst + static_cast<uint32_t>(tile), slot = n % KS;
-          if (b.qt == 1 || !(e & 1)) ok = ok && role_wait(&kfull[slot], (n / KS) & 1u, abort_flag, p.b.err);
-          if (!ok) return;
-          tc_fence_after();
-          const uint32_t qa = q0 + (b.qt == 2 ? (e & 1) * (128 * D * 2) : 0), ka = k0 + slot * S::kTile;
+    constexpr uint32_t idesc_s = attn_idesc<BF16>(128, KT, false), idesc_o = attn_idesc<BF16>(128, D, true);
+    const uint32_t on = elect_one();
+    const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+    const uint64_t qdesc = sw128_desc(smem_u32(s_q)), kdesc = sw128_desc(smem_u32(s_k));
+    const uint64_t vdesc = sw128_mn_desc(smem_u32(s_v), KT * 128);
+    uint32_t kslot = 0, kphase = 0, vslot = 0, vphase = 0;  // the next K and V tile to come
+    uint32_t pphase = 0;
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(bar, parity, abort_flag, p.b.err));
+    };
+    for (uint32_t serial = 0; ok && at < line.end; ++serial) {
+      const Block b = block_of<D, ROWS>(p, line, it, at);
+      const bool both = b.qt == 2;  // a key tile serves two events
+      wait(qfull, serial & 1u);
+      auto scores = [&](int e) {
+        const uint32_t buf = e & 1;
+        if (!both || buf == 0) wait(&kfull[kslot], kphase);
+        if (!ok) return;
+        tc_fence_after();
+        const uint64_t qa = qdesc + (both && buf ? (128 * D * 2) >> 4 : 0), ka = kdesc + kslot * (S::kTile >> 4);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            umma_f16(tmem + (e & 1) * KT, sw128_desc(qa + (kk >> 2) * (128 * 128) + (kk & 3) * 32),
-                     sw128_desc(ka + (kk >> 2) * (KT * 128) + (kk & 3) * 32), idesc_s, kk != 0 ? 1u : 0u);
-          umma_commit(&sfull[e & 1]);
-          if (b.qt == 1 || (e & 1)) umma_commit(&kempty[slot]);
-        };
-        scores(0);
-        if (b.events > 1) scores(1);
-        if (serial) ok = ok && role_wait(ofree, (serial - 1) & 1u, abort_flag, p.b.err);
-        for (int e = 0; ok && e < b.events; ++e) {
-          const uint32_t buf = e & 1;
-          const int tile = b.qt == 2 ? e >> 1 : e;
-          const uint32_t n = vfirst + static_cast<uint32_t>(tile), slot = n % VS;
-          ok = ok && role_wait(&pready[buf], (pphase >> buf) & 1u, abort_flag, p.b.err);
-          pphase ^= 1u << buf;
-          if (b.qt == 1 || !(e & 1)) ok = ok && role_wait(&vclean[slot], (n / VS) & 1u, abort_flag, p.b.err);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t va = v0 + slot * S::kTile;
-          const uint32_t od = tmem + S::kOCol + (NG == 2 ? buf * D : 0);
-          const bool first = e < NG;
-#pragma unroll
-          for (int kk = 0; kk < KT / 16; ++kk)
-            umma_ts(od, tmem + buf * KT + kk * 8, sw128_mn_desc(va + kk * 2048, KT * 128), idesc_o,
-                    !first || kk != 0 ? 1u : 0u);
-          if constexpr (NG == 1) umma_commit(pvdone);
-          if (b.qt == 1 || (e & 1)) umma_commit(&vempty[slot]);
-          if (e + 2 < b.events) scores(e + 2);
-          if (e + NG >= b.events) umma_commit(&ofull[NG == 2 ? buf : 0]);
+        for (int kk = 0; kk < D / 16; ++kk)
+          mma_ss(on, tm + buf * KT, qa + (((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4),
+                 ka + (((kk >> 2) * (KT * 128) + (kk & 3) * 32) >> 4), idesc_s, kk != 0 ? 1u : 0u);
+        commit(on, &sfull[buf]);
+        if (!both || buf) {
+          commit(on, &kempty[kslot]);
+          if (++kslot == KS) kslot = 0, kphase ^= 1u;
         }
-        kfirst += b.tiles, vfirst += b.tiles;
-        at += b.tiles;
-        if (at < line.end) line.next(p, it);
+      };
+      scores(0);
+      if (b.events > 1) scores(1);
+      if (serial) wait(ofree, (serial - 1) & 1u);
+      for (int e = 0; ok && e < b.events; ++e) {
+        const uint32_t buf = e & 1;
+        wait(&pready[buf], (pphase >> buf) & 1u);
+        pphase ^= 1u << buf;
+        if (!both || buf == 0) wait(&vclean[vslot], vphase);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t va = vdesc + vslot * (S::kTile >> 4);
+        const uint32_t od = tm + S::kOCol + (NG == 2 ? buf * D : 0);
+#pragma unroll
+        for (int kk = 0; kk < KT / 16; ++kk)
+          mma_ts(on, od, tm + buf * KT + kk * 8, va + ((kk * 2048) >> 4), idesc_o, e >= NG || kk != 0 ? 1u : 0u);
+        if constexpr (NG == 1) commit(on, pvdone);
+        if (!both || buf) {
+          commit(on, &vempty[vslot]);
+          if (++vslot == VS) vslot = 0, vphase ^= 1u;
+        }
+        if (e + 2 < b.events) scores(e + 2);
+        if (e + NG >= b.events) commit(on, &ofull[NG == 2 ? buf : 0]);
       }
-      umma_commit(fin);  // every MMA has finished before TMEM is released
-      if (!mbar_wait_bounded(fin, 0)) atomicOr(p.b.err, kErrWaitTimeout);
+      at += b.tiles;
+      if (at < line.end) line.next(p, it);
     }
+    commit(on, fin);  // every MMA has finished before TMEM is released
+    if (lane == 0 && !mbar_wait_bounded(fin, 0)) atomicOr(p.b.err, kErrWaitTimeout);
     __syncwarp();
   } else if (warp <= NG * 4 + 2) {
     // ---------------------------------------------------------------- K copies, V copies
@@ -489,7 +751,7 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
     uint32_t n = 0;
     bool ok = true;
     while (ok && at < line.end) {
-      const Block b = block_of<D>(p, line, it, at);
+      const Block b = block_of<D, ROWS>(p, line, it, at);
       const int32_t* tab = p.b.table + static_cast<int64_t>(it.seq) * p.b.max_pages;
       for (int t = 0; ok && t < b.tiles; ++t, ++n) {
         const uint32_t slot = n % slots;
@@ -504,7 +766,7 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
         }
         const uint32_t loads = __popc(__ballot_sync(0xFFFFFFFFu, id >= 0));
         if (n >= static_cast<uint32_t>(slots))
-          ok = role_wait(&empty[slot], (n / slots - 1) & 1u, abort_flag, p.b.err);
+          ok = wait_bar(&empty[slot], (n / slots - 1) & 1u, abort_flag, p.b.err);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&full[slot], loads * box_rows * 128);
@@ -527,10 +789,10 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
     uint32_t n = 0;
     bool ok = true;
     for (uint32_t serial = 0; ok && at < line.end; ++serial) {
-      const Block b = block_of<D>(p, line, it, at);
+      const Block b = block_of<D, ROWS>(p, line, it, at);
       for (int t = 0; ok && t < b.tiles; ++t, ++n) {
         const uint32_t slot = n % VS;
-        ok = role_wait(&vfull[slot], (n / VS) & 1u, abort_flag, p.b.err);
+        ok = wait_bar(&vfull[slot], (n / VS) & 1u, abort_flag, p.b.err);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
         const int key0 = (b.tile0 + t) * KT;
@@ -560,6 +822,7 @@ __global__ void __launch_bounds__(TcShape<D>::kThreads, 1)
       at += b.tiles;
       if (ok && at < line.end) line.next(p, it);
     }
+   }
   }
   tc_fence_before();
   __syncthreads();
@@ -605,11 +868,11 @@ bool encode(CUtensorMap& map, void* base, const AttnParams& p, int dim, int tile
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D>
+template <int D, int ROWS>
 cudaError_t launch_dim(const AttnParams& p, int sms, size_t partial_floats, cudaStream_t st) {
-  using S = TcShape<D>;
+  using S = TcShape<D, ROWS>;
   static KernelSetup setup[2];
-  auto kern = p.bf16 ? attn_tc_kernel<D, true> : attn_tc_kernel<D, false>;
+  auto kern = p.bf16 ? attn_tc_kernel<D, ROWS, true> : attn_tc_kernel<D, ROWS, false>;
   cudaError_t e = kernel_setup(setup[p.bf16 ? 1 : 0], kern, S::kThreads, S::kSmem);
   if (e != cudaSuccess) return e;
   CUtensorMap kmap, vmap;
@@ -637,10 +900,12 @@ cudaError_t launch_dim(const AttnParams& p, int sms, size_t partial_floats, cuda
 }  // namespace
 
 cudaError_t launch_attn_tc(const AttnParams& p, int dim, int sms, size_t partial_floats, cudaStream_t st) {
+  // one row tile where no block needs two: its second buffer then takes the next key tile, and more tiles fit
+  const bool one = static_cast<int64_t>(p.max_rows) * p.group <= 128;
   switch (dim) {
-    case 64: return launch_dim<64>(p, sms, partial_floats, st);
-    case 128: return launch_dim<128>(p, sms, partial_floats, st);
-    default: return launch_dim<256>(p, sms, partial_floats, st);
+    case 64: return (one ? launch_dim<64, 128> : launch_dim<64, 256>)(p, sms, partial_floats, st);
+    case 128: return (one ? launch_dim<128, 128> : launch_dim<128, 256>)(p, sms, partial_floats, st);
+    default: return launch_dim<256, 128>(p, sms, partial_floats, st);
   }
 }
 
