@@ -52,7 +52,8 @@ struct TcShape {
   static constexpr int VS = kSlots / 2, KS = kSlots - VS; // V and K tiles in flight
   static constexpr int kOCol = 256;                       // TMEM: S buffers at columns 0 and KT, O of group g at 256 + g * D
   static constexpr int kTmem = 512;
-  static constexpr int kBars = 2 * KS + 3 * VS + 2 + 2 + 2 + 5;
+  static constexpr int kParts = KT / 64;                  // P comes in parts of 64 keys, each a product of its own
+  static constexpr int kBars = 2 * KS + 3 * VS + 2 + 2 * kParts + 2 + 5;
   static constexpr int kSmem = kQBytes + kSlots * kTile + 2 * 128 * 8 + kBars * 8 + 64;
   static_assert(KS * kTile + VS * kTile + kQBytes <= 229376 && kSmem <= 232448, "shared memory");
   static_assert(VS <= 8, "the odd flags cover eight items");
@@ -166,6 +167,12 @@ __device__ __forceinline__ uint32_t elect_one() {
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(e));
   return e;
+}
+// The same value, known to the compiler to be one for the whole warp.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xFFFFFFFFu, v, 0); }
+// A descriptor `bytes` further on (its address field counts 16 bytes in the low word).
+__device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t lo_add) {
+  return (desc & 0xFFFFFFFF00000000ull) | (static_cast<uint32_t>(desc) + lo_add);
 }
 // D[tmem] (+)= A[smem] * B[smem]^T, where `on`
 __device__ __forceinline__ void mma_ss(uint32_t on, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
@@ -382,7 +389,7 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
   float2* s_ml = reinterpret_cast<float2*>(s_v + VS * S::kTile);  // [2][128]
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_ml + 256);
   uint64_t *kfull = bars, *kempty = kfull + KS, *vfull = kempty + KS, *vclean = vfull + VS, *vempty = vclean + VS;
-  uint64_t *sfull = vempty + VS, *pready = sfull + 2, *ofull = pready + 2;
+  uint64_t *sfull = vempty + VS, *pready = sfull + 2, *ofull = pready + 2 * S::kParts;
   uint64_t *qfull = ofull + 2, *ofree = qfull + 1, *xsync = ofree + 1, *pvdone = xsync + 1, *fin = pvdone + 1;
   uint32_t* words = reinterpret_cast<uint32_t*>(bars + S::kBars);
   uint32_t* s_tmem = words;
@@ -402,7 +409,8 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
   if (tid == 0) {
     for (int i = 0; i < KS; ++i) mbar_init(&kfull[i], 1), mbar_init(&kempty[i], 1);
     for (int i = 0; i < VS; ++i) mbar_init(&vfull[i], 1), mbar_init(&vclean[i], 1), mbar_init(&vempty[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&sfull[i], 1), mbar_init(&pready[i], 128), mbar_init(&ofull[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&sfull[i], 1), mbar_init(&ofull[i], 1);
+    for (int i = 0; i < 2 * S::kParts; ++i) mbar_init(&pready[i], 128);
     mbar_init(qfull, S::kSoft), mbar_init(ofree, S::kSoft), mbar_init(xsync, S::kSoft);
     mbar_init(pvdone, 1), mbar_init(fin, 1);
     fence_barrier_init();
@@ -489,7 +497,7 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
         ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(&sfull[buf], (sphase >> buf) & 1u, abort_flag, p.b.err));
         sphase ^= 1u << buf;
         if (idle) {  // none of the warp's rows is in the block: whatever P holds there is never read back
-          mbar_arrive(&pready[buf]);
+          for (int c = 0; c < S::kParts; ++c) mbar_arrive(&pready[buf * S::kParts + c]);
           continue;
         }
         tc_fence_after();
@@ -568,16 +576,16 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
               pk[i] = pack2<BF16>(e0, e1);  // (l keeps the f32 values)
             }
             tmem_st32(s_addr + c * 32, pk);
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&pready[buf * S::kParts + c]);
           }
         };
         if (partial) probabilities(std::true_type{});
         else probabilities(std::false_type{});
-        tmem_wait_st();
         float s0, s1;
         f2_split(add2(sum[0], sum[1]), s0, s1);
         l += s0 + s1;
-        tc_fence_before();
-        mbar_arrive(&pready[buf]);
       }
 
       // ---- the block's end: o / l, or a partial for the join
@@ -687,49 +695,62 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
     uint32_t pphase = 0;
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity))) return;
       ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(bar, parity, abort_flag, p.b.err));
     };
     for (uint32_t serial = 0; ok && at < line.end; ++serial) {
       const Block b = block_of<D, ROWS>(p, line, it, at);
       const bool both = b.qt == 2;  // a key tile serves two events
       wait(qfull, serial & 1u);
+      auto scores_wait = [&](int e) {
+        if (!both || !(e & 1)) wait(&kfull[kslot], kphase);
+      };
       auto scores = [&](int e) {
         const uint32_t buf = e & 1;
-        if (!both || buf == 0) wait(&kfull[kslot], kphase);
-        if (!ok) return;
-        tc_fence_after();
-        const uint64_t qa = qdesc + (both && buf ? (128 * D * 2) >> 4 : 0), ka = kdesc + kslot * (S::kTile >> 4);
+        const uint32_t qo = uniform(both && buf ? (128 * D * 2) >> 4 : 0), ko = uniform(kslot * (S::kTile >> 4));
+        const uint32_t sd = uniform(tm + buf * KT);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          mma_ss(on, tm + buf * KT, qa + (((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4),
-                 ka + (((kk >> 2) * (KT * 128) + (kk & 3) * 32) >> 4), idesc_s, kk != 0 ? 1u : 0u);
+          mma_ss(on, sd, desc_at(qdesc, qo + (((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4)),
+                 desc_at(kdesc, ko + (((kk >> 2) * (KT * 128) + (kk & 3) * 32) >> 4)), idesc_s, kk != 0 ? 1u : 0u);
         commit(on, &sfull[buf]);
         if (!both || buf) {
           commit(on, &kempty[kslot]);
           if (++kslot == KS) kslot = 0, kphase ^= 1u;
         }
       };
-      scores(0);
-      if (b.events > 1) scores(1);
+      for (int e = 0; e < 2 && e < b.events; ++e) {
+        scores_wait(e);
+        if (!ok) break;
+        tc_fence_after();
+        scores(e);
+      }
       if (serial) wait(ofree, (serial - 1) & 1u);
       for (int e = 0; ok && e < b.events; ++e) {
         const uint32_t buf = e & 1;
-        wait(&pready[buf], (pphase >> buf) & 1u);
-        pphase ^= 1u << buf;
+        // everything the event needs but P first: the products then follow one another
         if (!both || buf == 0) wait(&vclean[vslot], vphase);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t va = vdesc + vslot * (S::kTile >> 4);
-        const uint32_t od = tm + S::kOCol + (NG == 2 ? buf * D : 0);
+        if (e + 2 < b.events) scores_wait(e + 2);
+        const uint32_t vo = uniform(vslot * (S::kTile >> 4)), sd = uniform(tm + buf * KT);
+        const uint32_t od = uniform(tm + S::kOCol + (NG == 2 ? buf * D : 0)), more = uniform(e >= NG ? 1u : 0u);
+        const uint32_t pp = (pphase >> buf) & 1u;
+        pphase ^= 1u << buf;
 #pragma unroll
-        for (int kk = 0; kk < KT / 16; ++kk)
-          mma_ts(on, od, tm + buf * KT + kk * 8, va + ((kk * 2048) >> 4), idesc_o, e >= NG || kk != 0 ? 1u : 0u);
+        for (int c = 0; c < S::kParts; ++c) {
+          wait(&pready[buf * S::kParts + c], pp);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = c * 4; kk < c * 4 + 4; ++kk)
+            mma_ts(on, od, sd + kk * 8, desc_at(vdesc, vo + ((kk * 2048) >> 4)), idesc_o, kk != 0 ? 1u : more);
+        }
+        if (!ok) break;
+        if (e + 2 < b.events) scores(e + 2);
         if constexpr (NG == 1) commit(on, pvdone);
         if (!both || buf) {
           commit(on, &vempty[vslot]);
           if (++vslot == VS) vslot = 0, vphase ^= 1u;
         }
-        if (e + 2 < b.events) scores(e + 2);
         if (e + NG >= b.events) commit(on, &ofull[NG == 2 ? buf : 0]);
       }
       at += b.tiles;
