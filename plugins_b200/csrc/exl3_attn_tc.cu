@@ -25,8 +25,6 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
-#include <type_traits>
-
 #include "exl3_attn.h"
 #include "exl3_attn_dev.cuh"
 #include "exl3_common.cuh"
@@ -78,10 +76,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// the largest of three; NaN if one is
+// the largest of three (NaN is passed over: it shows in its own probability)
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -89,29 +87,6 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-// 2^y of a pair on the FMA pipe, to 2^-18 relative, for finite y <= 8 (below -126: about 2^-126): y = n + f with n the
-// nearest whole number (Cody and Waite's reduction; adding 1.5 x 2^23 leaves n in the low bits), a degree-4 polynomial
-// for 2^f on [-1/2, 1/2] (least relative error by Lawson's iteration), n added to the exponent.  The 16 exponentials a
-// clock of the special-function unit are otherwise what bounds a 256-row block: as many clocks as its two products.
-__device__ __forceinline__ void ex2_fma(uint64_t y, float& a, float& b) {
-  constexpr float kMagic = 12582912.f;
-  float y0, y1;
-  f2_split(y, y0, y1);
-  const uint64_t c = f2(fmaxf(y0, -126.f), fmaxf(y1, -126.f));
-  const uint64_t t = add2(c, f2(kMagic, kMagic));
-  const uint64_t f = fma2(add2(t, f2(-kMagic, -kMagic)), f2(-1.f, -1.f), c);
-  uint64_t r = f2(0.009570096619427204f, 0.009570096619427204f);
-  r = fma2(r, f, f2(0.05591786280274391f, 0.05591786280274391f));
-  r = fma2(r, f, f2(0.240247443318367f, 0.240247443318367f));
-  r = fma2(r, f, f2(0.6931217908859253f, 0.6931217908859253f));
-  r = fma2(r, f, f2(0.9999992847442627f, 0.9999992847442627f));
-  float r0, r1, t0, t1;
-  f2_split(r, r0, r1);
-  f2_split(t, t0, t1);
-  a = __uint_as_float(__float_as_uint(r0) + (__float_as_uint(t0) << 23));
-  b = __uint_as_float(__float_as_uint(r1) + (__float_as_uint(t1) << 23));
 }
 
 // Bounded wait (about two seconds) that also gives up when another role has.  The abort flag and the clock are read once
@@ -211,8 +186,6 @@ __device__ __forceinline__ void after_wait(uint32_t (&r)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i])::"memory");
 }
-
-constexpr int kFmaPairs = 2;  // of every eight pairs of exponentials, those on the FMA pipe
 
 // Moves registers from the copy and MMA warps to the softmax warps: a row's 128 scores stay in registers.  The shares
 // (8 x 32 x 200 + 4 x 32 x 104 = 64512) are what 384 threads were launched with (168 each).
@@ -507,8 +480,7 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
         tmem_wait_ld(x[0]);
 #pragma unroll
         for (int c = 1; c < KT / 32; ++c) after_wait(x[c]);
-        const bool partial = key0 + KT > b.full_keys;
-        if (partial) {
+        if (key0 + KT > b.full_keys) {
 #pragma unroll
           for (int c = 0; c < KT / 32; ++c) {
             const uint32_t mask = seen32(p.b, it, tok, key0 + c * 32);
@@ -529,8 +501,6 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
           }
         }
         const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale_log2;
-        // a visible score of NaN or +inf makes the row NaN; the exponentials below may not show it
-        if (!(top < INFINITY)) l = __uint_as_float(0x7FC00000u);
         const bool grow = top > m + 8.f;  // (m = -inf: as soon as anything is seen)
         if (e < NG) {
           m = top;
@@ -554,35 +524,24 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
         const float base = m == -INFINITY ? 0.f : m;
         const uint64_t scale2 = f2(p.scale_log2, p.scale_log2), base2 = f2(-base, -base);
         uint64_t sum[2] = {0, 0};
-        // (one straight run of code for each of the two: a branch per pair left every exponential's latency exposed)
-        auto probabilities = [&](auto masked) {
 #pragma unroll
-          for (int c = 0; c < KT / 64; ++c) {
-            uint32_t pk[32];
+        for (int c = 0; c < KT / 64; ++c) {
+          uint32_t pk[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int u = (2 * i) & 31;
-              const uint64_t y = fma2(f2(__uint_as_float(x[2 * c + (i >> 4)][u]), __uint_as_float(x[2 * c + (i >> 4)][u + 1])),
-                                      scale2, base2);
-              float e0, e1;
-              if (i % 8 < kFmaPairs && !decltype(masked)::value) {  // (masked scores need the other form's exact 0)
-                ex2_fma(y, e0, e1);
-              } else {
-                float y0, y1;
-                f2_split(y, y0, y1);
-                e0 = ex2(y0), e1 = ex2(y1);
-              }
-              sum[i & 1] = add2(sum[i & 1], f2(e0, e1));
-              pk[i] = pack2<BF16>(e0, e1);  // (l keeps the f32 values)
-            }
-            tmem_st32(s_addr + c * 32, pk);
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(&pready[buf * S::kParts + c]);
+          for (int i = 0; i < 32; ++i) {
+            const int u = (2 * i) & 31;
+            float y0, y1;
+            f2_split(fma2(f2(__uint_as_float(x[2 * c + (i >> 4)][u]), __uint_as_float(x[2 * c + (i >> 4)][u + 1])), scale2, base2),
+                     y0, y1);
+            y0 = ex2(y0), y1 = ex2(y1);
+            sum[i & 1] = add2(sum[i & 1], f2(y0, y1));
+            pk[i] = pack2<BF16>(y0, y1);  // (l keeps the f32 values)
           }
-        };
-        if (partial) probabilities(std::true_type{});
-        else probabilities(std::false_type{});
+          tmem_st32(s_addr + c * 32, pk);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&pready[buf * S::kParts + c]);
+        }
         float s0, s1;
         f2_split(add2(sum[0], sum[1]), s0, s1);
         l += s0 + s1;
