@@ -14,6 +14,7 @@ torch stream or ``stream``; refusals raise :class:`Exl3Error`.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -42,19 +43,52 @@ def _ints(t, shape, what: str, device=None, optional: bool = False):
     return t
 
 
-def _heads(t: torch.Tensor, device, what: str) -> L.Heads:
+# exl3_heads as bytes: a ctypes structure costs more than the rest of the checks
+_HEADS = struct.Struct("@Piiiiqq")
+assert _HEADS.size == ctypes.sizeof(L.Heads)
+
+
+def _heads(t: torch.Tensor, index: int, what: str) -> bytes:
     dt = _TORCH_DT.get(t.dtype)
-    if t.device != device:
+    if t.get_device() != index:
         _refuse(f"{what} does not lie on the cache's GPU")
     if dt is None:
         _refuse(f"dtype {t.dtype} is not served", L.EXL3_UNSUPPORTED)
-    if t.dim() != 3:
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3:
         _refuse(f"{what} is [rows, heads, head_dim]")
-    rows, heads, dim = t.shape
-    rs, hs, es = t.stride()
-    if es != 1 and dim > 1:
+    if stride[2] != 1 and shape[2] > 1:
         _refuse(f"{what}'s head vectors must be contiguous")
-    return L.Heads(t.data_ptr(), dt, rows, heads, dim, rs, hs)
+    return _HEADS.pack(t.data_ptr(), dt, shape[0], shape[1], shape[2], stride[0], stride[1])
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _on(stream, index: int) -> int:
+    """The stream's handle; without one, the current stream of the cache's GPU."""
+    if stream is not None:
+        return _stream(stream)
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _check(v: L.Verdict) -> None:
+    if v.code:
+        check(v)
+
+
+class _Calls:
+    """The library's per-layer calls taking addresses and packed structures."""
+    rope = attention = None
+
+    @classmethod
+    def load(cls) -> None:
+        p, c = ctypes.c_void_p, ctypes.c_char_p
+        lib = L.lib()
+        proto = ctypes.CFUNCTYPE(L.Verdict, p, ctypes.c_int32, p, c, c, c, p, p, c)
+        cls.rope = proto(ctypes.cast(lib.exl3_qk_norm_rope, p).value)
+        proto = ctypes.CFUNCTYPE(L.Verdict, p, ctypes.c_int32, p, c, ctypes.c_float, p, c, p)
+        cls.attention = proto(ctypes.cast(lib.exl3_tree_attention, p).value)
 
 
 def _used_on(stream, *tensors) -> None:
@@ -86,8 +120,11 @@ class KvCache:
         sl, sp, sh, st, _ = k.stride()
         self.raw = L.KvCache(ctypes.sizeof(L.KvCache), k.device.index, dt, layers, pages, page_size, kv_heads, dim,
                              k.data_ptr(), v.data_ptr(), sl, sp, sh, st)
-        self._ref = ctypes.byref(self.raw)
-        check(L.lib().exl3_kv_register(self._ref))
+        self._at, self._index = ctypes.addressof(self.raw), k.device.index
+        self._scale = dim ** -0.5
+        check(L.lib().exl3_kv_register(self.raw))
+        if _Calls.rope is None:
+            _Calls.load()
 
     @classmethod
     def empty(cls, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=torch.bfloat16,
@@ -135,16 +172,16 @@ class TreeBatch:
         self.raw = L.TreeBatch(ctypes.sizeof(L.TreeBatch), nseq, rows or 0, int(max_rows), int(max_context),
                                table.shape[1], tree.shape[1] if tree is not None else 0, ptr(row_start), ptr(context),
                                ptr(table), ptr(tree), ptr(position))
-        self._ref = ctypes.byref(self.raw)
+        self._at, self._index = ctypes.addressof(self.raw), dev.index
 
     def _for(self, cache: KvCache, rows: int):
         if self.rows is None:  # neither tree nor position nor rows said how many
             self.rows = self.raw.rows = rows
         if rows != self.rows:
             _refuse(f"the batch has {self.rows} rows, not {rows}")
-        if self.device != cache.device:
+        if self._index != cache._index:
             _refuse("the batch lies on another device than the cache")
-        return self._ref
+        return self._at
 
 
 class NormRope:
@@ -176,23 +213,23 @@ class NormRope:
         self.raw = L.NormRope(ctypes.sizeof(L.NormRope), 0 if inv_freq is None else 2 * inv_freq.shape[0],
                               int(bool(adjacent)), wdt, float(eps), float(weight_offset), ptr(q_weight), ptr(k_weight),
                               ptr(inv_freq))
-        self._ref = ctypes.byref(self.raw)
+        self._at = ctypes.addressof(self.raw)
 
 
 def qk_norm_rope(cache: KvCache, layer: int, batch: TreeBatch, q, k, v, rope: NormRope, out=None, stream=None):
     """q [rows, heads, head_dim] normed and rotated (returned, in ``out`` if given: in q's dtype or the cache's, q
     itself allowed), k and v [rows, kv_heads, head_dim] written to their slots of ``layer``: k normed and rotated, v as it is."""
-    dev = cache.device
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q)
     if rope.dim is not None and rope.dim != cache.raw.head_dim:
         _refuse("norm weights are [head_dim]")
-    if rope.device is not None and rope.device != dev:
+    if rope.device is not None and rope.device != cache.device:
         _refuse("the norm weights lie on another device than the cache")
-    hq, hk, hv, ho = _heads(q, dev, "q"), _heads(k, dev, "k"), _heads(v, dev, "v"), _heads(out, dev, "out")
-    _used_on(stream, q, k, v, out)
-    check(L.lib().exl3_qk_norm_rope(cache._ref, layer, batch._for(cache, hq.rows), hq, hk, hv, rope._ref,
-                                    _stream(stream), ho))
+    i = cache._index
+    hq, hk, hv, ho = _heads(q, i, "q"), _heads(k, i, "k"), _heads(v, i, "v"), _heads(out, i, "out")
+    if stream is not None:
+        _used_on(stream, q, k, v, out)
+    _check(_Calls.rope(cache._at, layer, batch._for(cache, q.shape[0]), hq, hk, hv, rope._at, _on(stream, i), ho))
     return out
 
 
@@ -201,21 +238,21 @@ def tree_attention(cache: KvCache, layer: int, batch: TreeBatch, q, scale: float
     """Attention of the batch's rows q [rows, heads, head_dim] over ``layer`` -> [rows, heads, head_dim] in the cache's
     dtype.  ``scale`` defaults to head_dim ** -0.5.  ``lse``: True returns (out, lse), the log-sum-exp f32
     [rows, heads] of each row's scores; a tensor receives it."""
-    dev = cache.device
+    i = cache._index
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    hq, ho = _heads(q, dev, "q"), _heads(out, dev, "out")
+        out = torch.empty_like(q)
+    hq, ho = _heads(q, i, "q"), _heads(out, i, "out")
     if lse is True:
-        lse = torch.empty((hq.rows, hq.heads), dtype=torch.float32, device=dev)
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
     elif lse is False:
         lse = None
-    elif lse is not None and (lse.dtype != torch.float32 or lse.device != dev or not lse.is_contiguous() or
-                              tuple(lse.shape) != (hq.rows, hq.heads)):
+    elif lse is not None and (lse.dtype != torch.float32 or lse.device != cache.device or not lse.is_contiguous() or
+                              lse.shape != q.shape[:2]):
         _refuse("lse is a contiguous f32 tensor [rows, heads] on the cache's GPU")
-    _used_on(stream, q, out, lse)
-    check(L.lib().exl3_tree_attention(cache._ref, layer, batch._for(cache, hq.rows), hq,
-                                      cache.raw.head_dim ** -0.5 if scale is None else scale, _stream(stream), ho,
-                                      None if lse is None else lse.data_ptr()))
+    if stream is not None:
+        _used_on(stream, q, out, lse)
+    _check(_Calls.attention(cache._at, layer, batch._for(cache, q.shape[0]), hq, cache._scale if scale is None else scale,
+                            _on(stream, i), ho, None if lse is None else lse.data_ptr()))
     return out if lse is None else (out, lse)
 
 
@@ -243,8 +280,13 @@ class PageState:
         n = self.raw.nseq if nseq is None else nseq
         pages, width = self.refs.shape[0], self.raw.max_pages
         flat = torch.empty(pages + n * (width + 2), dtype=torch.int32, device=self.refs.device)
-        t = pages + n * width
-        return PageState(flat[:pages], flat[pages:t].view(n, width), flat[t:t + n], flat[t + n:])
+        refs, table, held, lens = flat.split_with_sizes((pages, n * width, n, n))
+        new = PageState.__new__(PageState)  # (nothing to check)
+        new.refs, new.table, new.held, new.lens = refs, table.view(n, width), held, lens
+        at = flat.data_ptr()
+        new.raw = L.PageState(ctypes.sizeof(L.PageState), n, width, at, at + 4 * pages, at + 4 * (pages + n * width),
+                              at + 4 * (pages + n * width + n))
+        return new
 
 
 def _states(cache: KvCache, state: PageState, out: PageState | None, nseq: int | None = None):
@@ -266,7 +308,7 @@ def cache_fork(cache: KvCache, state: PageState, parent, out: PageState | None =
     _ints(parent, (None,), "parent", cache.device)
     out = _states(cache, state, out, parent.shape[0])
     _used_on(stream, parent, out.refs, out.table, out.held, out.lens)
-    check(L.lib().exl3_cache_fork(cache._ref, state.raw, parent.data_ptr(), _stream(stream), out.raw))
+    check(L.lib().exl3_cache_fork(cache.raw, state.raw, parent.data_ptr(), _on(stream, cache._index), out.raw))
     return out
 
 
@@ -280,7 +322,7 @@ def cache_grow(cache: KvCache, state: PageState, need, out: PageState | None = N
     else:
         _ints(missing, (), "missing", cache.device)
     _used_on(stream, need, missing, out.refs, out.table, out.held, out.lens)
-    check(L.lib().exl3_cache_grow(cache._ref, state.raw, need.data_ptr(), _stream(stream), out.raw,
+    check(L.lib().exl3_cache_grow(cache.raw, state.raw, need.data_ptr(), _on(stream, cache._index), out.raw,
                                   missing.data_ptr()))
     return out, missing
 
@@ -297,8 +339,9 @@ def cache_keep(cache: KvCache, batch: TreeBatch, path, kept, out=None, stream=No
     if batch.rows is None:
         _refuse("the batch does not know its rows yet: give rows to TreeBatch")
     _used_on(stream, path, kept, out)
-    check(L.lib().exl3_cache_keep(cache._ref, batch._for(cache, batch.rows), None if path is None else path.data_ptr(),
-                                  0 if path is None else path.shape[1], kept.data_ptr(), _stream(stream),
+    batch._for(cache, batch.rows)
+    check(L.lib().exl3_cache_keep(cache.raw, batch.raw, None if path is None else path.data_ptr(),
+                                  0 if path is None else path.shape[1], kept.data_ptr(), _on(stream, cache._index),
                                   out.data_ptr()))
     return out
 
@@ -307,5 +350,5 @@ def cache_compact(cache: KvCache, state: PageState, out: PageState | None = None
     """The live pages moved into the lowest ids, in every layer; tables and reference counts follow."""
     out = _states(cache, state, out)
     _used_on(stream, out.refs, out.table, out.held, out.lens)
-    check(L.lib().exl3_cache_compact(cache._ref, state.raw, _stream(stream), out.raw))
+    check(L.lib().exl3_cache_compact(cache.raw, state.raw, _on(stream, cache._index), out.raw))
     return out
