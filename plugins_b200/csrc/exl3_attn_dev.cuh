@@ -10,6 +10,12 @@
 
 namespace exl3 {
 
+__device__ __forceinline__ float ex2(float x) {  // 2^x
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 constexpr float kLn2 = 0.6931471805599453f;
 
 // ------------------------------------------------------------------ the work
@@ -366,7 +372,7 @@ __device__ void WorkLine::join(const AttnParams& p, const Item& it, int slot_row
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
           const float m2 = fmaxf(mx[u], ml[u].x), base = m2 == -INFINITY ? 0.f : m2;
-          const float fa = exp2f(mx[u] - base), fb = exp2f(ml[u].x - base);
+          const float fa = ex2(mx[u] - base), fb = ex2(ml[u].x - base);
           acc[u][0] = acc[u][0] * fa + v[u].x * fb, acc[u][1] = acc[u][1] * fa + v[u].y * fb;
           acc[u][2] = acc[u][2] * fa + v[u].z * fb, acc[u][3] = acc[u][3] * fa + v[u].w * fb;
           sum[u] = sum[u] * fa + ml[u].y * fb;

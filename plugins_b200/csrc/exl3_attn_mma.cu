@@ -80,6 +80,17 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const AttnParams p) 
     }
     __syncthreads();
 
+    // the query fragments stay in registers where they fit beside o
+    constexpr bool kQRegs = MT * D <= 128;
+    uint32_t qa[kQRegs ? D / 16 : 1][MT][4];
+    if constexpr (kQRegs) {
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+          ldmatrix_x4(smem_u32(s_q) + tile_off<D>(16u * i + (lane & 15u), 2u * kk + (lane >> 4)), qa[kk][i]);
+    }
+
     float o[MT][D / 8][4];
     float m[MT][2], l[MT][2];
 #pragma unroll
@@ -91,11 +102,17 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const AttnParams p) 
 
     const int32_t* tab = p.b.table + static_cast<int64_t>(it.seq) * p.b.max_pages;
     const int page_mask = (1 << p.b.page_shift) - 1;
+    auto page_at = [&](int t) {
+      const int key0 = (tile0 + t) * kTileKeys + static_cast<int>(warp) * kGroupKeys;
+      return t < tiles && key0 < it.keys ? tab[key0 >> p.b.page_shift] : -1;
+    };
+    int page = page_at(0);  // of the next tile to issue, looked up one tile ahead of its copies
     // this warp's 16 keys of tile t into ring stage st: rows past the sequence's last key are zeros
     auto issue = [&](int t, int st) {
       const int key0 = (tile0 + t) * kTileKeys + static_cast<int>(warp) * kGroupKeys;
+      int id = page;
+      page = page_at(t + 1);
       if (t < tiles && key0 < it.keys) {
-        int id = tab[key0 >> p.b.page_shift];
         const bool ok = id >= 0 && id < p.b.pages;
         if (!ok) {
           if (lane == 0) atomicOr(p.b.err, kErrBadShape);
@@ -137,10 +154,10 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const AttnParams p) 
           ldmatrix_x4(sk + tile_off<D>((lane & 7u) + ((lane >> 4) << 3), 2u * kk + ((lane >> 3) & 1u)), b);
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
-            uint32_t a[4];
-            ldmatrix_x4(smem_u32(s_q) + tile_off<D>(16u * i + (lane & 15u), 2u * kk + (lane >> 4)), a);
-            mma16816<BF16>(s[i][0], a, b[0], b[1]);
-            mma16816<BF16>(s[i][1], a, b[2], b[3]);
+            if constexpr (!kQRegs)
+              ldmatrix_x4(smem_u32(s_q) + tile_off<D>(16u * i + (lane & 15u), 2u * kk + (lane >> 4)), qa[0][i]);
+            mma16816<BF16>(s[i][0], qa[kQRegs ? kk : 0][i], b[0], b[1]);
+            mma16816<BF16>(s[i][1], qa[kQRegs ? kk : 0][i], b[2], b[3]);
           }
         }
         const bool tail = key0 + kGroupKeys > it.context;  // some key is not in the context: rows see it or not
@@ -168,12 +185,12 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const AttnParams p) 
             mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
             mx = fmaxf(mx, m[i][hh]);
             const float base = mx == -INFINITY ? 0.f : mx;  // nothing seen so far: every term below is 0
-            const float f = exp2f(m[i][hh] - base);
+            const float f = ex2(m[i][hh] - base);
             m[i][hh] = mx;
             float sum = 0.f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              x[j] = exp2f(x[j] - base);
+              x[j] = ex2(x[j] - base);
               sum += x[j];
             }
             l[i][hh] = l[i][hh] * f + sum;
@@ -259,7 +276,7 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const AttnParams p) 
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float2 ml = s_ml[r * kWarps + w];
-        const float f = exp2f(ml.x - base);
+        const float f = ex2(ml.x - base);
         const float4 v = *reinterpret_cast<const float4*>(s_o + (w * S::kRows + r) * D + d0);
         sum += ml.y * f;
         acc[0] += v.x * f, acc[1] += v.y * f, acc[2] += v.z * f, acc[3] += v.w * f;

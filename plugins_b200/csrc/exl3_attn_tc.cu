@@ -83,12 +83,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Bounded wait (about two seconds) that also gives up when another role has.  The abort flag and the clock are read once
 // in many polls: a read of the global timer between polls held each wait up, and every tile's chain has three of them
 // (a 256-row prompt block: 568 us with it, see the table of steps in the design notes).
