@@ -96,9 +96,15 @@ struct WorkLine {
     return v;
   }
 
-  int64_t mine_, upto_;  // this thread's sequence of the last scanned chunk
+  // Cuts the line and finds the item that holds this CTA's first tile (if it has any).
+  __device__ void start(const AttnParams& p, int rows_per_block_, int tile_keys_, int64_t* scratch, Item& it) {
+    int64_t mine, upto;  // this thread's sequence of the last scanned chunk
+    init(p, rows_per_block_, tile_keys_, scratch, mine, upto);
+    if (begin < end) locate(p, begin, it, scratch, mine, upto);
+  }
 
-  __device__ void init(const AttnParams& p, int rows_per_block_, int tile_keys_, int64_t* scratch) {
+  __device__ void init(const AttnParams& p, int rows_per_block_, int tile_keys_, int64_t* scratch, int64_t& mine_,
+                       int64_t& upto_) {
     rows_per_block = rows_per_block_, tile_keys = tile_keys_, tile_shift = 31 - __clz(tile_keys_);
     int64_t sum = 0;
     for (int base = 0; base < p.b.nseq; base += blockDim.x) {
@@ -128,8 +134,7 @@ struct WorkLine {
   }
 
   // The item that holds tile `at` of the line.
-  __device__ void locate(const AttnParams& p, int64_t at, Item& it, int64_t* scratch) const {
-    int64_t mine = mine_, upto = upto_;
+  __device__ void locate(const AttnParams& p, int64_t at, Item& it, int64_t* scratch, int64_t mine, int64_t upto) const {
     const bool one = p.b.nseq <= static_cast<int>(blockDim.x);  // init's scan is the whole
     int64_t sum = 0;
     for (int base = 0; base < p.b.nseq; base += blockDim.x) {

@@ -56,11 +56,10 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const AttnParams p) 
   pdl_wait();
 
   WorkLine line;
-  line.init(p, S::kRows, kTileKeys, reinterpret_cast<int64_t*>(smem));
+  Item it;
+  line.start(p, S::kRows, kTileKeys, reinterpret_cast<int64_t*>(smem), it);
   int64_t at = line.begin, end = line.end;
   if (at >= end) return;
-  Item it;
-  line.locate(p, at, it, reinterpret_cast<int64_t*>(smem));
 
   const uint32_t ring = smem_u32(smem + warp * S::kRing);
   while (at < end) {

@@ -46,13 +46,13 @@ struct TcShape {
   static constexpr int kSoft = NG * 128;                  // softmax threads
   static constexpr int kTile = KT * D * 2;                // bytes of a K or V tile
   static constexpr int kQBytes = kRows * D * 2;
-  static constexpr int kSlots = (229376 - kQBytes) / kTile > 12 ? 12 : (229376 - kQBytes) / kTile;
+  static constexpr int kSlots = (229376 - kQBytes) / kTile > 10 ? 10 : (229376 - kQBytes) / kTile;
   static constexpr int VS = kSlots / 2, KS = kSlots - VS; // V and K tiles in flight
   static constexpr int kOCol = 256;                       // TMEM: S buffers at columns 0 and KT, O of group g at 256 + g * D
   static constexpr int kTmem = 512;
   static constexpr int kParts = KT / 64;                  // P comes in parts of 64 keys, each a product of its own
   static constexpr int kBars = 2 * KS + 3 * VS + 2 + 2 * kParts + 2 + 5;
-  static constexpr int kSmem = kQBytes + kSlots * kTile + 2 * 128 * 8 + kBars * 8 + 64;
+  static constexpr int kSmem = kQBytes + kSlots * kTile + 2 * 128 * 8 + kBars * 8 + 48 + sizeof(WorkLine) + kThreads / 32 * sizeof(Item);
   static_assert(KS * kTile + VS * kTile + kQBytes <= 229376 && kSmem <= 232448, "shared memory");
   static_assert(VS <= 8, "the odd flags cover eight items");
 };
@@ -363,6 +363,8 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
   volatile uint32_t* abort_flag = words + 1;
   int* s_last = reinterpret_cast<int*>(words + 2);
   volatile uint32_t* s_odd = words + 4;  // [8]: serial + 1 of an item whose V held infinities or NaN
+  WorkLine* s_line = reinterpret_cast<WorkLine*>(words + 12);
+  Item* s_items = reinterpret_cast<Item*>(s_line + 1);  // one per warp
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
 
   if (smem_u32(smem) & 1023u) {  // the swizzle goes by address bits: not served
@@ -389,15 +391,30 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
     asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
   }
   pdl_wait();
-  WorkLine line;
-  line.init(p, S::kRows, KT, reinterpret_cast<int64_t*>(s_k));
-  Item it;
-  if (line.begin < line.end) line.locate(p, line.begin, it, reinterpret_cast<int64_t*>(s_k));
+  {
+    WorkLine own;
+    Item first;
+    own.start(p, S::kRows, KT, reinterpret_cast<int64_t*>(s_k), first);
+    if (tid == 0) *s_line = own;
+    if (lane == 0) s_items[warp] = first;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
+  // The line, and each warp's item on it, stay in shared memory: what did not fit in registers went to local memory,
+  // which the shared memory leaves next to no L1 for, and a block's end took as long as eight tiles.
+  const WorkLine& line = *s_line;
+  Item& it = s_items[warp];
   int64_t at = line.begin;
+  auto advance = [&](int tiles) {
+    at += tiles;
+    if (at < line.end) {
+      __syncwarp();
+      if (lane == 0) line.next(p, it);
+      __syncwarp();
+    }
+  };
 
   if (warp < NG * 4) {
     // ---------------------------------------------------------------- softmax groups
@@ -632,8 +649,7 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
       mbar_arrive(ofree);
       if (!whole) join_block<D, ROWS, BF16>(p, line, it, b.rows, s_last, group_sync);
       group_sync();  // every MMA of the block has finished, and its rows are read: Q may be replaced
-      at += b.tiles;
-      if (at < line.end) line.next(p, it);
+      advance(b.tiles);
     }
   } else {
    if constexpr (NG == 2) regs_down<104>();
@@ -706,8 +722,7 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
         }
         if (e + NG >= b.events) commit(on, &ofull[NG == 2 ? buf : 0]);
       }
-      at += b.tiles;
-      if (at < line.end) line.next(p, it);
+      advance(b.tiles);
     }
     commit(on, fin);  // every MMA has finished before TMEM is released
     if (lane == 0 && !mbar_wait_bounded(fin, 0)) atomicOr(p.b.err, kErrWaitTimeout);
@@ -748,8 +763,7 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
           tma_box(base + slot * S::kTile + blk * (KT * 128) + part * box_rows * 128, map, blk * 64,
                   key & ((1 << p.b.page_shift) - 1), it.kv_head, id, &full[slot]);
       }
-      at += b.tiles;
-      if (ok && at < line.end) line.next(p, it);
+      advance(b.tiles);
     }
     // no copy may outlive the CTA: wait (bounded) for the last fill of every slot
     const uint32_t last = min(n, static_cast<uint32_t>(slots));
@@ -793,8 +807,7 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
         }
         if (lane == 0) mbar_arrive(&vclean[slot]);
       }
-      at += b.tiles;
-      if (ok && at < line.end) line.next(p, it);
+      advance(b.tiles);
     }
    }
   }
