@@ -240,9 +240,7 @@ __device__ __noinline__ void add_odd(const AttnParams& p, const Item& it, int to
   if (tok >= it.ntok) return;
   const uint16_t* q = static_cast<const uint16_t*>(p.q.data) + static_cast<int64_t>(it.row0 + tok) * p.q.row_stride +
                       h * p.q.head_stride;
-  // only tiles that reach past full_keys were cleaned
-  constexpr int KT = TcShape<D, 128>::KT;
-  for (int key = max(key_lo, full_keys / KT * KT); key < min(key_hi, it.total_keys); ++key) {
+  for (int key = max(key_lo, full_keys); key < min(key_hi, it.total_keys); ++key) {
     if (!sees(p.b, it, tok, key)) continue;
     const int id = p.b.table[static_cast<int64_t>(it.seq) * p.b.max_pages + (key >> p.b.page_shift)];
     if (id < 0 || id >= p.b.pages) continue;
@@ -284,6 +282,7 @@ __device__ void join_block(const AttnParams& p, const WorkLine& line, const Item
     if (r < rows) {
       auto slot = [&](int c) { return p.partials + (static_cast<int64_t>(c) * 2 + (c == c0 ? 0 : 1)) * kFloats; };
       float m = -INFINITY, l = 0.f;
+#pragma unroll 4
       for (int c = c0; c <= c1; ++c) {
         const float2 ml = __ldcg(reinterpret_cast<const float2*>(slot(c) + ROWS * D) + r);
         const float top = fmaxf(m, ml.x), base = top == -INFINITY ? 0.f : top;
@@ -785,22 +784,35 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
         if (!ok) break;
         const int key0 = (b.tile0 + t) * KT;
         if (key0 + KT > b.full_keys) {
-          uint8_t* tile = s_v + slot * S::kTile;
+          // only the slots that some row does not see: a lane takes a 16-byte chunk of every fourth of them, in all
+          // 64-column blocks, kAhead slots in flight (one at a time, the last tile of a block waited 7k clocks on this)
+          constexpr int kAhead = 4, kBlocks = D / 64;
+          uint8_t* tile = s_v + slot * S::kTile + (lane & 7u) * 16;
+          const int r0 = max(0, b.full_keys - key0) + static_cast<int>(lane >> 3), end = min(KT, it.total_keys - key0);
           bool odd = false;
-#pragma unroll 4
-          for (int i = static_cast<int>(lane); i < S::kTile / 16; i += 32) {
-            const int key = key0 + (i >> 3) % KT;  // eight 16-byte chunks per row of a block
-            uint4* c = reinterpret_cast<uint4*>(tile) + i;
-            if (key >= it.total_keys) {
-              *c = make_uint4(0u, 0u, 0u, 0u);
-            } else {
-              const uint4 u = *c;
-              if (odd2<BF16>(u.x) || odd2<BF16>(u.y) || odd2<BF16>(u.z) || odd2<BF16>(u.w)) {
-                odd = true;
-                *c = make_uint4(zero_odd2<BF16>(u.x), zero_odd2<BF16>(u.y), zero_odd2<BF16>(u.z), zero_odd2<BF16>(u.w));
+          for (int r = r0; r < end; r += 4 * kAhead) {
+            uint4 u[kAhead][kBlocks];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+              for (int c = 0; c < kBlocks; ++c) {
+                u[i][c] = make_uint4(0u, 0u, 0u, 0u);
+                if (r + 4 * i < end) u[i][c] = *reinterpret_cast<const uint4*>(tile + (c * KT + r + 4 * i) * 128);
               }
-            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+              for (int c = 0; c < kBlocks; ++c)
+                if (odd2<BF16>(u[i][c].x) || odd2<BF16>(u[i][c].y) || odd2<BF16>(u[i][c].z) || odd2<BF16>(u[i][c].w)) {
+                  odd = true;
+                  *reinterpret_cast<uint4*>(tile + (c * KT + r + 4 * i) * 128) =
+                      make_uint4(zero_odd2<BF16>(u[i][c].x), zero_odd2<BF16>(u[i][c].y), zero_odd2<BF16>(u[i][c].z),
+                                 zero_odd2<BF16>(u[i][c].w));
+                }
           }
+          for (int r = max(end, 0) + static_cast<int>(lane >> 3); r < KT; r += 4)  // past the sequence
+#pragma unroll
+            for (int c = 0; c < kBlocks; ++c) *reinterpret_cast<uint4*>(tile + (c * KT + r) * 128) = make_uint4(0u, 0u, 0u, 0u);
           if (odd) s_odd[serial & 7u] = serial + 1u;
           fence_proxy_async_smem();
           __syncwarp();
