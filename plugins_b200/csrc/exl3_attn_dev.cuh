@@ -359,36 +359,22 @@ __device__ void WorkLine::join(const AttnParams& p, const Item& it, int slot_row
   if (*s_word) {
     __threadfence();
     const int floats = slot_rows * (D + 2);
-    constexpr int kBatch = 4;  // elements of a thread in flight, each over all the slots
-    for (int i0 = static_cast<int>(threadIdx.x); i0 < rows * (D / 4); i0 += threads * kBatch) {
-      float mx[kBatch], sum[kBatch], acc[kBatch][4];
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) mx[u] = -INFINITY, sum[u] = acc[u][0] = acc[u][1] = acc[u][2] = acc[u][3] = 0.f;
-      for (int c = c0; c <= c1; ++c) {
+    for (int i = static_cast<int>(threadIdx.x); i < rows * (D / 4); i += threads) {
+      const int r = i / (D / 4), d0 = (i % (D / 4)) * 4;
+      float mx = -INFINITY, sum = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+      for (int c = c0; c <= c1; ++c) {  // unrolled: the loads of several slots are in flight
         const float* s = p.partials + (static_cast<int64_t>(c) * 2 + (c == c0 ? 0 : 1)) * floats;
-        float2 ml[kBatch];
-        float4 v[kBatch];
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          const int i = min(i0 + u * threads, rows * (D / 4) - 1), r = i / (D / 4), d0 = (i % (D / 4)) * 4;
-          ml[u] = __ldcg(reinterpret_cast<const float2*>(s + slot_rows * D + 2 * r));
-          v[u] = __ldcg(reinterpret_cast<const float4*>(s + r * D + d0));
-        }
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          const float m2 = fmaxf(mx[u], ml[u].x), base = m2 == -INFINITY ? 0.f : m2;
-          const float fa = ex2(mx[u] - base), fb = ex2(ml[u].x - base);
-          acc[u][0] = acc[u][0] * fa + v[u].x * fb, acc[u][1] = acc[u][1] * fa + v[u].y * fb;
-          acc[u][2] = acc[u][2] * fa + v[u].z * fb, acc[u][3] = acc[u][3] * fa + v[u].w * fb;
-          sum[u] = sum[u] * fa + ml[u].y * fb;
-          mx[u] = m2;
-        }
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(s + slot_rows * D + 2 * r));
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(s + r * D + d0));
+        const float m2 = fmaxf(mx, ml.x), base = m2 == -INFINITY ? 0.f : m2;
+        const float fa = ex2(mx - base), fb = ex2(ml.x - base);
+        acc[0] = acc[0] * fa + v.x * fb, acc[1] = acc[1] * fa + v.y * fb;
+        acc[2] = acc[2] * fa + v.z * fb, acc[3] = acc[3] * fa + v.w * fb;
+        sum = sum * fa + ml.y * fb;
+        mx = m2;
       }
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int i = i0 + u * threads;
-        if (i < rows * (D / 4)) store_out4<BF16>(p, it, slot_rows, i / (D / 4), (i % (D / 4)) * 4, acc[u], mx[u], sum[u]);
-      }
+      store_out4<BF16>(p, it, slot_rows, r, d0, acc, mx, sum);
     }
   }
   sync();
