@@ -21,6 +21,10 @@
 // cannot be masked there (0 x inf = NaN), so in the tiles that hold such keys the cleaning warp zeroes slots past the
 // sequence and infinities and NaN; the latter are added back in the epilogue to the rows that see them.
 //
+// What bounds it: up to 128 rows HBM (32 sequences' 16-token trees over 4-8k slots: 147 us, 5.5 TB/s); with 256 rows the
+// softmax warps, whose chain with the products of their buffer is 3.4k clocks per 256 x 128 scores against 2.0k of
+// either the exponentials or the products alone (a 4096-row chunk on 4096 slots: 381 us, 1.08 PFLOP/s).
+//
 // Every mbarrier wait is bounded (wait_bar): one that gives up raises an abort flag that all roles poll.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -85,7 +89,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // Bounded wait (about two seconds) that also gives up when another role has.  The abort flag and the clock are read once
 // in many polls: a read of the global timer between polls held each wait up, and every tile's chain has three of them
-// (a 256-row prompt block: 568 us with it, see the table of steps in the design notes).
+// (32 x 16-token trees 207 us with it, 192 without).
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t* err) {
   uint64_t t0 = 0;
   for (uint32_t i = 1;; ++i) {
@@ -405,6 +409,10 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
   // which the shared memory leaves next to no L1 for, and a block's end took as long as eight tiles.
   const WorkLine& line = *s_line;
   Item& it = s_items[warp];
+  if constexpr (NG == 2) {
+    if (warp < NG * 4) regs_up<200>();
+    else regs_down<104>();
+  }
   int64_t at = line.begin;
   auto advance = [&](int tiles) {
     at += tiles;
@@ -417,7 +425,6 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
 
   if (warp < NG * 4) {
     // ---------------------------------------------------------------- softmax groups
-    if constexpr (NG == 2) regs_up<200>();
     const uint32_t g = warp >> 2, wq = warp & 3u, r128 = wq * 32 + lane;  // row of the 128-row tile = TMEM lane
     const uint32_t lane_off = (wq * 32u) << 16;
     uint32_t sphase = 0, ophase = 0, xphase = 0, pvphase = 0;  // sphase: a bit per buffer; ophase: per group
@@ -650,9 +657,7 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
       group_sync();  // every MMA of the block has finished, and its rows are read: Q may be replaced
       advance(b.tiles);
     }
-  } else {
-   if constexpr (NG == 2) regs_down<104>();
-   if (warp == NG * 4) {
+  } else if (warp == NG * 4) {
     // ---------------------------------------------------------------- MMA issuer
     constexpr uint32_t idesc_s = attn_idesc<BF16>(128, KT, false), idesc_o = attn_idesc<BF16>(128, D, true);
     const uint32_t on = elect_one();
@@ -821,7 +826,6 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
       }
       advance(b.tiles);
     }
-   }
   }
   tc_fence_before();
   __syncthreads();

