@@ -552,7 +552,7 @@ exl3_verdict exl3_qk_norm_rope(const exl3_kv_cache *cache, int32_t layer, const 
                                const exl3_norm_rope *opts, void *stream, const exl3_heads *q_out);
 
 /* Attention of the batch's rows over `layer`: out[r][h] = sum_j softmax_j(scale q[r][h] . k[j]) v[j] over the slots the
- * row sees, kv head h / (heads / kv_heads).  q and out in the cache's dtype; scale > 0.  `lse` (device f32
+ * row sees, kv head h / (heads / kv_heads).  q and out in the cache's dtype, not the same array; scale > 0.  `lse` (device f32
  * [rows][heads], or null) receives log sum_j exp(scale q . k[j]).  A row that sees nothing gets zeros and -inf.  What
  * lies in slots a row does not see -- stale pages, other branches of the tree, infinities, NaN -- does not reach it.
  * Any number of rows per sequence: one (a decode step), a drafted tree, a prompt chunk. */

@@ -84,6 +84,16 @@ exl3_verdict check_heads(const exl3_heads* h, const char* what, int32_t rows, in
   return kOk;
 }
 
+// Vectors that are written lie apart (those that are only read may repeat: a stride of 0 broadcasts).
+bool lies_apart(const exl3_heads* h) {
+  const auto step = [](int64_t s) { return s < 0 ? -s : s; };
+  const int64_t row = step(h->row_stride), head = step(h->head_stride);
+  const bool head_in = h->heads == 1 || head >= h->dim, row_in = h->rows <= 1 || row >= h->dim;
+  if (!head_in || !row_in) return false;
+  if (h->heads == 1 || h->rows <= 1) return true;
+  return row >= head ? row >= head * (h->heads - 1) + h->dim : head >= row * (h->rows - 1) + h->dim;
+}
+
 exl3::HeadsView view(const exl3_heads* h) {
   exl3::HeadsView v{};
   v.data = h->data, v.dtype = h->dtype, v.heads = h->heads, v.row_stride = h->row_stride, v.head_stride = h->head_stride;
@@ -172,6 +182,10 @@ exl3_verdict exl3_qk_norm_rope(const exl3_kv_cache* cache, int32_t layer, const 
   if (k->dtype != q->dtype || v->dtype != q->dtype) return refuse(EXL3_UNSUPPORTED, "exl3_b200: q, k and v have one dtype");
   if (q_out->dtype != q->dtype && q_out->dtype != cache->dtype)
     return refuse(EXL3_UNSUPPORTED, "exl3_b200: q_out has q's dtype or the cache's");
+  if (!lies_apart(q_out)) return refuse(EXL3_FAILED, "exl3_b200: q_out's vectors overlap");
+  if (q_out->data && q_out->data == q->data &&
+      (q_out->dtype != q->dtype || q_out->row_stride != q->row_stride || q_out->head_stride != q->head_stride))
+    return refuse(EXL3_FAILED, "exl3_b200: q_out lies over q in another layout");
   if (!opts || opts->size != sizeof(exl3_norm_rope)) return refuse(EXL3_FAILED, "exl3_b200: not norm and rotation options");
   if (opts->rot_dims < 0 || opts->rot_dims > dim || opts->rot_dims % 2 || (!opts->adjacent && opts->rot_dims % 16))
     return refuse(EXL3_UNSUPPORTED, "exl3_b200: rot_dims is even, at most head_dim, and a multiple of 16 for split halves");
@@ -205,11 +219,13 @@ exl3_verdict exl3_tree_attention(const exl3_kv_cache* cache, int32_t layer, cons
     return refuse(EXL3_UNSUPPORTED, "exl3_b200: q and out have the cache's dtype");
   if (out->heads != q->heads || q->heads % cache->kv_heads)
     return refuse(EXL3_FAILED, "exl3_b200: q and out have a whole number of heads per kv head");
+  if (!lies_apart(out)) return refuse(EXL3_FAILED, "exl3_b200: out's vectors overlap");
   if (q->heads > 4096) return refuse(EXL3_TOO_LARGE, "exl3_b200: more than 4096 query heads");
   if (static_cast<int64_t>(rows) * q->heads > (1ll << 30)) return refuse(EXL3_TOO_LARGE, "exl3_b200: more than 2^30 query vectors");
   if (!(scale > 0.f) || std::isinf(scale)) return refuse(EXL3_UNSUPPORTED, "exl3_b200: the scale is a positive number");
   if (batch->max_rows > rows) return refuse(EXL3_FAILED, "exl3_b200: max_rows is above the batch's rows");
   if (batch->nseq == 0 || rows == 0) return kOk;
+  if (out->data == q->data) return refuse(EXL3_FAILED, "exl3_b200: out is not q (a row may be read again at its end)");
   exl3::Workspace ws;
   if (!exl3::workspace_get(cache->device, ws)) return kNoWorkspace;
   OnDevice guard(cache->device);
@@ -221,7 +237,7 @@ exl3_verdict exl3_tree_attention(const exl3_kv_cache* cache, int32_t layer, cons
   p.bf16 = cache->dtype == EXL3_BF16;
   p.max_rows = batch->max_rows > 0 ? batch->max_rows : rows;
   const int64_t width = static_cast<int64_t>(batch->max_pages) * cache->page_size;
-  if (width > 0x7FFFFFFF) return refuse(EXL3_TOO_LARGE, "exl3_b200: the table spans 2^31 slots or more");
+  if (width > 0x7FFF0000) return refuse(EXL3_TOO_LARGE, "exl3_b200: the table spans 2^31 slots or more");
   p.max_context = static_cast<int32_t>(batch->max_context > 0 && batch->max_context < width ? batch->max_context : width);
   p.scale_log2 = scale * 1.4426950408889634f;
   p.partials = ws.partials, p.counters = ws.counters;

@@ -91,6 +91,8 @@ def test_a_batch_is_refused_by_name(kw, code, text):
     (dict(heads=4), dict(heads=2), 1, 0, L.EXL3_FAILED, "per kv head"),
     ({}, {}, 0.0, 0, L.EXL3_UNSUPPORTED, "scale"), ({}, {}, -1.0, 0, L.EXL3_UNSUPPORTED, "scale"),
     ({}, {}, math.nan, 0, L.EXL3_UNSUPPORTED, "scale"), ({}, {}, math.inf, 0, L.EXL3_UNSUPPORTED, "scale"),
+    ({}, dict(head_stride=0), 1, 0, L.EXL3_FAILED, "overlap"), ({}, dict(row_stride=64), 1, 0, L.EXL3_FAILED, "overlap"),
+    ({}, dict(head_stride=63), 1, 0, L.EXL3_FAILED, "overlap"),
     ({}, {}, 1, 2, L.EXL3_FAILED, "layer"), ({}, {}, 1, -1, L.EXL3_FAILED, "layer"),
 ])
 def test_attention_is_refused_by_name(q, out, scale, layer, code, text):
@@ -105,6 +107,8 @@ def test_attention_is_refused_by_name(q, out, scale, layer, code, text):
     (dict(dtype=L.F32), {}, {}, {}, {}, L.EXL3_UNSUPPORTED, "one dtype"),
     ({}, {}, {}, dict(dtype=L.F16), {}, L.EXL3_UNSUPPORTED, "q_out"),
     ({}, {}, {}, dict(dtype=L.F32), {}, L.EXL3_UNSUPPORTED, "q_out"),
+    ({}, {}, {}, dict(row_stride=0), {}, L.EXL3_FAILED, "overlap"),
+    ({}, {}, {}, dict(row_stride=512), {}, L.EXL3_FAILED, "another layout"),
     ({}, {}, {}, {}, dict(size=1), L.EXL3_FAILED, "options"), ({}, {}, {}, {}, dict(rot_dims=66), L.EXL3_UNSUPPORTED, "rot_dims"),
     ({}, {}, {}, {}, dict(rot_dims=24), L.EXL3_UNSUPPORTED, "rot_dims"),
     ({}, {}, {}, {}, dict(rot_dims=7, adjacent=1), L.EXL3_UNSUPPORTED, "rot_dims"),
@@ -130,7 +134,11 @@ def test_page_calls_are_refused_by_name():
     refused(lib.exl3_cache_fork(cache(), state(), AT, None, state(**other)), L.EXL3_FAILED, "exl3_kv_register")
     refused(lib.exl3_cache_keep(cache(), batch(), AT, 0, AT, None, AT), L.EXL3_FAILED, "without depth")
     refused(lib.exl3_cache_keep(cache(), batch(), AT, 1, None, None, AT), L.EXL3_FAILED, "without its arrays")
-    refused(lib.exl3_tree_attention(cache(), 0, batch(), heads(), 1.0, None, heads(), None), L.EXL3_FAILED, "exl3_kv_register")
+    refused(lib.exl3_tree_attention(cache(), 0, batch(), heads(), 1.0, None, heads(data=2 * AT), None), L.EXL3_FAILED,
+            "exl3_kv_register")
+    refused(lib.exl3_tree_attention(cache(), 0, batch(), heads(), 1.0, None, heads(), None), L.EXL3_FAILED, "out is not q")
+    refused(lib.exl3_tree_attention(cache(), 0, batch(max_rows=5), heads(), 1.0, None, heads(data=2 * AT), None),
+            L.EXL3_FAILED, "max_rows")
 
 
 def test_nothing_to_do_is_not_an_error():

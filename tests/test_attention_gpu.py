@@ -423,3 +423,19 @@ def test_slots_past_two_to_the_31_elements(A, rows):
     grown, missing = A.cache_grow(cache, state, i32([10, 9]))
     assert int(missing) == 0 and grown.table.tolist() == [[pages - 3], [pages - 1]]
     assert torch.equal(k[0, pages - 3], k[0, pages - 1]) and torch.equal(v[0, pages - 3], v[0, pages - 1])
+
+
+def test_broadcast_queries_and_one_key_for_all_heads(A):
+    """Inputs of stride 0: one query vector for every row and head, one k and v vector for every kv head."""
+    st = Step([3], [20], 2, 64, 16, "f16", seed=41)
+    cache, batch = st.device(A)
+    x = torch.randn((3, 1, 64), generator=torch.Generator().manual_seed(3)).half()
+    one = x.cuda().expand(3, 2, 64)
+    A.qk_norm_rope(cache, st.layer, batch, x.cuda()[:1].expand(3, 4, 64), one, one, A.NormRope(None))
+    pg, of = R.slots(st.table[0], 16, 20, 23)
+    st.k[st.layer, pg, :, of] = st.v[st.layer, pg, :, of] = x.expand(3, 2, 64)
+    assert torch.equal(cache.k.cpu(), st.k) and torch.equal(cache.v.cpu(), st.v)
+    q = x[:1].expand(3, 4, 64)
+    out, lse = A.tree_attention(cache, st.layer, batch, x.cuda()[:1].expand(3, 4, 64), lse=True,
+                                out=torch.empty((3, 4, 64), dtype=torch.float16, device="cuda"))
+    check_attention(out, lse, *st.want(q, 64 ** -0.5), st.dtype)
