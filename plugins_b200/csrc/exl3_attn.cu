@@ -241,7 +241,7 @@ exl3_verdict exl3_tree_attention(const exl3_kv_cache* cache, int32_t layer, cons
   p.max_context = static_cast<int32_t>(batch->max_context > 0 && batch->max_context < width ? batch->max_context : width);
   p.scale_log2 = scale * 1.4426950408889634f;
   p.partials = ws.partials, p.counters = ws.counters;
-  const bool few = static_cast<int64_t>(p.max_rows) * p.group <= exl3::kAttnFewRows;
+  const bool few = static_cast<int64_t>(p.max_rows) * p.group <= exl3::attn_few_rows(dim);
   return launched((few ? exl3::launch_attn_mma : exl3::launch_attn_tc)(p, dim, ws.sms, ws.partial_floats,
                                                                        static_cast<cudaStream_t>(stream)));
 }
