@@ -588,7 +588,8 @@ exl3_verdict exl3_cache_grow(const exl3_kv_cache *cache, const exl3_page_state *
 
 /* Keep a verified path: of each sequence's drafted rows, path[s][0 .. kept[s] - 1] (ascending row indices, [nseq][depth])
  * were accepted; their keys and values move, in every layer, from slots context + path[d] to context + d, and
- * lens[s] = context[s] + kept[s].  A null path keeps the first kept[s] rows where they are. */
+ * lens[s] = context[s] + kept[s].  A null path keeps the first kept[s] rows where they are.  `lens` may be the batch's
+ * context array itself, or `kept`. */
 exl3_verdict exl3_cache_keep(const exl3_kv_cache *cache, const exl3_tree_batch *batch, const int32_t *path,
                              int32_t depth, const int32_t *kept, void *stream, int32_t *lens);
 

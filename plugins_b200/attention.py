@@ -329,7 +329,8 @@ def cache_grow(cache: KvCache, state: PageState, need, out: PageState | None = N
 
 def cache_keep(cache: KvCache, batch: TreeBatch, path, kept, out=None, stream=None):
     """The accepted rows of each drafted tree, ``path[s][:kept[s]]`` (int32 [nseq, depth], ascending; None: the first
-    kept rows), moved behind the context in every layer -> the sequences' new lengths, context + kept."""
+    kept rows), moved behind the context in every layer -> the sequences' new lengths, context + kept (``out`` may be the
+    batch's own context tensor)."""
     _ints(kept, (batch.nseq,), "kept", cache.device)
     _ints(path, (batch.nseq, None), "path", cache.device, optional=True)
     if out is None:

@@ -158,7 +158,7 @@ exl3_verdict workspace_create(int device) { return ensure_device(device); }
 bool workspace_get(int device, Workspace& ws) {
   const DeviceState* d = device_state(device);
   if (!d) return false;
-  ws = {d->partials, d->partial_floats, d->counters, d->err, d->sms};
+  ws = {d->partials, d->partial_floats, d->counters, kCounterCount, d->err, d->sms};
   return true;
 }
 

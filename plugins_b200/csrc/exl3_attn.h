@@ -14,6 +14,7 @@ struct Workspace {
   float* partials;
   size_t partial_floats;
   uint32_t* counters;
+  uint32_t counter_count;
   uint32_t* err;
   int sms;
 };
@@ -97,9 +98,11 @@ struct KeepParams {
   PagedBatch b;
   const int32_t *path, *kept;
   int32_t depth;
-  int32_t* lens;
+  int32_t* lens;       // may be b.context, or kept
+  uint32_t* counters;  // one per sequence of a launch
+  int32_t seq0;        // the launch's first sequence
 };
-cudaError_t launch_cache_keep(const KeepParams& p, cudaStream_t st);
+cudaError_t launch_cache_keep(const KeepParams& p, uint32_t counters, cudaStream_t st);
 
 #if defined(__CUDACC__)
 // The sequence that owns `row`: the last s with row_start[s] <= row (empty sequences own none).  Called by a whole warp;

@@ -302,10 +302,11 @@ constexpr int kKeepThreads = 256;
 constexpr int kKeepBatch = 8;  // tokens read before any of them is written
 
 // One thread per (16-byte chunk of a head, kv head, k or v, layer) of one sequence (blockIdx.y): it walks the path.  The
-// path ascends, so path[d] >= d, and a slot is never read after a later token was written to it.
+// path ascends, so path[d] >= d, and a slot is never read after a later token was written to it.  lens[s] is written by the
+// sequence's last block to have read context[s] and kept[s]: it may be either of them (a loop's lengths kept in place).
 __global__ void __launch_bounds__(kKeepThreads) keep_kernel(const KeepParams p) {
   pdl_wait();
-  const int s = blockIdx.y;
+  const int s = p.seq0 + static_cast<int>(blockIdx.y);
   const int ctx = p.b.context[s];
   const int ntok = max(0, min(p.b.row_start[s + 1], p.b.rows) - max(p.b.row_start[s], 0));
   int kept = p.kept[s];
@@ -321,9 +322,19 @@ __global__ void __launch_bounds__(kKeepThreads) keep_kernel(const KeepParams p) 
   }
   const int64_t item = static_cast<int64_t>(blockIdx.x) * kKeepThreads + threadIdx.x;
   if (!ok) kept = 0;
-  if (item == 0) {
-    p.lens[s] = max(ctx, 0) + kept;
-    if (!ok) atomicOr(p.b.err, kErrBadShape);
+  __syncthreads();  // the block's reads of context and kept are done
+  if (threadIdx.x == 0) {
+    bool last = true;
+    if (gridDim.x > 1) {
+      __threadfence();
+      last = atomicAdd(p.counters + blockIdx.y, 1u) + 1u == gridDim.x;
+      __threadfence();
+    }
+    if (last) {
+      if (gridDim.x > 1) p.counters[blockIdx.y] = 0u;
+      p.lens[s] = max(ctx, 0) + kept;
+      if (!ok) atomicOr(p.b.err, kErrBadShape);
+    }
   }
   if (!path) return;
   const int per = p.pool.dim / 8;
@@ -406,11 +417,18 @@ cudaError_t launch_page_copy(const PagePool& pool, const int32_t* moves, int64_t
   return launch_pdl_k(page_copy_kernel, dim3(static_cast<unsigned>(grid)), dim3(kCopyThreads), st, pool, moves);
 }
 
-cudaError_t launch_cache_keep(const KeepParams& p, cudaStream_t st) {
-  if (p.b.nseq <= 0) return cudaSuccess;
+cudaError_t launch_cache_keep(const KeepParams& p, uint32_t counters, cudaStream_t st) {
   const int64_t items = p.path ? static_cast<int64_t>(p.pool.layers) * 2 * p.pool.kv_heads * (p.pool.dim / 8) : 1;
-  const dim3 grid(static_cast<unsigned>((items + kKeepThreads - 1) / kKeepThreads), static_cast<unsigned>(p.b.nseq));
-  return launch_pdl_k(keep_kernel, grid, dim3(kKeepThreads), st, p);
+  KeepParams part = p;
+  // a counter per sequence of a launch
+  for (part.seq0 = 0; part.seq0 < p.b.nseq; part.seq0 += static_cast<int>(counters)) {
+    const int left = p.b.nseq - part.seq0;
+    const dim3 grid(static_cast<unsigned>((items + kKeepThreads - 1) / kKeepThreads),
+                    left < static_cast<int>(counters) ? static_cast<unsigned>(left) : counters);
+    cudaError_t e = launch_pdl_k(keep_kernel, grid, dim3(kKeepThreads), st, part);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace exl3
