@@ -577,12 +577,13 @@ typedef struct exl3_page_state {
 exl3_verdict exl3_cache_fork(const exl3_kv_cache *cache, const exl3_page_state *in, const int32_t *parent, void *stream,
                              const exl3_page_state *out);
 
-/* Grow: every row gets pages for need[i] tokens, and sole ownership of the page its next token falls in.  A partly
- * filled last page that others share and the row will write is replaced by a copy (in every layer) -- except that when
- * all its sharers grow, the first of them keeps it.  Pages are given lowest id first, rows in order, a row's copy
- * before its new pages.  Rows never shrink; lens stay.  missing[0] (device) receives 0, or, when the free pages or the
- * table's width do not suffice, how many pages are lacking, and then `out` is `in` unchanged and nothing is copied.
- * out's arrays are not in's. */
+/* Grow: every row gets pages for need[i] tokens, and sole ownership of every page it is about to write, those of slots
+ * lens[i] .. need[i] - 1.  Such a page that others share is replaced in the row's table: by a copy (in every layer) where
+ * it holds tokens of the row, by a fresh page where it does not (pages a row holds beyond its tokens, as after rejected
+ * drafts, are shared by a fork like the others) -- except that when all its sharers write it, the first of them keeps it.
+ * Pages are given lowest id first, rows in order, a row's replaced pages (in table order) before its new ones.  Rows never
+ * shrink; lens stay.  missing[0] (device) receives 0, or, when the free pages or the table's width do not suffice, how
+ * many pages are lacking, and then `out` is `in` unchanged and nothing is copied.  out's arrays are not in's. */
 exl3_verdict exl3_cache_grow(const exl3_kv_cache *cache, const exl3_page_state *in, const int32_t *need, void *stream,
                              const exl3_page_state *out, int32_t *missing);
 

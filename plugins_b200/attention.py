@@ -313,8 +313,9 @@ def cache_fork(cache: KvCache, state: PageState, parent, out: PageState | None =
 
 
 def cache_grow(cache: KvCache, state: PageState, need, out: PageState | None = None, missing=None, stream=None):
-    """Pages for ``need[i]`` (int32) tokens in every row, a shared page that row i will write replaced by a copy ->
-    (the new state, ``missing``: an int32 scalar tensor, 0, or the pages lacking: then nothing changed)."""
+    """Pages for ``need[i]`` (int32) tokens in every row, each shared page that row i will write (slots ``lens[i]`` to
+    ``need[i]`` - 1) replaced by one of its own, with a copy where it holds tokens of the row -> (the new state,
+    ``missing``: an int32 scalar tensor, 0, or the pages lacking: then nothing changed)."""
     _ints(need, (state.raw.nseq,), "need", cache.device)
     out = _states(cache, state, out)
     if missing is None:

@@ -78,7 +78,8 @@ struct PageParams {
   int32_t *refs, *table, *held, *lens;
   const int32_t *parent, *need;
   int32_t* missing;
-  int32_t* moves;  // [1 + 2 * capacity]: count, then (source, destination) pages
+  int32_t* moves;    // [1 + 2 * capacity]: count, then (source, destination) pages
+  int32_t* scratch;  // grow: [2 * nseq + 2 * pages]
   uint32_t* err;
 };
 struct PagePool {

@@ -99,104 +99,140 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) for
 
 // ------------------------------------------------------------------ grow
 
+// The table places whose pages row r writes: those of the slots len .. need - 1, as far as it holds them.
+struct Writes {
+  int lo, hi;    // [lo, hi)
+  int len, held, want;  // the row's tokens and pages, the pages it needs (at most the table's width)
+  int over;      // pages it needs past that
+  __device__ __forceinline__ Writes(const PageParams& p, int r) {
+    const int page = 1 << p.page_shift, need = max(p.need[r], 0);
+    len = p.lens_in[r], held = held_of(p, r);
+    const int all = static_cast<int>((static_cast<int64_t>(need) + page - 1) >> p.page_shift);
+    want = min(all, p.width_in), over = all - want;
+    lo = hi = 0;
+    if (need > len && len >= 0) lo = min(len >> p.page_shift, held), hi = max(lo, min(want, held));
+  }
+};
+
+// A page with several references that a row writes is replaced in its table, by a copy where it holds tokens of the row:
+// the page of slot len, and pages past it that the row held without needing them (provided for drafts that were rejected)
+// when it was forked.  When every reference is a row's that writes the page, the first of these rows keeps it.
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) grow_kernel(const PageParams p) {
-  extern __shared__ int s_row[];  // [nseq] last pages of growing rows, asks before the row, copies before the row
+  extern __shared__ int s_row[];  // [nseq + 1] asks before the row, copies before the row
   __shared__ int s_warp[32], s_total, s_over;
-  int* s_last = s_row;
-  int* s_ask = s_row + p.nseq_in;
-  int* s_copy = s_ask + p.nseq_in + 1;
+  int* s_ask = s_row;
+  int* s_copy = s_row + p.nseq_in + 1;
   pdl_wait();
   const int tid = static_cast<int>(threadIdx.x);
   const int t = static_cast<int>(blockIdx.x) * kThreads + tid;
+  const int lane = t & 31, warp = t >> 5;
   const int n = p.nseq_in, page = 1 << p.page_shift;
-  for (int i = t; i < p.pages; i += kAll) p.refs[i] = p.refs_in[i];
+  int* asks = p.scratch;       // [nseq] pages each row asks for
+  int* copies = asks + n;      // [nseq] of them, copies
+  int* first = copies + n;     // [pages] of a shared page, the first row that writes it
+  int* order = first + p.pages;  // [pages] the free pages in the order they are given
+  // counts and tables as they are, and the free pages ranked
+  for (int i = t; i < p.pages; i += kAll) {
+    const int refs = p.refs_in[i];
+    p.refs[i] = refs;
+    if (refs > 1) first[i] = n;
+  }
   for (int64_t i = t; i < static_cast<int64_t>(n) * p.width_in; i += kAll) p.table[i] = p.table_in[i];
-  // every CTA: what each row asks for
-  for (int r = tid; r < n; r += kThreads) {
-    const int len = p.lens_in[r], held = held_of(p, r);
-    int last = -1;
-    if (p.need[r] > len && len >= 0 && (len & (page - 1)) && (len >> p.page_shift) < held) {
-      last = p.table_in[static_cast<int64_t>(r) * p.width_in + (len >> p.page_shift)];
-      if (last < 0 || last >= p.pages) {
-        last = -1;
-        atomicOr(p.err, kErrBadShape);
-      }
-    }
-    s_last[r] = last;
-  }
   if (tid == 0) s_over = 0;
-  __syncthreads();
-  int asked = 0, copied = 0;  // rows are scanned in runs of kThreads
-  for (int base = 0; base < n; base += kThreads) {
-    const int r = base + tid;
-    int ask = 0, copy = 0;
-    if (r < n) {
-      const int held = held_of(p, r);
-      const int64_t want = (static_cast<int64_t>(max(p.need[r], 0)) + page - 1) >> p.page_shift;
-      if (want > p.width_in) atomicAdd(&s_over, static_cast<int>(want - p.width_in));
-      ask = static_cast<int>(max(static_cast<int64_t>(0), min(want, static_cast<int64_t>(p.width_in)) - held));
-      const int last = s_last[r];
-      if (last >= 0) {
-        const int refs = p.refs_in[last];
-        if (refs > 1) {  // shared: copied, unless every sharer grows and this row is their first
-          int sharers = 0, first = r;
-          for (int o = 0; o < n; ++o)
-            if (s_last[o] == last) ++sharers, first = min(first, o);
-          copy = sharers == refs && first == r ? 0 : 1;
-        }
-      }
-      ask += copy;
-    }
-    int total;
-    const int a = cta_scan_excl(ask, s_warp, &total);
-    if (r < n) s_ask[r] = asked + a;
-    asked += total;
-    const int c = cta_scan_excl(copy, s_warp, &total);
-    if (r < n) s_copy[r] = copied + c;
-    copied += total;
-  }
-  if (tid == 0) s_ask[n] = asked, s_copy[n] = copied;
-  // the free pages, ranked
   const PageRun run(p.pages);
   int mine = 0, free_pages;
   for (int i = run.lo; i < run.hi; ++i) mine += p.refs_in[i] == 0 ? 1 : 0;
   int rank = cluster_scan_excl(mine, s_warp, &s_total, &free_pages);  // (its barrier: the copies above are in place)
+  // a shared page loses the references of the rows that write it (whole numbers: any order)
+  for (int r = warp; r < n; r += kAll / 32) {
+    const Writes w(p, r);
+    for (int j = w.lo + lane; j < w.hi; j += 32) {
+      const int id = p.table_in[static_cast<int64_t>(r) * p.width_in + j];
+      if (id < 0 || id >= p.pages) {
+        atomicOr(p.err, kErrBadShape);
+      } else if (p.refs_in[id] > 1) {
+        atomicSub(p.refs + id, 1);
+        atomicMin(first + id, r);
+      }
+    }
+  }
+  cluster_sync();
+  auto replaced = [&](const Writes& w, int r, int j, int& id) {
+    id = j < w.hi ? p.table_in[static_cast<int64_t>(r) * p.width_in + j] : -1;
+    if (id < 0 || id >= p.pages || p.refs_in[id] <= 1) return false;
+    return __ldcg(first + id) != r || __ldcg(p.refs + id) > 0;
+  };
+  for (int r = warp; r < n; r += kAll / 32) {
+    const Writes w(p, r);
+    int ask = max(0, w.want - w.held), copy = 0;
+    for (int j0 = w.lo; j0 < w.hi; j0 += 32) {
+      int id;
+      const uint32_t which = __ballot_sync(0xFFFFFFFFu, replaced(w, r, j0 + lane, id));
+      ask += __popc(which);
+      if (j0 == w.lo && (w.len & (page - 1))) copy = which & 1u;
+    }
+    if (lane == 0) asks[r] = ask, copies[r] = copy;
+  }
+  cluster_sync();
+  int asked = 0, copied = 0;  // every CTA: rows are scanned in runs of kThreads
+  for (int base = 0; base < n; base += kThreads) {
+    const int r = base + tid;
+    if (r < n) {
+      const int over = Writes(p, r).over;
+      if (over) atomicAdd(&s_over, over);
+    }
+    int total;
+    const int a = cta_scan_excl(r < n ? __ldcg(asks + r) : 0, s_warp, &total);
+    if (r < n) s_ask[r] = asked + a;
+    asked += total;
+    const int c = cta_scan_excl(r < n ? __ldcg(copies + r) : 0, s_warp, &total);
+    if (r < n) s_copy[r] = copied + c;
+    copied += total;
+  }
+  __syncthreads();
   const int missing = max(0, asked - free_pages) + s_over;
   if (t == 0) {
     p.missing[0] = missing;
     p.moves[0] = missing ? 0 : copied;
   }
   for (int r = t; r < n; r += kAll) {
-    const int held = held_of(p, r), got = s_ask[r + 1] - s_ask[r] - (s_copy[r + 1] - s_copy[r]);
-    p.held[r] = missing ? held : held + got;
-    p.lens[r] = p.lens_in[r];
+    const Writes w(p, r);
+    p.held[r] = missing ? w.held : max(w.held, w.want);
+    p.lens[r] = w.len;
   }
-  if (!missing) {
-    for (int i = run.lo; i < run.hi && rank < asked; ++i) {
-      if (p.refs_in[i] != 0) continue;
-      // the row whose ask holds this rank: the last with s_ask[r] <= rank
-      int lo = 0, hi = n;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (s_ask[mid] <= rank) lo = mid;
-        else hi = mid;
+  if (missing) {
+    for (int i = t; i < p.pages; i += kAll) p.refs[i] = p.refs_in[i];
+  } else {
+    for (int i = run.lo; i < run.hi && rank < asked; ++i)
+      if (p.refs_in[i] == 0) order[rank++] = i;
+  }
+  cluster_sync();  // (and no CTA leaves while another may read its shared words)
+  if (missing) return;
+  for (int r = warp; r < n; r += kAll / 32) {
+    const Writes w(p, r);
+    int32_t* row = p.table + static_cast<int64_t>(r) * p.width_in;
+    int at = s_ask[r];  // the row's next page in `order`
+    for (int j0 = w.lo; j0 < w.hi; j0 += 32) {
+      int id;
+      const bool mine_goes = replaced(w, r, j0 + lane, id);
+      const uint32_t which = __ballot_sync(0xFFFFFFFFu, mine_goes);
+      if (mine_goes) {
+        const int to = __ldcg(order + at + __popc(which & ((1u << lane) - 1u)));
+        row[j0 + lane] = to;
+        p.refs[to] = 1;
+        if (j0 + lane == w.lo && (w.len & (page - 1)))
+          p.moves[1 + 2 * s_copy[r]] = id, p.moves[2 + 2 * s_copy[r]] = to;
+      } else if (id >= 0 && id < p.pages && p.refs_in[id] > 1) {
+        p.refs[id] = 1;  // kept by the first of its rows (no other row's test reads this count)
       }
-      const int r = lo, copy = s_copy[r + 1] - s_copy[r];
-      const int64_t row = static_cast<int64_t>(r) * p.width_in;
-      const int j = rank - s_ask[r];
-      p.refs[i] = 1;
-      if (copy && j == 0) {
-        p.table[row + (p.lens_in[r] >> p.page_shift)] = i;
-        atomicSub(p.refs + s_last[r], 1);
-        p.moves[1 + 2 * s_copy[r]] = s_last[r];
-        p.moves[2 + 2 * s_copy[r]] = i;
-      } else {
-        p.table[row + held_of(p, r) + j - copy] = i;
-      }
-      ++rank;
+      at += __popc(which);
+    }
+    for (int j = w.held + lane; j < w.want; j += 32) {
+      const int to = __ldcg(order + at + j - w.held);
+      row[j] = to;
+      p.refs[to] = 1;
     }
   }
-  cluster_sync();  // no CTA leaves while another may read its shared words
 }
 
 // ------------------------------------------------------------------ compact
@@ -399,8 +435,8 @@ cudaError_t launch_cache_fork(const PageParams& p, cudaStream_t st) { return lau
 
 cudaError_t launch_cache_grow(const PageParams& p, cudaStream_t st) {
   static KernelSetup setup;
-  const size_t smem = (static_cast<size_t>(p.nseq_in) * 3 + 2) * sizeof(int);
-  cudaError_t e = kernel_setup(setup, grow_kernel, kThreads, (static_cast<size_t>(kMaxGrowRows) * 3 + 2) * sizeof(int));
+  const size_t smem = (static_cast<size_t>(p.nseq_in) + 1) * 2 * sizeof(int);
+  cudaError_t e = kernel_setup(setup, grow_kernel, kThreads, (static_cast<size_t>(kMaxGrowRows) + 1) * 2 * sizeof(int));
   if (e != cudaSuccess) return e;
   return launch_cluster(grow_kernel, smem, st, p);
 }
