@@ -92,7 +92,8 @@ class _Calls:
 
 
 def _used_on(stream, *tensors) -> None:
-    """Tensors the caching allocator must not hand out again before `stream` is done with them."""
+    """Tensors the caching allocator must not hand out again before `stream` is done with them: all that a call reads or
+    writes there.  (A stream given by its handle is the caller's to wait for.)"""
     if stream is not None and isinstance(stream, torch.cuda.Stream):
         for t in tensors:
             if t is not None:
@@ -228,7 +229,7 @@ def qk_norm_rope(cache: KvCache, layer: int, batch: TreeBatch, q, k, v, rope: No
     i = cache._index
     hq, hk, hv, ho = _heads(q, i, "q"), _heads(k, i, "k"), _heads(v, i, "v"), _heads(out, i, "out")
     if stream is not None:
-        _used_on(stream, q, k, v, out)
+        _used_on(stream, q, k, v, out, cache.k, cache.v, *batch._keep, *rope._keep)
     _check(_Calls.rope(cache._at, layer, batch._for(cache, q.shape[0]), hq, hk, hv, rope._at, _on(stream, i), ho))
     return out
 
@@ -250,7 +251,7 @@ def tree_attention(cache: KvCache, layer: int, batch: TreeBatch, q, scale: float
                               lse.shape != q.shape[:2]):
         _refuse("lse is a contiguous f32 tensor [rows, heads] on the cache's GPU")
     if stream is not None:
-        _used_on(stream, q, out, lse)
+        _used_on(stream, q, out, lse, cache.k, cache.v, *batch._keep)
     _check(_Calls.attention(cache._at, layer, batch._for(cache, q.shape[0]), hq, cache._scale if scale is None else scale,
                             _on(stream, i), ho, None if lse is None else lse.data_ptr()))
     return out if lse is None else (out, lse)
@@ -275,6 +276,9 @@ class PageState:
         """All pages free, ``nseq`` empty rows."""
         z = (lambda *s: torch.zeros(s, dtype=torch.int32, device=cache.device))
         return cls(z(cache.pages), z(nseq, max_pages) - 1, z(nseq), z(nseq))
+
+    def _tensors(self):
+        return self.refs, self.table, self.held, self.lens
 
     def _like(self, nseq: int | None = None) -> "PageState":
         n = self.raw.nseq if nseq is None else nseq
@@ -307,7 +311,8 @@ def cache_fork(cache: KvCache, state: PageState, parent, out: PageState | None =
     pages of rows nobody names become free."""
     _ints(parent, (None,), "parent", cache.device)
     out = _states(cache, state, out, parent.shape[0])
-    _used_on(stream, parent, out.refs, out.table, out.held, out.lens)
+    if stream is not None:
+        _used_on(stream, parent, *state._tensors(), *out._tensors())
     check(L.lib().exl3_cache_fork(cache.raw, state.raw, parent.data_ptr(), _on(stream, cache._index), out.raw))
     return out
 
@@ -322,7 +327,8 @@ def cache_grow(cache: KvCache, state: PageState, need, out: PageState | None = N
         missing = torch.empty((), dtype=torch.int32, device=cache.device)
     else:
         _ints(missing, (), "missing", cache.device)
-    _used_on(stream, need, missing, out.refs, out.table, out.held, out.lens)
+    if stream is not None:
+        _used_on(stream, need, missing, cache.k, cache.v, *state._tensors(), *out._tensors())
     check(L.lib().exl3_cache_grow(cache.raw, state.raw, need.data_ptr(), _on(stream, cache._index), out.raw,
                                   missing.data_ptr()))
     return out, missing
@@ -340,7 +346,8 @@ def cache_keep(cache: KvCache, batch: TreeBatch, path, kept, out=None, stream=No
         _ints(out, (batch.nseq,), "lens", cache.device)
     if batch.rows is None:
         _refuse("the batch does not know its rows yet: give rows to TreeBatch")
-    _used_on(stream, path, kept, out)
+    if stream is not None:
+        _used_on(stream, path, kept, out, cache.k, cache.v, *batch._keep)
     batch._for(cache, batch.rows)
     check(L.lib().exl3_cache_keep(cache.raw, batch.raw, None if path is None else path.data_ptr(),
                                   0 if path is None else path.shape[1], kept.data_ptr(), _on(stream, cache._index),
@@ -351,6 +358,7 @@ def cache_keep(cache: KvCache, batch: TreeBatch, path, kept, out=None, stream=No
 def cache_compact(cache: KvCache, state: PageState, out: PageState | None = None, stream=None) -> PageState:
     """The live pages moved into the lowest ids, in every layer; tables and reference counts follow."""
     out = _states(cache, state, out)
-    _used_on(stream, out.refs, out.table, out.held, out.lens)
+    if stream is not None:
+        _used_on(stream, cache.k, cache.v, *state._tensors(), *out._tensors())
     check(L.lib().exl3_cache_compact(cache.raw, state.raw, _on(stream, cache._index), out.raw))
     return out
