@@ -100,6 +100,18 @@ def _used_on(stream, *tensors) -> None:
                 t.record_stream(stream)
 
 
+def _made(stream, make, *args, **kw) -> torch.Tensor:
+    """A result that `stream` writes: from that stream's own memory (what the current stream has let go of it may still be
+    using), and kept for the current stream's later use of it."""
+    if stream is None or not isinstance(stream, torch.cuda.Stream):
+        return make(*args, **kw)
+    current = torch.cuda.current_stream(stream.device)
+    with torch.cuda.stream(stream):
+        t = make(*args, **kw)
+    t.record_stream(current)
+    return t
+
+
 class KvCache:
     """The paged cache of every layer: ``k`` and ``v`` [layers, pages, kv_heads, page_size, head_dim], f16 or bf16, of
     any strides (the same for both) with contiguous head vectors -- so also the transposed view of a pool stored
@@ -221,7 +233,7 @@ def qk_norm_rope(cache: KvCache, layer: int, batch: TreeBatch, q, k, v, rope: No
     """q [rows, heads, head_dim] normed and rotated (returned, in ``out`` if given: in q's dtype or the cache's, q
     itself allowed), k and v [rows, kv_heads, head_dim] written to their slots of ``layer``: k normed and rotated, v as it is."""
     if out is None:
-        out = torch.empty_like(q)
+        out = _made(stream, torch.empty_like, q)
     if rope.dim is not None and rope.dim != cache.raw.head_dim:
         _refuse("norm weights are [head_dim]")
     if rope.device is not None and rope.device != cache.device:
@@ -241,10 +253,10 @@ def tree_attention(cache: KvCache, layer: int, batch: TreeBatch, q, scale: float
     [rows, heads] of each row's scores; a tensor receives it."""
     i = cache._index
     if out is None:
-        out = torch.empty_like(q)
+        out = _made(stream, torch.empty_like, q)
     hq, ho = _heads(q, i, "q"), _heads(out, i, "out")
     if lse is True:
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        lse = _made(stream, torch.empty, q.shape[:2], dtype=torch.float32, device=q.device)
     elif lse is False:
         lse = None
     elif lse is not None and (lse.dtype != torch.float32 or lse.device != cache.device or not lse.is_contiguous() or
@@ -280,10 +292,9 @@ class PageState:
     def _tensors(self):
         return self.refs, self.table, self.held, self.lens
 
-    def _like(self, nseq: int | None = None) -> "PageState":
-        n = self.raw.nseq if nseq is None else nseq
+    def _like(self, n: int, stream) -> "PageState":
         pages, width = self.refs.shape[0], self.raw.max_pages
-        flat = torch.empty(pages + n * (width + 2), dtype=torch.int32, device=self.refs.device)
+        flat = _made(stream, torch.empty, pages + n * (width + 2), dtype=torch.int32, device=self.refs.device)
         refs, table, held, lens = flat.split_with_sizes((pages, n * width, n, n))
         new = PageState.__new__(PageState)  # (nothing to check)
         new.refs, new.table, new.held, new.lens = refs, table.view(n, width), held, lens
@@ -293,14 +304,14 @@ class PageState:
         return new
 
 
-def _states(cache: KvCache, state: PageState, out: PageState | None, nseq: int | None = None):
+def _states(cache: KvCache, state: PageState, out: PageState | None, stream, nseq: int | None = None):
     if state.refs.shape[0] != cache.pages or (out is not None and out.refs.shape[0] != cache.pages):
         _refuse("refs counts the cache's pages")
     if state.refs.device != cache.device or (out is not None and out.refs.device != cache.device):
         _refuse("the page state lies on another device than the cache")
     n = state.raw.nseq if nseq is None else nseq
     if out is None:
-        out = state._like(n)
+        out = state._like(n, stream)
     elif out.raw.nseq != n:
         _refuse(f"the new page state has {out.raw.nseq} rows, not {n}")
     return out
@@ -310,7 +321,7 @@ def cache_fork(cache: KvCache, state: PageState, parent, out: PageState | None =
     """Fork, reorder and free: row i of the result is row ``parent[i]`` (int32; -1: an empty row) sharing its pages; the
     pages of rows nobody names become free."""
     _ints(parent, (None,), "parent", cache.device)
-    out = _states(cache, state, out, parent.shape[0])
+    out = _states(cache, state, out, stream, parent.shape[0])
     if stream is not None:
         _used_on(stream, parent, *state._tensors(), *out._tensors())
     check(L.lib().exl3_cache_fork(cache.raw, state.raw, parent.data_ptr(), _on(stream, cache._index), out.raw))
@@ -322,9 +333,9 @@ def cache_grow(cache: KvCache, state: PageState, need, out: PageState | None = N
     ``need[i]`` - 1) replaced by one of its own, with a copy where it holds tokens of the row -> (the new state,
     ``missing``: an int32 scalar tensor, 0, or the pages lacking: then nothing changed)."""
     _ints(need, (state.raw.nseq,), "need", cache.device)
-    out = _states(cache, state, out)
+    out = _states(cache, state, out, stream)
     if missing is None:
-        missing = torch.empty((), dtype=torch.int32, device=cache.device)
+        missing = _made(stream, torch.empty, (), dtype=torch.int32, device=cache.device)
     else:
         _ints(missing, (), "missing", cache.device)
     if stream is not None:
@@ -341,7 +352,7 @@ def cache_keep(cache: KvCache, batch: TreeBatch, path, kept, out=None, stream=No
     _ints(kept, (batch.nseq,), "kept", cache.device)
     _ints(path, (batch.nseq, None), "path", cache.device, optional=True)
     if out is None:
-        out = torch.empty(batch.nseq, dtype=torch.int32, device=cache.device)
+        out = _made(stream, torch.empty, batch.nseq, dtype=torch.int32, device=cache.device)
     else:
         _ints(out, (batch.nseq,), "lens", cache.device)
     if batch.rows is None:
@@ -357,7 +368,7 @@ def cache_keep(cache: KvCache, batch: TreeBatch, path, kept, out=None, stream=No
 
 def cache_compact(cache: KvCache, state: PageState, out: PageState | None = None, stream=None) -> PageState:
     """The live pages moved into the lowest ids, in every layer; tables and reference counts follow."""
-    out = _states(cache, state, out)
+    out = _states(cache, state, out, stream)
     if stream is not None:
         _used_on(stream, cache.k, cache.v, *state._tensors(), *out._tensors())
     check(L.lib().exl3_cache_compact(cache.raw, state.raw, _on(stream, cache._index), out.raw))

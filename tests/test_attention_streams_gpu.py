@@ -65,7 +65,7 @@ def make(A, which):
     flat = (lambda s: (s.refs, s.table, s.held, s.lens, cache.k, cache.v))
     if which == "fork":
         parent = i32([1, 1, 0])
-        return lambda **kw: flat(A.cache_fork(cache, state, parent, **kw)), used + [parent]
+        return lambda **kw: flat(A.cache_fork(cache, state, parent, **kw))[:4], used + [parent]  # (no key or value moves)
     if which == "grow":
         need = i32([40, 33])
         return lambda **kw: flat(A.cache_grow(cache, state, need, **kw)[0]), used + [need, cache.k, cache.v]
@@ -103,3 +103,26 @@ def test_a_call_behind_other_work_outlives_its_arguments(A, which):
     torch.cuda.current_stream().wait_stream(side)
     assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))
     del junk
+
+
+@pytest.mark.parametrize("which", CALLS)
+def test_results_do_not_take_memory_that_the_current_stream_let_go(A, which):
+    """What was dropped on the current stream may still be in use there: a side stream that does not wait must not write
+    to it."""
+    call, used = make(A, which)
+    side = torch.cuda.Stream()
+    warm = call()
+    made = [t for t in warm if all(t.data_ptr() != u.data_ptr() for u in used)]
+    sizes = [(t.untyped_storage().nbytes(), t.untyped_storage().data_ptr()) for t in made]
+    assert sizes
+    torch.cuda.synchronize()
+    let_go = set()
+    freed = [torch.empty(n, dtype=torch.uint8, device="cuda") for n, _ in sizes for _ in range(4)]
+    for t in freed + made:
+        let_go.add(t.untyped_storage().data_ptr())
+    del warm, made, freed, t
+    got = call(stream=side)
+    torch.cuda.current_stream().wait_stream(side)
+    for t in got:
+        if all(t.data_ptr() != u.data_ptr() for u in used):
+            assert t.untyped_storage().data_ptr() not in let_go
