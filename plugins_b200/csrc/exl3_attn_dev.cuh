@@ -38,9 +38,9 @@ __device__ __forceinline__ void item_seq(const AttnParams& p, int s, Item& it) {
   it.row0 = max(0, min(r0, p.b.rows));
   it.ntok = max(0, min(r1, p.b.rows) - it.row0);
   const int64_t room = static_cast<int64_t>(p.b.max_pages) << p.b.page_shift;
-  it.context = max(0, ctx);
-  const int64_t keys = static_cast<int64_t>(it.context) + it.ntok;
+  const int64_t keys = static_cast<int64_t>(max(0, ctx)) + it.ntok;
   it.total_keys = static_cast<int>(min(keys, min(room, static_cast<int64_t>(0x7FFFFFFF))));
+  it.context = max(0, min(ctx, it.total_keys));  // (keys up to here fit 32 bits; context + a row's place need not)
   it.nrows = it.ntok * p.group;
   if ((ctx < 0 || keys > room || r0 < 0 || r1 < r0 || r1 > p.b.rows) && threadIdx.x == 0) atomicOr(p.b.err, kErrBadShape);
 }
@@ -49,7 +49,7 @@ __device__ __forceinline__ int block_keys(const AttnParams& p, const Item& it, i
   if (p.b.tree) return it.total_keys;
   // (rb + 1) rows_per_block is below nrows + a block: under 2^31
   const int last = min(it.ntok - 1, static_cast<int>(((rb + 1u) * rows_per_block - 1u) / static_cast<uint32_t>(p.group)));
-  return min(it.total_keys, it.context + last + 1);
+  return it.context + min(it.total_keys - it.context, last + 1);
 }
 
 // a / b for a >= 0, b > 0: nearly always in 32 bits
@@ -74,7 +74,7 @@ struct WorkLine {
     const int dq = rows_per_block / p.group, dr = rows_per_block % p.group;
     int64_t t = 0;
     for (int rb = 0; rb < nb; ++rb) {
-      t += (min(it.total_keys, it.context + min(it.ntok - 1, q) + 1) + tile_keys - 1) >> tile_shift;
+      t += (it.context + min(it.total_keys - it.context, min(it.ntok - 1, q) + 1) + tile_keys - 1) >> tile_shift;
       q += dq, r += dr;
       if (r >= p.group) ++q, r -= p.group;
     }

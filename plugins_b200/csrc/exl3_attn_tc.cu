@@ -206,8 +206,8 @@ __device__ __forceinline__ Block block_of(const AttnParams& p, const WorkLine& l
   b.qt = b.rows > 128 ? 2 : 1;
   b.events = b.qt * b.tiles;
   // the leading keys that every row sees
-  const int all = p.b.tree ? it.context : it.context + it.row_block * S::kRows / p.group + 1;
-  b.full_keys = min(all, it.total_keys);
+  const int own = p.b.tree ? 0 : it.row_block * S::kRows / p.group + 1;
+  b.full_keys = it.context + min(own, it.total_keys - it.context);
   return b;
 }
 

@@ -208,8 +208,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) norm_rope_kernel(const N
       continue;
     }
     const int s = seq_of_row(p.b.row_start, p.b.nseq, row, lane);
-    const int at = p.b.context[s] + row - p.b.row_start[s];
-    const int pg = at >> p.b.page_shift;
+    const int64_t at = static_cast<int64_t>(p.b.context[s]) + row - p.b.row_start[s];
+    const int64_t pg = at >> p.b.page_shift;
     int id = -1;
     if (at >= 0 && pg < p.b.max_pages) id = p.b.table[static_cast<int64_t>(s) * p.b.max_pages + pg];
     const bool ok = id >= 0 && id < p.b.pages;
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) norm_rope_kernel(const N
       if (!ok) atomicOr(p.b.err, kErrBadShape);
       s_slot[i] = ok ? id * p.b.page_stride + (at & ((1 << p.b.page_shift) - 1)) * p.b.token_stride : kOutside;
     }
-    const double pos = p.b.position ? p.b.position[row] : at;
+    const double pos = p.b.position ? p.b.position[row] : static_cast<double>(at);
     for (int f = static_cast<int>(lane); f < half; f += 32) {
       double t = pos * p.inv_freq[f] * kInvTwoPi;
       t -= rint(t);

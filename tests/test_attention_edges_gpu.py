@@ -1,0 +1,81 @@
+"""The attention side's kernels where their arithmetic is at its limits (plugins_b200/attention.py)."""
+import math
+
+import pytest
+import torch
+
+import attention_ref as R
+from plugins_b200 import _lib as L
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}  # half an ulp, relative
+
+
+@pytest.fixture()
+def A():
+    from plugins_b200 import attention
+    from plugins_b200 import quant as Q
+    Q.device_error(0, clear=True)
+    yield attention
+    assert Q.device_error(0, clear=True) == 0
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32).cuda()
+
+
+def close(out, lse, want, wlse, mass, dtype):
+    """One rounding of the result and one of the probabilities, relative to what they weigh; scores and sums in f32 (the
+    scores here stay below 2^5, their sums' errors below 2^-13)."""
+    tol = U[dtype] * want.abs() + (U[dtype] + 2.0 ** -13) * mass + 2.0 ** -25
+    err = (out.cpu().double() - want).abs()
+    assert bool((err <= tol).all()), f"worst {float((err / tol).max()):.2f} x the tolerance"
+    assert bool(((lse.cpu().double() - wlse).abs() <= 2.0 ** -13 + 2.0 ** -21 * wlse.abs()).all())
+
+
+@pytest.mark.parametrize("context", [2 ** 31 - 1, 2 ** 31 - 40, 1 << 30, 97])
+@pytest.mark.parametrize("rows", [2, 24, 90])
+@pytest.mark.parametrize("tree", [False, True])
+def test_a_context_past_the_table_harms_no_other_sequence(A, context, rows, tree):
+    """Contexts whose sums with a row's place pass 32 bits (and one slot too many): recorded, nothing of the sequence is
+    written, the sequences beside it are right."""
+    from plugins_b200 import quant as Q
+    g = torch.Generator().manual_seed(rows)
+    page, dim, dtype = 16, 128, torch.bfloat16
+    k, v = (torch.randn((1, 30, 2, page, dim), generator=g).to(dtype) for _ in range(2))
+    ids = torch.randperm(30, generator=g).int()
+    table = torch.full((3, 12), -1, dtype=torch.int32)
+    table[0, :12], table[1, :6], table[2, :12] = ids[:12], ids[12:18], ids[18:30]
+    lens = [70, context, 100]
+    if context == 97:  # the last new row of sequence 1 does not fit its table's six pages, and the seventh is -1
+        lens[1] = 6 * page - rows + 1
+    start = [0, rows, 2 * rows, 3 * rows]
+    bits = None
+    if tree:  # a chain
+        seen = [[((2 << i) - 1) >> (32 * w) & 0xFFFFFFFF for w in range(3)] for i in range(rows)]
+        bits = torch.tensor([[w - (1 << 32) if w >> 31 else w for w in row] for row in seen], dtype=torch.int32).repeat(3, 1)
+    cache = A.KvCache(k.cuda(), v.cuda())
+    batch = A.TreeBatch(i32(start), i32(lens), table.cuda(), max_rows=rows, rows=3 * rows,
+                        tree=None if bits is None else bits.cuda())
+    q = torch.randn((3 * rows, 8, dim), generator=g).to(dtype)
+    out, lse = A.tree_attention(cache, 0, batch, q.cuda(), lse=True)
+    assert Q.device_error(0, clear=True) == L.ERR_BAD_SHAPE
+    for s in (0, 2):
+        a, b = start[s], start[s + 1]
+        want = R.attention(k[0], v[0], q[a:b], [0, rows], [lens[s]], table[s:s + 1], dim ** -0.5,
+                           None if bits is None else bits[a:b])
+        close(out[a:b], lse[a:b], *want, dtype)
+    x = torch.randn((3 * rows, 4, dim), generator=g).to(dtype).cuda()
+    A.qk_norm_rope(cache, 0, batch, x[:, :2], x[:, :2], x[:, 2:], A.NormRope(None))
+    assert Q.device_error(0, clear=True) == L.ERR_BAD_SHAPE
+    for s in (0, 2):
+        pg, of = R.slots(table[s], page, lens[s], lens[s] + rows)
+        k[0, pg, :, of], v[0, pg, :, of] = x[start[s]:start[s + 1], :2].cpu(), x[start[s]:start[s + 1], 2:].cpu()
+    if context == 97:  # those of its rows that have a slot
+        pg, of = R.slots(table[1], page, lens[1], 6 * page)
+        k[0, pg, :, of], v[0, pg, :, of] = x[rows:2 * rows - 1, :2].cpu(), x[rows:2 * rows - 1, 2:].cpu()
+    assert torch.equal(cache.k.cpu(), k) and torch.equal(cache.v.cpu(), v)
+    lens2 = A.cache_keep(cache, batch, None, i32([1, 1, 1]))
+    if context != 97:
+        assert Q.device_error(0, clear=True) == L.ERR_BAD_SHAPE and lens2.tolist() == [71, context, 101]
