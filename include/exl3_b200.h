@@ -479,7 +479,8 @@ uint64_t exl3_resident_pending(void);
  * drafted tokens or of a prompt chunk over it, and the bookkeeping of its pages.  The calls follow the conventions at
  * the top of this file: they enqueue on `stream`, allocate nothing and do not synchronise; arrays named "device" are
  * read by the kernels when the call's work runs.  A device value out of range (a page id, a context, a path) is never
- * followed: the access is skipped and EXL3_ERR_BAD_SHAPE recorded. */
+ * followed: the access is skipped (attention takes a missing page's keys and values as zeros) and EXL3_ERR_BAD_SHAPE
+ * recorded. */
 
 /* The paged cache of every layer.  Token slot `t` of page `p` of kv head `h` of layer `l` is the head_dim contiguous
  * elements at k (v) + l * layer_stride + p * page_stride + h * head_stride + t * token_stride (elements; the same

@@ -754,7 +754,7 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
           id = tab[key >> p.b.page_shift];
           if (id < 0 || id >= p.b.pages) {
             atomicOr(p.b.err, kErrBadShape);
-            id = -1;
+            id = p.b.pages;  // past the map: the box arrives as zeros, as in the few-row kernel
           }
         }
         const uint32_t loads = __popc(__ballot_sync(0xFFFFFFFFu, id >= 0));

@@ -79,3 +79,33 @@ def test_a_context_past_the_table_harms_no_other_sequence(A, context, rows, tree
     lens2 = A.cache_keep(cache, batch, None, i32([1, 1, 1]))
     if context != 97:
         assert Q.device_error(0, clear=True) == L.ERR_BAD_SHAPE and lens2.tolist() == [71, context, 101]
+
+
+@pytest.mark.parametrize("rows,dim,page", [(2, 128, 16), (40, 128, 16), (90, 128, 64), (24, 64, 32), (40, 256, 16), (24, 256, 128)])
+@pytest.mark.parametrize("bad", [-1, 10 ** 6])
+def test_a_page_that_is_not_there_reads_as_zeros(A, rows, dim, page, bad):
+    """A page id out of range is recorded; its slots count as zero keys and values, whatever the kernel, and nothing that an
+    earlier launch or another sequence left on the chip shows."""
+    from plugins_b200 import quant as Q
+    g = torch.Generator().manual_seed(rows + dim)
+    dtype, ctx = torch.float16, 1000
+    held = -(-(ctx + rows) // page)
+    k, v = (torch.randn((1, held + 1, 2, page, dim), generator=g).to(dtype) for _ in range(2))
+    k[0, held], v[0, held] = 0, 0  # what the missing pages read as
+    table = torch.randperm(held, generator=g).int()[None]
+    lost = [held // 3, held // 2] if held > 8 else [held // 2]
+    cache = A.KvCache(k.cuda(), v.cuda())
+    q = torch.randn((rows, 8, dim), generator=g).to(dtype)
+
+    def run(t):
+        batch = A.TreeBatch(i32([0, rows]), i32([ctx]), t.cuda(), max_rows=rows, rows=rows)
+        return A.tree_attention(cache, 0, batch, q.cuda(), lse=True)
+
+    run(table)  # (leaves other keys behind)
+    assert Q.device_error(0, clear=True) == 0
+    holes = table.clone()
+    holes[0, lost] = bad
+    out, lse = run(holes)
+    assert Q.device_error(0, clear=True) == L.ERR_BAD_SHAPE
+    holes[0, lost] = held
+    close(out, lse, *R.attention(k[0], v[0], q, [0, rows], [ctx], holes, dim ** -0.5), dtype)
