@@ -18,6 +18,16 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x
 
 constexpr float kLn2 = 0.6931471805599453f;
 
+// The probabilities e^(s - m) are rounded to the element type for the product with V.  f16 has full precision down to 2^-14
+// only, and thousands of keys that far below the largest can weigh as much as it does: f16's are held 2^kLift higher, which
+// leaves 2^kSlack below its largest value for a running maximum that is behind (the many-row kernel's rescales O only when
+// the maximum has grown by more than that).  bf16 has f32's range.  Both kernels subtract kLift from m at an item's end:
+// l and o then refer to it.
+template <bool BF16>
+constexpr float kSlack = BF16 ? 8.f : 4.f;
+template <bool BF16>
+constexpr float kLift = BF16 ? 0.f : 11.f;
+
 // ------------------------------------------------------------------ the work
 
 // A row block of one sequence and kv head.  Its rows are (new token t, query head g) pairs, row = t * group + g.

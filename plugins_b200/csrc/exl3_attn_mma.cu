@@ -186,8 +186,9 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const AttnParams p) 
             mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
             mx = fmaxf(mx, m[i][hh]);
-            const float base = mx == -INFINITY ? 0.f : mx;  // nothing seen so far: every term below is 0
-            const float f = ex2(m[i][hh] - base);
+            const float top = mx == -INFINITY ? 0.f : mx;  // nothing seen so far: every term below is 0
+            const float base = top - kLift<BF16>;
+            const float f = ex2(m[i][hh] - top);
             m[i][hh] = mx;
             float sum = 0.f;
 #pragma unroll
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const AttnParams p) 
             l[i][hh] = l[i][hh] * f + sum;
 #pragma unroll
             for (int j = 0; j < D / 8; ++j) o[i][j][2 * hh] *= f, o[i][j][2 * hh + 1] *= f;
-            // e^(s - m) <= 1, rounded to the element type for the product with V (l keeps the f32 values)
+            // 2^kLift e^(s - m), rounded to the element type for the product with V (l keeps the f32 values)
             pa[i][hh] = pack2<BF16>(x[0], x[1]);
             pa[i][2 + hh] = pack2<BF16>(x[2], x[3]);
           }
@@ -257,7 +258,7 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const AttnParams p) 
         sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
         sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
         const uint32_t r = 16u * i + 8u * hh + g;
-        if (q4 == 0) s_ml[r * kWarps + warp] = make_float2(m[i][hh], sum);
+        if (q4 == 0) s_ml[r * kWarps + warp] = make_float2(m[i][hh] - kLift<BF16>, sum);
 #pragma unroll
         for (int j = 0; j < D / 8; ++j)
           *reinterpret_cast<float2*>(s_o + (warp * S::kRows + r) * D + j * 8 + q4 * 2) =

@@ -14,8 +14,9 @@
 //
 // Roles: NG groups of four softmax warps (a thread per row: tcgen05.ld of its scores, maximum, exponentials, P back by
 // tcgen05.st), then one warp each for the MMAs, K copies, V copies (TMA, one box per page and 64 columns, 128-byte
-// swizzle) and the V tiles' cleaning.  O is rescaled only when a row's maximum has grown by more than 2^8 (P then stays
-// below 2^8, and the f32 sums and the final division take out the difference); the old maximum is kept otherwise.
+// swizzle) and the V tiles' cleaning.  O is rescaled only when a row's maximum has grown by more than a factor (2^8; 2^4
+// for f16, whose probabilities have less room); the old maximum is kept otherwise, and the f32 sums and the final division
+// take out the difference.
 //
 // Keys that some row of the block does not see (stale slots, other branches) are masked in S by index; their V rows
 // cannot be masked there (0 x inf = NaN), so in the tiles that hold such keys the cleaning warp zeroes slots past the
@@ -518,7 +519,7 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
           }
         }
         const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale_log2;
-        const bool grow = top > m + 8.f;  // (m = -inf: as soon as anything is seen)
+        const bool grow = top > m + kSlack<BF16>;  // (m = -inf: as soon as anything is seen)
         if (e < NG) {
           m = top;
         } else if (__any_sync(0xFFFFFFFFu, grow)) {
@@ -538,7 +539,7 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
           }
           tmem_wait_st();
         }
-        const float base = m == -INFINITY ? 0.f : m;
+        const float base = (m == -INFINITY ? 0.f : m) - kLift<BF16>;
         const uint64_t scale2 = f2(p.scale_log2, p.scale_log2), base2 = f2(-base, -base);
         uint64_t sum[2] = {0, 0};
 #pragma unroll
@@ -565,6 +566,7 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
       }
 
       // ---- the block's end: o / l, or a partial for the join
+      m -= kLift<BF16>;
       const bool whole = b.tiles == it.tiles;
       const bool two = b.qt == 1 && NG == 2;  // two key halves of the same rows
       const int mine = two ? (b.events > static_cast<int>(g) ? 1 : 0) : 1;  // this group had a tile

@@ -109,3 +109,26 @@ def test_a_page_that_is_not_there_reads_as_zeros(A, rows, dim, page, bad):
     assert Q.device_error(0, clear=True) == L.ERR_BAD_SHAPE
     holes[0, lost] = held
     close(out, lse, *R.attention(k[0], v[0], q, [0, rows], [ctx], holes, dim ** -0.5), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,dim", [(1, 64), (24, 64), (40, 128), (20, 256)])
+def test_many_small_probabilities_beside_a_large_one(A, dtype, rows, dim):
+    """2^18 keys of some 2^-23.4 of the first one's probability each, which is below f16's full precision (and its smallest
+    numbers): together they are the whole result, since the first key's value is zero.  Enough sequences over the same
+    pages that a CTA's part of the keys is long."""
+    page, keys, nseq = 256, 1 << 18, 300 if rows == 1 else 40
+    dev = dict(dtype=dtype, device="cuda")
+    k, v = (torch.zeros((1, keys // page + 1, 1, page, dim), **dev) for _ in range(2))
+    v[:] = torch.linspace(0.5, 1.5, dim, **dev)
+    c = 23.4 * math.log(2) / math.sqrt(dim)
+    k[0, 0, 0, 0], v[0, 0, 0, 0] = c, 0
+    table = torch.arange(keys // page + 1, dtype=torch.int32)[None].expand(nseq, -1).contiguous().cuda()
+    start = [rows * s for s in range(nseq + 1)]
+    batch = A.TreeBatch(i32(start), i32([keys - 1] * nseq), table, max_rows=rows, rows=start[-1])
+    q = torch.ones((start[-1], 1, dim), **dev)
+    out, lse = A.tree_attention(A.KvCache(k, v), 0, batch, q, lse=True)
+    first = math.exp(float(k[0, 0, 0, 0].double().sum()) / math.sqrt(dim))
+    rest = torch.tensor([keys - 1 + i for i in range(rows)], dtype=torch.float64).repeat(nseq)[:, None]
+    want = (rest / (first + rest))[:, :, None] * v[0, 1, 0, 0].double().cpu()
+    close(out, lse, want, torch.log(first + rest), want, dtype)
