@@ -584,7 +584,8 @@ exl3_verdict exl3_cache_fork(const exl3_kv_cache *cache, const exl3_page_state *
  * drafts, are shared by a fork like the others) -- except that when all its sharers write it, the first of them keeps it.
  * Pages are given lowest id first, rows in order, a row's replaced pages (in table order) before its new ones.  Rows never
  * shrink; lens stay.  missing[0] (device) receives 0, or, when the free pages or the table's width do not suffice, how
- * many pages are lacking, and then `out` is `in` unchanged and nothing is copied.  out's arrays are not in's. */
+ * many pages are lacking (at most 2^31 - 1), and then `out` is `in` unchanged and nothing is copied.  At most 4096 rows.
+ * out's arrays are not in's. */
 exl3_verdict exl3_cache_grow(const exl3_kv_cache *cache, const exl3_page_state *in, const int32_t *need, void *stream,
                              const exl3_page_state *out, int32_t *missing);
 

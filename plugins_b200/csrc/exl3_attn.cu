@@ -267,7 +267,7 @@ exl3_verdict exl3_cache_grow(const exl3_kv_cache* cache, const exl3_page_state* 
   if (in->nseq != out->nseq) return refuse(EXL3_FAILED, "exl3_b200: grow keeps the rows");
   if (in->nseq > exl3::cache_grow_max_rows()) return refuse(EXL3_TOO_LARGE, "exl3_b200: grow takes at most 4096 rows");
   if (!missing || (!need && in->nseq > 0)) return refuse(EXL3_FAILED, "exl3_b200: grow without its arrays");
-  if (ws.partial_floats < static_cast<size_t>(in->nseq) * 4 + static_cast<size_t>(cache->pages) * 2 + 1)
+  if (ws.partial_floats < static_cast<size_t>(in->nseq) * 5 + static_cast<size_t>(cache->pages) * 2 + 1)
     return refuse(EXL3_TOO_LARGE, "exl3_b200: too many pages for the workspace");
   p.need = need, p.missing = missing;
   p.scratch = p.moves + 1 + 2 * in->nseq;

@@ -79,7 +79,7 @@ struct PageParams {
   const int32_t *parent, *need;
   int32_t* missing;
   int32_t* moves;    // [1 + 2 * capacity]: count, then (source, destination) pages
-  int32_t* scratch;  // grow: [2 * nseq + 2 * pages]
+  int32_t* scratch;  // grow: [3 * nseq + 2 * pages]
   uint32_t* err;
 };
 struct PagePool {

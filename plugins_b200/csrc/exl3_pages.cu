@@ -101,16 +101,27 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) for
 
 // The table places whose pages row r writes: those of the slots len .. need - 1, as far as it holds them.
 struct Writes {
-  int lo, hi;    // [lo, hi)
+  int lo = 0, hi = 0;   // [lo, hi)
   int len, held, want;  // the row's tokens and pages, the pages it needs (at most the table's width)
-  int over;      // pages it needs past that
-  __device__ __forceinline__ Writes(const PageParams& p, int r) {
+  int over;             // pages it needs past that
+  int id;               // the page at place lo + lane, or -1
+  bool shared;          // it has several references
+  Writes() = default;
+  __device__ __forceinline__ Writes(const PageParams& p, int r, int lane) {
     const int page = 1 << p.page_shift, need = max(p.need[r], 0);
     len = p.lens_in[r], held = held_of(p, r);
     const int all = static_cast<int>((static_cast<int64_t>(need) + page - 1) >> p.page_shift);
     want = min(all, p.width_in), over = all - want;
-    lo = hi = 0;
     if (need > len && len >= 0) lo = min(len >> p.page_shift, held), hi = max(lo, min(want, held));
+    place(p, r, lo + lane);
+  }
+  __device__ __forceinline__ void place(const PageParams& p, int r, int j) {
+    id = j < hi ? p.table_in[static_cast<int64_t>(r) * p.width_in + j] : -1;
+    if (j < hi && (id < 0 || id >= p.pages)) {
+      atomicOr(p.err, kErrBadShape);
+      id = -1;
+    }
+    shared = id >= 0 && p.refs_in[id] > 1;
   }
 };
 
@@ -119,7 +130,7 @@ struct Writes {
 // when it was forked.  When every reference is a row's that writes the page, the first of these rows keeps it.
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) grow_kernel(const PageParams p) {
   extern __shared__ int s_row[];  // [nseq + 1] asks before the row, copies before the row
-  __shared__ int s_warp[32], s_total, s_over;
+  __shared__ int s_warp[32], s_total;
   int* s_ask = s_row;
   int* s_copy = s_row + p.nseq_in + 1;
   pdl_wait();
@@ -127,10 +138,31 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) gro
   const int t = static_cast<int>(blockIdx.x) * kThreads + tid;
   const int lane = t & 31, warp = t >> 5;
   const int n = p.nseq_in, page = 1 << p.page_shift;
-  int* asks = p.scratch;       // [nseq] pages each row asks for
-  int* copies = asks + n;      // [nseq] of them, copies
-  int* first = copies + n;     // [pages] of a shared page, the first row that writes it
+  int* asks = p.scratch;         // [nseq] pages each row asks for
+  int* copies = asks + n;        // [nseq] of them, copies
+  int* overs = copies + n;       // [nseq] pages past the table's width
+  int* first = overs + n;        // [pages] of a shared page, the first row that writes it
   int* order = first + p.pages;  // [pages] the free pages in the order they are given
+  // a warp takes every 256th row; the first one's places are read once, under the copies
+  Writes own;
+  if (warp < n) own = Writes(p, warp, lane);
+  auto each_row = [&](auto&& f) {
+    for (int r = warp; r < n; r += kAll / 32) {
+      if (r == warp) {
+        f(r, own);
+      } else {
+        Writes w(p, r, lane);
+        f(r, w);
+      }
+    }
+  };
+  // f(its place, its 32 places begin at j0) for every place of the row, by lanes
+  auto each_place = [&](int r, Writes w, auto&& f) {
+    for (int j0 = w.lo; j0 < w.hi; j0 += 32) {
+      if (j0 > w.lo) w.place(p, r, j0 + lane);
+      f(w, j0);
+    }
+  };
   // counts and tables as they are, and the free pages ranked
   for (int i = t; i < p.pages; i += kAll) {
     const int refs = p.refs_in[i];
@@ -138,67 +170,52 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) gro
     if (refs > 1) first[i] = n;
   }
   for (int64_t i = t; i < static_cast<int64_t>(n) * p.width_in; i += kAll) p.table[i] = p.table_in[i];
-  if (tid == 0) s_over = 0;
   const PageRun run(p.pages);
   int mine = 0, free_pages;
   for (int i = run.lo; i < run.hi; ++i) mine += p.refs_in[i] == 0 ? 1 : 0;
   int rank = cluster_scan_excl(mine, s_warp, &s_total, &free_pages);  // (its barrier: the copies above are in place)
   // a shared page loses the references of the rows that write it (whole numbers: any order)
-  for (int r = warp; r < n; r += kAll / 32) {
-    const Writes w(p, r);
-    for (int j = w.lo + lane; j < w.hi; j += 32) {
-      const int id = p.table_in[static_cast<int64_t>(r) * p.width_in + j];
-      if (id < 0 || id >= p.pages) {
-        atomicOr(p.err, kErrBadShape);
-      } else if (p.refs_in[id] > 1) {
-        atomicSub(p.refs + id, 1);
-        atomicMin(first + id, r);
-      }
-    }
-  }
+  each_row([&](int r, const Writes& w) {
+    each_place(r, w, [&](const Writes& at, int) {
+      if (at.shared) atomicSub(p.refs + at.id, 1), atomicMin(first + at.id, r);
+    });
+  });
   cluster_sync();
-  auto replaced = [&](const Writes& w, int r, int j, int& id) {
-    id = j < w.hi ? p.table_in[static_cast<int64_t>(r) * p.width_in + j] : -1;
-    if (id < 0 || id >= p.pages || p.refs_in[id] <= 1) return false;
-    return __ldcg(first + id) != r || __ldcg(p.refs + id) > 0;
+  auto replaced = [&](int r, const Writes& at) {
+    return at.shared && (__ldcg(first + at.id) != r || __ldcg(p.refs + at.id) > 0);
   };
-  for (int r = warp; r < n; r += kAll / 32) {
-    const Writes w(p, r);
+  each_row([&](int r, const Writes& w) {
     int ask = max(0, w.want - w.held), copy = 0;
-    for (int j0 = w.lo; j0 < w.hi; j0 += 32) {
-      int id;
-      const uint32_t which = __ballot_sync(0xFFFFFFFFu, replaced(w, r, j0 + lane, id));
+    each_place(r, w, [&](const Writes& at, int j0) {
+      const uint32_t which = __ballot_sync(0xFFFFFFFFu, replaced(r, at));
       ask += __popc(which);
       if (j0 == w.lo && (w.len & (page - 1))) copy = which & 1u;
-    }
-    if (lane == 0) asks[r] = ask, copies[r] = copy;
-  }
+    });
+    if (lane == 0) asks[r] = ask, copies[r] = copy, overs[r] = w.over, p.lens[r] = w.len;
+  });
   cluster_sync();
-  int asked = 0, copied = 0;  // every CTA: rows are scanned in runs of kThreads
+  int asked = 0, copied = 0, over = 0;  // every CTA: rows are scanned in runs of kThreads
   for (int base = 0; base < n; base += kThreads) {
     const int r = base + tid;
-    if (r < n) {
-      const int over = Writes(p, r).over;
-      if (over) atomicAdd(&s_over, over);
-    }
     int total;
-    const int a = cta_scan_excl(r < n ? __ldcg(asks + r) : 0, s_warp, &total);
+    const int row_asks = r < n ? __ldcg(asks + r) : 0, row_copies = r < n ? __ldcg(copies + r) : 0;
+    over |= r < n ? __ldcg(overs + r) : 0;
+    const int a = cta_scan_excl(row_asks, s_warp, &total);
     if (r < n) s_ask[r] = asked + a;
     asked += total;
-    const int c = cta_scan_excl(r < n ? __ldcg(copies + r) : 0, s_warp, &total);
+    const int c = cta_scan_excl(row_copies, s_warp, &total);
     if (r < n) s_copy[r] = copied + c;
     copied += total;
   }
-  __syncthreads();
-  const int missing = max(0, asked - free_pages) + s_over;
+  int missing = max(0, asked - free_pages);
+  if (__syncthreads_or(over)) {  // (rare) the pages past the width, held below 2^31
+    int64_t sum = missing;
+    for (int r = 0; r < n; ++r) sum += __ldcg(overs + r);
+    missing = static_cast<int>(min(sum, static_cast<int64_t>(0x7FFFFFFF)));
+  }
   if (t == 0) {
     p.missing[0] = missing;
     p.moves[0] = missing ? 0 : copied;
-  }
-  for (int r = t; r < n; r += kAll) {
-    const Writes w(p, r);
-    p.held[r] = missing ? w.held : max(w.held, w.want);
-    p.lens[r] = w.len;
   }
   if (missing) {
     for (int i = t; i < p.pages; i += kAll) p.refs[i] = p.refs_in[i];
@@ -207,32 +224,31 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) gro
       if (p.refs_in[i] == 0) order[rank++] = i;
   }
   cluster_sync();  // (and no CTA leaves while another may read its shared words)
-  if (missing) return;
-  for (int r = warp; r < n; r += kAll / 32) {
-    const Writes w(p, r);
+  each_row([&](int r, const Writes& w) {
+    if (lane == 0) p.held[r] = missing ? w.held : max(w.held, w.want);
+    if (missing) return;
     int32_t* row = p.table + static_cast<int64_t>(r) * p.width_in;
-    int at = s_ask[r];  // the row's next page in `order`
-    for (int j0 = w.lo; j0 < w.hi; j0 += 32) {
-      int id;
-      const bool mine_goes = replaced(w, r, j0 + lane, id);
-      const uint32_t which = __ballot_sync(0xFFFFFFFFu, mine_goes);
-      if (mine_goes) {
-        const int to = __ldcg(order + at + __popc(which & ((1u << lane) - 1u)));
+    int next = s_ask[r];  // the row's next page in `order`
+    each_place(r, w, [&](const Writes& at, int j0) {
+      const bool goes = replaced(r, at);
+      const uint32_t which = __ballot_sync(0xFFFFFFFFu, goes);
+      if (goes) {
+        const int to = __ldcg(order + next + __popc(which & ((1u << lane) - 1u)));
         row[j0 + lane] = to;
         p.refs[to] = 1;
         if (j0 + lane == w.lo && (w.len & (page - 1)))
-          p.moves[1 + 2 * s_copy[r]] = id, p.moves[2 + 2 * s_copy[r]] = to;
-      } else if (id >= 0 && id < p.pages && p.refs_in[id] > 1) {
-        p.refs[id] = 1;  // kept by the first of its rows (no other row's test reads this count)
+          p.moves[1 + 2 * s_copy[r]] = at.id, p.moves[2 + 2 * s_copy[r]] = to;
+      } else if (at.shared) {
+        p.refs[at.id] = 1;  // kept by the first of its rows (no other row's test reads this count)
       }
-      at += __popc(which);
-    }
+      next += __popc(which);
+    });
     for (int j = w.held + lane; j < w.want; j += 32) {
-      const int to = __ldcg(order + at + j - w.held);
+      const int to = __ldcg(order + next + j - w.held);
       row[j] = to;
       p.refs[to] = 1;
     }
-  }
+  });
 }
 
 // ------------------------------------------------------------------ compact

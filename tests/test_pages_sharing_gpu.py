@@ -251,3 +251,16 @@ def test_a_forked_pair_that_diverges_decodes_as_unshared_rows_do(prompt, page):
     for a, b in zip(keep, keep2):
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     assert Q.device_error(0, clear=True) == 0
+
+
+@pytest.mark.parametrize("nseq", [0, 1, 40, 4096])
+def test_grow_asked_for_more_than_can_be_counted(A, nseq):
+    """No rows; and rows that together lack more pages than 32 bits hold: all of them said, nothing changed."""
+    cache = A.KvCache(*(torch.zeros((1, 8, 1, 16, 64), dtype=torch.float16, device="cuda") for _ in range(2)))
+    refs, table = [1] + [0] * 7, [[0]] + [[]] * (nseq - 1) if nseq else []
+    state = on_gpu(A, refs if nseq else [0] * 8, table, [3] + [0] * (nseq - 1) if nseq else [], 4)
+    out, missing = A.cache_grow(cache, state, i32([2 ** 31 - 1] * nseq).view(nseq))
+    asked = nseq * (2 ** 27 - 4) + max(0, 4 * nseq - (1 if nseq else 0) - (7 if nseq else 8))
+    assert int(missing) == min(asked, 2 ** 31 - 1)
+    assert out.refs.tolist() == state.refs.tolist() and out.table.tolist() == state.table.tolist()
+    assert out.held.tolist() == state.held.tolist() and out.lens.tolist() == state.lens.tolist()
