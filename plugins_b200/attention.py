@@ -14,6 +14,7 @@ torch stream or ``stream``; refusals raise :class:`Exl3Error`.
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 
 import torch
@@ -100,16 +101,18 @@ def _used_on(stream, *tensors) -> None:
                 t.record_stream(stream)
 
 
-def _made(stream, make, *args, **kw) -> torch.Tensor:
-    """A result that `stream` writes: from that stream's own memory (what the current stream has let go of it may still be
-    using), and kept for the current stream's later use of it."""
-    if stream is None or not isinstance(stream, torch.cuda.Stream):
-        return make(*args, **kw)
+def _made_on(stream, make, *args, **kw) -> torch.Tensor:
     current = torch.cuda.current_stream(stream.device)
     with torch.cuda.stream(stream):
         t = make(*args, **kw)
     t.record_stream(current)
     return t
+
+
+def _maker(stream, make):
+    """`make` for a result that `stream` writes: from that stream's own memory (what the current stream has let go of it may
+    still be using), and kept for the current stream's later use of it."""
+    return functools.partial(_made_on, stream, make) if isinstance(stream, torch.cuda.Stream) else make
 
 
 class KvCache:
@@ -233,7 +236,7 @@ def qk_norm_rope(cache: KvCache, layer: int, batch: TreeBatch, q, k, v, rope: No
     """q [rows, heads, head_dim] normed and rotated (returned, in ``out`` if given: in q's dtype or the cache's, q
     itself allowed), k and v [rows, kv_heads, head_dim] written to their slots of ``layer``: k normed and rotated, v as it is."""
     if out is None:
-        out = _made(stream, torch.empty_like, q)
+        out = _maker(stream, torch.empty_like)(q)
     if rope.dim is not None and rope.dim != cache.raw.head_dim:
         _refuse("norm weights are [head_dim]")
     if rope.device is not None and rope.device != cache.device:
@@ -253,10 +256,10 @@ def tree_attention(cache: KvCache, layer: int, batch: TreeBatch, q, scale: float
     [rows, heads] of each row's scores; a tensor receives it."""
     i = cache._index
     if out is None:
-        out = _made(stream, torch.empty_like, q)
+        out = _maker(stream, torch.empty_like)(q)
     hq, ho = _heads(q, i, "q"), _heads(out, i, "out")
     if lse is True:
-        lse = _made(stream, torch.empty, q.shape[:2], dtype=torch.float32, device=q.device)
+        lse = _maker(stream, torch.empty)(q.shape[:2], dtype=torch.float32, device=q.device)
     elif lse is False:
         lse = None
     elif lse is not None and (lse.dtype != torch.float32 or lse.device != cache.device or not lse.is_contiguous() or
@@ -294,7 +297,7 @@ class PageState:
 
     def _like(self, n: int, stream) -> "PageState":
         pages, width = self.refs.shape[0], self.raw.max_pages
-        flat = _made(stream, torch.empty, pages + n * (width + 2), dtype=torch.int32, device=self.refs.device)
+        flat = _maker(stream, torch.empty)(pages + n * (width + 2), dtype=torch.int32, device=self.refs.device)
         refs, table, held, lens = flat.split_with_sizes((pages, n * width, n, n))
         new = PageState.__new__(PageState)  # (nothing to check)
         new.refs, new.table, new.held, new.lens = refs, table.view(n, width), held, lens
@@ -335,7 +338,7 @@ def cache_grow(cache: KvCache, state: PageState, need, out: PageState | None = N
     _ints(need, (state.raw.nseq,), "need", cache.device)
     out = _states(cache, state, out, stream)
     if missing is None:
-        missing = _made(stream, torch.empty, (), dtype=torch.int32, device=cache.device)
+        missing = _maker(stream, torch.empty)((), dtype=torch.int32, device=cache.device)
     else:
         _ints(missing, (), "missing", cache.device)
     if stream is not None:
@@ -352,7 +355,7 @@ def cache_keep(cache: KvCache, batch: TreeBatch, path, kept, out=None, stream=No
     _ints(kept, (batch.nseq,), "kept", cache.device)
     _ints(path, (batch.nseq, None), "path", cache.device, optional=True)
     if out is None:
-        out = _made(stream, torch.empty, batch.nseq, dtype=torch.int32, device=cache.device)
+        out = _maker(stream, torch.empty)(batch.nseq, dtype=torch.int32, device=cache.device)
     else:
         _ints(out, (batch.nseq,), "lens", cache.device)
     if batch.rows is None:
