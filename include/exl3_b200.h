@@ -477,10 +477,10 @@ uint64_t exl3_resident_pending(void);
  * Between a layer's q|k|v linears and its o linear (no counterpart in the reference's EXL3 path, whose host keeps its
  * own attention): a paged key/value cache, the norms and rotation that fill it, attention of one token, of a tree of
  * drafted tokens or of a prompt chunk over it, and the bookkeeping of its pages.  The calls follow the conventions at
- * the top of this file: they enqueue on `stream`, allocate nothing and do not synchronise; arrays named "device" are
- * read by the kernels when the call's work runs.  A device value out of range (a page id, a context, a path) is never
- * followed: the access is skipped (attention takes a missing page's keys and values as zeros) and EXL3_ERR_BAD_SHAPE
- * recorded. */
+ * the top of this file: they enqueue on `stream`, allocate nothing and do not synchronise.  Arrays named "device" are read
+ * by the kernels when the call's work runs; a result that shares a byte with what its call reads is refused, except where
+ * the call allows it.  A device value out of range (a page id, a context, a path) is never followed: the access is skipped
+ * (attention takes a missing page's keys and values as zeros) and EXL3_ERR_BAD_SHAPE recorded. */
 
 /* The paged cache of every layer.  Token slot `t` of page `p` of kv head `h` of layer `l` is the head_dim contiguous
  * elements at k (v) + l * layer_stride + p * page_stride + h * head_stride + t * token_stride (elements; the same
@@ -545,7 +545,7 @@ typedef struct exl3_norm_rope {
   const double *inv_freq; /* device, [rot_dims / 2] radians per position (null with rot_dims 0) */
 } exl3_norm_rope;
 
-/* One pass over a layer's q, k, v rows: q normed and rotated into q_out (may be q itself), k normed and rotated and v
+/* One pass over a layer's q, k, v rows: q normed and rotated into q_out (may be q itself, in its dtype), k normed and rotated and v
  * as it is into their slots of `layer`.  f16, bf16 or f32 in one dtype; q_out in that dtype or the cache's; the
  * arithmetic is f32, the angle exact to 2^-52 turns of position * inv_freq, each output rounded once. */
 exl3_verdict exl3_qk_norm_rope(const exl3_kv_cache *cache, int32_t layer, const exl3_tree_batch *batch,
@@ -553,7 +553,7 @@ exl3_verdict exl3_qk_norm_rope(const exl3_kv_cache *cache, int32_t layer, const 
                                const exl3_norm_rope *opts, void *stream, const exl3_heads *q_out);
 
 /* Attention of the batch's rows over `layer`: out[r][h] = sum_j softmax_j(scale q[r][h] . k[j]) v[j] over the slots the
- * row sees, kv head h / (heads / kv_heads).  q and out in the cache's dtype, not the same array; scale > 0.  `lse` (device f32
+ * row sees, kv head h / (heads / kv_heads).  q and out in the cache's dtype, apart; scale > 0.  `lse` (device f32
  * [rows][heads], or null) receives log sum_j exp(scale q . k[j]).  A row that sees nothing gets zeros and -inf.  What
  * lies in slots a row does not see -- stale pages, other branches of the tree, infinities, NaN -- does not reach it.
  * Any number of rows per sequence: one (a decode step), a drafted tree, a prompt chunk. */

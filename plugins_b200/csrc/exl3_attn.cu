@@ -94,6 +94,80 @@ bool lies_apart(const exl3_heads* h) {
   return row >= head ? row >= head * (h->heads - 1) + h->dim : head >= row * (h->rows - 1) + h->dim;
 }
 
+// The bytes of an array of rows of heads: runs of `len` from `base` on, in up to two strides.
+struct Runs {
+  int64_t base, len;
+  int dims = 0;
+  int64_t step[2], count[2];
+};
+Runs runs_of(const exl3_heads* h) {
+  const int64_t size = h->dtype == EXL3_F32 ? 4 : 2;
+  Runs r{reinterpret_cast<intptr_t>(h->data), h->dim * size};
+  std::pair<int64_t, int64_t> d[2] = {{h->head_stride * size, h->heads}, {h->row_stride * size, h->rows}};
+  for (auto& [step, count] : d)
+    if (step < 0) r.base += step * (count - 1), step = -step;
+  if (d[0].first > d[1].first) std::swap(d[0], d[1]);
+  for (const auto& [step, count] : d) {
+    if (step == 0 || count <= 1) continue;
+    if (r.dims == 0 && step == r.len) r.len *= count;  // one run after the other
+    else r.step[r.dims] = step, r.count[r.dims++] = count;
+  }
+  return r;
+}
+Runs runs_of(const void* p, int64_t bytes) { return {reinterpret_cast<intptr_t>(p), bytes}; }
+
+// Whether some integers k_i in [lo_i, hi_i] bring delta + sum k_i step_i between (below, above): by the longest step first,
+// where few k are left.  (Gives up, and says yes, on layouts that need more than `budget` trials.)
+struct Term {
+  int64_t step, lo, hi;
+};
+bool hits(const Term* t, int n, int64_t delta, int64_t below, int64_t above, int& budget) {
+  if (n == 0) return below < delta && delta < above;
+  int64_t least = 0, most = 0;  // what the shorter steps can add
+  for (int i = 1; i < n; ++i) least += t[i].lo * t[i].step, most += t[i].hi * t[i].step;
+  const auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0 ? 1 : 0); };
+  const int64_t lo = std::max(t->lo, floor_div(below - delta - most, t->step) + 1);
+  const int64_t hi = std::min(t->hi, -floor_div(-(above - delta - least), t->step) - 1);
+  for (int64_t k = lo; k <= hi; ++k) {
+    if (--budget < 0) return true;
+    if (hits(t + 1, n - 1, delta + k * t->step, below, above, budget)) return true;
+  }
+  return false;
+}
+
+// Whether two arrays have a byte in common.
+bool meet(const Runs& a, const Runs& b) {
+  if (a.len <= 0 || b.len <= 0) return false;
+  const auto end = [](const Runs& r) {
+    int64_t e = r.base + r.len;
+    for (int i = 0; i < r.dims; ++i) e += r.step[i] * (r.count[i] - 1);
+    return e;
+  };
+  if (end(a) <= b.base || end(b) <= a.base) return false;
+  Term t[4];
+  int n = 0;
+  for (int i = 0; i < a.dims; ++i) t[n++] = {a.step[i], -(a.count[i] - 1), 0};
+  for (int i = 0; i < b.dims; ++i) {
+    int j = 0;
+    while (j < a.dims && t[j].step != b.step[i]) ++j;
+    if (j < a.dims) t[j].hi = b.count[i] - 1;
+    else t[n++] = {b.step[i], 0, b.count[i] - 1};
+  }
+  for (int i = 1; i < n; ++i)
+    for (int j = i; j > 0 && t[j].step > t[j - 1].step; --j) std::swap(t[j], t[j - 1]);
+  int budget = 4096;
+  return hits(t, n, b.base - a.base, -b.len, a.len, budget);
+}
+bool meet(const exl3_heads* a, const exl3_heads* b) { return meet(runs_of(a), runs_of(b)); }
+bool meet(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  return a && b && meet(runs_of(a, a_bytes), runs_of(b, b_bytes));
+}
+// Whether q_out is q itself: each element is then read by the thread that writes it.
+bool same_vectors(const exl3_heads* a, const exl3_heads* b) {
+  return a->data == b->data && a->dtype == b->dtype && a->rows == b->rows && a->heads == b->heads &&
+         (a->rows <= 1 || a->row_stride == b->row_stride) && (a->heads <= 1 || a->head_stride == b->head_stride);
+}
+
 exl3::HeadsView view(const exl3_heads* h) {
   exl3::HeadsView v{};
   v.data = h->data, v.dtype = h->dtype, v.heads = h->heads, v.row_stride = h->row_stride, v.head_stride = h->head_stride;
@@ -134,15 +208,30 @@ exl3_verdict check_state(const exl3_page_state* s) {
   return kOk;
 }
 
-// What the page calls share; `moves` in the workspace.
+// What the page calls share; `moves` in the workspace.  `asked`: the rows' parents or needs.
 exl3_verdict page_params(const exl3_kv_cache* cache, const exl3_page_state* in, const exl3_page_state* out,
-                         exl3::Workspace& ws, exl3::PageParams& p) {
+                         const int32_t* asked, int64_t asked_bytes, const int32_t* missing, exl3::Workspace& ws,
+                         exl3::PageParams& p) {
   exl3_verdict v = check_cache(cache);
   if (v.code != EXL3_OK) return v;
   if ((v = check_state(in)).code != EXL3_OK || (v = check_state(out)).code != EXL3_OK) return v;
   if (in->max_pages != out->max_pages) return refuse(EXL3_FAILED, "exl3_b200: the two tables have one width");
-  if (in->refs == out->refs || (in->nseq > 0 && (in->table == out->table || in->held == out->held || in->lens == out->lens)))
-    return refuse(EXL3_FAILED, "exl3_b200: the new page state has its own arrays");
+  const struct {
+    const void* at;
+    int64_t bytes;
+  } old[4] = {{in->refs, cache->pages * 4ll}, {in->table, in->nseq * 4ll * in->max_pages}, {in->held, in->nseq * 4ll},
+              {in->lens, in->nseq * 4ll}},
+    made[5] = {{out->refs, cache->pages * 4ll}, {out->table, out->nseq * 4ll * out->max_pages}, {out->held, out->nseq * 4ll},
+               {out->lens, out->nseq * 4ll}, {missing, 4}};
+  for (const auto& m : made) {
+    for (const auto& o : old)
+      if (meet(m.at, m.bytes, o.at, o.bytes)) return refuse(EXL3_FAILED, "exl3_b200: the new page state has its own arrays");
+    if (meet(m.at, m.bytes, asked, asked_bytes))
+      return refuse(EXL3_FAILED, "exl3_b200: the new page state lies over the call's arguments");
+  }
+  for (int i = 0; i < 4; ++i)
+    if (meet(missing, 4, made[i].at, made[i].bytes))
+      return refuse(EXL3_FAILED, "exl3_b200: the new page state lies over the call's arguments");
   if (!exl3::workspace_get(cache->device, ws)) return kNoWorkspace;
   p = {};
   p.pages = cache->pages;
@@ -183,8 +272,7 @@ exl3_verdict exl3_qk_norm_rope(const exl3_kv_cache* cache, int32_t layer, const 
   if (q_out->dtype != q->dtype && q_out->dtype != cache->dtype)
     return refuse(EXL3_UNSUPPORTED, "exl3_b200: q_out has q's dtype or the cache's");
   if (!lies_apart(q_out)) return refuse(EXL3_FAILED, "exl3_b200: q_out's vectors overlap");
-  if (q_out->data && q_out->data == q->data &&
-      (q_out->dtype != q->dtype || q_out->row_stride != q->row_stride || q_out->head_stride != q->head_stride))
+  if (q_out->data && meet(q_out, q) && !same_vectors(q_out, q))
     return refuse(EXL3_FAILED, "exl3_b200: q_out lies over q in another layout");
   if (!opts || opts->size != sizeof(exl3_norm_rope)) return refuse(EXL3_FAILED, "exl3_b200: not norm and rotation options");
   if (opts->rot_dims < 0 || opts->rot_dims > dim || opts->rot_dims % 2 || (!opts->adjacent && opts->rot_dims % 16))
@@ -195,6 +283,7 @@ exl3_verdict exl3_qk_norm_rope(const exl3_kv_cache* cache, int32_t layer, const 
     return refuse(EXL3_UNSUPPORTED, "exl3_b200: norm weights are f16, bf16 or f32");
   if (!(opts->eps >= 0.f)) return refuse(EXL3_FAILED, "exl3_b200: eps is not negative");
   if (batch->nseq == 0 || rows == 0) return kOk;
+  if (meet(q_out, k) || meet(q_out, v)) return refuse(EXL3_FAILED, "exl3_b200: q_out lies over k or v");
   exl3::Workspace ws;
   if (!exl3::workspace_get(cache->device, ws)) return kNoWorkspace;
   OnDevice guard(cache->device);
@@ -225,7 +314,11 @@ exl3_verdict exl3_tree_attention(const exl3_kv_cache* cache, int32_t layer, cons
   if (!(scale > 0.f) || std::isinf(scale)) return refuse(EXL3_UNSUPPORTED, "exl3_b200: the scale is a positive number");
   if (batch->max_rows > rows) return refuse(EXL3_FAILED, "exl3_b200: max_rows is above the batch's rows");
   if (batch->nseq == 0 || rows == 0) return kOk;
-  if (out->data == q->data) return refuse(EXL3_FAILED, "exl3_b200: out is not q (a row may be read again at its end)");
+  if (meet(out, q)) return refuse(EXL3_FAILED, "exl3_b200: out is not q (a row may be read again at its end)");
+  if (lse) {
+    const Runs l = runs_of(lse, static_cast<int64_t>(rows) * q->heads * 4);
+    if (meet(l, runs_of(q)) || meet(l, runs_of(out))) return refuse(EXL3_FAILED, "exl3_b200: lse lies over q or out");
+  }
   exl3::Workspace ws;
   if (!exl3::workspace_get(cache->device, ws)) return kNoWorkspace;
   OnDevice guard(cache->device);
@@ -250,7 +343,7 @@ exl3_verdict exl3_cache_fork(const exl3_kv_cache* cache, const exl3_page_state* 
                              const exl3_page_state* out) {
   exl3::Workspace ws;
   exl3::PageParams p;
-  exl3_verdict v = page_params(cache, in, out, ws, p);
+  exl3_verdict v = page_params(cache, in, out, parent, out ? out->nseq * 4ll : 0, nullptr, ws, p);
   if (v.code != EXL3_OK) return v;
   if (!parent && out->nseq > 0) return refuse(EXL3_FAILED, "exl3_b200: fork without parents");
   p.parent = parent;
@@ -262,7 +355,7 @@ exl3_verdict exl3_cache_grow(const exl3_kv_cache* cache, const exl3_page_state* 
                              const exl3_page_state* out, int32_t* missing) {
   exl3::Workspace ws;
   exl3::PageParams p;
-  exl3_verdict v = page_params(cache, in, out, ws, p);
+  exl3_verdict v = page_params(cache, in, out, need, in ? in->nseq * 4ll : 0, missing, ws, p);
   if (v.code != EXL3_OK) return v;
   if (in->nseq != out->nseq) return refuse(EXL3_FAILED, "exl3_b200: grow keeps the rows");
   if (in->nseq > exl3::cache_grow_max_rows()) return refuse(EXL3_TOO_LARGE, "exl3_b200: grow takes at most 4096 rows");
@@ -282,7 +375,7 @@ exl3_verdict exl3_cache_compact(const exl3_kv_cache* cache, const exl3_page_stat
                                 const exl3_page_state* out) {
   exl3::Workspace ws;
   exl3::PageParams p;
-  exl3_verdict v = page_params(cache, in, out, ws, p);
+  exl3_verdict v = page_params(cache, in, out, nullptr, 0, nullptr, ws, p);
   if (v.code != EXL3_OK) return v;
   if (in->nseq != out->nseq) return refuse(EXL3_FAILED, "exl3_b200: compact keeps the rows");
   if (ws.partial_floats < static_cast<size_t>(cache->pages) * 4 + 1)
@@ -301,6 +394,11 @@ exl3_verdict exl3_cache_keep(const exl3_kv_cache* cache, const exl3_tree_batch* 
   if (batch->nseq == 0) return kOk;
   if (!kept || !lens) return refuse(EXL3_FAILED, "exl3_b200: keep without its arrays");
   if (path && depth < 1) return refuse(EXL3_FAILED, "exl3_b200: a path without depth");
+  const int64_t bytes = batch->nseq * 4ll;
+  if ((lens != batch->context && meet(lens, bytes, batch->context, bytes)) || (lens != kept && meet(lens, bytes, kept, bytes)) ||
+      meet(lens, bytes, path, bytes * depth) || meet(lens, bytes, batch->table, bytes * batch->max_pages) ||
+      meet(lens, bytes, batch->row_start, bytes + 4))
+    return refuse(EXL3_FAILED, "exl3_b200: lens lies over the call's arguments");
   exl3::Workspace ws;
   if (!exl3::workspace_get(cache->device, ws)) return kNoWorkspace;
   OnDevice guard(cache->device);
