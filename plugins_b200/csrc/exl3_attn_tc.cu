@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(TcShape<D, ROWS>::kThreads, 1)
   {
     WorkLine own;
     Item first;
-    own.start(p, S::kRows, KT, reinterpret_cast<int64_t*>(s_k), first);
+    own.start(p, S::kRows, KT, reinterpret_cast<int64_t*>(s_ml), first);  // (not where TMA will write: that is another proxy)
     if (tid == 0) *s_line = own;
     if (lane == 0) s_items[warp] = first;
   }

@@ -132,3 +132,37 @@ def test_many_small_probabilities_beside_a_large_one(A, dtype, rows, dim):
     rest = torch.tensor([keys - 1 + i for i in range(rows)], dtype=torch.float64).repeat(nseq)[:, None]
     want = (rest / (first + rest))[:, :, None] * v[0, 1, 0, 0].double().cpu()
     close(out, lse, want, torch.log(first + rest), want, dtype)
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 128), (4, 64), (20, 128), (40, 64), (10, 256)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_more_sequences_than_threads(A, rows, dim, tree):
+    """The line of work is scanned in several runs of sequences, many of them without rows; launches follow one another."""
+    nseq, page, dtype = 1000, 16, torch.bfloat16
+    g = torch.Generator().manual_seed(rows)
+    lens = torch.randint(0, 60, (nseq,), generator=g).tolist()
+    count = [rows if x < 0.7 else (1 if x < 0.8 else 0) for x in torch.rand(nseq, generator=g).tolist()]
+    start = [0]
+    for c in count:
+        start.append(start[-1] + c)
+    width = (60 + rows) // page + 1
+    pages = 512  # (read only: the sequences may share them)
+    table = torch.randint(0, pages, (nseq, width), generator=g).int()
+    k, v = (torch.randn((1, pages, 1, page, dim), generator=g).to(dtype) for _ in range(2))
+    bits = torch.randint(0, 1 << 30, (start[-1], 2), generator=g).int() if tree else None
+    batch = A.TreeBatch(i32(start), i32(lens), table.cuda(), max_rows=rows, rows=start[-1], tree=None if bits is None else bits.cuda())
+    cache = A.KvCache(k.cuda(), v.cuda())
+    q = torch.randn((start[-1], 2, dim), generator=g).to(dtype)
+    dev = q.cuda()
+    outs = [A.tree_attention(cache, 0, batch, dev, lse=True) for _ in range(4)]
+    for out, lse in outs[1:]:
+        assert torch.equal(out, outs[0][0]) and torch.equal(lse, outs[0][1])
+    out, lse = outs[0]
+    sample = [0, 1, 255, 256, 257, 383, 384, 385, 640, nseq - 1] + torch.randint(0, nseq, (25,), generator=g).tolist()
+    for s in sample:
+        a, b = start[s], start[s + 1]
+        want, wlse, mass = R.attention(k[0], v[0], q[a:b], [0, b - a], [lens[s]], table[s:s + 1], dim ** -0.5,
+                                       None if bits is None else bits[a:b])
+        empty = torch.isneginf(wlse)
+        assert torch.equal(torch.isneginf(lse[a:b].cpu()), empty)
+        close(out[a:b], torch.where(empty, 0.0, lse[a:b].cpu()), want, torch.where(empty, 0.0, wlse), mass, dtype)
