@@ -86,10 +86,10 @@ class _Calls:
     def load(cls) -> None:
         p, c = ctypes.c_void_p, ctypes.c_char_p
         lib = L.lib()
-        proto = ctypes.CFUNCTYPE(L.Verdict, p, ctypes.c_int32, p, c, c, c, p, p, c)
-        cls.rope = proto(ctypes.cast(lib.exl3_qk_norm_rope, p).value)
         proto = ctypes.CFUNCTYPE(L.Verdict, p, ctypes.c_int32, p, c, ctypes.c_float, p, c, p)
         cls.attention = proto(ctypes.cast(lib.exl3_tree_attention, p).value)
+        proto = ctypes.CFUNCTYPE(L.Verdict, p, ctypes.c_int32, p, c, c, c, p, p, c)
+        cls.rope = proto(ctypes.cast(lib.exl3_qk_norm_rope, p).value)  # last: another thread takes it for all there
 
 
 def _used_on(stream, *tensors) -> None:
