@@ -574,7 +574,7 @@ typedef struct exl3_page_state {
 
 /* Fork, reorder and free: row i of `out` becomes row parent[i] of `in` (-1: an empty row), sharing its pages; each
  * page's references follow the rows that hold it, so the pages of rows nobody names become free.  No key or value
- * moves.  out->nseq rows; out's arrays are not in's. */
+ * moves.  out->nseq rows, in->nseq * out->nseq at most 2^32; out's arrays are not in's. */
 exl3_verdict exl3_cache_fork(const exl3_kv_cache *cache, const exl3_page_state *in, const int32_t *parent, void *stream,
                              const exl3_page_state *out);
 

@@ -341,6 +341,9 @@ exl3_verdict exl3_tree_attention(const exl3_kv_cache* cache, int32_t layer, cons
 
 exl3_verdict exl3_cache_fork(const exl3_kv_cache* cache, const exl3_page_state* in, const int32_t* parent, void* stream,
                              const exl3_page_state* out) {
+  // every old row looks through the new rows for its children
+  if (in && out && in->nseq > 0 && out->nseq > 0 && static_cast<int64_t>(in->nseq) * out->nseq > (1ll << 32))
+    return refuse(EXL3_TOO_LARGE, "exl3_b200: fork takes at most 2^32 pairs of an old and a new row");
   exl3::Workspace ws;
   exl3::PageParams p;
   exl3_verdict v = page_params(cache, in, out, parent, out ? out->nseq * 4ll : 0, nullptr, ws, p);

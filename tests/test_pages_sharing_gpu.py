@@ -264,3 +264,9 @@ def test_grow_asked_for_more_than_can_be_counted(A, nseq):
     assert int(missing) == min(asked, 2 ** 31 - 1)
     assert out.refs.tolist() == state.refs.tolist() and out.table.tolist() == state.table.tolist()
     assert out.held.tolist() == state.held.tolist() and out.lens.tolist() == state.lens.tolist()
+
+
+def test_grow_of_too_many_rows_is_refused(A):
+    cache = A.KvCache(*(torch.zeros((1, 8, 1, 16, 64), dtype=torch.float16, device="cuda") for _ in range(2)))
+    with pytest.raises(A.Exl3Error, match="4096"):
+        A.cache_grow(cache, A.PageState.empty(cache, 4097, 2), i32([0] * 4097))
