@@ -181,6 +181,8 @@ class TreeBatch:
         if rows is None:
             rows = next((t.shape[0] for t in (tree, position) if t is not None), None)
         _ints(tree, (rows, None), "tree", dev, optional=True)
+        if tree is not None and tree.shape[1] == 0:
+            _refuse("a tree without words")  # (whose address is null: it would read as no tree)
         _ints(position, (rows,), "position", dev, optional=True)
         self.rows, self.nseq, self.device = rows, nseq, dev
         self._keep = (row_start, context, table, tree, position)

@@ -166,3 +166,8 @@ def test_more_sequences_than_threads(A, rows, dim, tree):
         empty = torch.isneginf(wlse)
         assert torch.equal(torch.isneginf(lse[a:b].cpu()), empty)
         close(out[a:b], torch.where(empty, 0.0, lse[a:b].cpu()), want, torch.where(empty, 0.0, wlse), mass, dtype)
+
+
+def test_a_tree_without_words_is_refused(A):
+    with pytest.raises(A.Exl3Error, match="without words"):
+        A.TreeBatch(i32([0, 2]), i32([3]), i32([[0]]), max_rows=2, tree=torch.empty((2, 0), dtype=torch.int32, device="cuda"))
