@@ -87,6 +87,8 @@ class TreeDecoder:
 
     def prompt(self, prompts: list[list[int]]) -> list[int]:
         """Every sequence's prompt in one pass -> its next token."""
+        if len(prompts) != len(self.lens) or not all(prompts):
+            raise ValueError(f"a prompt of at least one token for each of the {len(self.lens)} sequences")
         batch = self._batch([len(p) for p in prompts])
         x = self.forward(torch.tensor([t for p in prompts for t in p], device=self.embed.device), batch)
         ends = [0]
@@ -98,6 +100,8 @@ class TreeDecoder:
 
     def step(self, trees: list[list[tuple[int, int]]]) -> list[list[int]]:
         """One pass over every sequence's last token (row 0 of its tree) and its drafts -> the tokens each gained."""
+        if len(trees) != len(self.lens) or any(not -1 <= p < i for tree in trees for i, (p, _) in enumerate(tree)):
+            raise ValueError(f"a tree for each of the {len(self.lens)} sequences, every parent -1 or before its child")
         tokens, parents, counts = [], [], []
         for last, tree in zip(self.last, trees):
             tokens += [last] + [t for _, t in tree]
@@ -135,6 +139,8 @@ class TreeDecoder:
 
     def reorder(self, parent: list[int]) -> None:
         """Row i becomes row parent[i] (a fork when named twice); rows nobody names give their pages back."""
+        if not all(0 <= p < len(self.lens) for p in parent):
+            raise ValueError(f"parents are among the {len(self.lens)} rows")
         self.state = A.cache_fork(self.cache, self.state, self._ints(parent))
         self.lens, self.last = [self.lens[p] for p in parent], [self.last[p] for p in parent]
 
