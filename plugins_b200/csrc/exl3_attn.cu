@@ -409,7 +409,7 @@ exl3_verdict exl3_cache_keep(const exl3_kv_cache* cache, const exl3_tree_batch* 
   p.pool = pool_of(cache);
   p.b = paged(cache, 0, batch, ws.err);
   p.path = path, p.depth = depth, p.kept = kept, p.lens = lens;
-  p.counters = ws.counters;
+  if (lens == batch->context || lens == kept) p.counters = ws.counters;
   return launched(exl3::launch_cache_keep(p, ws.counter_count, static_cast<cudaStream_t>(stream)));
 }
 

@@ -100,7 +100,7 @@ struct KeepParams {
   const int32_t *path, *kept;
   int32_t depth;
   int32_t* lens;       // may be b.context, or kept
-  uint32_t* counters;  // one per sequence of a launch
+  uint32_t* counters;  // where it is, one per sequence of a launch; else null
   int32_t seq0;        // the launch's first sequence
 };
 cudaError_t launch_cache_keep(const KeepParams& p, uint32_t counters, cudaStream_t st);

@@ -354,8 +354,9 @@ constexpr int kKeepThreads = 256;
 constexpr int kKeepBatch = 8;  // tokens read before any of them is written
 
 // One thread per (16-byte chunk of a head, kv head, k or v, layer) of one sequence (blockIdx.y): it walks the path.  The
-// path ascends, so path[d] >= d, and a slot is never read after a later token was written to it.  lens[s] is written by the
-// sequence's last block to have read context[s] and kept[s]: it may be either of them (a loop's lengths kept in place).
+// path ascends, so path[d] >= d, and a slot is never read after a later token was written to it.  lens may be context or kept
+// (a loop's lengths kept in place): lens[s] is then written by the sequence's last block to have read them.  The count takes
+// 2 us of 16 (32 trees, 36 layers); lengths apart from both are written at once.
 __global__ void __launch_bounds__(kKeepThreads) keep_kernel(const KeepParams p) {
   pdl_wait();
   const int s = p.seq0 + static_cast<int>(blockIdx.y);
@@ -374,19 +375,20 @@ __global__ void __launch_bounds__(kKeepThreads) keep_kernel(const KeepParams p) 
   }
   const int64_t item = static_cast<int64_t>(blockIdx.x) * kKeepThreads + threadIdx.x;
   if (!ok) kept = 0;
-  __syncthreads();  // the block's reads of context and kept are done
-  if (threadIdx.x == 0) {
-    bool last = true;
-    if (gridDim.x > 1) {
+  bool last = item == 0;
+  if (p.counters) {
+    __syncthreads();  // the block's reads of context and kept are done
+    last = false;
+    if (threadIdx.x == 0) {
       __threadfence();
       last = atomicAdd(p.counters + blockIdx.y, 1u) + 1u == gridDim.x;
       __threadfence();
+      if (last) p.counters[blockIdx.y] = 0u;
     }
-    if (last) {
-      if (gridDim.x > 1) p.counters[blockIdx.y] = 0u;
-      p.lens[s] = max(ctx, 0) + kept;
-      if (!ok) atomicOr(p.b.err, kErrBadShape);
-    }
+  }
+  if (last) {
+    p.lens[s] = max(ctx, 0) + kept;
+    if (!ok) atomicOr(p.b.err, kErrBadShape);
   }
   if (!path) return;
   const int per = p.pool.dim / 8;
@@ -472,11 +474,10 @@ cudaError_t launch_page_copy(const PagePool& pool, const int32_t* moves, int64_t
 cudaError_t launch_cache_keep(const KeepParams& p, uint32_t counters, cudaStream_t st) {
   const int64_t items = p.path ? static_cast<int64_t>(p.pool.layers) * 2 * p.pool.kv_heads * (p.pool.dim / 8) : 1;
   KeepParams part = p;
-  // a counter per sequence of a launch
-  for (part.seq0 = 0; part.seq0 < p.b.nseq; part.seq0 += static_cast<int>(counters)) {
+  const int most = p.counters ? static_cast<int>(counters) : p.b.nseq;  // sequences of a launch
+  for (part.seq0 = 0; part.seq0 < p.b.nseq; part.seq0 += most) {
     const int left = p.b.nseq - part.seq0;
-    const dim3 grid(static_cast<unsigned>((items + kKeepThreads - 1) / kKeepThreads),
-                    left < static_cast<int>(counters) ? static_cast<unsigned>(left) : counters);
+    const dim3 grid(static_cast<unsigned>((items + kKeepThreads - 1) / kKeepThreads), static_cast<unsigned>(left < most ? left : most));
     cudaError_t e = launch_pdl_k(keep_kernel, grid, dim3(kKeepThreads), st, part);
     if (e != cudaSuccess) return e;
   }
