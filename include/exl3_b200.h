@@ -560,7 +560,7 @@ exl3_verdict exl3_qk_norm_rope(const exl3_kv_cache *cache, int32_t layer, const 
 exl3_verdict exl3_tree_attention(const exl3_kv_cache *cache, int32_t layer, const exl3_tree_batch *batch,
                                  const exl3_heads *q, float scale, void *stream, const exl3_heads *out, float *lse);
 
-/* The host's page bookkeeping, on the device: how many rows refer to each page (0: free), each row's page ids (-1 past
+/* The host's page bookkeeping, on the device: how many rows refer to each page (none: free), each row's page ids (-1 past
  * its `held` pages), and its tokens. */
 typedef struct exl3_page_state {
   uint32_t size;      /* sizeof(exl3_page_state) */

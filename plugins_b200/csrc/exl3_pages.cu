@@ -172,7 +172,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) gro
   for (int64_t i = t; i < static_cast<int64_t>(n) * p.width_in; i += kAll) p.table[i] = p.table_in[i];
   const PageRun run(p.pages);
   int mine = 0, free_pages;
-  for (int i = run.lo; i < run.hi; ++i) mine += p.refs_in[i] == 0 ? 1 : 0;
+  for (int i = run.lo; i < run.hi; ++i) mine += p.refs_in[i] <= 0 ? 1 : 0;
   int rank = cluster_scan_excl(mine, s_warp, &s_total, &free_pages);  // (its barrier: the copies above are in place)
   // a shared page loses the references of the rows that write it (whole numbers: any order)
   each_row([&](int r, const Writes& w) {
@@ -221,7 +221,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) gro
     for (int i = t; i < p.pages; i += kAll) p.refs[i] = p.refs_in[i];
   } else {
     for (int i = run.lo; i < run.hi && rank < asked; ++i)
-      if (p.refs_in[i] == 0) order[rank++] = i;
+      if (p.refs_in[i] <= 0) order[rank++] = i;
   }
   cluster_sync();  // (and no CTA leaves while another may read its shared words)
   each_row([&](int r, const Writes& w) {

@@ -270,3 +270,17 @@ def test_grow_of_too_many_rows_is_refused(A):
     cache = A.KvCache(*(torch.zeros((1, 8, 1, 16, 64), dtype=torch.float16, device="cuda") for _ in range(2)))
     with pytest.raises(A.Exl3Error, match="4096"):
         A.cache_grow(cache, A.PageState.empty(cache, 4097, 2), i32([0] * 4097))
+
+
+def test_a_page_without_references_is_free_to_every_call(A):
+    """Counts that a host kept too low fall below zero when its rows end (the page of row 0 here): grow and compact both
+    take such a page as free."""
+    cache = A.KvCache(*(torch.randn((1, 6, 1, 16, 64), device="cuda").half() for _ in range(2)))
+    state = A.cache_fork(cache, on_gpu(A, [0, 1, 0, 0, 1, 0], [[0], [1], [4]], [9, 9, 9], 3), i32([1, 2]))
+    assert state.refs.tolist() == [-1, 1, 0, 0, 1, 0]
+    grown, missing = A.cache_grow(cache, state, i32([33, 17]))
+    assert int(missing) == 0 and grown.table.tolist() == [[1, 0, 2], [4, 3, -1]] and grown.refs.tolist() == [1, 1, 1, 1, 1, 0]
+    k = cache.k.clone()
+    packed = A.cache_compact(cache, state)
+    assert packed.table.tolist() == [[1, -1, -1], [0, -1, -1]] and packed.refs.tolist() == [1, 1, 0, 0, 0, 0]
+    assert torch.equal(cache.k[:, 0], k[:, 4])
