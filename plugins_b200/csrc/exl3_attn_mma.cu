@@ -2,8 +2,8 @@
 //
 // One pass over the keys with the running maximum m and sum l of a softmax (all in f32):
 //   s = scale q . k,  m' = max(m, s),  l = l e^(m - m') + e^(s - m'),  o = o e^(m - m') + e^(s - m') v;   out = o / l.
-// The rows that share a kv head (its query heads x the sequence's new tokens) are packed into m16n8k16 row tiles, so a
-// key is read once for all of them.  Bound by HBM: K and V once, 16 x rows / 16-bit element operations against them.
+// The rows that share a kv head (its query heads x the sequence's new tokens) are packed into one m16n8k16 row tile,
+// so a key is read once for all of them.  Bound by HBM: K and V once, 16 x rows / 16-bit element operations against them.
 //
 // Work: the (sequence, kv head, row block) items' keys, in tiles of 64, form one line that the CTAs cut into equal
 // parts, whatever the sequences' lengths.  A CTA's four warps take 16 keys of each tile, every warp with its own ring of
@@ -29,9 +29,9 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kGroupKeys = 16;                   // keys a warp takes per step: inside one page
 constexpr int kTileKeys = kWarps * kGroupKeys;
 
-template <int D, int MT>
+template <int D>
 struct MmaShape {
-  static constexpr int kRows = 16 * MT;
+  static constexpr int kRows = 16;
   static constexpr int kGroupBytes = kGroupKeys * D * 2;       // K or V of one warp step
   static constexpr int kStages = D == 64 ? 6 : 3;
   static constexpr int kRing = kStages * 2 * kGroupBytes;      // per warp
@@ -47,9 +47,9 @@ __device__ __forceinline__ uint32_t tile_off(uint32_t r, uint32_t c) {
   return r * (D * 2) + ((c ^ (r & 7u)) << 4);
 }
 
-template <int D, int MT, bool BF16>
+template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const AttnParams p) {
-  using S = MmaShape<D, MT>;
+  using S = MmaShape<D>;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* s_q = smem + kWarps * S::kRing;
   float2* s_ml = reinterpret_cast<float2*>(s_q + S::kQBytes);  // [rows][warps]
@@ -83,24 +83,17 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const AttnParams p) 
     __syncthreads();
 
     // the query fragments stay in registers where they fit beside o
-    constexpr bool kQRegs = MT * D <= 128;
-    uint32_t qa[kQRegs ? D / 16 : 1][MT][4];
+    constexpr bool kQRegs = D <= 128;
+    uint32_t qa[kQRegs ? D / 16 : 1][4];
     if constexpr (kQRegs) {
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-          ldmatrix_x4(smem_u32(s_q) + tile_off<D>(16u * i + (lane & 15u), 2u * kk + (lane >> 4)), qa[kk][i]);
+      for (int kk = 0; kk < D / 16; ++kk) ldmatrix_x4(smem_u32(s_q) + tile_off<D>(lane & 15u, 2u * kk + (lane >> 4)), qa[kk]);
     }
 
-    float o[MT][D / 8][4];
-    float m[MT][2], l[MT][2];
+    float o[D / 8][4];
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // rows g and g + 8
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      m[i][0] = m[i][1] = -INFINITY, l[i][0] = l[i][1] = 0.f;
-#pragma unroll
-      for (int j = 0; j < D / 8; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
-    }
+    for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
     const int32_t* tab = p.b.table + static_cast<int64_t>(it.seq) * p.b.max_pages;
     const int page_mask = (1 << p.b.page_shift) - 1;
@@ -145,86 +138,72 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const AttnParams p) 
       const int key0 = (tile0 + t) * kTileKeys + static_cast<int>(warp) * kGroupKeys;
       if (key0 < it.keys) {
         const uint32_t sk = ring + (t % S::kStages) * 2 * S::kGroupBytes, sv = sk + S::kGroupBytes;
-        float s[MT][2][4];
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) s[i][j][0] = s[i][j][1] = s[i][j][2] = s[i][j][3] = 0.f;
+        float s[2][4] = {};
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           uint32_t b[4];  // keys 0..7 (k low, high), keys 8..15 (k low, high)
           ldmatrix_x4(sk + tile_off<D>((lane & 7u) + ((lane >> 4) << 3), 2u * kk + ((lane >> 3) & 1u)), b);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            if constexpr (!kQRegs)
-              ldmatrix_x4(smem_u32(s_q) + tile_off<D>(16u * i + (lane & 15u), 2u * kk + (lane >> 4)), qa[0][i]);
-            mma16816<BF16>(s[i][0], qa[kQRegs ? kk : 0][i], b[0], b[1]);
-            mma16816<BF16>(s[i][1], qa[kQRegs ? kk : 0][i], b[2], b[3]);
-          }
+          if constexpr (!kQRegs) ldmatrix_x4(smem_u32(s_q) + tile_off<D>(lane & 15u, 2u * kk + (lane >> 4)), qa[0]);
+          mma16816<BF16>(s[0], qa[kQRegs ? kk : 0], b[0], b[1]);
+          mma16816<BF16>(s[1], qa[kQRegs ? kk : 0], b[2], b[3]);
         }
         const bool tail = key0 + kGroupKeys > it.context;  // some key is not in the context: rows see it or not
         uint32_t odd = 0;                                  // a tail key's V holds an infinity or NaN
         if (tail) odd = odd_values<D, BF16>(sv, lane);
-        uint32_t pa[MT][4];
+        uint32_t pa[4];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
+        for (int hh = 0; hh < 2; ++hh) {  // rows g and g + 8 of the row tile
+          float x[4] = {s[0][2 * hh], s[0][2 * hh + 1], s[1][2 * hh], s[1][2 * hh + 1]};
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {  // rows g and g + 8 of the row tile
-            float x[4] = {s[i][0][2 * hh], s[i][0][2 * hh + 1], s[i][1][2 * hh], s[i][1][2 * hh + 1]};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] *= p.scale_log2;
-            if (tail) {
-              const int r = it.row_block * S::kRows + 16 * i + 8 * hh + static_cast<int>(g);
-              const int tok = r / p.group;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int key = key0 + (j >> 1) * 8 + static_cast<int>(q4) * 2 + (j & 1);
-                if (!sees(p.b, it, tok, key)) x[j] = -INFINITY;
-              }
-            }
-            float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
-            mx = fmaxf(mx, m[i][hh]);
-            const float top = mx == -INFINITY ? 0.f : mx;  // nothing seen so far: every term below is 0
-            const float base = top - kLift<BF16>;
-            const float f = ex2(m[i][hh] - top);
-            m[i][hh] = mx;
-            float sum = 0.f;
+          for (int j = 0; j < 4; ++j) x[j] *= p.scale_log2;
+          if (tail) {
+            const int r = it.row_block * S::kRows + 8 * hh + static_cast<int>(g);
+            const int tok = r / p.group;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              x[j] = ex2(x[j] - base);
-              sum += x[j];
+              const int key = key0 + (j >> 1) * 8 + static_cast<int>(q4) * 2 + (j & 1);
+              if (!sees(p.b, it, tok, key)) x[j] = -INFINITY;
             }
-            l[i][hh] = l[i][hh] * f + sum;
-#pragma unroll
-            for (int j = 0; j < D / 8; ++j) o[i][j][2 * hh] *= f, o[i][j][2 * hh + 1] *= f;
-            // 2^kLift e^(s - m), rounded to the element type for the product with V (l keeps the f32 values)
-            pa[i][hh] = pack2<BF16>(x[0], x[1]);
-            pa[i][2 + hh] = pack2<BF16>(x[2], x[3]);
           }
+          float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
+          mx = fmaxf(mx, m[hh]);
+          const float top = mx == -INFINITY ? 0.f : mx;  // nothing seen so far: every term below is 0
+          const float base = top - kLift<BF16>;
+          const float f = ex2(m[hh] - top);
+          m[hh] = mx;
+          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[j] = ex2(x[j] - base);
+            sum += x[j];
+          }
+          l[hh] = l[hh] * f + sum;
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j) o[j][2 * hh] *= f, o[j][2 * hh + 1] *= f;
+          // 2^kLift e^(s - m), rounded to the element type for the product with V (l keeps the f32 values)
+          pa[hh] = pack2<BF16>(x[0], x[1]);
+          pa[2 + hh] = pack2<BF16>(x[2], x[3]);
         }
         if (__any_sync(0xFFFFFFFFu, odd != 0u)) {
           // rare: an infinity or NaN in V reaches the rows that see its key and no others, so it cannot go through
           // the product (0 x inf = NaN); add it by hand, then zero it in shared memory
 #pragma unroll 1
           for (int key = 0; key < kGroupKeys; ++key) {
+            const int src = static_cast<int>((lane & ~3u) | ((key & 7u) >> 1));
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              const int src = static_cast<int>((lane & ~3u) | ((key & 7u) >> 1));
+            for (int hh = 0; hh < 2; ++hh) {
+              const uint32_t w = __shfl_sync(0xFFFFFFFFu, key < 8 ? pa[hh] : pa[2 + hh], src);
+              const float pv = unpack1<BF16>(w, key & 1);
+              const int r = it.row_block * S::kRows + 8 * hh + static_cast<int>(g);
+              const bool see = key0 + key < it.keys && sees(p.b, it, r / p.group, key0 + key);
 #pragma unroll
-              for (int hh = 0; hh < 2; ++hh) {
-                const uint32_t w = __shfl_sync(0xFFFFFFFFu, key < 8 ? pa[i][hh] : pa[i][2 + hh], src);
-                const float pv = unpack1<BF16>(w, key & 1);
-                const int r = it.row_block * S::kRows + 16 * i + 8 * hh + static_cast<int>(g);
-                const bool see = key0 + key < it.keys && sees(p.b, it, r / p.group, key0 + key);
-#pragma unroll
-                for (int j = 0; j < D / 8; ++j) {
-                  const uint32_t v2 = lds32(sv + tile_off<D>(static_cast<uint32_t>(key), static_cast<uint32_t>(j)) + q4 * 4u);
-                  const float v0 = unpack1<BF16>(v2, 0), v1 = unpack1<BF16>(v2, 1);
-                  if (see && !isfinite(v0)) o[i][j][2 * hh] += pv * v0;
-                  if (see && !isfinite(v1)) o[i][j][2 * hh + 1] += pv * v1;
-                }
+              for (int j = 0; j < D / 8; ++j) {
+                const uint32_t v2 = lds32(sv + tile_off<D>(static_cast<uint32_t>(key), static_cast<uint32_t>(j)) + q4 * 4u);
+                const float v0 = unpack1<BF16>(v2, 0), v1 = unpack1<BF16>(v2, 1);
+                if (see && !isfinite(v0)) o[j][2 * hh] += pv * v0;
+                if (see && !isfinite(v1)) o[j][2 * hh + 1] += pv * v1;
               }
             }
           }
@@ -236,11 +215,8 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const AttnParams p) 
         for (int jj = 0; jj < D / 16; ++jj) {
           uint32_t b[4];  // d 16 jj .. + 7 (keys low, high), d 16 jj + 8 .. (keys low, high)
           ldmatrix_x4_trans(sv + tile_off<D>(lane & 15u, 2u * jj + (lane >> 4)), b);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            mma16816<BF16>(o[i][2 * jj], pa[i], b[0], b[1]);
-            mma16816<BF16>(o[i][2 * jj + 1], pa[i], b[2], b[3]);
-          }
+          mma16816<BF16>(o[2 * jj], pa, b[0], b[1]);
+          mma16816<BF16>(o[2 * jj + 1], pa, b[2], b[3]);
         }
       }
       __syncwarp();  // the stage may be refilled
@@ -251,19 +227,16 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const AttnParams p) 
     // ---- join the four warps: m and l per row, then o scaled to the common maximum, summed in warp order
     float* s_o = reinterpret_cast<float*>(smem);  // [warps][rows][D]
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
+    for (int hh = 0; hh < 2; ++hh) {
+      float sum = l[hh];
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+      const uint32_t r = 8u * hh + g;
+      if (q4 == 0) s_ml[r * kWarps + warp] = make_float2(m[hh] - kLift<BF16>, sum);
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        float sum = l[i][hh];
-        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
-        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-        const uint32_t r = 16u * i + 8u * hh + g;
-        if (q4 == 0) s_ml[r * kWarps + warp] = make_float2(m[i][hh] - kLift<BF16>, sum);
-#pragma unroll
-        for (int j = 0; j < D / 8; ++j)
-          *reinterpret_cast<float2*>(s_o + (warp * S::kRows + r) * D + j * 8 + q4 * 2) =
-              make_float2(o[i][j][2 * hh], o[i][j][2 * hh + 1]);
-      }
+      for (int j = 0; j < D / 8; ++j)
+        *reinterpret_cast<float2*>(s_o + (warp * S::kRows + r) * D + j * 8 + q4 * 2) =
+            make_float2(o[j][2 * hh], o[j][2 * hh + 1]);
     }
     __syncthreads();
     const bool whole = tiles == it.tiles;
@@ -297,11 +270,11 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(const AttnParams p) 
   }
 }
 
-template <int D, int MT>
+template <int D>
 cudaError_t launch_dim(const AttnParams& p, int sms, size_t partial_floats, cudaStream_t st) {
-  using S = MmaShape<D, MT>;
+  using S = MmaShape<D>;
   static KernelSetup setup[2];
-  auto kern = p.bf16 ? attn_mma_kernel<D, MT, true> : attn_mma_kernel<D, MT, false>;
+  auto kern = p.bf16 ? attn_mma_kernel<D, true> : attn_mma_kernel<D, false>;
   int per_sm = 1;
   cudaError_t e = kernel_setup(setup[p.bf16 ? 1 : 0], kern, kThreads, S::kSmem, false, &per_sm, 4);
   if (e != cudaSuccess) return e;
@@ -330,9 +303,9 @@ cudaError_t launch_dim(const AttnParams& p, int sms, size_t partial_floats, cuda
 
 cudaError_t launch_attn_mma(const AttnParams& p, int dim, int sms, size_t partial_floats, cudaStream_t st) {
   switch (dim) {
-    case 64: return launch_dim<64, 1>(p, sms, partial_floats, st);
-    case 128: return launch_dim<128, 1>(p, sms, partial_floats, st);
-    default: return launch_dim<256, 1>(p, sms, partial_floats, st);
+    case 64: return launch_dim<64>(p, sms, partial_floats, st);
+    case 128: return launch_dim<128>(p, sms, partial_floats, st);
+    default: return launch_dim<256>(p, sms, partial_floats, st);
   }
 }
 
