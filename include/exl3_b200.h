@@ -547,7 +547,8 @@ typedef struct exl3_norm_rope {
 
 /* One pass over a layer's q, k, v rows: q normed and rotated into q_out (may be q itself, in its dtype), k normed and rotated and v
  * as it is into their slots of `layer`.  f16, bf16 or f32 in one dtype; q_out in that dtype or the cache's; the
- * arithmetic is f32, the angle exact to 2^-52 turns of position * inv_freq, each output rounded once. */
+ * arithmetic is f32, each output rounded once.  The angle position * inv_freq is formed and reduced to turns in f64 (a
+ * relative error of 2^-52), then rounded to f32 (2^-26 turns) for its sine and cosine. */
 exl3_verdict exl3_qk_norm_rope(const exl3_kv_cache *cache, int32_t layer, const exl3_tree_batch *batch,
                                const exl3_heads *q, const exl3_heads *k, const exl3_heads *v,
                                const exl3_norm_rope *opts, void *stream, const exl3_heads *q_out);
@@ -556,6 +557,8 @@ exl3_verdict exl3_qk_norm_rope(const exl3_kv_cache *cache, int32_t layer, const 
  * row sees, kv head h / (heads / kv_heads).  q and out in the cache's dtype, apart; scale > 0.  `lse` (device f32
  * [rows][heads], or null) receives log sum_j exp(scale q . k[j]).  A row that sees nothing gets zeros and -inf.  What
  * lies in slots a row does not see -- stale pages, other branches of the tree, infinities, NaN -- does not reach it.
+ * Scores, the softmax's maximum and sum and the sums over v are f32; the probabilities are rounded to the cache's dtype for
+ * the product with v (half an ulp each; f16's keep that down to 2^-25 of the row's largest), the result once.
  * Any number of rows per sequence: one (a decode step), a drafted tree, a prompt chunk. */
 exl3_verdict exl3_tree_attention(const exl3_kv_cache *cache, int32_t layer, const exl3_tree_batch *batch,
                                  const exl3_heads *q, float scale, void *stream, const exl3_heads *out, float *lse);

@@ -65,7 +65,8 @@ struct AttnParams {
 // Rows per kv head up to which the few-row kernel runs: its one 16-row tile, or half of it with 256-wide heads.  Measured,
 // few-row / tensor-core kernel: 32 sequences over 1500-9001 slots, 128-wide heads, 4 rows 121 / 130 us, 16 rows 128 / 136,
 // 20 rows (two tiles, K and V read twice) 215 / 141; 64-wide, 8 rows 55 / 63; five sequences over 20-33k slots, 256-wide, 2
-// rows 174 / 180, 8 rows 180 / 180, up to 16 rows 192 / 182; one token over 301 slots 14 / 18.
+// rows 174 / 180, 8 rows 180 / 180, up to 16 rows 192 / 182; one token over 301 slots 14 / 18 (one call between two events;
+// the other figures likewise).
 constexpr int attn_few_rows(int dim) { return dim == 256 ? 8 : 16; }
 // the tensor-core kernel (exl3_attn_tc.cu) and the few-row kernel (exl3_attn_mma.cu)
 cudaError_t launch_attn_tc(const AttnParams& p, int dim, int sms, size_t partial_floats, cudaStream_t st);

@@ -22,9 +22,10 @@
 // cannot be masked there (0 x inf = NaN), so in the tiles that hold such keys the cleaning warp zeroes slots past the
 // sequence and infinities and NaN; the latter are added back in the epilogue to the rows that see them.
 //
-// What bounds it: up to 128 rows HBM (32 sequences' 16-token trees over 4-8k slots: 147 us, 5.5 TB/s); with 256 rows the
-// softmax warps, whose chain with the products of their buffer is 3.4k clocks per 256 x 128 scores against 2.0k of
-// either the exponentials or the products alone (a 4096-row chunk on 4096 slots: 381 us, 1.08 PFLOP/s).
+// What bounds it: up to 128 rows HBM (32 sequences' 16-token trees over 4-8k slots: 148 us, 5.5 TB/s; 154 us, 5.2 TB/s back
+// to back); with 256 rows the softmax warps, whose chain with the products of their buffer is 3.4k clocks per 256 x 128
+// scores against 2.0k of either the exponentials or the products alone (a 4096-row chunk on 4096 slots: 386 us, 1.07 PFLOP/s;
+// back to back, where power limits the clock, 420 us, 0.98 PFLOP/s).
 //
 // Every mbarrier wait is bounded (wait_bar): one that gives up raises an abort flag that all roles poll.
 #include <cuda.h>

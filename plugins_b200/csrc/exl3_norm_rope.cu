@@ -8,7 +8,8 @@
 // and the rotation's partner element are shuffles inside them; the row's sines and cosines stay in registers over its
 // heads.  The angle is reduced to turns in f64 (its error is the
 // product's rounding, also at long positions) and its sine and cosine are shared through shared memory by all heads of
-// the row.  Measured: 8192 rows of 48 128-wide heads, bf16: 58-63 us (3.2-3.5 TB/s; the same path as a bare copy 45 us).
+// the row.  Measured: 8192 rows of 48 128-wide heads, bf16: 56 us in a graph (3.6 TB/s; the same path as a bare copy 45 us,
+// one call between events 63).
 #include <cuda_runtime.h>
 
 #include "exl3_attn.h"
@@ -20,10 +21,15 @@ namespace exl3 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxRowsPerCta = 8;  // measured at 8192 rows of 48 heads: 2 / 4 / 6 / 8 / 16 rows 74 / 64 / 68 / 63 / 72 us
+// Measured at 8192 rows of 48 heads: 2 / 4 / 6 / 8 / 16 rows 74 / 64 / 68 / 63 / 72 us.  The steps are those of the waves (9.2,
+// 4.6, 3.1, 2.3, 1.2): no number is best for every count of rows; 8 pays the search and the fill once for enough of them.
+constexpr int kMaxRowsPerCta = 8;
 constexpr int kCtasPerSm = 3;
 constexpr int kDepth = 2;  // rows a thread has in flight
-constexpr int kBatch = 3;  // head vectors a thread has in flight
+// Head vectors a thread has in flight.  Measured at 8190 rows, 2 / 3 / 4 of them: 48 vectors of 128, bf16, which are three
+// passes, 70 / 63 / 74 us; 32 of them 47 / 51 / 61; 64 of them 80 / 90 / 88; 32 f32 vectors of 256, four passes, 121 / 155 /
+// 172.  So 3 where it divides the passes, else 2 would be the better: one number serves all as yet.
+constexpr int kBatch = 3;
 constexpr int64_t kOutside = -1;  // the row's slot is not in the table
 constexpr int64_t kPadding = -2;  // no sequence owns the row
 constexpr double kInvTwoPi = 0.15915494309189533576888;
