@@ -284,3 +284,55 @@ def test_a_page_without_references_is_free_to_every_call(A):
     packed = A.cache_compact(cache, state)
     assert packed.table.tolist() == [[1, -1, -1], [0, -1, -1]] and packed.refs.tolist() == [1, 1, 0, 0, 0, 0]
     assert torch.equal(cache.k[:, 0], k[:, 4])
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_chains_of_page_calls_keep_every_rows_tokens(A, seed):
+    """Grow (also for more than is kept), append, keep in place, fork, compact and lengths cut back, in a random order: every
+    row's tokens, in every layer, are those it was given, and no page a row grew into is another's."""
+    r = random.Random(seed)
+    page, layers, kv_heads, pages, width = r.choice([16, 32]), 3, 2, 200, 8
+    cache = A.KvCache(*(torch.zeros((layers, pages, kv_heads, page, 64), dtype=torch.float16, device="cuda") for _ in range(2)))
+    tokens, state, copy, last = [[] for _ in range(5)], A.PageState.empty(cache, 5, width), A.NormRope(None), 0
+    for _ in range(60):
+        what, n = r.choice(["grow", "grow", "grow", "fork", "compact", "cut"]), len(tokens)
+        if what == "grow":
+            rows = [min(r.choice([0, 1, r.randrange(1, 40)]), width * page - len(t)) for t in tokens]
+            need = [min(len(t) + c + r.choice([0, 0, page, 50]), width * page) for t, c in zip(tokens, rows)]
+            grown, missing = A.cache_grow(cache, state, i32(need))
+            if int(missing) or not sum(rows):
+                continue
+            state = grown
+            held = [row[:h] for row, h in zip(state.table.tolist(), state.held.tolist())]
+            apart(held, state.refs.tolist(), [len(t) for t in tokens], need, page)
+            start = [0]
+            for c in rows:
+                start.append(start[-1] + c)
+            new = [(last + i) % 2000 for i in range(start[-1])]
+            last += start[-1]
+            batch = A.TreeBatch(i32(start), state.lens, state.table, max_rows=max(rows), rows=start[-1])
+            x = torch.tensor(new, device="cuda").half()[:, None, None].expand(-1, kv_heads, 64).contiguous()
+            for layer in range(layers):
+                A.qk_norm_rope(cache, layer, batch, x, x, x + layer + 1, copy)
+            path = [sorted(r.sample(range(c), r.randrange(c + 1))) for c in rows]
+            deep = max(1, *map(len, path))
+            A.cache_keep(cache, batch, i32([p + [-1] * (deep - len(p)) for p in path]), i32([len(p) for p in path]),
+                         out=state.lens)
+            for t, p, a in zip(tokens, path, start):
+                t += [new[a + j] for j in p]
+        elif what == "fork":
+            parent = [r.randrange(-1, n) for _ in range(r.randrange(1, 9))]
+            state = A.cache_fork(cache, state, i32(parent))
+            tokens = [list(tokens[p]) if p >= 0 else [] for p in parent]
+        elif what == "compact":
+            state = A.cache_compact(cache, state)
+        else:
+            tokens = [t[:r.randrange(len(t) + 1)] if r.random() < 0.3 else t for t in tokens]
+            state.lens.copy_(i32([len(t) for t in tokens]))
+        assert state.lens.tolist() == [len(t) for t in tokens]
+        for row, t in zip(state.table.cpu().long(), tokens):
+            at = torch.arange(len(t))
+            want = torch.tensor(t, dtype=torch.float16)[:, None, None]
+            k, v = (p.cpu()[:, row[at // page], :, at % page] for p in (cache.k, cache.v))
+            assert bool((k == want[..., None]).all())
+            assert bool((v == (want + torch.arange(1, layers + 1).half()[:, None])[..., None]).all())
