@@ -605,6 +605,41 @@ exl3_verdict exl3_cache_keep(const exl3_kv_cache *cache, const exl3_tree_batch *
 exl3_verdict exl3_cache_compact(const exl3_kv_cache *cache, const exl3_page_state *in, void *stream,
                                 const exl3_page_state *out);
 
+/* One step's drafted tokens.  Row 0 of a sequence is its newest token, the others are drafts: row i continues row
+ * parent[i] < i of its own sequence (without `parent`, row i - 1).  logits row r is the target's for what follows row r;
+ * draft row r (or null: a drafter without probabilities) the probabilities that row r's children were drawn from. */
+typedef struct exl3_draft {
+  uint32_t size;            /* sizeof(exl3_draft) */
+  int32_t vocab;            /* 1 .. 393216 */
+  int32_t logits_dtype;     /* EXL3_F16, EXL3_BF16 or EXL3_F32 */
+  int32_t draft_dtype;      /* likewise */
+  int64_t logits_stride;    /* elements from row to row */
+  int64_t draft_stride;
+  const void *logits;       /* device, [rows][vocab] */
+  const void *draft;        /* device, [rows][vocab], or null */
+  const int32_t *tokens;    /* device, [rows] (row 0's is not read) */
+  const int32_t *parent;    /* device, [rows], or null */
+  const float *uniform;     /* device, [rows][2], in [0, 1): for the row's own token, for the token that follows the row */
+  const float *temperature; /* device, [nseq], 0 (greedy) or a positive number, or null: 1 */
+} exl3_draft;
+
+/* Verification of drafted tokens: the path of accepted rows from row 0 down, and the token that follows it, together
+ * distributed as tokens drawn one by one from p = softmax(logits / temperature) -- whatever the drafter.  At a node, r = p
+ * and Z = 1.  Its children are tried in row order: row c with token x is accepted if uniform[c][0] q(x) Z < r(x) and is the
+ * next node; otherwise r becomes max(r - Z q, 0) and Z its sum (where nothing is left: p and 1 again).  Without draft, q is
+ * one at x.  Where no child is accepted the path ends, and the next token is the first v with
+ * sum_{w <= v} r(w) > uniform[node][1] Z (the last with r(v) > 0 where rounding leaves none).  Temperature 0: p and q are one
+ * at the largest logit (the lowest of equals) and at x.  A path ends at the latest at its `depth`-th row, whose children
+ * are not tried.
+ * path [nseq][depth] receives the accepted rows, ascending, -1 past them, kept [nseq] their number (row 0 counts; 0 for a
+ * sequence without rows), as exl3_cache_keep takes them; token [nseq] the token that follows (-1: no rows, or no logit above
+ * -inf).  Logits: NaN counts as -inf, +inf as the largest finite number, and a token 2^-100 below the likeliest has no
+ * probability; draft: NaN and negative numbers count as 0; a child whose token is outside the vocabulary is not tried.
+ * Exponentials are f32 to a few ulp, their sums, r and Z f64.  At most 1024 rows a sequence.  The batch's context and table
+ * are not read. */
+exl3_verdict exl3_draft_verify(const exl3_kv_cache *cache, const exl3_tree_batch *batch, const exl3_draft *draft,
+                               void *stream, int32_t *path, int32_t depth, int32_t *kept, int32_t *token);
+
 /* Device error bits the kernels recorded on `device`; `clear` resets them. */
 #define EXL3_ERR_WAIT_TIMEOUT 1u  /* a bounded mbarrier wait gave up (the kernel left its loop and returned) */
 #define EXL3_ERR_BAD_SHAPE 2u     /* a launch saw a shape its host validation should have refused */

@@ -42,7 +42,7 @@ EXPORTS = (
     "exl3_model_claims", "exl3_model_parse", "exl3_model_bill", "exl3_model_load", "exl3_model_unload",
     "exl3_model_weight", "exl3_model_linear", "exl3_model_linears", "exl3_model_mlp", "exl3_model_experts", "exl3_resident", "exl3_resident_pending",
     "exl3_kv_register", "exl3_qk_norm_rope", "exl3_tree_attention", "exl3_cache_fork", "exl3_cache_grow",
-    "exl3_cache_keep", "exl3_cache_compact",
+    "exl3_cache_keep", "exl3_cache_compact", "exl3_draft_verify",
 )
 
 
@@ -154,6 +154,14 @@ class PageState(ctypes.Structure):
     _fields_ = [("size", ctypes.c_uint32), ("nseq", ctypes.c_int32), ("max_pages", ctypes.c_int32),
                 ("refs", ctypes.c_void_p), ("table", ctypes.c_void_p), ("held", ctypes.c_void_p),
                 ("lens", ctypes.c_void_p)]
+
+
+class Draft(ctypes.Structure):
+    """exl3_draft: a step's drafted tokens, the target's logits and the drafter's probabilities."""
+    _fields_ = [("size", ctypes.c_uint32), ("vocab", ctypes.c_int32), ("logits_dtype", ctypes.c_int32),
+                ("draft_dtype", ctypes.c_int32), ("logits_stride", ctypes.c_int64), ("draft_stride", ctypes.c_int64),
+                ("logits", ctypes.c_void_p), ("draft", ctypes.c_void_p), ("tokens", ctypes.c_void_p),
+                ("parent", ctypes.c_void_p), ("uniform", ctypes.c_void_p), ("temperature", ctypes.c_void_p)]
 
 
 _lock = threading.Lock()
@@ -331,6 +339,9 @@ def lib() -> ctypes.CDLL:
                                           ctypes.c_void_p, ctypes.c_void_p]
             L.exl3_cache_compact.restype = Verdict
             L.exl3_cache_compact.argtypes = [P(KvCache), P(PageState), ctypes.c_void_p, P(PageState)]
+            L.exl3_draft_verify.restype = Verdict
+            L.exl3_draft_verify.argtypes = [P(KvCache), P(TreeBatch), P(Draft), ctypes.c_void_p, ctypes.c_void_p,
+                                            ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]
             L.exl3_version.restype = ctypes.c_char_p
             L.exl3_version.argtypes = []
             _lib = L

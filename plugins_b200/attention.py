@@ -24,7 +24,7 @@ from ._lib import Exl3Error, check
 from .quant import _TORCH_DT, _stream
 
 __all__ = ["Exl3Error", "KvCache", "TreeBatch", "NormRope", "PageState", "qk_norm_rope", "tree_attention", "cache_fork",
-           "cache_grow", "cache_keep", "cache_compact"]
+           "cache_grow", "cache_keep", "cache_compact", "draft_verify"]
 
 
 def _refuse(why: str, code: int = L.EXL3_FAILED):
@@ -378,3 +378,64 @@ def cache_compact(cache: KvCache, state: PageState, out: PageState | None = None
         _used_on(stream, cache.k, cache.v, *state._tensors(), *out._tensors())
     check(L.lib().exl3_cache_compact(cache.raw, state.raw, _on(stream, cache._index), out.raw))
     return out
+
+
+def _floats(t, shape, what: str, device):
+    """A contiguous f32 GPU tensor of this shape."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != device or not t.is_contiguous():
+        _refuse(f"{what} is a contiguous f32 tensor on the cache's GPU")
+    if tuple(t.shape) != tuple(shape):
+        _refuse(f"{what} has shape {list(t.shape)}, not {list(shape)}")
+
+
+def _vocab_rows(t, rows: int, vocab, what: str, device):
+    """[rows, vocab] with contiguous rows -> its dtype."""
+    if not isinstance(t, torch.Tensor) or t.device != device or t.dim() != 2 or t.shape[0] != rows or \
+            (vocab is not None and t.shape[1] != vocab) or (t.stride(1) != 1 and t.shape[1] > 1):
+        _refuse(f"{what} is [rows, vocab] on the cache's GPU, its rows contiguous")
+    dt = _TORCH_DT.get(t.dtype)
+    if dt not in (L.F16, L.BF16, L.F32):
+        _refuse(f"{what} is f16, bf16 or f32", L.EXL3_UNSUPPORTED)
+    return dt
+
+
+def draft_verify(cache: KvCache, batch: TreeBatch, logits, tokens, parent, uniform, temperature=None, draft=None,
+                 depth: int | None = None, path=None, kept=None, token=None, stream=None):
+    """Which drafted tokens stay, and the token after them -> (``path`` [nseq, depth], ``kept`` [nseq], as
+    :func:`cache_keep` takes them, ``token`` [nseq]; int32).
+
+    Row 0 of a sequence is its newest token, the others are drafts: ``tokens`` (int32 [rows]) and ``parent`` (int32 [rows],
+    rows of the same sequence, a parent before its children; None: chains).  ``logits`` [rows, vocab]: the target's, f16, bf16
+    or f32; ``draft`` [rows, vocab]: the probabilities that the children of each row were drawn from (None: a drafter without
+    any).  ``uniform`` (f32 [rows, 2], in [0, 1)): a number for the row's own token and one for the token that follows the
+    row.  ``temperature`` (f32 [nseq], 0: greedy; None: 1).  The path and the token are distributed as tokens drawn one by one
+    from softmax(logits / temperature).  ``depth``: the most rows of a path (max_rows, if not given)."""
+    dev, n = cache.device, batch.nseq
+    rows = batch.rows if batch.rows is not None else logits.shape[0]
+    dt = _vocab_rows(logits, rows, None, "logits", dev)
+    vocab = logits.shape[1]
+    qt = L.F32 if draft is None else _vocab_rows(draft, rows, vocab, "draft", dev)
+    _ints(tokens, (rows,), "tokens", dev)
+    _ints(parent, (rows,), "parent", dev, optional=True)
+    _floats(uniform, (rows, 2), "uniform", dev)
+    if temperature is not None:
+        _floats(temperature, (n,), "temperature", dev)
+    depth = max(1, batch.raw.max_rows if depth is None else int(depth))
+    make = _maker(stream, torch.empty)
+    if path is None and kept is None and token is None:  # one allocation
+        path, kept, token = make(n * (depth + 2), dtype=torch.int32, device=dev).split_with_sizes((n * depth, n, n))
+        path = path.view(n, depth)
+    else:
+        path = make((n, depth), dtype=torch.int32, device=dev) if path is None else _ints(path, (n, depth), "path", dev)
+        kept = make(n, dtype=torch.int32, device=dev) if kept is None else _ints(kept, (n,), "kept", dev)
+        token = make(n, dtype=torch.int32, device=dev) if token is None else _ints(token, (n,), "token", dev)
+    batch._for(cache, rows)
+    if stream is not None:
+        _used_on(stream, logits, tokens, parent, uniform, temperature, draft, path, kept, token, *batch._keep)
+    raw = L.Draft(ctypes.sizeof(L.Draft), vocab, dt, qt, logits.stride(0), 0 if draft is None else draft.stride(0),
+                  logits.data_ptr(), None if draft is None else draft.data_ptr(), tokens.data_ptr(),
+                  None if parent is None else parent.data_ptr(), uniform.data_ptr(),
+                  None if temperature is None else temperature.data_ptr())
+    check(L.lib().exl3_draft_verify(cache.raw, batch.raw, raw, _on(stream, cache._index), path.data_ptr(), depth,
+                                    kept.data_ptr(), token.data_ptr()))
+    return path, kept, token

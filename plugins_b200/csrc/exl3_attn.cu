@@ -413,4 +413,53 @@ exl3_verdict exl3_cache_keep(const exl3_kv_cache* cache, const exl3_tree_batch* 
   return launched(exl3::launch_cache_keep(p, ws.counter_count, static_cast<cudaStream_t>(stream)));
 }
 
+exl3_verdict exl3_draft_verify(const exl3_kv_cache* cache, const exl3_tree_batch* batch, const exl3_draft* draft,
+                               void* stream, int32_t* path, int32_t depth, int32_t* kept, int32_t* token) {
+  exl3_verdict r = check_cache(cache);
+  if (r.code != EXL3_OK || (r = check_batch(batch)).code != EXL3_OK) return r;
+  if (!draft || draft->size != sizeof(exl3_draft)) return refuse(EXL3_FAILED, "exl3_b200: not a draft");
+  if (draft->vocab < 1) return refuse(EXL3_FAILED, "exl3_b200: an empty vocabulary");
+  if (draft->vocab > exl3::kDraftMaxVocab) return refuse(EXL3_TOO_LARGE, "exl3_b200: a vocabulary of more than 393216 tokens");
+  const auto floats = [](int32_t t) { return t == EXL3_F16 || t == EXL3_BF16 || t == EXL3_F32; };
+  if (!floats(draft->logits_dtype) || (draft->draft && !floats(draft->draft_dtype)))
+    return refuse(EXL3_UNSUPPORTED, "exl3_b200: logits and draft are f16, bf16 or f32");
+  if (depth < 1) return refuse(EXL3_FAILED, "exl3_b200: a path without depth");
+  if (batch->max_rows > batch->rows) return refuse(EXL3_FAILED, "exl3_b200: max_rows is above the batch's rows");
+  if (batch->nseq == 0) return kOk;
+  const int32_t max_rows = batch->max_rows > 0 ? batch->max_rows : batch->rows;
+  if (max_rows > exl3::kDraftMaxRows) return refuse(EXL3_TOO_LARGE, "exl3_b200: more than 1024 drafted rows of one sequence");
+  if (!path || !kept || !token || (batch->rows > 0 && (!draft->logits || !draft->tokens || !draft->uniform)))
+    return refuse(EXL3_FAILED, "exl3_b200: verify without its arrays");
+  const auto width = [](int32_t t) { return t == EXL3_F32 ? 4 : 2; };
+  if (reinterpret_cast<uintptr_t>(draft->logits) % width(draft->logits_dtype) ||
+      reinterpret_cast<uintptr_t>(draft->draft) % width(draft->draft_dtype))
+    return refuse(EXL3_UNSUPPORTED, "exl3_b200: logits and draft lie on multiples of their elements");
+  const int64_t rows = batch->rows, n = batch->nseq;
+  const exl3_heads x{const_cast<void*>(draft->logits), draft->logits_dtype, batch->rows, 1, draft->vocab, draft->logits_stride, 0};
+  const exl3_heads q{const_cast<void*>(draft->draft), draft->draft_dtype, batch->rows, 1, draft->vocab, draft->draft_stride, 0};
+  const Runs read[] = {runs_of(&x), draft->draft ? runs_of(&q) : runs_of(nullptr, 0), runs_of(draft->tokens, rows * 4),
+                       runs_of(draft->parent, draft->parent ? rows * 4 : 0), runs_of(draft->uniform, rows * 8),
+                       runs_of(draft->temperature, draft->temperature ? n * 4 : 0), runs_of(batch->row_start, (n + 1) * 4)};
+  const Runs made[] = {runs_of(path, n * depth * 4), runs_of(kept, n * 4), runs_of(token, n * 4)};
+  for (int i = 0; i < 3; ++i) {
+    for (const Runs& o : read)
+      if (rows > 0 && meet(made[i], o)) return refuse(EXL3_FAILED, "exl3_b200: verify's results lie over its arguments");
+    for (int j = 0; j < i; ++j)
+      if (meet(made[i], made[j])) return refuse(EXL3_FAILED, "exl3_b200: verify's results lie over one another");
+  }
+  exl3::Workspace ws;
+  if (!exl3::workspace_get(cache->device, ws)) return kNoWorkspace;
+  OnDevice guard(cache->device);
+  exl3::DraftParams p{};
+  p.logits = draft->logits, p.draft = draft->draft;
+  p.logits_stride = draft->logits_stride, p.draft_stride = draft->draft_stride;
+  p.logits_dtype = draft->logits_dtype, p.draft_dtype = draft->draft_dtype;
+  p.rows = batch->rows, p.max_rows = max_rows, p.vocab = draft->vocab, p.depth = depth;
+  p.row_start = batch->row_start, p.tokens = draft->tokens, p.parent = draft->parent;
+  p.uniform = draft->uniform, p.temperature = draft->temperature;
+  p.path = path, p.kept = kept, p.token = token;
+  p.err = ws.err;
+  return launched(exl3::launch_draft_verify(p, batch->nseq, static_cast<cudaStream_t>(stream)));
+}
+
 }  // extern "C"

@@ -106,6 +106,22 @@ struct KeepParams {
 };
 cudaError_t launch_cache_keep(const KeepParams& p, uint32_t counters, cudaStream_t st);
 
+constexpr int kDraftMaxRows = 1024;     // rows of one sequence
+constexpr int kDraftMaxVocab = 393216;  // a slice of an eighth, as f32, fits in shared memory
+struct DraftParams {
+  const void *logits, *draft;  // [rows][vocab]; draft may be null
+  int64_t logits_stride, draft_stride;
+  int32_t logits_dtype, draft_dtype;
+  int32_t rows, max_rows, vocab;
+  int32_t slice;               // the vocabulary's share of a CTA
+  int32_t depth;
+  const int32_t *row_start, *tokens, *parent;
+  const float *uniform, *temperature;
+  int32_t *path, *kept, *token;
+  uint32_t* err;
+};
+cudaError_t launch_draft_verify(const DraftParams& p, int nseq, cudaStream_t st);
+
 #if defined(__CUDACC__)
 // The sequence that owns `row`: the last s with row_start[s] <= row (empty sequences own none).  Called by a whole warp;
 // 32-way search, so two loads deep up to 1024 sequences.
