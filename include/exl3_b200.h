@@ -563,6 +563,27 @@ exl3_verdict exl3_qk_norm_rope(const exl3_kv_cache *cache, int32_t layer, const 
 exl3_verdict exl3_tree_attention(const exl3_kv_cache *cache, int32_t layer, const exl3_tree_batch *batch,
                                  const exl3_heads *q, float scale, void *stream, const exl3_heads *out, float *lse);
 
+/* How much each cached token was attended to: f32 weights of a row's slots in order, head h of row r of layer l at
+ * data + l * layer_stride + r * row_stride + h * head_stride (elements).  They go by the row's slots and not by pages, so
+ * rows that share pages have their own (a fork copies its parent's rows). */
+typedef struct exl3_kv_weight {
+  uint32_t size;   /* sizeof(exl3_kv_weight) */
+  int32_t layers, nseq;
+  int32_t slots;   /* >= 1 */
+  float *data;     /* device, [layers][nseq][kv_heads][slots] */
+  int64_t layer_stride, row_stride, head_stride;
+} exl3_kv_weight;
+
+/* Accumulates one layer's attention into `weight` (layers 1, the batch's nseq): for every sequence with rows and its slots
+ * j < context + rows, w[j] becomes (j < context ? decay * w[j] : 0) + sum exp(scale q[r][h] . k[j] - lse[r][h]) over the rows
+ * r that see slot j and the query heads h of the kv head.  q, scale and lse are exl3_tree_attention's (call it first); a row
+ * whose lse is -inf saw nothing and adds nothing, decay 0 does not read w.  0 <= decay <= 1.  What lies in other slots, or in
+ * rows that do not see a slot, does not reach its weight; other sequences' and slots' weights stay.  Products and sums are
+ * f32, in an order that does not vary.  Slots from `slots` on have no weight (EXL3_ERR_BAD_SHAPE is recorded). */
+exl3_verdict exl3_attention_weight(const exl3_kv_cache *cache, int32_t layer, const exl3_tree_batch *batch,
+                                   const exl3_heads *q, float scale, const float *lse, float decay, void *stream,
+                                   const exl3_kv_weight *weight);
+
 /* The host's page bookkeeping, on the device: how many rows refer to each page (none: free), each row's page ids (-1 past
  * its `held` pages), and its tokens. */
 typedef struct exl3_page_state {

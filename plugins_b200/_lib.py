@@ -42,7 +42,7 @@ EXPORTS = (
     "exl3_model_claims", "exl3_model_parse", "exl3_model_bill", "exl3_model_load", "exl3_model_unload",
     "exl3_model_weight", "exl3_model_linear", "exl3_model_linears", "exl3_model_mlp", "exl3_model_experts", "exl3_resident", "exl3_resident_pending",
     "exl3_kv_register", "exl3_qk_norm_rope", "exl3_tree_attention", "exl3_cache_fork", "exl3_cache_grow",
-    "exl3_cache_keep", "exl3_cache_compact", "exl3_draft_verify",
+    "exl3_cache_keep", "exl3_cache_compact", "exl3_draft_verify", "exl3_attention_weight",
 )
 
 
@@ -154,6 +154,13 @@ class PageState(ctypes.Structure):
     _fields_ = [("size", ctypes.c_uint32), ("nseq", ctypes.c_int32), ("max_pages", ctypes.c_int32),
                 ("refs", ctypes.c_void_p), ("table", ctypes.c_void_p), ("held", ctypes.c_void_p),
                 ("lens", ctypes.c_void_p)]
+
+
+class KvWeight(ctypes.Structure):
+    """exl3_kv_weight: how much each cached token was attended to, strides in elements."""
+    _fields_ = [("size", ctypes.c_uint32), ("layers", ctypes.c_int32), ("nseq", ctypes.c_int32),
+                ("slots", ctypes.c_int32), ("data", ctypes.c_void_p), ("layer_stride", ctypes.c_int64),
+                ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
 
 
 class Draft(ctypes.Structure):
@@ -339,6 +346,9 @@ def lib() -> ctypes.CDLL:
                                           ctypes.c_void_p, ctypes.c_void_p]
             L.exl3_cache_compact.restype = Verdict
             L.exl3_cache_compact.argtypes = [P(KvCache), P(PageState), ctypes.c_void_p, P(PageState)]
+            L.exl3_attention_weight.restype = Verdict
+            L.exl3_attention_weight.argtypes = [P(KvCache), ctypes.c_int32, P(TreeBatch), ctypes.c_char_p, ctypes.c_float,
+                                                ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p, P(KvWeight)]
             L.exl3_draft_verify.restype = Verdict
             L.exl3_draft_verify.argtypes = [P(KvCache), P(TreeBatch), P(Draft), ctypes.c_void_p, ctypes.c_void_p,
                                             ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]

@@ -24,7 +24,7 @@ from ._lib import Exl3Error, check
 from .quant import _TORCH_DT, _stream
 
 __all__ = ["Exl3Error", "KvCache", "TreeBatch", "NormRope", "PageState", "qk_norm_rope", "tree_attention", "cache_fork",
-           "cache_grow", "cache_keep", "cache_compact", "draft_verify"]
+           "cache_grow", "cache_keep", "cache_compact", "draft_verify", "attention_weight"]
 
 
 def _refuse(why: str, code: int = L.EXL3_FAILED):
@@ -272,6 +272,36 @@ def tree_attention(cache: KvCache, layer: int, batch: TreeBatch, q, scale: float
     _check(_Calls.attention(cache._at, layer, batch._for(cache, q.shape[0]), hq, cache._scale if scale is None else scale,
                             _on(stream, i), ho, None if lse is None else lse.data_ptr()))
     return out if lse is None else (out, lse)
+
+
+def _kv_weight(t, layers: int, nseq: int, cache: KvCache) -> L.KvWeight:
+    """[layers, nseq, kv_heads, slots] f32 on the cache's GPU, a head's slots contiguous."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != cache.device or t.dim() != 4:
+        _refuse("weights are f32 [layers, rows, kv_heads, slots] on the cache's GPU")
+    if tuple(t.shape[:3]) != (layers, nseq, cache.raw.kv_heads):
+        _refuse(f"the weights have shape {list(t.shape)}, not {[layers, nseq, cache.raw.kv_heads, 'any']}")
+    if t.stride(3) != 1 and t.shape[3] > 1:
+        _refuse("the weights of a head's slots must be contiguous")
+    return L.KvWeight(ctypes.sizeof(L.KvWeight), layers, nseq, t.shape[3], t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+
+
+def attention_weight(cache: KvCache, layer: int, batch: TreeBatch, q, lse, weight, scale: float | None = None,
+                     decay: float = 1.0, stream=None):
+    """How much the batch's rows attended to each cached token of ``layer``, added to ``weight`` (f32
+    [nseq, kv_heads, slots], in place, returned): slots of the context keep ``decay`` of what they had, the rows' own slots
+    begin anew.  ``q``, ``scale`` and ``lse`` (f32 [rows, heads]) are :func:`tree_attention`'s, which comes first."""
+    i = cache._index
+    hq = _heads(q, i, "q")
+    _floats(lse, q.shape[:2], "lse", cache.device)
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 3:
+        _refuse("a layer's weights are f32 [nseq, kv_heads, slots]")
+    raw = _kv_weight(weight[None], 1, batch.nseq, cache)
+    if stream is not None:
+        _used_on(stream, q, lse, weight, cache.k, cache.v, *batch._keep)
+    batch._for(cache, q.shape[0])
+    check(L.lib().exl3_attention_weight(cache.raw, layer, batch.raw, hq, cache._scale if scale is None else scale,
+                                        lse.data_ptr(), decay, _on(stream, i), raw))
+    return weight
 
 
 class PageState:

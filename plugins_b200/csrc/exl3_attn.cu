@@ -244,6 +244,25 @@ exl3_verdict page_params(const exl3_kv_cache* cache, const exl3_page_state* in, 
   return kOk;
 }
 
+// `weight`: what a row's slots and heads span, one after the other or in any other order of nested strides.
+exl3_verdict check_weight(const exl3_kv_weight* w, int32_t layers, int32_t nseq, int32_t kv_heads, int64_t* bytes) {
+  if (!w || w->size != sizeof(exl3_kv_weight)) return refuse(EXL3_FAILED, "exl3_b200: not a cache's weights");
+  if (w->layers != layers || w->nseq != nseq) return refuse(EXL3_FAILED, "exl3_b200: the weights have other layers or rows");
+  if (w->slots < 1) return refuse(EXL3_FAILED, "exl3_b200: weights without slots");
+  if (nseq > 0 && !w->data) return refuse(EXL3_FAILED, "exl3_b200: not a cache's weights");
+  if (reinterpret_cast<uintptr_t>(w->data) % 4) return refuse(EXL3_UNSUPPORTED, "exl3_b200: weights lie on multiples of 4 bytes");
+  std::pair<int64_t, int64_t> dims[3] = {{w->head_stride, kv_heads}, {w->row_stride, nseq}, {w->layer_stride, layers}};
+  std::sort(dims, dims + 3);
+  int64_t span = w->slots;
+  for (const auto& d : dims) {
+    if (d.second <= 1) continue;
+    if (d.first < span) return refuse(EXL3_FAILED, "exl3_b200: weights overlap");
+    span += d.first * (d.second - 1);
+  }
+  *bytes = nseq > 0 ? span * 4 : 0;
+  return kOk;
+}
+
 }  // namespace
 
 extern "C" {
@@ -337,6 +356,50 @@ exl3_verdict exl3_tree_attention(const exl3_kv_cache* cache, int32_t layer, cons
   const bool few = static_cast<int64_t>(p.max_rows) * p.group <= exl3::attn_few_rows(dim);
   return launched((few ? exl3::launch_attn_mma : exl3::launch_attn_tc)(p, dim, ws.sms, ws.partial_floats,
                                                                        static_cast<cudaStream_t>(stream)));
+}
+
+exl3_verdict exl3_attention_weight(const exl3_kv_cache* cache, int32_t layer, const exl3_tree_batch* batch,
+                                   const exl3_heads* q, float scale, const float* lse, float decay, void* stream,
+                                   const exl3_kv_weight* weight) {
+  exl3_verdict r = check_layer(cache, layer);
+  if (r.code != EXL3_OK || (r = check_batch(batch)).code != EXL3_OK) return r;
+  const int32_t rows = batch->rows, dim = cache->head_dim;
+  if ((r = check_heads(q, "exl3_b200: q is [rows, heads, head_dim]", rows, dim)).code != EXL3_OK) return r;
+  if (q->dtype != cache->dtype) return refuse(EXL3_UNSUPPORTED, "exl3_b200: q has the cache's dtype");
+  if (q->heads % cache->kv_heads) return refuse(EXL3_FAILED, "exl3_b200: q has a whole number of heads per kv head");
+  if (q->heads > 4096) return refuse(EXL3_TOO_LARGE, "exl3_b200: more than 4096 query heads");
+  if (static_cast<int64_t>(rows) * q->heads > (1ll << 30)) return refuse(EXL3_TOO_LARGE, "exl3_b200: more than 2^30 query vectors");
+  if (!(scale > 0.f) || std::isinf(scale)) return refuse(EXL3_UNSUPPORTED, "exl3_b200: the scale is a positive number");
+  if (!(decay >= 0.f && decay <= 1.f)) return refuse(EXL3_UNSUPPORTED, "exl3_b200: the decay is between 0 and 1");
+  if (batch->max_rows > rows) return refuse(EXL3_FAILED, "exl3_b200: max_rows is above the batch's rows");
+  int64_t bytes = 0;
+  if ((r = check_weight(weight, 1, batch->nseq, cache->kv_heads, &bytes)).code != EXL3_OK) return r;
+  if (batch->nseq == 0 || rows == 0) return kOk;
+  if (!lse) return refuse(EXL3_FAILED, "exl3_b200: weights without the attention's log-sum-exp");
+  const int64_t n = batch->nseq;
+  const Runs w = runs_of(weight->data, bytes);
+  const Runs read[] = {runs_of(q), runs_of(lse, static_cast<int64_t>(rows) * q->heads * 4), runs_of(batch->row_start, n * 4 + 4),
+                       runs_of(batch->context, n * 4), runs_of(batch->table, n * 4 * batch->max_pages),
+                       runs_of(batch->tree, batch->tree ? rows * 4ll * batch->tree_words : 0)};
+  for (const Runs& o : read)
+    if (meet(w, o)) return refuse(EXL3_FAILED, "exl3_b200: the weights lie over the call's arguments");
+  exl3::Workspace ws;
+  if (!exl3::workspace_get(cache->device, ws)) return kNoWorkspace;
+  OnDevice guard(cache->device);
+  exl3::WeightParams p{};
+  p.a.b = paged(cache, layer, batch, ws.err);
+  p.a.q = view(q);
+  p.a.group = q->heads / cache->kv_heads;
+  p.a.bf16 = cache->dtype == EXL3_BF16;
+  p.a.max_rows = batch->max_rows > 0 ? batch->max_rows : rows;
+  const int64_t width = static_cast<int64_t>(batch->max_pages) * cache->page_size;
+  if (width > 0x7FFF0000) return refuse(EXL3_TOO_LARGE, "exl3_b200: the table spans 2^31 slots or more");
+  p.a.max_context = static_cast<int32_t>(batch->max_context > 0 && batch->max_context < width ? batch->max_context : width);
+  p.a.scale_log2 = scale * 1.4426950408889634f;
+  p.a.partials = ws.partials, p.a.counters = ws.counters;
+  p.lse = lse, p.w = weight->data, p.row_stride = weight->row_stride, p.head_stride = weight->head_stride;
+  p.slots = weight->slots, p.decay = decay;
+  return launched(exl3::launch_attn_weight(p, dim, ws.sms, ws.partial_floats, static_cast<cudaStream_t>(stream)));
 }
 
 exl3_verdict exl3_cache_fork(const exl3_kv_cache* cache, const exl3_page_state* in, const int32_t* parent, void* stream,

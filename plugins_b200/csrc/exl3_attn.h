@@ -72,6 +72,17 @@ constexpr int attn_few_rows(int dim) { return dim == 256 ? 8 : 16; }
 cudaError_t launch_attn_tc(const AttnParams& p, int dim, int sms, size_t partial_floats, cudaStream_t st);
 cudaError_t launch_attn_mma(const AttnParams& p, int dim, int sms, size_t partial_floats, cudaStream_t st);
 
+// The attention's parameters (out and lse unused), and one layer's weights [nseq][kv_heads][slots].
+struct WeightParams {
+  AttnParams a;
+  const float* lse;  // [rows][heads]
+  float* w;
+  int64_t row_stride, head_stride;
+  int32_t slots;
+  float decay;
+};
+cudaError_t launch_attn_weight(const WeightParams& p, int dim, int sms, size_t partial_floats, cudaStream_t st);
+
 struct PageParams {
   int32_t pages, page_shift;
   int32_t nseq_in, nseq_out, width_in, width_out;
