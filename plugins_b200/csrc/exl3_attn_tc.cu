@@ -33,6 +33,7 @@
 
 #include "exl3_attn.h"
 #include "exl3_attn_dev.cuh"
+#include "exl3_attn_tc.cuh"
 #include "exl3_common.cuh"
 #include "exl3_internal.h"
 #include "exl3_tc.cuh"
@@ -62,130 +63,6 @@ struct TcShape {
   static_assert(KS * kTile + VS * kTile + kQBytes <= 229376 && kSmem <= 232448, "shared memory");
   static_assert(VS <= 8, "the odd flags cover eight items");
 };
-
-// Two f32 in one 64-bit register pair: one issue slot for both.
-__device__ __forceinline__ uint64_t f2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void f2_split(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-// the largest of three (NaN is passed over: it shows in its own probability)
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
-// Bounded wait (about two seconds) that also gives up when another role has.  The abort flag and the clock are read once
-// in many polls: a read of the global timer between polls held each wait up, and every tile's chain has three of them
-// (32 x 16-token trees 207 us with it, 192 without).
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t* err) {
-  uint64_t t0 = 0;
-  for (uint32_t i = 1;; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 63u) != 0u) continue;
-    if (*abort_flag) return false;
-    if ((i & 1023u) != 0u) continue;
-    const uint64_t now = global_timer_ns();
-    if (t0 == 0) t0 = now;
-    else if (now - t0 > 2000000000ull) {
-      *abort_flag = 1u;
-      atomicOr(err, kErrWaitTimeout);
-      return false;
-    }
-  }
-}
-
-// A box of the cache: 64 columns from x, the rows from `tok` of one page and head.
-__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int tok, int head, int page,
-                                        uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
-          "r"(dst),
-      "l"(map), "r"(x), "r"(tok), "r"(head), "r"(page), "r"(smem_u32(bar))
-      : "memory");
-}
-
-// Shared-memory descriptor of an operand whose rows are k (keys) and whose contiguous direction is M or N: 64-element
-// blocks of 128-byte swizzled rows, `block_bytes` apart; 8-key groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t block_bytes) {
-  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>((block_bytes >> 4) & 0x3FFFu) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
-}
-
-// Instruction descriptor of kind::f16 with f32 accumulators; b_mn: B's contiguous direction is N.
-template <bool BF16>
-constexpr uint32_t attn_idesc(int m, int n, bool b_mn) {
-  return umma_idesc(m, n) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u);
-}
-
-// The MMA warp runs converged and one elected lane issues: its operands then stay in uniform registers.  (Issued inside
-// a one-lane branch, each MMA took some 100 clocks to issue, against the 64 it runs for: 4.1k clocks per 256 x 128 tile.)
-__device__ __forceinline__ uint32_t elect_one() {
-  uint32_t e;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xFFFFFFFF;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(e));
-  return e;
-}
-// The same value, known to the compiler to be one for the whole warp.
-__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xFFFFFFFFu, v, 0); }
-// A descriptor `bytes` further on (its address field counts 16 bytes in the low word).
-__device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t lo_add) {
-  return (desc & 0xFFFFFFFF00000000ull) | (static_cast<uint32_t>(desc) + lo_add);
-}
-// D[tmem] (+)= A[smem] * B[smem]^T, where `on`
-__device__ __forceinline__ void mma_ss(uint32_t on, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                       uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on)
-      : "memory");
-}
-// D[tmem] (+)= A[tmem] * B[smem], where `on`
-__device__ __forceinline__ void mma_ts(uint32_t on, uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                       uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on)
-      : "memory");
-}
-// Arrives on `bar` when every tcgen05 operation the elected lane issued before has completed.
-__device__ __forceinline__ void commit(uint32_t on, uint64_t* bar) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\t"
-      "setp.ne.b32 q, %1, 0;\n\t"
-      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
-      "r"(on)
-      : "memory");
-}
-
-// Orders uses of registers loaded by tmem_ld32 after an earlier wait (tmem_wait_ld of another load).
-__device__ __forceinline__ void after_wait(uint32_t (&r)[32]) {
-#pragma unroll
-  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i])::"memory");
-}
 
 // Moves registers from the copy and MMA warps to the softmax warps: a row's 128 scores stay in registers.  The shares
 // (8 x 32 x 200 + 4 x 32 x 104 = 64512) are what 384 threads were launched with (168 each).
@@ -856,24 +733,6 @@ EncodeFn encode_fn() {
   return fn;
 }
 
-// The layer's K or V as [pages][kv_heads][page_size][dim], in boxes of 64 columns by min(page_size, key tile) rows.
-bool encode(CUtensorMap& map, void* base, const AttnParams& p, int dim, int tile_keys) {
-  const EncodeFn fn = encode_fn();
-  if (!fn) return false;
-  const cuuint64_t page = 1ull << p.b.page_shift;
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(dim), page, static_cast<cuuint64_t>(p.b.kv_heads),
-                              static_cast<cuuint64_t>(p.b.pages)};
-  // (a dimension of one takes no steps: its stride need not mean anything)
-  const cuuint64_t row = static_cast<cuuint64_t>(p.b.token_stride) * 2;
-  const cuuint64_t strides[3] = {row, p.b.kv_heads > 1 ? static_cast<cuuint64_t>(p.b.head_stride) * 2 : row,
-                                 p.b.pages > 1 ? static_cast<cuuint64_t>(p.b.page_stride) * 2 : row};
-  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(page < static_cast<cuuint64_t>(tile_keys) ? page : tile_keys), 1, 1};
-  const cuuint32_t step[4] = {1, 1, 1, 1};
-  return fn(&map, p.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims, strides, box,
-            step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int D, int ROWS>
 cudaError_t launch_dim(const AttnParams& p, int sms, size_t partial_floats, cudaStream_t st) {
   using S = TcShape<D, ROWS>;
@@ -882,7 +741,7 @@ cudaError_t launch_dim(const AttnParams& p, int sms, size_t partial_floats, cuda
   cudaError_t e = kernel_setup(setup[p.bf16 ? 1 : 0], kern, S::kThreads, S::kSmem);
   if (e != cudaSuccess) return e;
   CUtensorMap kmap, vmap;
-  if (!encode(kmap, p.b.k, p, D, S::KT) || !encode(vmap, p.b.v, p, D, S::KT)) return cudaErrorInvalidValue;
+  if (!kv_tensor_map(kmap, p.b.k, p, D, S::KT) || !kv_tensor_map(vmap, p.b.v, p, D, S::KT)) return cudaErrorInvalidValue;
   const int64_t blocks = (static_cast<int64_t>(p.max_rows) * p.group + S::kRows - 1) / S::kRows;
   const int64_t tiles = static_cast<int64_t>(p.b.nseq) * p.b.kv_heads * blocks * ((p.max_context + S::KT - 1) / S::KT);
   int64_t grid = sms;
@@ -904,6 +763,24 @@ cudaError_t launch_dim(const AttnParams& p, int sms, size_t partial_floats, cuda
 }
 
 }  // namespace
+
+// The layer's K or V as [pages][kv_heads][page_size][dim], in boxes of 64 columns by min(page_size, key tile) rows.
+bool kv_tensor_map(CUtensorMap& map, void* base, const AttnParams& p, int dim, int tile_keys) {
+  const EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t page = 1ull << p.b.page_shift;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(dim), page, static_cast<cuuint64_t>(p.b.kv_heads),
+                              static_cast<cuuint64_t>(p.b.pages)};
+  // (a dimension of one takes no steps: its stride need not mean anything)
+  const cuuint64_t row = static_cast<cuuint64_t>(p.b.token_stride) * 2;
+  const cuuint64_t strides[3] = {row, p.b.kv_heads > 1 ? static_cast<cuuint64_t>(p.b.head_stride) * 2 : row,
+                                 p.b.pages > 1 ? static_cast<cuuint64_t>(p.b.page_stride) * 2 : row};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(page < static_cast<cuuint64_t>(tile_keys) ? page : tile_keys), 1, 1};
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  return fn(&map, p.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims, strides, box,
+            step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 cudaError_t launch_attn_tc(const AttnParams& p, int dim, int sms, size_t partial_floats, cudaStream_t st) {
   // blocks of one row tile where no sequence needs two: a slot more for K and V in the second tile's place (32 sequences' 8,

@@ -1,99 +1,589 @@
 // exl3_attn_weight.cu -- how much every cached token was attended to: the column sums of the attention's probabilities,
-// accumulated over steps (exl3_attention_weight, include/exl3_b200.h).
+// accumulated over steps (exl3_attention_weight, include/exl3_b200.h), on the 5th-generation tensor cores.
 //
-// w[s][g][j] = (j < context ? decay w[s][g][j] : 0) + sum_i sum_{h in g} exp(scale q_ih . k_j - lse_ih) over the rows i of
-// sequence s that see slot j.  A thread per slot; a block of 128 slots takes the rows sixteen at a time.
+//   w[s][g][j] = (j < context ? decay w[s][g][j] : 0) + sum_i sum_{h in g} exp(scale q_ih . k_j - lse_ih)
+//
+// over the rows i of sequence s that see slot j.  The log-sum-exps are given, so a slot's sum needs nothing of the other
+// slots: S^T = K Q^T with the keys as the MMA's M dimension puts a key on a TMEM lane and hence in one thread, which sums its
+// probabilities over the columns (rows of Q) with no exchange; each thread's own f32 sum runs over its columns in order.
+//
+// The work: (sequence, kv head, block of keys) items, an item's tiles its query row tiles, all items' tiles on one line cut
+// into equal parts, one per CTA.  An item's keys stay in shared memory while the row tiles stream by; where a sequence has
+// one row tile (decoding, small trees) that stays, and the keys stream.  An item cut between CTAs is joined by the last of
+// them to finish, its partial sums added in the line's order: the bits do not depend on which CTA that is.
+//
+// Roles: two groups of four warps for the exponentials and sums (a thread per key), then one warp each for the MMAs and the
+// copies of K (TMA, one box per page and 64 columns, 128-byte swizzle), and four that bring the query rows (cp.async; row
+// t * group + g is token t's query head g).  Heads up to 128 wide: an item is 256 keys, a group per half.  256 wide: 128 keys,
+// whose columns the groups share.
+//
+// Every mbarrier wait is bounded (wait_bar): one that gives up raises an abort flag that all roles poll.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include "exl3_attn.h"
 #include "exl3_attn_dev.cuh"
+#include "exl3_attn_tc.cuh"
 #include "exl3_common.cuh"
 #include "exl3_internal.h"
 
 namespace exl3 {
 
+using namespace tc;
+
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kRows = 16;
+constexpr float kLog2e = 1.4426950408889634f;
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads) weight_kernel(const WeightParams p) {
-  __shared__ float s_q[kRows][D];
-  __shared__ float s_lse[kRows];
-  __shared__ int s_tok[kRows];
-  pdl_wait();
-  Item it;
-  item_seq(p.a, static_cast<int>(blockIdx.y), it);
-  it.kv_head = static_cast<int>(blockIdx.z);
-  const PagedBatch& b = p.a.b;
-  if (it.ntok == 0) return;
-  for (int key0 = static_cast<int>(blockIdx.x) * kThreads; key0 < min(it.total_keys, p.slots); key0 += gridDim.x * kThreads) {
-    const int key = key0 + static_cast<int>(threadIdx.x);
-    int id = -1;
-    if (key < it.total_keys) {
-      id = b.table[static_cast<int64_t>(it.seq) * b.max_pages + (key >> b.page_shift)];
-      if (id < 0 || id >= b.pages) {
-        atomicOr(b.err, kErrBadShape);
-        id = -1;
-      }
-    }
-    const uint16_t* k = b.k + id * b.page_stride + (key & ((1 << b.page_shift) - 1)) * b.token_stride + it.kv_head * b.head_stride;
-    float sum = 0.f;
-    for (int r0 = 0; r0 < it.nrows; r0 += kRows) {
+template <int D>
+struct WtShape {
+  static constexpr int HB = D == 256 ? 1 : 2;       // 128-key halves of an item
+  static constexpr int KB = HB * 128;               // keys of an item
+  static constexpr int RT = D == 256 ? 64 : 128;    // query rows of a tile
+  static constexpr int kBufs = D == 256 ? 4 : 2;    // accumulators of a half
+  static constexpr int kKTile = 128 * D * 2;
+  static constexpr int kQTile = RT * D * 2;
+  static constexpr int KS = D == 256 ? 2 : D == 128 ? 4 : 6;  // K halves in flight
+  static constexpr int QS = D == 64 ? 3 : 2;                  // query tiles in flight
+  static constexpr int kEpi = 256;                  // threads of the sums
+  static constexpr int kLoad = 128;                 // threads that bring the queries
+  static constexpr int kThreads = kEpi + 64 + kLoad;
+  static constexpr int kTmem = D == 256 ? 256 : 512;
+  static constexpr int kBars = 2 * KS + 2 * QS + 2 * HB * kBufs + 2;
+  static constexpr int kSmem = KS * kKTile + QS * kQTile + QS * RT * 4 + 2 * 128 * 4 + kBars * 8 + 64;
+  static_assert(HB * kBufs * RT <= kTmem && kSmem <= 232448 - 2048, "shared memory or TMEM");
+};
+
+// A block of keys of one sequence and kv head, with the row tiles that see any of it.
+struct WtItem {
+  Item s;                  // the sequence (item_seq) and kv head
+  int block, nblocks;
+  int row_tiles;           // of the sequence
+  int first_tile, tiles;   // the block's: first_tile .. row_tiles - 1
+  int64_t first;           // its first tile on the line
+};
+
+template <int D>
+struct WtLine : WorkLine {
+  using S = WtShape<D>;
+  __device__ __forceinline__ static void set_seq(const WeightParams& p, WtItem& it) {
+    if (it.s.total_keys > p.slots) atomicOr(p.a.b.err, kErrBadShape);
+    it.s.total_keys = min(it.s.total_keys, p.slots);
+    it.s.context = min(it.s.context, it.s.total_keys);
+    it.nblocks = it.s.nrows ? (it.s.total_keys + S::KB - 1) / S::KB : 0;
+    it.row_tiles = (it.s.nrows + S::RT - 1) / S::RT;
+  }
+  // The first row tile that sees any key of the block: without a tree, slot context + d is seen from token d on.
+  __device__ __forceinline__ static int first_of(const WeightParams& p, const WtItem& it, int block) {
+    const int d = block * S::KB - it.s.context;
+    return p.a.b.tree || d <= 0 ? 0 : static_cast<int>(static_cast<int64_t>(d) * p.a.group / S::RT);
+  }
+  __device__ __forceinline__ static void set_block(const WeightParams& p, WtItem& it) {
+    it.first_tile = first_of(p, it, it.block);
+    it.tiles = it.row_tiles - it.first_tile;
+  }
+  __device__ __forceinline__ static int64_t tiles_of_head(const WeightParams& p, const WtItem& it) {
+    int64_t t = static_cast<int64_t>(it.nblocks) * it.row_tiles;
+    if (!p.a.b.tree && it.row_tiles > 1)
+      for (int b = it.s.context / S::KB; b < it.nblocks; ++b) t -= first_of(p, it, b);
+    return t;
+  }
+  __device__ __forceinline__ int64_t seq_tiles(const WeightParams& p, int s) const {
+    if (s >= p.a.b.nseq) return 0;
+    WtItem it;
+    item_seq(p.a, s, it.s);
+    set_seq(p, it);
+    return tiles_of_head(p, it) * p.a.b.kv_heads;
+  }
+  // Cuts the line and finds the item that holds this CTA's first tile (if it has any).  scratch: 36 words.
+  __device__ void begin_line(const WeightParams& p, int64_t* scratch, WtItem& it) {
+    int64_t sum = 0, mine = 0, upto = 0;
+    for (int base = 0; base < p.a.b.nseq; base += blockDim.x) {
+      mine = seq_tiles(p, base + static_cast<int>(threadIdx.x));
+      upto = sum + scan(mine, scratch);
+      if (threadIdx.x == blockDim.x - 1) scratch[33] = upto;
       __syncthreads();
-      for (int i = static_cast<int>(threadIdx.x); i < kRows * D; i += kThreads) {
-        const int r = r0 + i / D, t = r / p.a.group, h = it.kv_head * p.a.group + r % p.a.group;
-        float v = 0.f;
-        if (r < it.nrows)
-          v = unpack1<BF16>(static_cast<const uint16_t*>(p.a.q.data)[(it.row0 + t) * p.a.q.row_stride + h * p.a.q.head_stride + i % D], 0);
-        s_q[i / D][i % D] = v;
-        if (i % D == 0) {
-          s_tok[i / D] = r < it.nrows ? t : it.ntok;
-          const float l = r < it.nrows ? p.lse[static_cast<int64_t>(it.row0 + t) * p.a.q.heads + h] : 0.f;
-          s_lse[i / D] = l == -INFINITY ? INFINITY : l * 1.4426950408889634f;
-        }
-      }
+      sum = scratch[33];
       __syncthreads();
-      float dot[kRows];
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) dot[r] = 0.f;
-      if (id >= 0) {
-        for (int d = 0; d < D; d += 2) {
-          const uint32_t u = *reinterpret_cast<const uint32_t*>(k + d);
-          const float x = unpack1<BF16>(u, 0), y = unpack1<BF16>(u, 1);
-#pragma unroll
-          for (int r = 0; r < kRows; ++r) dot[r] = fmaf(s_q[r][d + 1], y, fmaf(s_q[r][d], x, dot[r]));
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < kRows; ++r)
-        if (sees(b, it, s_tok[r], key)) sum += ex2(fmaf(dot[r], p.a.scale_log2, -s_lse[r]));
     }
-    if (key < it.total_keys && key < p.slots) {
-      float* w = p.w + it.seq * p.row_stride + it.kv_head * p.head_stride + key;
-      *w = key < it.context && p.decay != 0.f ? fmaf(p.decay, *w, sum) : sum;
+    total = sum;
+    parts = static_cast<int>(min(static_cast<int64_t>(gridDim.x), total));
+    begin = end = 0;
+    if (static_cast<int>(blockIdx.x) >= parts) return;
+    share = divide(total, parts);
+    extra = static_cast<int>(total - share * parts);
+    const int c = static_cast<int>(blockIdx.x);
+    begin = share * c + min(c, extra);
+    end = begin + share + (c < extra ? 1 : 0);
+    const bool one = p.a.b.nseq <= static_cast<int>(blockDim.x);  // the scan above is the whole
+    sum = 0;
+    for (int base = 0; base < p.a.b.nseq; base += blockDim.x) {
+      const int s = base + static_cast<int>(threadIdx.x);
+      if (!one) {
+        mine = seq_tiles(p, s);
+        upto = sum + scan(mine, scratch);
+      }
+      if (threadIdx.x == blockDim.x - 1) scratch[33] = upto;
+      if (begin < upto && begin >= upto - mine) scratch[34] = s, scratch[35] = upto - mine;
+      __syncthreads();
+      sum = scratch[33];
+      if (begin < sum) break;
+      __syncthreads();
+    }
+    const int s = static_cast<int>(scratch[34]);
+    const int64_t first = scratch[35];
+    __syncthreads();
+    item_seq(p.a, s, it.s);
+    set_seq(p, it);
+    const int64_t per_head = tiles_of_head(p, it);
+    it.s.kv_head = static_cast<int>(divide(begin - first, per_head));
+    it.first = first + it.s.kv_head * per_head;
+    // the blocks that begin in the context have all row tiles
+    const int whole = p.a.b.tree ? it.nblocks : min(it.nblocks, it.s.context / S::KB + 1);
+    it.block = static_cast<int>(min(divide(begin - it.first, it.row_tiles), static_cast<int64_t>(whole - 1)));
+    it.first += static_cast<int64_t>(it.block) * it.row_tiles;
+    set_block(p, it);
+    while (begin >= it.first + it.tiles) {
+      it.first += it.tiles;
+      ++it.block;
+      set_block(p, it);
     }
   }
-  if (it.total_keys > p.slots && threadIdx.x == 0) atomicOr(b.err, kErrBadShape);
+  // The item after `it` (there is one).
+  __device__ __forceinline__ static void step(const WeightParams& p, WtItem& it) {
+    it.first += it.tiles;
+    if (++it.block == it.nblocks) {
+      it.block = 0;
+      if (++it.s.kv_head == p.a.b.kv_heads) {
+        it.s.kv_head = 0;
+        int s = it.s.seq;
+        do item_seq(p.a, ++s, it.s);
+        while (it.s.ntok == 0 && s + 1 < p.a.b.nseq);
+        set_seq(p, it);
+      }
+    }
+    set_block(p, it);
+  }
+};
+
+// Which of the rows row0 .. row0 + 31 of the sequence (row t * group + g: token t) see slot context + d (d >= 0).
+__device__ __forceinline__ uint32_t seeing32(const WeightParams& p, const Item& it, int row0, int d) {
+  if (!p.a.b.tree) {
+    const int64_t n = static_cast<int64_t>(d) * p.a.group - row0;  // the first that does
+    return n <= 0 ? ~0u : n >= 32 ? 0u : ~0u << n;
+  }
+  const int word = d >> 5;
+  if (word >= p.a.b.tree_words) return 0u;
+  uint32_t m = 0;
+  int t = row0 / p.a.group, next = (t + 1) * p.a.group - row0;
+  for (int i = 0; i < 32; ++t) {
+    const uint32_t bit = t < it.ntok ? (p.a.b.tree[static_cast<int64_t>(it.row0 + t) * p.a.b.tree_words + word] >> (d & 31)) & 1u : 0u;
+    const int to = min(next, 32);
+    if (bit) m |= (to == 32 ? ~0u : (1u << to) - 1u) & ~((1u << i) - 1u);
+    i = to;
+    next += p.a.group;
+  }
+  return m;
+}
+
+// The sum of 2^(scale x - lse) over 32 accumulators; lse in shared memory, in units of log 2.
+__device__ __forceinline__ void add32(const uint32_t (&x)[32], const float* lse, uint64_t scale2, uint64_t (&sum)[2]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) {
+    const float4 l = *reinterpret_cast<const float4*>(lse + i);
+    float a, b, c, d;
+    f2_split(fma2(f2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, f2(l.x, l.y)), a, b);
+    f2_split(fma2(f2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), scale2, f2(l.z, l.w)), c, d);
+    sum[0] = add2(sum[0], f2(ex2(a), ex2(b)));
+    sum[1] = add2(sum[1], f2(ex2(c), ex2(d)));
+  }
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
+    weight_kernel(const __grid_constant__ WeightParams p, const __grid_constant__ CUtensorMap kmap) {
+  using S = WtShape<D>;
+  constexpr int HB = S::HB, KS = S::KS, QS = S::QS, RT = S::RT, kBufs = S::kBufs;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ WtLine<D> line;
+  __shared__ WtItem s_items[S::kThreads / 32];
+  uint8_t* s_k = smem;                           // [slot][64-column block][128 keys][128 bytes], swizzled
+  uint8_t* s_q = s_k + KS * S::kKTile;           // [slot][64-column block][RT rows][128 bytes], swizzled
+  float* s_lse = reinterpret_cast<float*>(s_q + QS * S::kQTile);  // [slot][RT], negated, in units of log 2
+  float* s_half = s_lse + QS * RT;               // [2][128]: the second group's sums
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_half + 256);
+  uint64_t *kfull = bars, *kempty = kfull + KS, *qfull = kempty + KS, *qempty = qfull + QS;
+  uint64_t *afull = qempty + QS, *aempty = afull + HB * kBufs, *xsync = aempty + HB * kBufs, *fin = xsync + 1;
+  uint32_t* words = reinterpret_cast<uint32_t*>(bars + S::kBars);
+  uint32_t* s_tmem = words;
+  volatile uint32_t* abort_flag = words + 1;
+  int* s_last = reinterpret_cast<int*>(words + 2);
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  const PagedBatch& b = p.a.b;
+
+  if (smem_u32(smem) & 1023u) {  // the swizzle goes by address bits: not served
+    if (tid == 0) atomicOr(b.err, kErrBadShape);
+    return;
+  }
+  if (warp == 8) {
+    tmem_alloc(smem_u32(s_tmem), S::kTmem);
+    tmem_relinquish();
+  }
+  if (tid == 0) {
+    for (int i = 0; i < KS; ++i) mbar_init(&kfull[i], 1), mbar_init(&kempty[i], 1);
+    for (int i = 0; i < QS; ++i) mbar_init(&qfull[i], S::kLoad), mbar_init(&qempty[i], 1 + 8);
+    for (int i = 0; i < HB * kBufs; ++i) mbar_init(&afull[i], 1), mbar_init(&aempty[i], HB == 2 ? 4 : 8);
+    mbar_init(xsync, S::kEpi), mbar_init(fin, 1);
+    fence_barrier_init();
+    *abort_flag = 0u;
+  }
+  if (tid == 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
+  pdl_wait();
+  {
+    WtLine<D> own;
+    WtItem first;
+    own.begin_line(p, reinterpret_cast<int64_t*>(s_half), first);  // (no place that TMA writes: that is another proxy)
+    if (tid == 0) line = own;
+    if (lane == 0) s_items[warp] = first;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  WtItem& it = s_items[warp];
+  int64_t at = line.begin;
+  const int64_t end = line.end;
+  auto advance = [&](int tiles) {
+    at += tiles;
+    if (at < end) {
+      __syncwarp();
+      if (lane == 0) WtLine<D>::step(p, it);
+      __syncwarp();
+    }
+  };
+  // Whether the tile needs its queries brought: not where the sequence's one tile is there already.
+  int held_seq = -1, held_head = -1;
+  auto brings = [&]() {
+    const bool there = it.row_tiles == 1 && it.s.seq == held_seq && it.s.kv_head == held_head;
+    held_seq = it.s.seq, held_head = it.s.kv_head;
+    return !there;
+  };
+  auto tiles_here = [&]() { return static_cast<int>(min(end - at, it.tiles - (at - it.first))); };
+  auto first_here = [&]() { return it.first_tile + static_cast<int>(at - it.first); };
+  auto halves_here = [&]() { return min(HB, (it.s.total_keys - it.block * S::KB + 127) / 128); };
+  auto rows_of = [&](int tile) { return min(RT, it.s.nrows - tile * RT); };
+
+  if (warp < 8) {
+    // ---------------------------------------------------------------- exponentials and sums: a thread per key
+    const uint32_t g = warp >> 2, wq = warp & 3u, r128 = wq * 32 + lane;  // key of the half = TMEM lane
+    const uint32_t lane_off = (wq * 32u) << 16;
+    const int half = HB == 2 ? static_cast<int>(g) : 0;
+    const uint64_t scale2 = f2(p.a.scale_log2, p.a.scale_log2);
+    uint32_t q_slot = QS - 1, q_phase = 1, buf = 0, a_phase = 0, x_phase = 0, turn = 0;  // (the first tile goes to slot 0, phase 0)
+    bool ok = true, any_q = false;
+    auto group_sync = [&]() {  // both groups
+      mbar_arrive(xsync);
+      ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(xsync, x_phase, abort_flag, b.err));
+      x_phase ^= 1u;
+    };
+    while (ok && at < end) {
+      const int tiles = tiles_here(), tile0 = first_here(), halves = halves_here();
+      const int key = it.block * S::KB + half * 128 + static_cast<int>(r128);
+      const bool mine = half < halves;
+      const bool writes = mine && key < it.s.total_keys && (HB == 2 || g == 0);
+      float* w = p.w + it.s.seq * p.row_stride + it.s.kv_head * p.head_stride + key;
+      const bool keeps = writes && key < it.s.context && p.decay != 0.f;
+      const float old = keeps ? __ldcg(w) : 0.f;
+      const int d = key - it.s.context;
+      float total = 0.f;
+      for (int i = 0; ok && i < tiles; ++i) {
+        const int rows = rows_of(tile0 + i), row0 = (tile0 + i) * RT;
+        if (brings()) {
+          if (any_q && lane == 0) mbar_arrive(&qempty[q_slot]);
+          any_q = true;
+          if (++q_slot == QS) q_slot = 0, q_phase ^= 1u;
+          ok = __all_sync(0xFFFFFFFFu, wait_bar(&qfull[q_slot], q_phase, abort_flag, b.err));
+        }
+        if (!mine) continue;
+        const uint32_t ab = half * kBufs + buf;
+        ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(&afull[ab], a_phase, abort_flag, b.err));
+        tc_fence_after();
+        const float* lse = s_lse + q_slot * RT;
+        const uint32_t acc = tmem + lane_off + ab * RT;
+        // every row of the tile is there and sees every key of the half
+        const int last = it.block * S::KB + half * 128 + 127 - it.s.context;  // the last key's place among the new tokens
+        const bool whole = (rows & 31) == 0 && (last < 0 || (!b.tree && static_cast<int64_t>(last) * p.a.group <= row0));
+        const int c_lo = HB == 2 ? 0 : static_cast<int>(g) * 32, c_hi = HB == 2 ? rows : min(rows, c_lo + 32);
+        uint64_t sum[2] = {0, 0};
+        float odd = 0.f;
+#pragma unroll 1
+        for (int c = c_lo; c < c_hi; c += 32) {
+          uint32_t x[32];
+          tmem_ld32(acc + c, x);
+          uint32_t see = ~0u;
+          if (!whole) {
+            if (d >= 0) see = seeing32(p, it.s, row0 + c, d);
+            if (rows - c < 32) see &= (1u << (rows - c)) - 1u;
+          }
+          tmem_wait_ld(x);
+          if (whole) {
+            add32(x, lse + c, scale2, sum);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float e = ex2(fmaf(__uint_as_float(x[j]), p.a.scale_log2, lse[c + j]));
+              if (see & (1u << j)) odd += e;
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&aempty[ab]);
+        if (++buf == kBufs) buf = 0, a_phase ^= 1u;
+        float s0, s1;
+        f2_split(add2(sum[0], sum[1]), s0, s1);
+        total += (s0 + s1) + odd;
+      }
+      if constexpr (HB == 1) {  // the groups' columns together
+        float* there = s_half + (turn++ & 1u) * 128;
+        if (g == 1) there[r128] = total;
+        group_sync();
+        if (g == 0) total += there[r128];
+      }
+      if (tiles == it.tiles) {
+        if (writes) *w = keeps ? fmaf(p.decay, old, total) : total;
+      } else {
+        // a part of the item: the last of its CTAs adds them up, in the line's order
+        if (writes) line.slot(p.a, S::KB, at != it.first)[half * 128 + r128] = total;
+        const int c0 = line.part_of(it.first), c1 = line.part_of(it.first + it.tiles - 1);
+        __threadfence();
+        group_sync();
+        if (tid == 0) {
+          const bool last = atomicAdd(p.a.counters + c0, 1u) + 1u == static_cast<uint32_t>(c1 - c0 + 1);
+          if (last) p.a.counters[c0] = 0u;
+          *s_last = last;
+        }
+        group_sync();
+        if (ok && *s_last) {
+          __threadfence();
+          if (writes) {
+            float all = 0.f;
+#pragma unroll 4
+            for (int c = c0; c <= c1; ++c)
+              all += __ldcg(p.a.partials + (static_cast<int64_t>(c) * 2 + (c == c0 ? 0 : 1)) * S::KB + half * 128 + r128);
+            *w = keeps ? fmaf(p.decay, old, all) : all;
+          }
+        }
+        group_sync();  // s_last is read
+      }
+      advance(tiles);
+    }
+  } else if (warp == 8) {
+    // ---------------------------------------------------------------- MMA issuer: converged, one elected lane issues
+    const uint32_t on = elect_one();
+    const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+    const uint64_t qdesc = sw128_desc(smem_u32(s_q)), kdesc = sw128_desc(smem_u32(s_k));
+    uint32_t k_slot = 0, k_phase = 0, q_slot = QS - 1, q_phase = 1;
+    uint32_t used[HB] = {};  // tiles a half's accumulators have served
+    bool ok = true, any_q = false;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity))) return;
+      ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(bar, parity, abort_flag, b.err));
+    };
+    while (ok && at < end) {
+      const int tiles = tiles_here(), tile0 = first_here(), halves = halves_here();
+      uint32_t ks[HB];
+#pragma unroll
+      for (int h = 0; h < HB; ++h) {
+        if (h >= halves) break;
+        ks[h] = k_slot;
+        wait(&kfull[k_slot], k_phase);
+        if (++k_slot == KS) k_slot = 0, k_phase ^= 1u;
+      }
+      for (int i = 0; ok && i < tiles; ++i) {
+        const int rows = rows_of(tile0 + i);
+        if (brings()) {
+          if (any_q) commit(on, &qempty[q_slot]);
+          any_q = true;
+          if (++q_slot == QS) q_slot = 0, q_phase ^= 1u;
+          wait(&qfull[q_slot], q_phase);
+        }
+        const uint32_t idesc = uniform((attn_idesc<BF16>(128, 0, false)) | (static_cast<uint32_t>(((rows + 31) & ~31) >> 3) << 17));
+#pragma unroll
+        for (int h = 0; h < HB; ++h) {
+          if (h >= halves) break;
+          const uint32_t ab = h * kBufs + used[h] % kBufs;
+          if (used[h] >= kBufs) wait(&aempty[ab], (used[h] / kBufs - 1) & 1u);
+          ++used[h];
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t qo = uniform(q_slot * (S::kQTile >> 4)), ko = uniform(ks[h] * (S::kKTile >> 4));
+          const uint32_t ad = uniform(tm + ab * RT);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            mma_ss(on, ad, desc_at(kdesc, ko + (((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4)),
+                   desc_at(qdesc, qo + (((kk >> 2) * (RT * 128) + (kk & 3) * 32) >> 4)), idesc, kk != 0 ? 1u : 0u);
+          commit(on, &afull[ab]);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < HB; ++h)
+        if (h < halves) commit(on, &kempty[ks[h]]);
+      advance(tiles);
+    }
+    commit(on, fin);  // every MMA has finished before TMEM is released
+    if (lane == 0 && !mbar_wait_bounded(fin, 0)) atomicOr(b.err, kErrWaitTimeout);
+    __syncwarp();
+  } else if (warp == 9) {
+    // ---------------------------------------------------------------- K copies
+    const uint32_t base = smem_u32(s_k);
+    const int box_rows = min(1 << b.page_shift, 128);
+    const int parts = 128 / box_rows, boxes = parts * (D / 64);  // at most 32: a lane each
+    const int blk = static_cast<int>(lane) % (D / 64), part = static_cast<int>(lane) / (D / 64);
+    uint32_t n = 0;
+    bool ok = true;
+    while (ok && at < end) {
+      const int32_t* tab = b.table + static_cast<int64_t>(it.s.seq) * b.max_pages;
+      const int halves = halves_here(), tiles = tiles_here();
+      for (int h = 0; ok && h < halves; ++h, ++n) {
+        const uint32_t slot = n % KS;
+        const int key = it.block * S::KB + h * 128 + part * box_rows;
+        int id = -1;
+        if (static_cast<int>(lane) < boxes && key < it.s.total_keys) {
+          id = tab[key >> b.page_shift];
+          if (id < 0 || id >= b.pages) {
+            atomicOr(b.err, kErrBadShape);
+            id = b.pages;  // past the map: the box arrives as zeros
+          }
+        }
+        const uint32_t loads = __popc(__ballot_sync(0xFFFFFFFFu, id >= 0));
+        if (n >= KS) ok = wait_bar(&kempty[slot], (n / KS - 1) & 1u, abort_flag, b.err);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&kfull[slot], loads * box_rows * 128);
+        if (id >= 0)
+          tma_box(base + slot * S::kKTile + blk * (128 * 128) + part * box_rows * 128, &kmap, blk * 64,
+                  key & ((1 << b.page_shift) - 1), it.s.kv_head, id, &kfull[slot]);
+      }
+      advance(tiles);
+    }
+    // no copy may outlive the CTA: wait (bounded) for the last fill of every slot
+    const uint32_t last = min(n, static_cast<uint32_t>(KS));
+    for (uint32_t i = 1; i <= last; ++i) {
+      const uint32_t f = n - i;
+      if (!mbar_wait_bounded(&kfull[f % KS], (f / KS) & 1u)) atomicOr(b.err, kErrWaitTimeout);
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- queries and their log-sum-exps
+    const uint32_t t128 = tid - (S::kEpi + 64);
+    constexpr int kChunks = D / 8, kPerPass = S::kLoad / kChunks;  // a row's 16-byte chunks lie on neighbouring lanes
+    const int c = static_cast<int>(t128) % kChunks, r_first = static_cast<int>(t128) / kChunks;
+    uint32_t n = 0;        // tiles brought
+    bool ok = true, pending = false;  // the last one's copies are on their way: not published yet
+    auto publish = [&](uint32_t which) {
+      fence_proxy_async_smem();
+      mbar_arrive(&qfull[which % QS]);
+    };
+    auto flush = [&]() {
+      if (!pending) return;
+      cp_async_wait<0>();
+      publish(n - 1);
+      pending = false;
+    };
+    while (ok && at < end) {
+      const int tiles = tiles_here(), tile0 = first_here();
+      for (int i = 0; ok && i < tiles; ++i) {
+        if (!brings()) {
+          flush();
+          continue;
+        }
+        const uint32_t slot = n % QS;
+        if (n >= QS && !__all_sync(0xFFFFFFFFu, mbar_try_wait(&qempty[slot], (n / QS - 1) & 1u))) {
+          flush();
+          ok = __all_sync(0xFFFFFFFFu, wait_bar(&qempty[slot], (n / QS - 1) & 1u, abort_flag, b.err));
+          if (!ok) break;
+        }
+        const int rows = rows_of(tile0 + i), wide = (rows + 31) & ~31, row0 = (tile0 + i) * RT;
+        uint8_t* dst = s_q + slot * S::kQTile + (c >> 3) * (RT * 128);
+        for (int r = r_first; r < wide; r += kPerPass) {
+          const int rr = row0 + r, t = rr / p.a.group, h = it.s.kv_head * p.a.group + rr % p.a.group;
+          const uint32_t to = smem_u32(dst + image_offset(static_cast<uint32_t>(r), static_cast<uint32_t>((c & 7) * 8)));
+          const bool in = r < rows;
+          if (p.a.q.vec) {
+            const uint16_t* src = static_cast<const uint16_t*>(p.a.q.data);
+            if (in) src += static_cast<int64_t>(it.s.row0 + t) * p.a.q.row_stride + static_cast<int64_t>(h) * p.a.q.head_stride + c * 8;
+            cp_async16(to, src, in);
+          } else {
+            const uint4 u = in ? load_q8(p.a.q, it.s.row0 + t, h, c * 8) : make_uint4(0u, 0u, 0u, 0u);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+          }
+        }
+        cp_async_commit();
+        if (static_cast<int>(t128) < RT) {
+          const int rr = row0 + static_cast<int>(t128);
+          float l = -INFINITY;
+          if (static_cast<int>(t128) < rows)
+            l = p.lse[static_cast<int64_t>(it.s.row0 + rr / p.a.group) * p.a.q.heads + it.s.kv_head * p.a.group + rr % p.a.group];
+          // a row that saw nothing (or is not there) adds nothing: 2^(x - inf)
+          s_lse[slot * RT + t128] = l == -INFINITY ? -INFINITY : -l * kLog2e;
+        }
+        if (pending) {
+          cp_async_wait<1>();
+          publish(n - 1);
+        }
+        pending = true;
+        ++n;
+      }
+      advance(tiles);
+    }
+    flush();
+    cp_async_wait<0>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S::kTmem);
+  }
 }
 
 template <int D>
-cudaError_t launch_dim(const WeightParams& p, cudaStream_t st) {
-  const int tiles = (p.a.max_context + kThreads - 1) / kThreads;
-  const dim3 grid(static_cast<unsigned>(tiles < 1 ? 1 : tiles > 65535 ? 65535 : tiles), static_cast<unsigned>(p.a.b.nseq),
-                  static_cast<unsigned>(p.a.b.kv_heads));
-  return p.a.bf16 ? launch_pdl_k(weight_kernel<D, true>, grid, dim3(kThreads), st, p)
-                  : launch_pdl_k(weight_kernel<D, false>, grid, dim3(kThreads), st, p);
+cudaError_t launch_dim(const WeightParams& p, int sms, size_t partial_floats, cudaStream_t st) {
+  using S = WtShape<D>;
+  static KernelSetup setup[2];
+  auto kern = p.a.bf16 ? weight_kernel<D, true> : weight_kernel<D, false>;
+  cudaError_t e = kernel_setup(setup[p.a.bf16 ? 1 : 0], kern, S::kThreads, S::kSmem);
+  if (e != cudaSuccess) return e;
+  CUtensorMap kmap;
+  if (!kv_tensor_map(kmap, p.a.b.k, p.a, D, 128)) return cudaErrorInvalidValue;
+  const int64_t tiles = static_cast<int64_t>(p.a.b.nseq) * p.a.b.kv_heads * ((p.a.max_context + S::KB - 1) / S::KB) *
+                        ((static_cast<int64_t>(p.a.max_rows) * p.a.group + S::RT - 1) / S::RT);
+  int64_t grid = sms;
+  if (grid > tiles) grid = tiles;
+  const int64_t fit = static_cast<int64_t>(partial_floats / (2 * S::KB));
+  if (grid > fit) grid = fit;
+  if (grid < 1) grid = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, p, kmap);
 }
 
 }  // namespace
 
 cudaError_t launch_attn_weight(const WeightParams& p, int dim, int sms, size_t partial_floats, cudaStream_t st) {
   switch (dim) {
-    case 64: return launch_dim<64>(p, st);
-    case 128: return launch_dim<128>(p, st);
-    default: return launch_dim<256>(p, st);
+    case 64: return launch_dim<64>(p, sms, partial_floats, st);
+    case 128: return launch_dim<128>(p, sms, partial_floats, st);
+    default: return launch_dim<256>(p, sms, partial_floats, st);
   }
 }
 
