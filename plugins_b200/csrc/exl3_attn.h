@@ -80,6 +80,8 @@ struct WeightParams {
   int64_t row_stride, head_stride;
   int32_t slots;
   float decay;
+  int32_t row_tile;    // query rows of a tile (the launch's)
+  int32_t box_tokens;  // tokens of a TMA box of queries; 0: the queries are not fetched by TMA
 };
 cudaError_t launch_attn_weight(const WeightParams& p, int dim, int sms, size_t partial_floats, cudaStream_t st);
 

@@ -782,6 +782,24 @@ bool kv_tensor_map(CUtensorMap& map, void* base, const AttnParams& p, int dim, i
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Queries as [rows][kv_heads][group][dim], in boxes of 64 columns by one kv head's query heads by `tokens`.
+bool q_tensor_map(CUtensorMap& map, const AttnParams& p, int dim, int tokens) {
+  const EncodeFn fn = encode_fn();
+  if (!fn || p.q.row_stride < 0 || p.q.head_stride < 0) return false;
+  const cuuint64_t head = static_cast<cuuint64_t>(p.q.head_stride) * 2, row = static_cast<cuuint64_t>(p.q.row_stride) * 2;
+  const cuuint64_t some = static_cast<cuuint64_t>(dim) * 2;  // of a dimension of one, which takes no steps
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(p.group),
+                              static_cast<cuuint64_t>(p.b.kv_heads), static_cast<cuuint64_t>(p.b.rows)};
+  const cuuint64_t strides[3] = {p.group > 1 ? head : some, p.b.kv_heads > 1 ? head * p.group : some, p.b.rows > 1 ? row : some};
+  for (const cuuint64_t s : strides)
+    if (s == 0) return false;  // a broadcast
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(p.group), 1, static_cast<cuuint32_t>(tokens)};
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  return fn(&map, p.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, p.q.data, dims, strides, box,
+            step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 cudaError_t launch_attn_tc(const AttnParams& p, int dim, int sms, size_t partial_floats, cudaStream_t st) {
   // blocks of one row tile where no sequence needs two: a slot more for K and V in the second tile's place (32 sequences' 8,
   // 16 and 32-token trees over 4-8k slots: 143 / 148 / 158 us, with room for two tiles 145 / 148 / 161)

@@ -10,8 +10,9 @@
 
 namespace exl3 {
 
-// The layer's K or V as a tensor map (exl3_attn_tc.cu).
+// The layer's K or V, and the queries, as tensor maps (exl3_attn_tc.cu).
 bool kv_tensor_map(CUtensorMap& map, void* base, const AttnParams& p, int dim, int tile_keys);
+bool q_tensor_map(CUtensorMap& map, const AttnParams& p, int dim, int tokens);
 
 namespace tc {
 

@@ -13,8 +13,9 @@
 // them to finish, its partial sums added in the line's order: the bits do not depend on which CTA that is.
 //
 // Roles: two groups of four warps for the exponentials and sums (a thread per key), then one warp each for the MMAs and the
-// copies of K (TMA, one box per page and 64 columns, 128-byte swizzle), and four that bring the query rows (cp.async; row
-// t * group + g is token t's query head g).  Heads up to 128 wide: an item is 256 keys, a group per half.  256 wide: 128 keys,
+// copies of K (TMA, one box per page and 64 columns, 128-byte swizzle) and of the query rows (row t * group + g is token t's
+// query head g: a box of the kv head's query heads by tokens).  Queries whose addresses TMA does not take, or with more heads
+// per kv head than a tile has rows, are brought by four warps instead.  Heads up to 128 wide: an item is 256 keys, a group per half.  256 wide: 128 keys,
 // whose columns the groups share.
 //
 // Every mbarrier wait is bounded (wait_bar): one that gives up raises an abort flag that all roles poll.
@@ -71,12 +72,12 @@ struct WtLine : WorkLine {
     it.s.total_keys = min(it.s.total_keys, p.slots);
     it.s.context = min(it.s.context, it.s.total_keys);
     it.nblocks = it.s.nrows ? (it.s.total_keys + S::KB - 1) / S::KB : 0;
-    it.row_tiles = (it.s.nrows + S::RT - 1) / S::RT;
+    it.row_tiles = (it.s.nrows + p.row_tile - 1) / p.row_tile;
   }
   // The first row tile that sees any key of the block: without a tree, slot context + d is seen from token d on.
   __device__ __forceinline__ static int first_of(const WeightParams& p, const WtItem& it, int block) {
     const int d = block * S::KB - it.s.context;
-    return p.a.b.tree || d <= 0 ? 0 : static_cast<int>(static_cast<int64_t>(d) * p.a.group / S::RT);
+    return p.a.b.tree || d <= 0 ? 0 : static_cast<int>(static_cast<int64_t>(d) * p.a.group / p.row_tile);
   }
   __device__ __forceinline__ static void set_block(const WeightParams& p, WtItem& it) {
     it.first_tile = first_of(p, it, it.block);
@@ -201,7 +202,8 @@ __device__ __forceinline__ void add32(const uint32_t (&x)[32], const float* lse,
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
-    weight_kernel(const __grid_constant__ WeightParams p, const __grid_constant__ CUtensorMap kmap) {
+    weight_kernel(const __grid_constant__ WeightParams p, const __grid_constant__ CUtensorMap kmap,
+                  const __grid_constant__ CUtensorMap qmap) {
   using S = WtShape<D>;
   constexpr int HB = S::HB, KS = S::KS, QS = S::QS, RT = S::RT, kBufs = S::kBufs;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -231,13 +233,14 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
   }
   if (tid == 0) {
     for (int i = 0; i < KS; ++i) mbar_init(&kfull[i], 1), mbar_init(&kempty[i], 1);
-    for (int i = 0; i < QS; ++i) mbar_init(&qfull[i], S::kLoad), mbar_init(&qempty[i], 1 + 8);
+    for (int i = 0; i < QS; ++i) mbar_init(&qfull[i], p.box_tokens ? 32 : S::kLoad), mbar_init(&qempty[i], 1 + 8);
     for (int i = 0; i < HB * kBufs; ++i) mbar_init(&afull[i], 1), mbar_init(&aempty[i], HB == 2 ? 4 : 8);
     mbar_init(xsync, S::kEpi), mbar_init(fin, 1);
     fence_barrier_init();
     *abort_flag = 0u;
   }
   if (tid == 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
+  if (tid == 64 && p.box_tokens) asm volatile("prefetch.tensormap [%0];" ::"l"(&qmap) : "memory");
   pdl_wait();
   {
     WtLine<D> own;
@@ -271,7 +274,7 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
   auto tiles_here = [&]() { return static_cast<int>(min(end - at, it.tiles - (at - it.first))); };
   auto first_here = [&]() { return it.first_tile + static_cast<int>(at - it.first); };
   auto halves_here = [&]() { return min(HB, (it.s.total_keys - it.block * S::KB + 127) / 128); };
-  auto rows_of = [&](int tile) { return min(RT, it.s.nrows - tile * RT); };
+  auto rows_of = [&](int tile) { return min(p.row_tile, it.s.nrows - tile * p.row_tile); };
 
   if (warp < 8) {
     // ---------------------------------------------------------------- exponentials and sums: a thread per key
@@ -297,7 +300,7 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
       const int d = key - it.s.context;
       float total = 0.f;
       for (int i = 0; ok && i < tiles; ++i) {
-        const int rows = rows_of(tile0 + i), row0 = (tile0 + i) * RT;
+        const int rows = rows_of(tile0 + i), row0 = (tile0 + i) * p.row_tile;
         if (brings()) {
           if (any_q && lane == 0) mbar_arrive(&qempty[q_slot]);
           any_q = true;
@@ -316,23 +319,39 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
         const int c_lo = HB == 2 ? 0 : static_cast<int>(g) * 32, c_hi = HB == 2 ? rows : min(rows, c_lo + 32);
         uint64_t sum[2] = {0, 0};
         float odd = 0.f;
+        if (whole && c_hi - c_lo == 128) {  // the loads of 64 columns under the exponentials of the 64 before
+          uint32_t x[2][2][32];
+          tmem_ld32(acc, x[0][0]);
+          tmem_ld32(acc + 32, x[0][1]);
+          tmem_wait_ld(x[0][0]);
+          after_wait(x[0][1]);
+          tmem_ld32(acc + 64, x[1][0]);
+          tmem_ld32(acc + 96, x[1][1]);
+          add32(x[0][0], lse, scale2, sum);
+          add32(x[0][1], lse + 32, scale2, sum);
+          tmem_wait_ld(x[1][0]);
+          after_wait(x[1][1]);
+          add32(x[1][0], lse + 64, scale2, sum);
+          add32(x[1][1], lse + 96, scale2, sum);
+        } else {
 #pragma unroll 1
-        for (int c = c_lo; c < c_hi; c += 32) {
-          uint32_t x[32];
-          tmem_ld32(acc + c, x);
-          uint32_t see = ~0u;
-          if (!whole) {
-            if (d >= 0) see = seeing32(p, it.s, row0 + c, d);
-            if (rows - c < 32) see &= (1u << (rows - c)) - 1u;
-          }
-          tmem_wait_ld(x);
-          if (whole) {
-            add32(x, lse + c, scale2, sum);
-          } else {
+          for (int c = c_lo; c < c_hi; c += 32) {
+            uint32_t x[32];
+            tmem_ld32(acc + c, x);
+            uint32_t see = ~0u;
+            if (!whole) {
+              if (d >= 0) see = seeing32(p, it.s, row0 + c, d);
+              if (rows - c < 32) see &= (1u << (rows - c)) - 1u;
+            }
+            tmem_wait_ld(x);
+            if (whole) {
+              add32(x, lse + c, scale2, sum);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float e = ex2(fmaf(__uint_as_float(x[j]), p.a.scale_log2, lse[c + j]));
-              if (see & (1u << j)) odd += e;
+              for (int j = 0; j < 32; ++j) {
+                const float e = ex2(fmaf(__uint_as_float(x[j]), p.a.scale_log2, lse[c + j]));
+                if (see & (1u << j)) odd += e;
+              }
             }
           }
         }
@@ -474,8 +493,49 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
       if (!mbar_wait_bounded(&kfull[f % KS], (f / KS) & 1u)) atomicOr(b.err, kErrWaitTimeout);
     }
     __syncwarp();
+  } else if (p.box_tokens) {
+    // ---------------------------------------------------------------- queries (TMA) and their log-sum-exps: one warp
+    uint32_t n = 0;
+    bool ok = warp == 10;
+    while (ok && at < end) {
+      const int tiles = tiles_here(), tile0 = first_here();
+      for (int i = 0; ok && i < tiles; ++i) {
+        if (!brings()) continue;
+        const uint32_t slot = n % QS;
+        const int rows = rows_of(tile0 + i), row0 = (tile0 + i) * p.row_tile;
+        const int64_t l_at = static_cast<int64_t>(it.s.row0) * p.a.q.heads + it.s.kv_head * p.a.group;
+        float l[RT / 32];
+#pragma unroll
+        for (int j = 0; j < RT / 32; ++j) {
+          const int r = j * 32 + static_cast<int>(lane), rr = row0 + r;
+          l[j] = r < rows ? p.lse[l_at + static_cast<int64_t>(rr / p.a.group) * p.a.q.heads + rr % p.a.group] : -INFINITY;
+        }
+        if (n >= QS) ok = __all_sync(0xFFFFFFFFu, wait_bar(&qempty[slot], (n / QS - 1) & 1u, abort_flag, b.err));
+        if (!ok) break;
+        // a row that saw nothing (or is not there) adds nothing: 2^(x - inf)
+#pragma unroll
+        for (int j = 0; j < RT / 32; ++j) s_lse[slot * RT + j * 32 + lane] = l[j] == -INFINITY ? -INFINITY : -l[j] * kLog2e;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&qfull[slot], p.box_tokens * p.a.group * D * 2);
+          for (int c = 0; c < D / 64; ++c)
+            tma_box(smem_u32(s_q) + slot * S::kQTile + c * (RT * 128), &qmap, c * 64, 0, it.s.kv_head,
+                    it.s.row0 + row0 / p.a.group, &qfull[slot]);
+        } else {
+          mbar_arrive(&qfull[slot]);
+        }
+        ++n;
+      }
+      advance(tiles);
+    }
+    // no copy may outlive the CTA
+    const uint32_t last = min(n, static_cast<uint32_t>(QS));
+    for (uint32_t i = 1; i <= last; ++i) {
+      const uint32_t f = n - i;
+      if (!mbar_wait_bounded(&qfull[f % QS], (f / QS) & 1u)) atomicOr(b.err, kErrWaitTimeout);
+    }
+    __syncwarp();
   } else {
-    // ---------------------------------------------------------------- queries and their log-sum-exps
+    // ---------------------------------------------------------------- queries that TMA cannot fetch, likewise: four warps
     const uint32_t t128 = tid - (S::kEpi + 64);
     constexpr int kChunks = D / 8, kPerPass = S::kLoad / kChunks;  // a row's 16-byte chunks lie on neighbouring lanes
     const int c = static_cast<int>(t128) % kChunks, r_first = static_cast<int>(t128) / kChunks;
@@ -504,7 +564,7 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
           ok = __all_sync(0xFFFFFFFFu, wait_bar(&qempty[slot], (n / QS - 1) & 1u, abort_flag, b.err));
           if (!ok) break;
         }
-        const int rows = rows_of(tile0 + i), wide = (rows + 31) & ~31, row0 = (tile0 + i) * RT;
+        const int rows = rows_of(tile0 + i), wide = (rows + 31) & ~31, row0 = (tile0 + i) * p.row_tile;
         uint8_t* dst = s_q + slot * S::kQTile + (c >> 3) * (RT * 128);
         for (int r = r_first; r < wide; r += kPerPass) {
           const int rr = row0 + r, t = rr / p.a.group, h = it.s.kv_head * p.a.group + rr % p.a.group;
@@ -549,16 +609,24 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
 }
 
 template <int D>
-cudaError_t launch_dim(const WeightParams& p, int sms, size_t partial_floats, cudaStream_t st) {
+cudaError_t launch_dim(const WeightParams& params, int sms, size_t partial_floats, cudaStream_t st) {
   using S = WtShape<D>;
   static KernelSetup setup[2];
+  WeightParams p = params;
   auto kern = p.a.bf16 ? weight_kernel<D, true> : weight_kernel<D, false>;
   cudaError_t e = kernel_setup(setup[p.a.bf16 ? 1 : 0], kern, S::kThreads, S::kSmem);
   if (e != cudaSuccess) return e;
   CUtensorMap kmap;
   if (!kv_tensor_map(kmap, p.a.b.k, p.a, D, 128)) return cudaErrorInvalidValue;
+  // whole tokens to a tile where they fit: then a tile of queries is a box
+  p.row_tile = p.a.group <= S::RT ? S::RT / p.a.group * p.a.group : S::RT;
+  CUtensorMap qmap = kmap;
+  if (p.a.q.vec && p.a.group <= S::RT) {
+    const int tokens = S::RT / p.a.group < p.a.max_rows ? S::RT / p.a.group : p.a.max_rows;
+    if (q_tensor_map(qmap, p.a, D, tokens)) p.box_tokens = tokens;
+  }
   const int64_t tiles = static_cast<int64_t>(p.a.b.nseq) * p.a.b.kv_heads * ((p.a.max_context + S::KB - 1) / S::KB) *
-                        ((static_cast<int64_t>(p.a.max_rows) * p.a.group + S::RT - 1) / S::RT);
+                        ((static_cast<int64_t>(p.a.max_rows) * p.a.group + p.row_tile - 1) / p.row_tile);
   int64_t grid = sms;
   if (grid > tiles) grid = tiles;
   const int64_t fit = static_cast<int64_t>(partial_floats / (2 * S::KB));
@@ -574,7 +642,7 @@ cudaError_t launch_dim(const WeightParams& p, int sms, size_t partial_floats, cu
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, p, kmap);
+  return cudaLaunchKernelEx(&cfg, kern, p, kmap, qmap);
 }
 
 }  // namespace
