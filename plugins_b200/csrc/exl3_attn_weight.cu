@@ -46,12 +46,13 @@ struct WtShape {
   static constexpr int kQTile = RT * D * 2;
   static constexpr int KS = D == 256 ? 2 : D == 128 ? 4 : 6;  // K halves in flight
   static constexpr int QS = D == 64 ? 3 : 2;                  // query tiles in flight
+  static constexpr int LS = 4;                      // log-sum-exps of query tiles: used later than the tiles themselves
   static constexpr int kEpi = 256;                  // threads of the sums
   static constexpr int kLoad = 128;                 // threads that bring the queries
   static constexpr int kThreads = kEpi + 64 + kLoad;
   static constexpr int kTmem = D == 256 ? 256 : 512;
-  static constexpr int kBars = 2 * KS + 2 * QS + 2 * HB * kBufs + 2;
-  static constexpr int kSmem = KS * kKTile + QS * kQTile + QS * RT * 4 + 2 * 128 * 4 + kBars * 8 + 64;
+  static constexpr int kBars = 2 * KS + 2 * QS + 2 * LS + 2 * HB * kBufs + 2;
+  static constexpr int kSmem = KS * kKTile + QS * kQTile + LS * RT * 4 + 2 * 128 * 4 + kBars * 8 + 64;
   static_assert(HB * kBufs * RT <= kTmem && kSmem <= 232448 - 2048, "shared memory or TMEM");
 };
 
@@ -205,17 +206,17 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
     weight_kernel(const __grid_constant__ WeightParams p, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap qmap) {
   using S = WtShape<D>;
-  constexpr int HB = S::HB, KS = S::KS, QS = S::QS, RT = S::RT, kBufs = S::kBufs;
+  constexpr int HB = S::HB, KS = S::KS, QS = S::QS, LS = S::LS, RT = S::RT, kBufs = S::kBufs;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ WtLine<D> line;
   __shared__ WtItem s_items[S::kThreads / 32];
   uint8_t* s_k = smem;                           // [slot][64-column block][128 keys][128 bytes], swizzled
   uint8_t* s_q = s_k + KS * S::kKTile;           // [slot][64-column block][RT rows][128 bytes], swizzled
   float* s_lse = reinterpret_cast<float*>(s_q + QS * S::kQTile);  // [slot][RT], negated, in units of log 2
-  float* s_half = s_lse + QS * RT;               // [2][128]: the second group's sums
+  float* s_half = s_lse + S::LS * RT;               // [2][128]: the second group's sums
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_half + 256);
-  uint64_t *kfull = bars, *kempty = kfull + KS, *qfull = kempty + KS, *qempty = qfull + QS;
-  uint64_t *afull = qempty + QS, *aempty = afull + HB * kBufs, *xsync = aempty + HB * kBufs, *fin = xsync + 1;
+  uint64_t *kfull = bars, *kempty = kfull + KS, *qfull = kempty + KS, *qempty = qfull + QS, *lfull = qempty + QS;
+  uint64_t *lempty = lfull + LS, *afull = lempty + LS, *aempty = afull + HB * kBufs, *xsync = aempty + HB * kBufs, *fin = xsync + 1;
   uint32_t* words = reinterpret_cast<uint32_t*>(bars + S::kBars);
   uint32_t* s_tmem = words;
   volatile uint32_t* abort_flag = words + 1;
@@ -233,7 +234,8 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
   }
   if (tid == 0) {
     for (int i = 0; i < KS; ++i) mbar_init(&kfull[i], 1), mbar_init(&kempty[i], 1);
-    for (int i = 0; i < QS; ++i) mbar_init(&qfull[i], p.box_tokens ? 32 : S::kLoad), mbar_init(&qempty[i], 1 + 8);
+    for (int i = 0; i < QS; ++i) mbar_init(&qfull[i], p.box_tokens ? 1 : S::kLoad), mbar_init(&qempty[i], 1);
+    for (int i = 0; i < LS; ++i) mbar_init(&lfull[i], p.box_tokens ? 32 : S::kLoad), mbar_init(&lempty[i], 8);
     for (int i = 0; i < HB * kBufs; ++i) mbar_init(&afull[i], 1), mbar_init(&aempty[i], HB == 2 ? 4 : 8);
     mbar_init(xsync, S::kEpi), mbar_init(fin, 1);
     fence_barrier_init();
@@ -282,8 +284,8 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
     const uint32_t lane_off = (wq * 32u) << 16;
     const int half = HB == 2 ? static_cast<int>(g) : 0;
     const uint64_t scale2 = f2(p.a.scale_log2, p.a.scale_log2);
-    uint32_t q_slot = QS - 1, q_phase = 1, buf = 0, a_phase = 0, x_phase = 0, turn = 0;  // (the first tile goes to slot 0, phase 0)
-    bool ok = true, any_q = false;
+    uint32_t brought = 0, buf = 0, a_phase = 0, x_phase = 0, turn = 0;  // brought: query tiles so far
+    bool ok = true;
     auto group_sync = [&]() {  // both groups
       mbar_arrive(xsync);
       ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(xsync, x_phase, abort_flag, b.err));
@@ -302,16 +304,15 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
       for (int i = 0; ok && i < tiles; ++i) {
         const int rows = rows_of(tile0 + i), row0 = (tile0 + i) * p.row_tile;
         if (brings()) {
-          if (any_q && lane == 0) mbar_arrive(&qempty[q_slot]);
-          any_q = true;
-          if (++q_slot == QS) q_slot = 0, q_phase ^= 1u;
-          ok = __all_sync(0xFFFFFFFFu, wait_bar(&qfull[q_slot], q_phase, abort_flag, b.err));
+          if (brought && lane == 0) mbar_arrive(&lempty[(brought - 1) % LS]);
+          ok = __all_sync(0xFFFFFFFFu, wait_bar(&lfull[brought % LS], brought / LS & 1u, abort_flag, b.err));
+          ++brought;
         }
         if (!mine) continue;
         const uint32_t ab = half * kBufs + buf;
         ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(&afull[ab], a_phase, abort_flag, b.err));
         tc_fence_after();
-        const float* lse = s_lse + q_slot * RT;
+        const float* lse = s_lse + (brought - 1) % LS * RT;
         const uint32_t acc = tmem + lane_off + ab * RT;
         // every row of the tile is there and sees every key of the half
         const int last = it.block * S::KB + half * 128 + 127 - it.s.context;  // the last key's place among the new tokens
@@ -511,18 +512,18 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
           l[j] = r < rows ? p.lse[l_at + static_cast<int64_t>(rr / p.a.group) * p.a.q.heads + rr % p.a.group] : -INFINITY;
         }
         if (n >= QS) ok = __all_sync(0xFFFFFFFFu, wait_bar(&qempty[slot], (n / QS - 1) & 1u, abort_flag, b.err));
+        if (n >= LS) ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(&lempty[n % LS], (n / LS - 1) & 1u, abort_flag, b.err));
         if (!ok) break;
         // a row that saw nothing (or is not there) adds nothing: 2^(x - inf)
 #pragma unroll
-        for (int j = 0; j < RT / 32; ++j) s_lse[slot * RT + j * 32 + lane] = l[j] == -INFINITY ? -INFINITY : -l[j] * kLog2e;
+        for (int j = 0; j < RT / 32; ++j) s_lse[n % LS * RT + j * 32 + lane] = l[j] == -INFINITY ? -INFINITY : -l[j] * kLog2e;
         if (lane == 0) {
           mbar_arrive_expect_tx(&qfull[slot], p.box_tokens * p.a.group * D * 2);
           for (int c = 0; c < D / 64; ++c)
             tma_box(smem_u32(s_q) + slot * S::kQTile + c * (RT * 128), &qmap, c * 64, 0, it.s.kv_head,
                     it.s.row0 + row0 / p.a.group, &qfull[slot]);
-        } else {
-          mbar_arrive(&qfull[slot]);
         }
+        mbar_arrive(&lfull[n % LS]);
         ++n;
       }
       advance(tiles);
@@ -564,6 +565,11 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
           ok = __all_sync(0xFFFFFFFFu, wait_bar(&qempty[slot], (n / QS - 1) & 1u, abort_flag, b.err));
           if (!ok) break;
         }
+        if (n >= LS && !__all_sync(0xFFFFFFFFu, mbar_try_wait(&lempty[n % LS], (n / LS - 1) & 1u))) {
+          flush();
+          ok = __all_sync(0xFFFFFFFFu, wait_bar(&lempty[n % LS], (n / LS - 1) & 1u, abort_flag, b.err));
+          if (!ok) break;
+        }
         const int rows = rows_of(tile0 + i), wide = (rows + 31) & ~31, row0 = (tile0 + i) * p.row_tile;
         uint8_t* dst = s_q + slot * S::kQTile + (c >> 3) * (RT * 128);
         for (int r = r_first; r < wide; r += kPerPass) {
@@ -586,8 +592,9 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
           if (static_cast<int>(t128) < rows)
             l = p.lse[static_cast<int64_t>(it.s.row0 + rr / p.a.group) * p.a.q.heads + it.s.kv_head * p.a.group + rr % p.a.group];
           // a row that saw nothing (or is not there) adds nothing: 2^(x - inf)
-          s_lse[slot * RT + t128] = l == -INFINITY ? -INFINITY : -l * kLog2e;
+          s_lse[n % LS * RT + t128] = l == -INFINITY ? -INFINITY : -l * kLog2e;
         }
+        mbar_arrive(&lfull[n % LS]);
         if (pending) {
           cp_async_wait<1>();
           publish(n - 1);
