@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
       float* w = p.w + it.s.seq * p.row_stride + it.s.kv_head * p.head_stride + key;
       const bool keeps = writes && key < it.s.context && p.decay != 0.f;
       const float old = keeps ? __ldcg(w) : 0.f;
-      const int d = key - it.s.context;
+      const int d = key - it.s.context, d_last = d + 31 - static_cast<int>(lane);  // place among the new tokens; the warp's last
       float total = 0.f;
       for (int i = 0; ok && i < tiles; ++i) {
         const int rows = rows_of(tile0 + i), row0 = (tile0 + i) * p.row_tile;
@@ -314,13 +314,14 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
         tc_fence_after();
         const float* lse = s_lse + (brought - 1) % LS * RT;
         const uint32_t acc = tmem + lane_off + ab * RT;
-        // every row of the tile is there and sees every key of the half
-        const int last = it.block * S::KB + half * 128 + 127 - it.s.context;  // the last key's place among the new tokens
-        const bool whole = (rows & 31) == 0 && (last < 0 || (!b.tree && static_cast<int64_t>(last) * p.a.group <= row0));
+        // The rows from `full` on see every key of the warp, those before `some` none.
+        const bool all = d_last < 0, by_place = !b.tree;
+        const int64_t full = all ? 0 : by_place ? static_cast<int64_t>(d_last) * p.a.group - row0 : 1 << 30;
+        const int64_t some = all || !by_place ? 0 : static_cast<int64_t>(max(d_last - 31, 0)) * p.a.group - row0;
         const int c_lo = HB == 2 ? 0 : static_cast<int>(g) * 32, c_hi = HB == 2 ? rows : min(rows, c_lo + 32);
         uint64_t sum[2] = {0, 0};
         float odd = 0.f;
-        if (whole && c_hi - c_lo == 128) {  // the loads of 64 columns under the exponentials of the 64 before
+        if (full <= 0 && c_hi - c_lo == 128) {  // the loads of 64 columns under the exponentials of the 64 before
           uint32_t x[2][2][32];
           tmem_ld32(acc, x[0][0]);
           tmem_ld32(acc + 32, x[0][1]);
@@ -337,22 +338,21 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
         } else {
 #pragma unroll 1
           for (int c = c_lo; c < c_hi; c += 32) {
+            if (c + 31 < some) continue;
             uint32_t x[32];
             tmem_ld32(acc + c, x);
-            uint32_t see = ~0u;
-            if (!whole) {
-              if (d >= 0) see = seeing32(p, it.s, row0 + c, d);
-              if (rows - c < 32) see &= (1u << (rows - c)) - 1u;
-            }
-            tmem_wait_ld(x);
-            if (whole) {
+            if (c >= full && c + 32 <= c_hi) {
+              tmem_wait_ld(x);
               add32(x, lse + c, scale2, sum);
-            } else {
+              continue;
+            }
+            uint32_t see = d >= 0 ? seeing32(p, it.s, row0 + c, d) : ~0u;
+            if (rows - c < 32) see &= (1u << (rows - c)) - 1u;
+            tmem_wait_ld(x);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const float e = ex2(fmaf(__uint_as_float(x[j]), p.a.scale_log2, lse[c + j]));
-                if (see & (1u << j)) odd += e;
-              }
+            for (int j = 0; j < 32; ++j) {
+              const float e = ex2(fmaf(__uint_as_float(x[j]), p.a.scale_log2, lse[c + j]));
+              if (see & (1u << j)) odd += e;
             }
           }
         }
