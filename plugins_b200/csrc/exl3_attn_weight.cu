@@ -15,7 +15,7 @@
 // Roles: two groups of four warps for the exponentials and sums (a thread per key), then one warp each for the MMAs and the
 // copies of K (TMA, one box per page and 64 columns, 128-byte swizzle) and of the query rows (row t * group + g is token t's
 // query head g: a box of the kv head's query heads by tokens).  Queries whose addresses TMA does not take, or with more heads
-// per kv head than a tile has rows, are brought by four warps instead.  Heads up to 128 wide: an item is 256 keys, a group per half.  256 wide: 128 keys,
+// per kv head than a tile has rows, are brought by two warps instead.  Heads up to 128 wide: an item is 256 keys, a group per half.  256 wide: 128 keys,
 // whose columns the groups share.
 //
 // Every mbarrier wait is bounded (wait_bar): one that gives up raises an abort flag that all roles poll.
@@ -48,7 +48,7 @@ struct WtShape {
   static constexpr int QS = D == 64 ? 3 : 2;                  // query tiles in flight
   static constexpr int LS = 4;                      // log-sum-exps of query tiles: used later than the tiles themselves
   static constexpr int kEpi = 256;                  // threads of the sums
-  static constexpr int kLoad = 128;                 // threads that bring the queries
+  static constexpr int kLoad = 64;                  // threads that bring the queries
   static constexpr int kThreads = kEpi + 64 + kLoad;
   static constexpr int kTmem = D == 256 ? 256 : 512;
   static constexpr int kBars = 2 * KS + 2 * QS + 2 * LS + 2 * HB * kBufs + 2;
@@ -78,7 +78,7 @@ struct WtLine : WorkLine {
   // The first row tile that sees any key of the block: without a tree, slot context + d is seen from token d on.
   __device__ __forceinline__ static int first_of(const WeightParams& p, const WtItem& it, int block) {
     const int d = block * S::KB - it.s.context;
-    return p.a.b.tree || d <= 0 ? 0 : static_cast<int>(static_cast<int64_t>(d) * p.a.group / p.row_tile);
+    return p.a.b.tree || d <= 0 ? 0 : static_cast<int>(divide(static_cast<int64_t>(d) * p.a.group, p.row_tile));
   }
   __device__ __forceinline__ static void set_block(const WeightParams& p, WtItem& it) {
     it.first_tile = first_of(p, it, it.block);
@@ -300,69 +300,77 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
       const bool keeps = writes && key < it.s.context && p.decay != 0.f;
       const float old = keeps ? __ldcg(w) : 0.f;
       const int d = key - it.s.context, d_last = d + 31 - static_cast<int>(lane);  // place among the new tokens; the warp's last
+      const int nrows = it.s.nrows;
+      const bool all = d_last < 0, by_place = !b.tree;
+      // a sequence of one query tile may have it here already; those of more bring each
+      bool bring = brings();
+      int row0 = tile0 * p.row_tile;
+      // The rows from `full` on see every key of the warp, those before `some` none, counted from the tile's first row.
+      // (A call has at most 2^30 query vectors: a key's place times the group stays below 2^31.)
+      int full = all ? -(1 << 30) : by_place ? d_last * p.a.group - row0 : 1 << 30;
+      int some = all || !by_place ? -(1 << 30) : max(d_last - 31, 0) * p.a.group - row0;
       float total = 0.f;
       for (int i = 0; ok && i < tiles; ++i) {
-        const int rows = rows_of(tile0 + i), row0 = (tile0 + i) * p.row_tile;
-        if (brings()) {
+        const int rows = min(p.row_tile, nrows - row0);
+        if (bring) {
           if (brought && lane == 0) mbar_arrive(&lempty[(brought - 1) % LS]);
-          ok = __all_sync(0xFFFFFFFFu, wait_bar(&lfull[brought % LS], brought / LS & 1u, abort_flag, b.err));
           ++brought;
         }
-        if (!mine) continue;
-        const uint32_t ab = half * kBufs + buf;
-        ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(&afull[ab], a_phase, abort_flag, b.err));
-        tc_fence_after();
-        const float* lse = s_lse + (brought - 1) % LS * RT;
-        const uint32_t acc = tmem + lane_off + ab * RT;
-        // The rows from `full` on see every key of the warp, those before `some` none.
-        const bool all = d_last < 0, by_place = !b.tree;
-        const int64_t full = all ? 0 : by_place ? static_cast<int64_t>(d_last) * p.a.group - row0 : 1 << 30;
-        const int64_t some = all || !by_place ? 0 : static_cast<int64_t>(max(d_last - 31, 0)) * p.a.group - row0;
-        const int c_lo = HB == 2 ? 0 : static_cast<int>(g) * 32, c_hi = HB == 2 ? rows : min(rows, c_lo + 32);
-        uint64_t sum[2] = {0, 0};
-        float odd = 0.f;
-        if (full <= 0 && c_hi - c_lo == 128) {  // the loads of 64 columns under the exponentials of the 64 before
-          uint32_t x[2][2][32];
-          tmem_ld32(acc, x[0][0]);
-          tmem_ld32(acc + 32, x[0][1]);
-          tmem_wait_ld(x[0][0]);
-          after_wait(x[0][1]);
-          tmem_ld32(acc + 64, x[1][0]);
-          tmem_ld32(acc + 96, x[1][1]);
-          add32(x[0][0], lse, scale2, sum);
-          add32(x[0][1], lse + 32, scale2, sum);
-          tmem_wait_ld(x[1][0]);
-          after_wait(x[1][1]);
-          add32(x[1][0], lse + 64, scale2, sum);
-          add32(x[1][1], lse + 96, scale2, sum);
-        } else {
+        bring = true;
+        if (mine) {
+          const uint32_t ab = half * kBufs + buf;
+          ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(&afull[ab], a_phase, abort_flag, b.err));
+          tc_fence_after();
+          const float* lse = s_lse + (brought - 1) % LS * RT;
+          const uint32_t acc = tmem + lane_off + ab * RT;
+          const int c_lo = HB == 2 ? 0 : static_cast<int>(g) * 32, c_hi = HB == 2 ? rows : min(rows, c_lo + 32);
+          uint64_t sum[2] = {0, 0};
+          float odd = 0.f;
+          if (full <= 0 && c_hi - c_lo == 128) {  // the loads of 64 columns under the exponentials of the 64 before
+            uint32_t x[2][2][32];
+            tmem_ld32(acc, x[0][0]);
+            tmem_ld32(acc + 32, x[0][1]);
+            tmem_wait_ld(x[0][0]);
+            after_wait(x[0][1]);
+            tmem_ld32(acc + 64, x[1][0]);
+            tmem_ld32(acc + 96, x[1][1]);
+            add32(x[0][0], lse, scale2, sum);
+            add32(x[0][1], lse + 32, scale2, sum);
+            tmem_wait_ld(x[1][0]);
+            after_wait(x[1][1]);
+            add32(x[1][0], lse + 64, scale2, sum);
+            add32(x[1][1], lse + 96, scale2, sum);
+          } else {
 #pragma unroll 1
-          for (int c = c_lo; c < c_hi; c += 32) {
-            if (c + 31 < some) continue;
-            uint32_t x[32];
-            tmem_ld32(acc + c, x);
-            if (c >= full && c + 32 <= c_hi) {
+            for (int c = c_lo; c < c_hi; c += 32) {
+              if (c + 31 < some) continue;
+              uint32_t x[32];
+              tmem_ld32(acc + c, x);
+              if (c >= full && c + 32 <= c_hi) {
+                tmem_wait_ld(x);
+                add32(x, lse + c, scale2, sum);
+                continue;
+              }
+              uint32_t see = d >= 0 ? seeing32(p, it.s, row0 + c, d) : ~0u;
+              if (rows - c < 32) see &= (1u << (rows - c)) - 1u;
               tmem_wait_ld(x);
-              add32(x, lse + c, scale2, sum);
-              continue;
-            }
-            uint32_t see = d >= 0 ? seeing32(p, it.s, row0 + c, d) : ~0u;
-            if (rows - c < 32) see &= (1u << (rows - c)) - 1u;
-            tmem_wait_ld(x);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float e = ex2(fmaf(__uint_as_float(x[j]), p.a.scale_log2, lse[c + j]));
-              if (see & (1u << j)) odd += e;
+              for (int j = 0; j < 32; ++j) {
+                const float e = ex2(fmaf(__uint_as_float(x[j]), p.a.scale_log2, lse[c + j]));
+                if (see & (1u << j)) odd += e;
+              }
             }
           }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&aempty[ab]);
+          if (++buf == kBufs) buf = 0, a_phase ^= 1u;
+          float s0, s1;
+          f2_split(add2(sum[0], sum[1]), s0, s1);
+          total += (s0 + s1) + odd;
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&aempty[ab]);
-        if (++buf == kBufs) buf = 0, a_phase ^= 1u;
-        float s0, s1;
-        f2_split(add2(sum[0], sum[1]), s0, s1);
-        total += (s0 + s1) + odd;
+        row0 += p.row_tile;
+        if (!all && by_place) full -= p.row_tile, some -= p.row_tile;
       }
       if constexpr (HB == 1) {  // the groups' columns together
         float* there = s_half + (turn++ & 1u) * 128;
@@ -403,7 +411,7 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
     const uint32_t on = elect_one();
     const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
     const uint64_t qdesc = sw128_desc(smem_u32(s_q)), kdesc = sw128_desc(smem_u32(s_k));
-    uint32_t k_slot = 0, k_phase = 0, q_slot = QS - 1, q_phase = 1;
+    uint32_t k_slot = 0, k_phase = 0, q_slot = QS - 1, q_phase = 1, brought = 0;
     uint32_t used[HB] = {};  // tiles a half's accumulators have served
     bool ok = true, any_q = false;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -426,6 +434,8 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
           if (any_q) commit(on, &qempty[q_slot]);
           any_q = true;
           if (++q_slot == QS) q_slot = 0, q_phase ^= 1u;
+          wait(&lfull[brought % LS], brought / LS & 1u);  // the sums read them when this tile's product is there
+          ++brought;
           wait(&qfull[q_slot], q_phase);
         }
         const uint32_t idesc = uniform((attn_idesc<BF16>(128, 0, false)) | (static_cast<uint32_t>(((rows + 31) & ~31) >> 3) << 17));
@@ -536,10 +546,10 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
     }
     __syncwarp();
   } else {
-    // ---------------------------------------------------------------- queries that TMA cannot fetch, likewise: four warps
-    const uint32_t t128 = tid - (S::kEpi + 64);
+    // ---------------------------------------------------------------- queries that TMA cannot fetch, likewise: two warps
+    const uint32_t t = tid - (S::kEpi + 64);
     constexpr int kChunks = D / 8, kPerPass = S::kLoad / kChunks;  // a row's 16-byte chunks lie on neighbouring lanes
-    const int c = static_cast<int>(t128) % kChunks, r_first = static_cast<int>(t128) / kChunks;
+    const int c = static_cast<int>(t) % kChunks, r_first = static_cast<int>(t) / kChunks;
     uint32_t n = 0;        // tiles brought
     bool ok = true, pending = false;  // the last one's copies are on their way: not published yet
     auto publish = [&](uint32_t which) {
@@ -573,26 +583,26 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
         const int rows = rows_of(tile0 + i), wide = (rows + 31) & ~31, row0 = (tile0 + i) * p.row_tile;
         uint8_t* dst = s_q + slot * S::kQTile + (c >> 3) * (RT * 128);
         for (int r = r_first; r < wide; r += kPerPass) {
-          const int rr = row0 + r, t = rr / p.a.group, h = it.s.kv_head * p.a.group + rr % p.a.group;
+          const int rr = row0 + r, tok = rr / p.a.group, h = it.s.kv_head * p.a.group + rr % p.a.group;
           const uint32_t to = smem_u32(dst + image_offset(static_cast<uint32_t>(r), static_cast<uint32_t>((c & 7) * 8)));
           const bool in = r < rows;
           if (p.a.q.vec) {
             const uint16_t* src = static_cast<const uint16_t*>(p.a.q.data);
-            if (in) src += static_cast<int64_t>(it.s.row0 + t) * p.a.q.row_stride + static_cast<int64_t>(h) * p.a.q.head_stride + c * 8;
+            if (in) src += static_cast<int64_t>(it.s.row0 + tok) * p.a.q.row_stride + static_cast<int64_t>(h) * p.a.q.head_stride + c * 8;
             cp_async16(to, src, in);
           } else {
-            const uint4 u = in ? load_q8(p.a.q, it.s.row0 + t, h, c * 8) : make_uint4(0u, 0u, 0u, 0u);
+            const uint4 u = in ? load_q8(p.a.q, it.s.row0 + tok, h, c * 8) : make_uint4(0u, 0u, 0u, 0u);
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
           }
         }
         cp_async_commit();
-        if (static_cast<int>(t128) < RT) {
-          const int rr = row0 + static_cast<int>(t128);
+        for (int r = static_cast<int>(t); r < RT; r += S::kLoad) {
+          const int rr = row0 + r;
           float l = -INFINITY;
-          if (static_cast<int>(t128) < rows)
+          if (r < rows)
             l = p.lse[static_cast<int64_t>(it.s.row0 + rr / p.a.group) * p.a.q.heads + it.s.kv_head * p.a.group + rr % p.a.group];
           // a row that saw nothing (or is not there) adds nothing: 2^(x - inf)
-          s_lse[n % LS * RT + t128] = l == -INFINITY ? -INFINITY : -l * kLog2e;
+          s_lse[n % LS * RT + r] = l == -INFINITY ? -INFINITY : -l * kLog2e;
         }
         mbar_arrive(&lfull[n % LS]);
         if (pending) {
