@@ -12,11 +12,11 @@
 // one row tile (decoding, small trees) that stays, and the keys stream.  An item cut between CTAs is joined by the last of
 // them to finish, its partial sums added in the line's order: the bits do not depend on which CTA that is.
 //
-// Roles: two groups of four warps for the exponentials and sums (a thread per key), then one warp each for the MMAs and the
+// Roles: four groups of four warps for the exponentials and sums (a thread per key), then one warp each for the MMAs and the
 // copies of K (TMA, one box per page and 64 columns, 128-byte swizzle) and of the query rows (row t * group + g is token t's
 // query head g: a box of the kv head's query heads by tokens).  Queries whose addresses TMA does not take, or with more heads
-// per kv head than a tile has rows, are brought by two warps instead.  Heads up to 128 wide: an item is 256 keys, a group per half.  256 wide: 128 keys,
-// whose columns the groups share.
+// per kv head than a tile has rows, are brought by two warps instead.  Heads up to 128 wide: an item is 256 keys, two groups per half
+// that take its row tiles by turns.  256 wide: 128 keys, all four by turns.
 //
 // Every mbarrier wait is bounded (wait_bar): one that gives up raises an abort flag that all roles poll.
 #include <cuda.h>
@@ -35,6 +35,7 @@ using namespace tc;
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kPolyEvery = 8;  // one pair of this many numbers takes the FMA pipe
 
 template <int D>
 struct WtShape {
@@ -47,12 +48,13 @@ struct WtShape {
   static constexpr int KS = D == 256 ? 2 : D == 128 ? 4 : 6;  // K halves in flight
   static constexpr int QS = D == 64 ? 3 : 2;                  // query tiles in flight
   static constexpr int LS = 4;                      // log-sum-exps of query tiles: used later than the tiles themselves
-  static constexpr int kEpi = 256;                  // threads of the sums
+  static constexpr int kEpi = 512;                  // threads of the sums: four groups of four warps
+  static constexpr int GH = 4 / HB;                 // groups of a half, which take its tiles by turns
   static constexpr int kLoad = 64;                  // threads that bring the queries
   static constexpr int kThreads = kEpi + 64 + kLoad;
   static constexpr int kTmem = D == 256 ? 256 : 512;
   static constexpr int kBars = 2 * KS + 2 * QS + 2 * LS + 2 * HB * kBufs + 2;
-  static constexpr int kSmem = KS * kKTile + QS * kQTile + LS * RT * 4 + 2 * 128 * 4 + kBars * 8 + 64;
+  static constexpr int kSmem = KS * kKTile + QS * kQTile + LS * RT * 4 + 2 * 3 * 128 * 4 + kBars * 8 + 64;
   static_assert(HB * kBufs * RT <= kTmem && kSmem <= 232448 - 2048, "shared memory or TMEM");
 };
 
@@ -188,6 +190,31 @@ __device__ __forceinline__ uint32_t seeing32(const WeightParams& p, const Item& 
   return m;
 }
 
+// 2^x of two numbers at most about 0 on the FMA pipe: x = n + f with |f| <= 1/2, a polynomial of degree 5 for 2^f (the
+// minimax of its relative error, 7.5e-8, by Remez' exchange) and n into the exponent.  Below -125 exactly zero, NaN stays.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t exp2_fma(float a, float b) {
+  constexpr float kRound = 12582912.f;  // 1.5 x 2^23: what is added to it loses its fraction
+  const uint64_t x = f2(max_nan(a, -125.f), max_nan(b, -125.f));
+  const uint64_t t = add2(x, f2(kRound, kRound));
+  const uint64_t f = fma2(add2(t, f2(-kRound, -kRound)), f2(-1.f, -1.f), x);
+  uint64_t y = fma2(f2(0.0013276472f, 0.0013276472f), f, f2(0.00967554133f, 0.00967554133f));
+  y = fma2(y, f, f2(0.0555071327f, 0.0555071327f));
+  y = fma2(y, f, f2(0.240221197f, 0.240221197f));
+  y = fma2(y, f, f2(0.693146967f, 0.693146967f));
+  y = fma2(y, f, f2(1.00000007f, 1.00000007f));
+  float t0, t1, y0, y1;
+  f2_split(t, t0, t1), f2_split(y, y0, y1);
+  y0 = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23));
+  y1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23));
+  constexpr float kLeast = 2.35098887e-38f * 1.00000007f;  // what x = -125 comes to
+  return add2(f2(y0, y1), f2(-kLeast, -kLeast));
+}
+
 // The sum of 2^(scale x - lse) over 32 accumulators; lse in shared memory, in units of log 2.
 __device__ __forceinline__ void add32(const uint32_t (&x)[32], const float* lse, uint64_t scale2, uint64_t (&sum)[2]) {
 #pragma unroll
@@ -197,7 +224,7 @@ __device__ __forceinline__ void add32(const uint32_t (&x)[32], const float* lse,
     f2_split(fma2(f2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, f2(l.x, l.y)), a, b);
     f2_split(fma2(f2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), scale2, f2(l.z, l.w)), c, d);
     sum[0] = add2(sum[0], f2(ex2(a), ex2(b)));
-    sum[1] = add2(sum[1], f2(ex2(c), ex2(d)));
+    sum[1] = add2(sum[1], i % kPolyEvery == 0 ? exp2_fma(c, d) : f2(ex2(c), ex2(d)));
   }
 }
 
@@ -213,8 +240,8 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
   uint8_t* s_k = smem;                           // [slot][64-column block][128 keys][128 bytes], swizzled
   uint8_t* s_q = s_k + KS * S::kKTile;           // [slot][64-column block][RT rows][128 bytes], swizzled
   float* s_lse = reinterpret_cast<float*>(s_q + QS * S::kQTile);  // [slot][RT], negated, in units of log 2
-  float* s_half = s_lse + S::LS * RT;               // [2][128]: the second group's sums
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_half + 256);
+  float* s_sums = s_lse + LS * RT;               // [2][3][128]: the other groups' sums, by turns
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_sums + 768);
   uint64_t *kfull = bars, *kempty = kfull + KS, *qfull = kempty + KS, *qempty = qfull + QS, *lfull = qempty + QS;
   uint64_t *lempty = lfull + LS, *afull = lempty + LS, *aempty = afull + HB * kBufs, *xsync = aempty + HB * kBufs, *fin = xsync + 1;
   uint32_t* words = reinterpret_cast<uint32_t*>(bars + S::kBars);
@@ -228,16 +255,16 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
     if (tid == 0) atomicOr(b.err, kErrBadShape);
     return;
   }
-  if (warp == 8) {
+  if (warp == 16) {
     tmem_alloc(smem_u32(s_tmem), S::kTmem);
     tmem_relinquish();
   }
   if (tid == 0) {
     for (int i = 0; i < KS; ++i) mbar_init(&kfull[i], 1), mbar_init(&kempty[i], 1);
     for (int i = 0; i < QS; ++i) mbar_init(&qfull[i], p.box_tokens ? 1 : S::kLoad), mbar_init(&qempty[i], 1);
-    for (int i = 0; i < LS; ++i) mbar_init(&lfull[i], p.box_tokens ? 32 : S::kLoad), mbar_init(&lempty[i], 8);
-    for (int i = 0; i < HB * kBufs; ++i) mbar_init(&afull[i], 1), mbar_init(&aempty[i], HB == 2 ? 4 : 8);
-    mbar_init(xsync, S::kEpi), mbar_init(fin, 1);
+    for (int i = 0; i < LS; ++i) mbar_init(&lfull[i], p.box_tokens ? 32 : S::kLoad), mbar_init(&lempty[i], 16);
+    for (int i = 0; i < HB * kBufs; ++i) mbar_init(&afull[i], 1), mbar_init(&aempty[i], 4);
+    mbar_init(xsync, 16), mbar_init(fin, 1);
     fence_barrier_init();
     *abort_flag = 0u;
   }
@@ -247,7 +274,7 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
   {
     WtLine<D> own;
     WtItem first;
-    own.begin_line(p, reinterpret_cast<int64_t*>(s_half), first);  // (no place that TMA writes: that is another proxy)
+    own.begin_line(p, reinterpret_cast<int64_t*>(s_sums), first);  // (no place that TMA writes: that is another proxy)
     if (tid == 0) line = own;
     if (lane == 0) s_items[warp] = first;
   }
@@ -278,16 +305,18 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
   auto halves_here = [&]() { return min(HB, (it.s.total_keys - it.block * S::KB + 127) / 128); };
   auto rows_of = [&](int tile) { return min(p.row_tile, it.s.nrows - tile * p.row_tile); };
 
-  if (warp < 8) {
+  if (warp < 16) {
     // ---------------------------------------------------------------- exponentials and sums: a thread per key
+    constexpr uint32_t GH = S::GH;
     const uint32_t g = warp >> 2, wq = warp & 3u, r128 = wq * 32 + lane;  // key of the half = TMEM lane
     const uint32_t lane_off = (wq * 32u) << 16;
-    const int half = HB == 2 ? static_cast<int>(g) : 0;
+    const int half = static_cast<int>(g / GH);
     const uint64_t scale2 = f2(p.a.scale_log2, p.a.scale_log2);
-    uint32_t brought = 0, buf = 0, a_phase = 0, x_phase = 0, turn = 0;  // brought: query tiles so far
+    uint32_t brought = 0, served = 0, x_phase = 0, turn = 0;  // query tiles so far; the half's tiles so far
     bool ok = true;
-    auto group_sync = [&]() {  // both groups
-      mbar_arrive(xsync);
+    auto group_sync = [&]() {  // all groups
+      __syncwarp();
+      if (lane == 0) mbar_arrive(xsync);
       ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(xsync, x_phase, abort_flag, b.err));
       x_phase ^= 1u;
     };
@@ -295,7 +324,9 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
       const int tiles = tiles_here(), tile0 = first_here(), halves = halves_here();
       const int key = it.block * S::KB + half * 128 + static_cast<int>(r128);
       const bool mine = half < halves;
-      const bool writes = mine && key < it.s.total_keys && (HB == 2 || g == 0);
+      const bool solo = it.row_tiles == 1;  // its one tile's group has nobody to wait for
+      const uint32_t writer = half * GH + (solo ? served % GH : 0u);
+      const bool writes = mine && key < it.s.total_keys && g == writer;
       float* w = p.w + it.s.seq * p.row_stride + it.s.kv_head * p.head_stride + key;
       const bool keeps = writes && key < it.s.context && p.decay != 0.f;
       const float old = keeps ? __ldcg(w) : 0.f;
@@ -317,36 +348,32 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
           ++brought;
         }
         bring = true;
-        if (mine) {
-          const uint32_t ab = half * kBufs + buf;
-          ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(&afull[ab], a_phase, abort_flag, b.err));
+        const uint32_t use = served;
+        if (mine) ++served;
+        if (mine && use % GH == g % GH) {
+          const uint32_t ab = half * kBufs + use % kBufs;
+          ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(&afull[ab], use / kBufs & 1u, abort_flag, b.err));
           tc_fence_after();
           const float* lse = s_lse + (brought - 1) % LS * RT;
           const uint32_t acc = tmem + lane_off + ab * RT;
-          const int c_lo = HB == 2 ? 0 : static_cast<int>(g) * 32, c_hi = HB == 2 ? rows : min(rows, c_lo + 32);
           uint64_t sum[2] = {0, 0};
           float odd = 0.f;
-          if (full <= 0 && c_hi - c_lo == 128) {  // the loads of 64 columns under the exponentials of the 64 before
-            uint32_t x[2][2][32];
-            tmem_ld32(acc, x[0][0]);
-            tmem_ld32(acc + 32, x[0][1]);
-            tmem_wait_ld(x[0][0]);
-            after_wait(x[0][1]);
-            tmem_ld32(acc + 64, x[1][0]);
-            tmem_ld32(acc + 96, x[1][1]);
-            add32(x[0][0], lse, scale2, sum);
-            add32(x[0][1], lse + 32, scale2, sum);
-            tmem_wait_ld(x[1][0]);
-            after_wait(x[1][1]);
-            add32(x[1][0], lse + 64, scale2, sum);
-            add32(x[1][1], lse + 96, scale2, sum);
+          if (full <= 0 && rows == RT) {  // the loads of 32 columns under the exponentials of the 32 before
+            uint32_t x[2][32];
+            tmem_ld32(acc, x[0]);
+#pragma unroll
+            for (int c = 0; c < RT; c += 32) {
+              tmem_wait_ld(x[c / 32 & 1]);
+              if (c + 32 < RT) tmem_ld32(acc + c + 32, x[~(c / 32) & 1]);
+              add32(x[c / 32 & 1], lse + c, scale2, sum);
+            }
           } else {
 #pragma unroll 1
-            for (int c = c_lo; c < c_hi; c += 32) {
+            for (int c = 0; c < rows; c += 32) {
               if (c + 31 < some) continue;
               uint32_t x[32];
               tmem_ld32(acc + c, x);
-              if (c >= full && c + 32 <= c_hi) {
+              if (c >= full && c + 32 <= rows) {
                 tmem_wait_ld(x);
                 add32(x, lse + c, scale2, sum);
                 continue;
@@ -364,7 +391,6 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&aempty[ab]);
-          if (++buf == kBufs) buf = 0, a_phase ^= 1u;
           float s0, s1;
           f2_split(add2(sum[0], sum[1]), s0, s1);
           total += (s0 + s1) + odd;
@@ -372,11 +398,13 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
         row0 += p.row_tile;
         if (!all && by_place) full -= p.row_tile, some -= p.row_tile;
       }
-      if constexpr (HB == 1) {  // the groups' columns together
-        float* there = s_half + (turn++ & 1u) * 128;
-        if (g == 1) there[r128] = total;
+      if (!solo) {  // the groups' sums together, in their order
+        float* there = s_sums + (turn++ & 1u) * 384;
+        if (g % GH != 0) there[(g - 1) * 128 + r128] = total;
         group_sync();
-        if (g == 0) total += there[r128];
+        if (g % GH == 0)
+#pragma unroll
+          for (uint32_t o = 1; o < GH; ++o) total += there[(g + o - 1) * 128 + r128];
       }
       if (tiles == it.tiles) {
         if (writes) *w = keeps ? fmaf(p.decay, old, total) : total;
@@ -406,7 +434,7 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
       }
       advance(tiles);
     }
-  } else if (warp == 8) {
+  } else if (warp == 16) {
     // ---------------------------------------------------------------- MMA issuer: converged, one elected lane issues
     const uint32_t on = elect_one();
     const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
@@ -464,7 +492,7 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
     commit(on, fin);  // every MMA has finished before TMEM is released
     if (lane == 0 && !mbar_wait_bounded(fin, 0)) atomicOr(b.err, kErrWaitTimeout);
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == 17) {
     // ---------------------------------------------------------------- K copies
     const uint32_t base = smem_u32(s_k);
     const int box_rows = min(1 << b.page_shift, 128);
@@ -507,7 +535,7 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
   } else if (p.box_tokens) {
     // ---------------------------------------------------------------- queries (TMA) and their log-sum-exps: one warp
     uint32_t n = 0;
-    bool ok = warp == 10;
+    bool ok = warp == 18;
     while (ok && at < end) {
       const int tiles = tiles_here(), tile0 = first_here();
       for (int i = 0; ok && i < tiles; ++i) {
@@ -619,7 +647,7 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem, S::kTmem);
   }
