@@ -53,7 +53,7 @@ struct WtShape {
   static constexpr int kLoad = 64;                  // threads that bring the queries
   static constexpr int kThreads = kEpi + 64 + kLoad;
   static constexpr int kTmem = D == 256 ? 256 : 512;
-  static constexpr int kBars = 2 * KS + 2 * QS + 2 * LS + 2 * HB * kBufs + 2;
+  static constexpr int kBars = 2 * KS + 2 * QS + LS + 2 * HB * kBufs + 2;
   static constexpr int kSmem = KS * kKTile + QS * kQTile + LS * RT * 4 + 2 * 3 * 128 * 4 + kBars * 8 + 64;
   static_assert(HB * kBufs * RT <= kTmem && kSmem <= 232448 - 2048, "shared memory or TMEM");
 };
@@ -242,8 +242,8 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
   float* s_lse = reinterpret_cast<float*>(s_q + QS * S::kQTile);  // [slot][RT], negated, in units of log 2
   float* s_sums = s_lse + LS * RT;               // [2][3][128]: the other groups' sums, by turns
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_sums + 768);
-  uint64_t *kfull = bars, *kempty = kfull + KS, *qfull = kempty + KS, *qempty = qfull + QS, *lfull = qempty + QS;
-  uint64_t *lempty = lfull + LS, *afull = lempty + LS, *aempty = afull + HB * kBufs, *xsync = aempty + HB * kBufs, *fin = xsync + 1;
+  uint64_t *kfull = bars, *kempty = kfull + KS, *qfull = kempty + KS, *qempty = qfull + QS, *lempty = qempty + QS;
+  uint64_t *afull = lempty + LS, *aempty = afull + HB * kBufs, *xsync = aempty + HB * kBufs, *fin = xsync + 1;
   uint32_t* words = reinterpret_cast<uint32_t*>(bars + S::kBars);
   uint32_t* s_tmem = words;
   volatile uint32_t* abort_flag = words + 1;
@@ -261,8 +261,8 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
   }
   if (tid == 0) {
     for (int i = 0; i < KS; ++i) mbar_init(&kfull[i], 1), mbar_init(&kempty[i], 1);
-    for (int i = 0; i < QS; ++i) mbar_init(&qfull[i], p.box_tokens ? 1 : S::kLoad), mbar_init(&qempty[i], 1);
-    for (int i = 0; i < LS; ++i) mbar_init(&lfull[i], p.box_tokens ? 32 : S::kLoad), mbar_init(&lempty[i], 16);
+    for (int i = 0; i < QS; ++i) mbar_init(&qfull[i], p.box_tokens ? 1 + 32 : S::kLoad), mbar_init(&qempty[i], 1);
+    for (int i = 0; i < LS; ++i) mbar_init(&lempty[i], 16);
     for (int i = 0; i < HB * kBufs; ++i) mbar_init(&afull[i], 1), mbar_init(&aempty[i], 4);
     mbar_init(xsync, 16), mbar_init(fin, 1);
     fence_barrier_init();
@@ -439,7 +439,8 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
     const uint32_t on = elect_one();
     const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
     const uint64_t qdesc = sw128_desc(smem_u32(s_q)), kdesc = sw128_desc(smem_u32(s_k));
-    uint32_t k_slot = 0, k_phase = 0, q_slot = QS - 1, q_phase = 1, brought = 0;
+    constexpr uint32_t kIdesc = attn_idesc<BF16>(128, 0, false);
+    uint32_t k_slot = 0, k_phase = 0, q_slot = QS - 1, q_phase = 1;
     uint32_t used[HB] = {};  // tiles a half's accumulators have served
     bool ok = true, any_q = false;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -447,46 +448,47 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
       ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(bar, parity, abort_flag, b.err));
     };
     while (ok && at < end) {
-      const int tiles = tiles_here(), tile0 = first_here(), halves = halves_here();
-      uint32_t ks[HB];
+      const int tiles = tiles_here(), halves = halves_here();
+      int left = it.s.nrows - first_here() * p.row_tile;  // rows from the tile on
+      bool bring = brings();
+      uint32_t ks[HB] = {};
 #pragma unroll
       for (int h = 0; h < HB; ++h) {
         if (h >= halves) break;
-        ks[h] = k_slot;
+        ks[h] = uniform(k_slot * (S::kKTile >> 4));
         wait(&kfull[k_slot], k_phase);
         if (++k_slot == KS) k_slot = 0, k_phase ^= 1u;
       }
-      for (int i = 0; ok && i < tiles; ++i) {
-        const int rows = rows_of(tile0 + i);
-        if (brings()) {
+      for (int i = 0; ok && i < tiles; ++i, left -= p.row_tile) {
+        if (bring) {
           if (any_q) commit(on, &qempty[q_slot]);
           any_q = true;
           if (++q_slot == QS) q_slot = 0, q_phase ^= 1u;
-          wait(&lfull[brought % LS], brought / LS & 1u);  // the sums read them when this tile's product is there
-          ++brought;
           wait(&qfull[q_slot], q_phase);
         }
-        const uint32_t idesc = uniform((attn_idesc<BF16>(128, 0, false)) | (static_cast<uint32_t>(((rows + 31) & ~31) >> 3) << 17));
+        bring = true;
+        // as many columns as the tile has rows, in whole chunks of 32
+        const uint32_t idesc = uniform(kIdesc | static_cast<uint32_t>((min(left, p.row_tile) + 31) >> 5) << 19);
+        const uint32_t qo = uniform(q_slot * (S::kQTile >> 4));
 #pragma unroll
         for (int h = 0; h < HB; ++h) {
           if (h >= halves) break;
-          const uint32_t ab = h * kBufs + used[h] % kBufs;
+          const uint32_t ab = uniform(h * kBufs + used[h] % kBufs);
           if (used[h] >= kBufs) wait(&aempty[ab], (used[h] / kBufs - 1) & 1u);
           ++used[h];
           if (!ok) break;
           tc_fence_after();
-          const uint32_t qo = uniform(q_slot * (S::kQTile >> 4)), ko = uniform(ks[h] * (S::kKTile >> 4));
-          const uint32_t ad = uniform(tm + ab * RT);
+          const uint32_t ad = tm + ab * RT;
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            mma_ss(on, ad, desc_at(kdesc, ko + (((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4)),
+            mma_ss(on, ad, desc_at(kdesc, ks[h] + (((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4)),
                    desc_at(qdesc, qo + (((kk >> 2) * (RT * 128) + (kk & 3) * 32) >> 4)), idesc, kk != 0 ? 1u : 0u);
           commit(on, &afull[ab]);
         }
       }
 #pragma unroll
       for (int h = 0; h < HB; ++h)
-        if (h < halves) commit(on, &kempty[ks[h]]);
+        if (h < halves) commit(on, &kempty[(k_slot + KS - halves + h) % KS]);
       advance(tiles);
     }
     commit(on, fin);  // every MMA has finished before TMEM is released
@@ -534,45 +536,63 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
     __syncwarp();
   } else if (p.box_tokens) {
     // ---------------------------------------------------------------- queries (TMA) and their log-sum-exps: one warp
-    uint32_t n = 0;
-    bool ok = warp == 18;
-    while (ok && at < end) {
-      const int tiles = tiles_here(), tile0 = first_here();
-      for (int i = 0; ok && i < tiles; ++i) {
-        if (!brings()) continue;
-        const uint32_t slot = n % QS;
-        const int rows = rows_of(tile0 + i), row0 = (tile0 + i) * p.row_tile;
-        const int64_t l_at = static_cast<int64_t>(it.s.row0) * p.a.q.heads + it.s.kv_head * p.a.group;
-        float l[RT / 32];
+    if (warp == 18) {
+      const int tokens = p.row_tile / p.a.group;  // of a tile
+      int64_t off[RT / 32];                       // a lane's rows lie at the same places of every tile
 #pragma unroll
-        for (int j = 0; j < RT / 32; ++j) {
-          const int r = j * 32 + static_cast<int>(lane), rr = row0 + r;
-          l[j] = r < rows ? p.lse[l_at + static_cast<int64_t>(rr / p.a.group) * p.a.q.heads + rr % p.a.group] : -INFINITY;
-        }
-        if (n >= QS) ok = __all_sync(0xFFFFFFFFu, wait_bar(&qempty[slot], (n / QS - 1) & 1u, abort_flag, b.err));
-        if (n >= LS) ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(&lempty[n % LS], (n / LS - 1) & 1u, abort_flag, b.err));
-        if (!ok) break;
-        // a row that saw nothing (or is not there) adds nothing: 2^(x - inf)
-#pragma unroll
-        for (int j = 0; j < RT / 32; ++j) s_lse[n % LS * RT + j * 32 + lane] = l[j] == -INFINITY ? -INFINITY : -l[j] * kLog2e;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&qfull[slot], p.box_tokens * p.a.group * D * 2);
-          for (int c = 0; c < D / 64; ++c)
-            tma_box(smem_u32(s_q) + slot * S::kQTile + c * (RT * 128), &qmap, c * 64, 0, it.s.kv_head,
-                    it.s.row0 + row0 / p.a.group, &qfull[slot]);
-        }
-        mbar_arrive(&lfull[n % LS]);
-        ++n;
+      for (int j = 0; j < RT / 32; ++j) {
+        const int r = j * 32 + static_cast<int>(lane);
+        off[j] = static_cast<int64_t>(r / p.a.group) * p.a.q.heads + r % p.a.group;
       }
-      advance(tiles);
+      uint32_t n = 0;
+      bool ok = true;
+      while (ok && at < end) {
+        const int tiles = tiles_here();
+        bool bring = brings();
+        if (!bring) {
+          advance(tiles);
+          continue;
+        }
+        const int tile0 = first_here(), kv_head = it.s.kv_head;
+        int left = it.s.nrows - tile0 * p.row_tile, token = it.s.row0 + tile0 * tokens;  // the tile's rows, its first token
+        const float* lse = p.lse + static_cast<int64_t>(token) * p.a.q.heads + kv_head * p.a.group;
+        float l[RT / 32], next[RT / 32];
+        auto fetch = [&]() {
+#pragma unroll
+          for (int j = 0; j < RT / 32; ++j)
+            next[j] = j * 32 + static_cast<int>(lane) < min(left, p.row_tile) ? lse[off[j]] : -INFINITY;
+        };
+        fetch();
+        for (int i = 0; ok && i < tiles; ++i, token += tokens) {
+          const uint32_t slot = n % QS;
+          if (n >= QS) ok = __all_sync(0xFFFFFFFFu, wait_bar(&qempty[slot], (n / QS - 1) & 1u, abort_flag, b.err));
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&qfull[slot], p.box_tokens * p.a.group * D * 2);
+            for (int c = 0; c < D / 64; ++c)
+              tma_box(smem_u32(s_q) + slot * S::kQTile + c * (RT * 128), &qmap, c * 64, 0, kv_head, token, &qfull[slot]);
+          }
+#pragma unroll
+          for (int j = 0; j < RT / 32; ++j) l[j] = next[j];
+          left -= p.row_tile, lse += static_cast<int64_t>(tokens) * p.a.q.heads;
+          if (i + 1 < tiles) fetch();  // (a tile ahead)
+          if (n >= LS) ok = __all_sync(0xFFFFFFFFu, wait_bar(&lempty[n % LS], (n / LS - 1) & 1u, abort_flag, b.err));
+          // a row that saw nothing (or is not there) adds nothing: 2^(x - inf)
+#pragma unroll
+          for (int j = 0; j < RT / 32; ++j) s_lse[n % LS * RT + j * 32 + lane] = l[j] == -INFINITY ? -INFINITY : -l[j] * kLog2e;
+          mbar_arrive(&qfull[slot]);
+          ++n;
+        }
+        advance(tiles);
+      }
+      // no copy may outlive the CTA
+      const uint32_t last = min(n, static_cast<uint32_t>(QS));
+      for (uint32_t i = 1; i <= last; ++i) {
+        const uint32_t f = n - i;
+        if (!mbar_wait_bounded(&qfull[f % QS], (f / QS) & 1u)) atomicOr(b.err, kErrWaitTimeout);
+      }
+      __syncwarp();
     }
-    // no copy may outlive the CTA
-    const uint32_t last = min(n, static_cast<uint32_t>(QS));
-    for (uint32_t i = 1; i <= last; ++i) {
-      const uint32_t f = n - i;
-      if (!mbar_wait_bounded(&qfull[f % QS], (f / QS) & 1u)) atomicOr(b.err, kErrWaitTimeout);
-    }
-    __syncwarp();
   } else {
     // ---------------------------------------------------------------- queries that TMA cannot fetch, likewise: two warps
     const uint32_t t = tid - (S::kEpi + 64);
@@ -632,7 +652,6 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
           // a row that saw nothing (or is not there) adds nothing: 2^(x - inf)
           s_lse[n % LS * RT + r] = l == -INFINITY ? -INFINITY : -l * kLog2e;
         }
-        mbar_arrive(&lfull[n % LS]);
         if (pending) {
           cp_async_wait<1>();
           publish(n - 1);
