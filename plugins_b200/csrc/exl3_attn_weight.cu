@@ -83,7 +83,7 @@ struct WtLine : WorkLine {
     return p.a.b.tree || d <= 0 ? 0 : static_cast<int>(divide(static_cast<int64_t>(d) * p.a.group, p.row_tile));
   }
   __device__ __forceinline__ static void set_block(const WeightParams& p, WtItem& it) {
-    it.first_tile = first_of(p, it, it.block);
+    it.first_tile = it.row_tiles == 1 ? 0 : first_of(p, it, it.block);
     it.tiles = it.row_tiles - it.first_tile;
   }
   __device__ __forceinline__ static int64_t tiles_of_head(const WeightParams& p, const WtItem& it) {
@@ -156,7 +156,8 @@ struct WtLine : WorkLine {
   // The item after `it` (there is one).
   __device__ __forceinline__ static void step(const WeightParams& p, WtItem& it) {
     it.first += it.tiles;
-    if (++it.block == it.nblocks) {
+    if (++it.block < it.nblocks && it.row_tiles == 1) return;  // (its one tile)
+    if (it.block == it.nblocks) {
       it.block = 0;
       if (++it.s.kv_head == p.a.b.kv_heads) {
         it.s.kv_head = 0;
