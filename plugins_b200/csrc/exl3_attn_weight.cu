@@ -37,16 +37,16 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kPolyEvery = 8;  // one pair of this many numbers takes the FMA pipe
 
-template <int D>
+template <int D, bool FEW>
 struct WtShape {
   static constexpr int HB = D == 256 ? 1 : 2;       // 128-key halves of an item
   static constexpr int KB = HB * 128;               // keys of an item
-  static constexpr int RT = D == 256 ? 64 : 128;    // query rows of a tile
+  static constexpr int RT = FEW ? 32 : D == 256 ? 64 : 128;  // query rows of a tile
   static constexpr int kBufs = D == 256 ? 4 : 2;    // accumulators of a half
   static constexpr int kKTile = 128 * D * 2;
   static constexpr int kQTile = RT * D * 2;
-  static constexpr int KS = D == 256 ? 2 : D == 128 ? 4 : 6;  // K halves in flight
-  static constexpr int QS = D == 64 ? 3 : 2;                  // query tiles in flight
+  static constexpr int QS = FEW && D == 256 ? 1 : D == 64 ? 3 : 2;                         // query tiles in flight
+  static constexpr int KS = FEW ? (D == 256 ? 3 : D == 128 ? 6 : 12) : D == 256 ? 2 : D == 128 ? 4 : 6;  // K halves
   static constexpr int LS = 4;                      // log-sum-exps of query tiles: used later than the tiles themselves
   static constexpr int kEpi = 512;                  // threads of the sums: four groups of four warps
   static constexpr int GH = 4 / HB;                 // groups of a half, which take its tiles by turns
@@ -67,9 +67,9 @@ struct WtItem {
   int64_t first;           // its first tile on the line
 };
 
-template <int D>
+template <int D, bool FEW>
 struct WtLine : WorkLine {
-  using S = WtShape<D>;
+  using S = WtShape<D, FEW>;
   __device__ __forceinline__ static void set_seq(const WeightParams& p, WtItem& it) {
     if (it.s.total_keys > p.slots) atomicOr(p.a.b.err, kErrBadShape);
     it.s.total_keys = min(it.s.total_keys, p.slots);
@@ -229,14 +229,14 @@ __device__ __forceinline__ void add32(const uint32_t (&x)[32], const float* lse,
   }
 }
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
+template <int D, bool FEW, bool BF16>
+__global__ void __launch_bounds__(WtShape<D, FEW>::kThreads, 1)
     weight_kernel(const __grid_constant__ WeightParams p, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap qmap) {
-  using S = WtShape<D>;
+  using S = WtShape<D, FEW>;
   constexpr int HB = S::HB, KS = S::KS, QS = S::QS, LS = S::LS, RT = S::RT, kBufs = S::kBufs;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ WtLine<D> line;
+  __shared__ WtLine<D, FEW> line;
   __shared__ WtItem s_items[S::kThreads / 32];
   uint8_t* s_k = smem;                           // [slot][64-column block][128 keys][128 bytes], swizzled
   uint8_t* s_q = s_k + KS * S::kKTile;           // [slot][64-column block][RT rows][128 bytes], swizzled
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
   if (tid == 64 && p.box_tokens) asm volatile("prefetch.tensormap [%0];" ::"l"(&qmap) : "memory");
   pdl_wait();
   {
-    WtLine<D> own;
+    WtLine<D, FEW> own;
     WtItem first;
     own.begin_line(p, reinterpret_cast<int64_t*>(s_sums), first);  // (no place that TMA writes: that is another proxy)
     if (tid == 0) line = own;
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
     at += tiles;
     if (at < end) {
       __syncwarp();
-      if (lane == 0) WtLine<D>::step(p, it);
+      if (lane == 0) WtLine<D, FEW>::step(p, it);
       __syncwarp();
     }
   };
@@ -673,12 +673,12 @@ __global__ void __launch_bounds__(WtShape<D>::kThreads, 1)
   }
 }
 
-template <int D>
+template <int D, bool FEW>
 cudaError_t launch_dim(const WeightParams& params, int sms, size_t partial_floats, cudaStream_t st) {
-  using S = WtShape<D>;
+  using S = WtShape<D, FEW>;
   static KernelSetup setup[2];
   WeightParams p = params;
-  auto kern = p.a.bf16 ? weight_kernel<D, true> : weight_kernel<D, false>;
+  auto kern = p.a.bf16 ? weight_kernel<D, FEW, true> : weight_kernel<D, FEW, false>;
   cudaError_t e = kernel_setup(setup[p.a.bf16 ? 1 : 0], kern, S::kThreads, S::kSmem);
   if (e != cudaSuccess) return e;
   CUtensorMap kmap;
@@ -713,10 +713,12 @@ cudaError_t launch_dim(const WeightParams& params, int sms, size_t partial_float
 }  // namespace
 
 cudaError_t launch_attn_weight(const WeightParams& p, int dim, int sms, size_t partial_floats, cudaStream_t st) {
+  // blocks with room for 32 query rows leave it to the keys
+  const bool few = static_cast<int64_t>(p.a.max_rows) * p.a.group <= 32;
   switch (dim) {
-    case 64: return launch_dim<64>(p, sms, partial_floats, st);
-    case 128: return launch_dim<128>(p, sms, partial_floats, st);
-    default: return launch_dim<256>(p, sms, partial_floats, st);
+    case 64: return (few ? launch_dim<64, true> : launch_dim<64, false>)(p, sms, partial_floats, st);
+    case 128: return (few ? launch_dim<128, true> : launch_dim<128, false>)(p, sms, partial_floats, st);
+    default: return (few ? launch_dim<256, true> : launch_dim<256, false>)(p, sms, partial_floats, st);
   }
 }
 
