@@ -626,6 +626,20 @@ exl3_verdict exl3_cache_keep(const exl3_kv_cache *cache, const exl3_tree_batch *
 exl3_verdict exl3_cache_compact(const exl3_kv_cache *cache, const exl3_page_state *in, void *stream,
                                 const exl3_page_state *out);
 
+/* Evict: every row with more tokens than n = max(budget[i], sink + recent) keeps n of them -- in each layer and kv head its
+ * first `sink`, its last `recent` and the heaviest of the others by `weight` (of equal weights the lowest slots; NaN counts
+ * above all) -- in their order, in slots 0 .. n - 1, with their weights in `kept_weight`; lens becomes n, and the pages past
+ * ceil(n / page_size) lose the row.  Pages among the others that several rows refer to are left to them: free pages, lowest
+ * id first, rows in order and a row's in table order, take their places in the row's table.  Other rows stay as they are,
+ * their weights copied to kept_weight.  Keys keep the rotation they were written with, so positions are the host's to carry
+ * on (exl3_tree_batch's `position`).  missing[0] (device) receives 0, or, when the free pages do not suffice, how many are
+ * lacking: then `out` is `in` unchanged and nothing moves.  kept_weight may be weight itself; slots from a row's new length
+ * on are not written.  At most 4096 rows; out's arrays are not in's.  A row whose budget is negative or whose lens is
+ * beyond its pages or the weights' slots stays as it is (EXL3_ERR_BAD_SHAPE is recorded). */
+exl3_verdict exl3_cache_evict(const exl3_kv_cache *cache, const exl3_page_state *in, const exl3_kv_weight *weight,
+                              const int32_t *budget, int32_t sink, int32_t recent, void *stream,
+                              const exl3_page_state *out, const exl3_kv_weight *kept_weight, int32_t *missing);
+
 /* One step's drafted tokens.  Row 0 of a sequence is its newest token, the others are drafts: row i continues row
  * parent[i] < i of its own sequence (without `parent`, row i - 1).  logits row r is the target's for what follows row r;
  * draft row r (or null: a drafter without probabilities) the probabilities that row r's children were drawn from. */

@@ -24,7 +24,8 @@ from ._lib import Exl3Error, check
 from .quant import _TORCH_DT, _stream
 
 __all__ = ["Exl3Error", "KvCache", "TreeBatch", "NormRope", "PageState", "qk_norm_rope", "tree_attention", "cache_fork",
-           "cache_grow", "cache_keep", "cache_compact", "draft_verify", "attention_weight"]
+           "cache_grow", "cache_keep", "cache_compact", "cache_evict", "draft_verify",
+           "attention_weight"]
 
 
 def _refuse(why: str, code: int = L.EXL3_FAILED):
@@ -408,6 +409,28 @@ def cache_compact(cache: KvCache, state: PageState, out: PageState | None = None
         _used_on(stream, cache.k, cache.v, *state._tensors(), *out._tensors())
     check(L.lib().exl3_cache_compact(cache.raw, state.raw, _on(stream, cache._index), out.raw))
     return out
+
+
+def cache_evict(cache: KvCache, state: PageState, weight, budget, sink: int = 0, recent: int = 0,
+                out: PageState | None = None, weight_out=None, missing=None, stream=None):
+    """Rows of more than max(``budget[i]`` (int32), ``sink`` + ``recent``) tokens keep that many: in every layer and kv head the
+    first ``sink``, the last ``recent`` and the heaviest of the others by ``weight`` (f32 [layers, rows, kv_heads, slots]),
+    moved together in their order -> (the new state, ``missing``: an int32 scalar tensor, 0, or the free pages lacking to part
+    from shared ones: then nothing changed).  The tokens' weights move with them, in place or to ``weight_out``."""
+    n = state.raw.nseq
+    _ints(budget, (n,), "budget", cache.device)
+    raw = _kv_weight(weight, cache.raw.layers, n, cache)
+    kept = raw if weight_out is None else _kv_weight(weight_out, cache.raw.layers, n, cache)
+    out = _states(cache, state, out, stream)
+    if missing is None:
+        missing = _maker(stream, torch.empty)((), dtype=torch.int32, device=cache.device)
+    else:
+        _ints(missing, (), "missing", cache.device)
+    if stream is not None:
+        _used_on(stream, budget, missing, weight, weight_out, cache.k, cache.v, *state._tensors(), *out._tensors())
+    check(L.lib().exl3_cache_evict(cache.raw, state.raw, raw, budget.data_ptr(), sink, recent, _on(stream, cache._index),
+                                   out.raw, kept, missing.data_ptr()))
+    return out, missing
 
 
 def _floats(t, shape, what: str, device):

@@ -476,6 +476,59 @@ exl3_verdict exl3_cache_keep(const exl3_kv_cache* cache, const exl3_tree_batch* 
   return launched(exl3::launch_cache_keep(p, ws.counter_count, static_cast<cudaStream_t>(stream)));
 }
 
+exl3_verdict exl3_cache_evict(const exl3_kv_cache* cache, const exl3_page_state* in, const exl3_kv_weight* weight,
+                              const int32_t* budget, int32_t sink, int32_t recent, void* stream,
+                              const exl3_page_state* out, const exl3_kv_weight* kept_weight, int32_t* missing) {
+  exl3_verdict v = check_cache(cache);
+  if (v.code != EXL3_OK) return v;
+  if ((v = check_state(in)).code != EXL3_OK || (v = check_state(out)).code != EXL3_OK) return v;
+  if (in->nseq != out->nseq) return refuse(EXL3_FAILED, "exl3_b200: evict keeps the rows");
+  if (in->nseq > exl3::cache_grow_max_rows()) return refuse(EXL3_TOO_LARGE, "exl3_b200: evict takes at most 4096 rows");
+  if (sink < 0 || recent < 0) return refuse(EXL3_FAILED, "exl3_b200: negative counts of tokens that stay");
+  int64_t bytes = 0, kept_bytes = 0;
+  if ((v = check_weight(weight, cache->layers, in->nseq, cache->kv_heads, &bytes)).code != EXL3_OK) return v;
+  if ((v = check_weight(kept_weight, cache->layers, in->nseq, cache->kv_heads, &kept_bytes)).code != EXL3_OK) return v;
+  if (weight->slots != kept_weight->slots) return refuse(EXL3_FAILED, "exl3_b200: the weights have one number of slots");
+  if (!missing || (!budget && in->nseq > 0)) return refuse(EXL3_FAILED, "exl3_b200: evict without its arrays");
+  const int64_t n = in->nseq;
+  const bool in_place = weight->data == kept_weight->data && weight->layer_stride == kept_weight->layer_stride &&
+                        weight->row_stride == kept_weight->row_stride && weight->head_stride == kept_weight->head_stride;
+  if (!in_place && meet(weight->data, bytes, kept_weight->data, kept_bytes))
+    return refuse(EXL3_FAILED, "exl3_b200: the kept weights lie over the weights in another layout");
+  const struct {
+    const void* at;
+    int64_t bytes;
+  } state[] = {{in->refs, cache->pages * 4ll},  {in->table, n * 4 * in->max_pages},   {in->held, n * 4},  {in->lens, n * 4},
+               {out->refs, cache->pages * 4ll}, {out->table, n * 4 * out->max_pages}, {out->held, n * 4}, {out->lens, n * 4},
+               {budget, n * 4},                 {missing, 4}};
+  for (const auto& x : state)
+    if (meet(kept_weight->data, kept_bytes, x.at, x.bytes) || meet(weight->data, bytes, x.at, x.bytes))
+      return refuse(EXL3_FAILED, "exl3_b200: the weights lie over the page state");
+  const int64_t units = n * cache->layers * cache->kv_heads;
+  if (units > 0x7FFFFFFF) return refuse(EXL3_TOO_LARGE, "exl3_b200: more than 2^31 rows of a layer and head");
+  exl3::Workspace ws;
+  exl3::PageParams p;
+  v = page_params(cache, in, out, budget, n * 4, missing, ws, p);
+  if (v.code != EXL3_OK) return v;
+  if (ws.partial_floats < static_cast<size_t>(n) + cache->pages)
+    return refuse(EXL3_TOO_LARGE, "exl3_b200: too many pages for the workspace");
+  p.need = budget, p.missing = missing, p.sink = sink, p.recent = recent, p.slots = weight->slots;
+  p.scratch = p.moves;
+  OnDevice guard(cache->device);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  v = launched(exl3::launch_evict_pages(p, st));
+  if (v.code != EXL3_OK || units == 0) return v;
+  exl3::EvictParams e{};
+  e.pool = pool_of(cache);
+  e.pages = cache->pages, e.page_shift = p.page_shift, e.nseq = in->nseq, e.width = in->max_pages;
+  e.table_in = in->table, e.lens_in = in->lens, e.table = out->table, e.lens = out->lens;
+  e.w = weight->data, e.w_layer = weight->layer_stride, e.w_row = weight->row_stride, e.w_head = weight->head_stride;
+  e.w_out = kept_weight->data;
+  e.out_layer = kept_weight->layer_stride, e.out_row = kept_weight->row_stride, e.out_head = kept_weight->head_stride;
+  e.sink = sink, e.recent = recent, e.err = ws.err;
+  return launched(exl3::launch_evict_tokens(e, st));
+}
+
 exl3_verdict exl3_draft_verify(const exl3_kv_cache* cache, const exl3_tree_batch* batch, const exl3_draft* draft,
                                void* stream, int32_t* path, int32_t depth, int32_t* kept, int32_t* token) {
   exl3_verdict r = check_cache(cache);

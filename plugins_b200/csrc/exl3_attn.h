@@ -90,10 +90,11 @@ struct PageParams {
   int32_t nseq_in, nseq_out, width_in, width_out;
   const int32_t *refs_in, *table_in, *held_in, *lens_in;
   int32_t *refs, *table, *held, *lens;
-  const int32_t *parent, *need;
+  const int32_t *parent, *need;  // need: evict's budgets
+  int32_t sink, recent, slots;   // evict: the tokens that always stay; the weights' slots
   int32_t* missing;
   int32_t* moves;    // [1 + 2 * capacity]: count, then (source, destination) pages
-  int32_t* scratch;  // grow: [3 * nseq + 2 * pages]
+  int32_t* scratch;  // grow: [3 * nseq + 2 * pages]; evict: [nseq + pages]
   uint32_t* err;
 };
 struct PagePool {
@@ -118,6 +119,21 @@ struct KeepParams {
   int32_t seq0;        // the launch's first sequence
 };
 cudaError_t launch_cache_keep(const KeepParams& p, uint32_t counters, cudaStream_t st);
+
+// Evict's tokens and weights: rows whose lens became fewer (the page state as launch_evict_pages left it).
+struct EvictParams {
+  PagePool pool;
+  int32_t pages, page_shift, nseq, width;
+  const int32_t *table_in, *lens_in;
+  const int32_t *table, *lens;  // the new state's
+  const float* w;               // [layers][nseq][kv_heads][slots]
+  float* w_out;                 // may be w
+  int64_t w_layer, w_row, w_head, out_layer, out_row, out_head;
+  int32_t sink, recent;
+  uint32_t* err;
+};
+cudaError_t launch_evict_pages(const PageParams& p, cudaStream_t st);
+cudaError_t launch_evict_tokens(const EvictParams& p, cudaStream_t st);
 
 constexpr int kDraftMaxRows = 1024;     // rows of one sequence
 constexpr int kDraftMaxVocab = 393216;  // a slice of an eighth, as f32, fits in shared memory

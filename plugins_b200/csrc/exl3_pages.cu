@@ -252,6 +252,97 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) gro
   });
 }
 
+// ------------------------------------------------------------------ evict: the pages
+
+// What a row keeps and the pages that takes.  A row whose numbers make no sense keeps all it has.
+struct Cut {
+  int len, keep, held, want;  // tokens, those that stay; pages, those that stay
+  bool cut;
+  __device__ __forceinline__ Cut(const PageParams& p, int r, bool tell) {
+    const int64_t always = static_cast<int64_t>(p.sink) + p.recent;
+    len = p.lens_in[r], held = held_of(p, r);
+    const int budget = p.need[r];
+    const bool sense = budget >= 0 && len >= 0 && len <= p.slots && len <= static_cast<int64_t>(held) << p.page_shift;
+    if (!sense && tell) atomicOr(p.err, kErrBadShape);
+    const int64_t stay = max(static_cast<int64_t>(budget), always);
+    cut = sense && stay < len;
+    keep = cut ? static_cast<int>(stay) : len;
+    want = cut ? static_cast<int>((static_cast<int64_t>(keep) + (1 << p.page_shift) - 1) >> p.page_shift) : held;
+  }
+};
+
+// A cut row gives back the pages past its tokens; a page among the others that has several references is left to them, and
+// a free one takes its place (the moves of evict_kernel fill it).
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) evict_pages_kernel(const PageParams p) {
+  extern __shared__ int s_ask[];  // [nseq] asks before the row
+  __shared__ int s_warp[32], s_total;
+  pdl_wait();
+  const int tid = static_cast<int>(threadIdx.x);
+  const int t = static_cast<int>(blockIdx.x) * kThreads + tid;
+  const int lane = t & 31, warp = t >> 5, n = p.nseq_in;
+  int* asks = p.scratch;   // [nseq] pages each row asks for
+  int* order = asks + n;   // [pages] the free pages in the order they are given
+  for (int i = t; i < p.pages; i += kAll) p.refs[i] = p.refs_in[i];
+  for (int64_t i = t; i < static_cast<int64_t>(n) * p.width_in; i += kAll) p.table[i] = p.table_in[i];
+  auto page_at = [&](int r, int j) {
+    const int id = p.table_in[static_cast<int64_t>(r) * p.width_in + j];
+    if (id >= 0 && id < p.pages) return id;
+    atomicOr(p.err, kErrBadShape);
+    return -1;
+  };
+  for (int r = warp; r < n; r += kAll / 32) {
+    const Cut c(p, r, lane == 0);
+    int ask = 0;
+    if (c.cut)
+      for (int j = lane; j < c.want; j += 32) {
+        const int id = page_at(r, j);
+        ask += id >= 0 && p.refs_in[id] > 1 ? 1 : 0;
+      }
+    ask = __reduce_add_sync(0xFFFFFFFFu, ask);
+    if (lane == 0) asks[r] = ask;
+  }
+  const PageRun run(p.pages);
+  int mine = 0, free_pages;
+  for (int i = run.lo; i < run.hi; ++i) mine += p.refs_in[i] <= 0 ? 1 : 0;
+  int rank = cluster_scan_excl(mine, s_warp, &s_total, &free_pages);  // (its barrier: the copies and asks are in place)
+  int asked = 0;  // every CTA: rows are scanned in runs of kThreads
+  for (int base = 0; base < n; base += kThreads) {
+    const int r = base + tid;
+    int total;
+    const int a = cta_scan_excl(r < n ? __ldcg(asks + r) : 0, s_warp, &total);
+    if (r < n) s_ask[r] = asked + a;
+    asked += total;
+  }
+  const int missing = max(0, asked - free_pages);
+  if (t == 0) p.missing[0] = missing;
+  if (!missing)
+    for (int i = run.lo; i < run.hi && rank < asked; ++i)
+      if (p.refs_in[i] <= 0) order[rank++] = i;
+  cluster_sync();  // (and no CTA leaves while another may read its shared words)
+  for (int r = warp; r < n; r += kAll / 32) {
+    const Cut c(p, r, false);
+    const bool cut = c.cut && !missing;
+    if (lane == 0) p.held[r] = cut ? c.want : p.held_in[r], p.lens[r] = cut ? c.keep : p.lens_in[r];
+    if (!cut) continue;
+    int32_t* row = p.table + static_cast<int64_t>(r) * p.width_in;
+    int next = s_ask[r];
+    for (int j0 = 0; j0 < c.held; j0 += 32) {
+      const int j = j0 + lane;
+      const int id = j < c.held ? page_at(r, j) : -1;
+      const bool goes = j < c.want && id >= 0 && p.refs_in[id] > 1;
+      const uint32_t which = __ballot_sync(0xFFFFFFFFu, goes);
+      if (goes) {
+        const int to = __ldcg(order + next + __popc(which & ((1u << lane) - 1u)));
+        row[j] = to;
+        p.refs[to] = 1;
+      }
+      if (id >= 0 && (goes || j >= c.want)) atomicSub(p.refs + id, 1);  // (whole numbers: any order)
+      if (j >= c.want && j < c.held) row[j] = -1;
+      next += __popc(which);
+    }
+  }
+}
+
 // ------------------------------------------------------------------ compact
 
 // scratch: [2 * pages] after the moves: the live pages by their rank, then the free pages below the live count by theirs
@@ -458,6 +549,10 @@ cudaError_t launch_cache_grow(const PageParams& p, cudaStream_t st) {
   cudaError_t e = kernel_setup(setup, grow_kernel, kThreads, (static_cast<size_t>(kMaxGrowRows) + 1) * 2 * sizeof(int));
   if (e != cudaSuccess) return e;
   return launch_cluster(grow_kernel, smem, st, p);
+}
+
+cudaError_t launch_evict_pages(const PageParams& p, cudaStream_t st) {
+  return launch_cluster(evict_pages_kernel, static_cast<size_t>(p.nseq_in) * sizeof(int) + 4, st, p);
 }
 
 cudaError_t launch_cache_compact(const PageParams& p, cudaStream_t st) {
