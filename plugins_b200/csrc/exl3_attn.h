@@ -142,7 +142,7 @@ struct DraftParams {
   int64_t logits_stride, draft_stride;
   int32_t logits_dtype, draft_dtype;
   int32_t rows, max_rows, vocab;
-  int32_t slice;               // the vocabulary's share of a CTA
+  int32_t slice;               // the vocabulary's share of a warp
   int32_t depth;
   const int32_t *row_start, *tokens, *parent;
   const float *uniform, *temperature;

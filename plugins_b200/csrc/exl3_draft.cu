@@ -7,10 +7,12 @@
 // Without q a rejected token simply leaves p.  The path ends at the node none of whose children is accepted; its last r
 // gives the next token by its cumulative sums.
 //
-// One cluster per sequence walks its path, a slice of the vocabulary per CTA: the row's exponentials e^((x - m) / T), m the
-// slice's own maximum, stay in shared memory as f32; the sums over them are f64, so that r, which can be a small rest of p,
-// keeps what the exponentials have (an f32 sum would leave 2^-24 of all of p in it).  Each CTA sends its slice's (m, sum)
-// to all others, and every CTA then takes the same decisions from the same numbers.  Only rows on the path are read.
+// One cluster per sequence walks its path; each of sixteen warps per CTA has a slice of the vocabulary.  A node costs one
+// pass over its row and one cluster barrier: a warp takes its slice's maximum m_w and the exponentials e^((x - m_w) / T) (kept
+// in shared memory as f32) by itself, sends (m_w, their sum) to every CTA, and each CTA's seventeenth warp then takes the same
+// decisions from the same numbers.  The sums are f64, so that r, which can be a small rest of p, keeps what the exponentials have (an f32 sum would
+// leave 2^-24 of all of p in it).  Only rows on the path are read, and each node's first child, whose slice is on its way to
+// registers while the node is decided: the chain of a node (row, exponentials, barrier, decision) is what bounds the call.
 #include <cuda_runtime.h>
 #include <float.h>
 
@@ -22,9 +24,12 @@ namespace exl3 {
 
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
+constexpr int kWarps = 16;                   // with a slice each
+constexpr int kThreads = (kWarps + 1) * 32;  // and one that decides
 constexpr int kCluster = 8;
+constexpr int kSlices = kCluster * kWarps;
+constexpr int kOwn = kSlices / 32;  // slices that a lane of a deciding warp looks after, neighbours
+constexpr int kChunks = 8;          // 16-byte chunks of a lane's slice in registers
 constexpr double kLog2e = 1.4426950408889634;
 constexpr double kNone = 0x1p-100;  // a token this far below the likeliest has no probability
 
@@ -55,6 +60,13 @@ __device__ __forceinline__ float widen(typename Elem<DT>::type v) {
 }
 // A logit as it counts: NaN as -inf, +inf as the largest finite number.
 __device__ __forceinline__ float logit(float x) { return x == x ? fminf(x, FLT_MAX) : -INFINITY; }
+// Element k of a chunk, as a logit.
+template <int DT>
+__device__ __forceinline__ float chunk_logit(const uint4& u, int k) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  if constexpr (DT == EXL3_F32) return logit(__uint_as_float(w[k]));
+  else return logit(widen<DT>(static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1)))));
+}
 // A drafter's probability: NaN and negative numbers as 0.
 template <int DT>
 __device__ __forceinline__ float draft_p(const void* row, int64_t i) {
@@ -64,85 +76,29 @@ __device__ __forceinline__ float draft_at(const void* row, int dtype, int64_t i)
   return dtype == EXL3_F32 ? draft_p<EXL3_F32>(row, i) : dtype == EXL3_F16 ? draft_p<EXL3_F16>(row, i) : draft_p<EXL3_BF16>(row, i);
 }
 
-// 2^((x - m) c), c = c1 + c2 = log2(e) / T.  The rounding of the difference and of the product, up to 2^-24 of an
-// exponent of 100, is carried along: what is left is the exponential's own.
+// 2^((x - m) c), c = c1 + c2 = log2(e) / T.  What the product and c's first part leave out, up to 2^-24 of an exponent of
+// 100, is carried along (and what the difference does, where x is f32: of 16-bit numbers it is exact): what is left is the
+// exponential's own error.
 struct Scale {
   float c1, c2;
 };
-__device__ __forceinline__ float power(float x, float m, Scale c) {
-  if (x == -INFINITY) return 0.f;
-  const float d = x - m, b = d - x, d2 = (x - (d - b)) + (-m - b);
-  const float z = d * c.c1;
-  if (!(z > -150.f)) return 0.f;
-  const float z2 = fmaf(d, c.c1, -z) + fmaf(d, c.c2, d2 * c.c1);
-  return exp2f(z) * fmaf(z2, 0.6931472f, 1.f);
-}
-
-// The elements of a slice [0, n) at `src`, by 16-byte chunks where the address allows: f(index, values, count).
 template <int DT>
-__device__ __forceinline__ int head_of(const typename Elem<DT>::type* src, int n) {
-  constexpr int kVec = Elem<DT>::kVec;
-  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(src) % 16 / sizeof(typename Elem<DT>::type));
-  return min(n, (kVec - off) % kVec);
-}
-template <int DT, typename F>
-__device__ __forceinline__ void each_chunk(const typename Elem<DT>::type* src, int n, F&& f) {
-  using E = Elem<DT>;
-  constexpr int kVec = E::kVec;
-  const int head = head_of<DT>(src, n), chunks = (n - head) / kVec, tail = head + chunks * kVec;
-  const int t = static_cast<int>(threadIdx.x);
-  constexpr int kAhead = 4;
-  for (int i0 = t; i0 < chunks; i0 += kThreads * kAhead) {
-    uint4 u[kAhead];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (i0 + j * kThreads < chunks) u[j] = *(reinterpret_cast<const uint4*>(src + head) + i0 + j * kThreads);
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      if (i0 + j * kThreads >= chunks) break;
-      float v[kVec];
-      const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        if constexpr (DT == EXL3_F32) v[k] = __uint_as_float(w[k]);
-        else v[k] = widen<DT>(static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1))));
-      }
-      f(head + (i0 + j * kThreads) * kVec, v, kVec);
-    }
+__device__ __forceinline__ float power(float x, float m, Scale c) {
+  const float d = x - m, z = d * c.c1;
+  float z2 = fmaf(d, c.c2, fmaf(d, c.c1, -z));
+  if constexpr (DT == EXL3_F32) {
+    const float b = d - x;
+    z2 = fmaf((x - (d - b)) + (-m - b), c.c1, z2);
   }
-  for (int i = t; i < head + (n - tail); i += kThreads) {
-    const int at = i < head ? i : tail + i - head;
-    float v[kVec];
-    v[0] = widen<DT>(src[at]);
-    f(at, v, 1);
-  }
+  const float e = exp2f(z);
+  return z > -150.f ? fmaf(e * 0.6931472f, z2, e) : 0.f;  // (x of -inf: z is -inf, or NaN beside m = -inf)
 }
 
-// The drafter's probabilities of a slice: f(index, q).
-template <int DT, typename F>
-__device__ __forceinline__ void each_draft_of(const DraftParams& p, int64_t row, int v0, int n, F&& f) {
-  const void* q = p.draft;
-  const int64_t base = row * p.draft_stride + v0;
-#pragma unroll 8
-  for (int i = static_cast<int>(threadIdx.x); i < n; i += kThreads) f(i, draft_p<DT>(q, base + i));
+__device__ __forceinline__ uint32_t ordered(float x) {  // whole numbers in the order of the floats
+  const uint32_t u = __float_as_uint(x);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-template <typename F>
-__device__ __forceinline__ void each_draft(const DraftParams& p, int64_t row, int v0, int n, F&& f) {
-  if (p.draft_dtype == EXL3_F32) each_draft_of<EXL3_F32>(p, row, v0, n, f);
-  else if (p.draft_dtype == EXL3_F16) each_draft_of<EXL3_F16>(p, row, v0, n, f);
-  else each_draft_of<EXL3_BF16>(p, row, v0, n, f);
-}
-
-struct Block {
-  double sum[kWarps];
-  double2 slice[2][kCluster];  // (maximum, sum) of every CTA's slice, sent by its owner; two, by turns
-  float top[kWarps];
-  int at[kWarps];
-  // the walk, as warp 0 leaves it
-  int command, node, owner, token, found, last;
-  double a, lift, unit, target;  // A; e^((m_slice - m) / T) of this CTA's slice; 1 / the row's sum; what is left to pass
-};
-enum : int { kNext = 0, kStop = 1, kCut = 2 };  // on to a child; the path ends; r has to be summed
+__device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u); }
 
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
@@ -150,19 +106,100 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
+struct Block {
+  double2 slice[2][kSlices];  // every slice's (maximum, sum), sent by its warp; two, by turns
+  float top[kSlices];         // their maxima and e^((m_w - m) / T)
+  double lift[kSlices];
+  // the walk, as the deciding warp leaves it
+  int command, node, owner, token;
+  float a, cut;               // A; what is none, in units of p
+  double unit, target;        // 1 / the row's sum; what is left to pass in the owner's slice
+  // the sequence's rows
+  int parent[kDraftMaxRows], tokens[kDraftMaxRows], first[kDraftMaxRows];  // first: a row's first child, or none
+  int out[kDraftMaxRows];     // the node's rejected tokens, where there is no q
+};
+enum : int { kNext = 0, kStop = 1, kCut = 2 };  // on to a child; the path ends; r has to be summed
+
+// r of an element after rejections: e its exponential, lu what makes that p.
+__device__ __forceinline__ float rest_of(float e, float lu, float a, float q, float cut) {
+  const float v = e * lu;
+  return v < cut ? 0.f : fmaxf(fmaf(-a, q, v), 0.f);
+}
+
+// Where elements of a row lie in s_e: whole 16-byte chunks of the row on multiples of four.
 template <int DT>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) verify_kernel(const DraftParams p) {
+__device__ __forceinline__ int chunks_begin(const typename Elem<DT>::type* src) {
+  constexpr int kVec = Elem<DT>::kVec;
+  return (kVec - static_cast<int>(reinterpret_cast<uintptr_t>(src) % 16 / sizeof(typename Elem<DT>::type))) % kVec;
+}
+template <int DT>
+__device__ __forceinline__ int pad_of(const typename Elem<DT>::type* src) { return (4 - (chunks_begin<DT>(src) & 3)) & 3; }
+
+// A lane's part of a slice of n elements: `head` and tail elements outside of whole 16-byte chunks, one a lane.
+template <int DT>
+struct Part {
+  using T = typename Elem<DT>::type;
+  static constexpr int kVec = Elem<DT>::kVec;
+  const T* src;
+  int n, head, chunks, lane;
+  int odd;  // this lane's single element, or -1
+  __device__ __forceinline__ Part(const T* s, int n_, int lane_) : src(s), n(n_), lane(lane_) {
+    head = min(n, chunks_begin<DT>(s));
+    chunks = (n - head) / kVec;
+    const int tail = n - head - chunks * kVec;
+    odd = lane < head ? lane : lane < head + tail ? chunks * kVec + lane : -1;
+  }
+  __device__ __forceinline__ void load(int from, uint4 (&u)[kChunks]) const {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      u[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (from + i * 32 + lane < chunks) u[i] = reinterpret_cast<const uint4*>(src + head)[from + i * 32 + lane];
+    }
+  }
+};
+
+// f(e, q) for the elements of a warp's slice, four neighbours a lane.
+template <int DT, typename F>
+__device__ __forceinline__ void each_draft_of(const void* draft, int64_t at, const float* own, int pad, int n, int lane, F&& f) {
+  using T = typename Elem<DT>::type;
+  const T* q = static_cast<const T*>(draft) + at - pad;
+  const bool vec = reinterpret_cast<uintptr_t>(q) % (4 * sizeof(T)) == 0;
+#pragma unroll 4
+  for (int t = lane * 4; t < pad + n; t += 128) {
+    const float4 e = *reinterpret_cast<const float4*>(own + t);
+    if (vec && t >= pad && t + 4 <= pad + n) {
+      T v[4];
+      if constexpr (DT == EXL3_F32) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(q + t);
+      else *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(q + t);
+      f(e.x, fmaxf(widen<DT>(v[0]), 0.f)), f(e.y, fmaxf(widen<DT>(v[1]), 0.f));
+      f(e.z, fmaxf(widen<DT>(v[2]), 0.f)), f(e.w, fmaxf(widen<DT>(v[3]), 0.f));
+    } else {
+      const float es[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (t + k >= pad && t + k < pad + n) f(es[k], fmaxf(widen<DT>(q[t + k]), 0.f));
+    }
+  }
+}
+template <typename F>
+__device__ __forceinline__ void each_draft(const DraftParams& p, int64_t at, const float* own, int pad, int n, int lane, F&& f) {
+  if (p.draft_dtype == EXL3_F32) each_draft_of<EXL3_F32>(p.draft, at, own, pad, n, lane, f);
+  else if (p.draft_dtype == EXL3_F16) each_draft_of<EXL3_F16>(p.draft, at, own, pad, n, lane, f);
+  else each_draft_of<EXL3_BF16>(p.draft, at, own, pad, n, lane, f);
+}
+
+template <int DT>
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) verify_kernel(const DraftParams p) {
   using T = typename Elem<DT>::type;
   constexpr int kVec = Elem<DT>::kVec;
   extern __shared__ __align__(16) float s_e[];  // [slice + 8]
   __shared__ Block b;
-  __shared__ int s_out[kDraftMaxRows];  // the node's rejected tokens, where there is no q
   pdl_wait();
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int rank = static_cast<int>(blockIdx.x) % kCluster, s = static_cast<int>(blockIdx.x) / kCluster;
   const int r0 = p.row_start[s], r1 = p.row_start[s + 1];
-  const int row0 = max(0, min(r0, p.rows)), all = max(0, min(r1, p.rows) - row0), ntok = min(all, p.max_rows);
   const float temp = p.temperature ? p.temperature[s] : 1.f;
+  const int row0 = max(0, min(r0, p.rows)), all = max(0, min(r1, p.rows) - row0), ntok = min(all, p.max_rows);
   const bool warm = temp > 0.f && temp <= FLT_MAX;
   if (tid == 0 && rank == 0 && (r0 < 0 || r1 < r0 || r1 > p.rows || all > ntok || (!warm && temp != 0.f)))
     atomicOr(p.err, kErrBadShape);
@@ -174,299 +211,368 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) ver
     }
     return;
   }
+  const bool decides = warp == kWarps;
+  // this warp's slice, of p.slice elements but for the last
+  const int mine = rank * kWarps + warp;
+  const int v0 = min(mine * p.slice, p.vocab), n = decides ? 0 : min(p.vocab - v0, p.slice);
+  auto row_of = [&](int i) { return static_cast<const T*>(p.logits) + (row0 + static_cast<int64_t>(i)) * p.logits_stride; };
+  uint4 raw[kChunks];
+  T odd = {};  // the lane's single element
+  auto fetch = [&](int i) {
+    const Part<DT> part(row_of(i) + v0, n, lane);
+    if (part.chunks <= kChunks * 32) part.load(0, raw);  // (else they are loaded as they are used)
+    if (part.odd >= 0) odd = part.src[part.odd];
+  };
+  if (!decides) fetch(0);
+  for (int i = tid; i < ntok; i += kThreads) {
+    b.parent[i] = p.parent ? p.parent[row0 + i] : i - 1;
+    b.tokens[i] = p.tokens[row0 + i];
+    b.first[i] = kDraftMaxRows;
+  }
   Scale c{0.f, 0.f};
   if (warm) {
     const double cd = kLog2e / static_cast<double>(temp);
     c.c1 = static_cast<float>(fmin(cd, static_cast<double>(FLT_MAX)));
     c.c2 = cd < 1e30 ? static_cast<float>(cd - static_cast<double>(c.c1)) : 0.f;
   }
-  const int v0 = min(rank * p.slice, p.vocab), n = min(p.vocab - v0, p.slice);
+  __syncthreads();
+  for (int i = tid; i < ntok; i += kThreads) {
+    const int a = b.parent[i];
+    if (a >= 0 && a < i) atomicMin(&b.first[a], i);
+  }
+  __syncthreads();
   const bool has_q = p.draft != nullptr && warm;
   int node = 0, kept = 0;
   uint32_t turn = 0;
 
-  // This CTA's pair to all, and theirs into b.slice[the returned turn].
-  auto exchange = [&](double x, double y) {
-    const uint32_t which = turn++ & 1u;
-    if (tid < kCluster) cluster_store(&b.slice[which][rank], tid, x, y);
-    cluster_sync();
-    return which;
-  };
-  auto block_sum = [&](double v) {  // in every thread
-    v = warp_sum(v);
-    if (lane == 0) b.sum[warp] = v;
-    __syncthreads();
-    double t = 0.0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) t += b.sum[w];
-    return t;
-  };
-
-  for (;;) {
-    // ---- the node's row: its maximum, its exponentials and their sum
-    const int64_t row = row0 + node;
-    const T* logits = static_cast<const T*>(p.logits) + row * p.logits_stride;
-    const int pad = (4 - (head_of<DT>(logits + v0, n) & 3)) & 3;  // whole chunks lie on multiples of four in s_e
-    const int end = pad + n;
-    if (tid < pad) s_e[tid] = -INFINITY;
-    if (tid < 4 && end + tid < ((end + 3) & ~3)) s_e[end + tid] = -INFINITY;
-    float top = -INFINITY;
-    int at = 0x7FFFFFFF;
-    each_chunk<DT>(logits + v0, n, [&](int i, const float (&v)[kVec], int count) {
-      float x[kVec];
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        x[k] = k < count ? logit(v[k]) : -INFINITY;
-        // (a thread meets its places in ascending order, but for the few outside whole chunks, which come last)
-        if (x[k] > top || (x[k] == top && i + k < at && x[k] != -INFINITY)) top = x[k], at = i + k;
-      }
-      if (count == 1) {
-        s_e[pad + i] = x[0];
-      } else {
-#pragma unroll
-        for (int k = 0; k < kVec; k += 4)
-          *reinterpret_cast<float4*>(s_e + pad + i + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
-      }
-    });
-#pragma unroll
-    for (int d = 16; d; d >>= 1) {
-      const float o = __shfl_xor_sync(0xFFFFFFFFu, top, d);
-      const int oat = __shfl_xor_sync(0xFFFFFFFFu, at, d);
-      if (o > top || (o == top && oat < at)) top = o, at = oat;
-    }
-    if (lane == 0) b.top[warp] = top, b.at[warp] = at;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w)
-      if (b.top[w] > top || (b.top[w] == top && b.at[w] < at)) top = b.top[w], at = b.at[w];
-    double sum = 0.0;
-    if (warm) {
-      for (int i = tid * 4; i < end; i += kThreads * 4) {
-        float4 e = *reinterpret_cast<const float4*>(s_e + i);
-        e.x = power(e.x, top, c), e.y = power(e.y, top, c), e.z = power(e.z, top, c), e.w = power(e.w, top, c);
-        *reinterpret_cast<float4*>(s_e + i) = e;
-        sum += (static_cast<double>(e.x) + static_cast<double>(e.y)) + (static_cast<double>(e.z) + static_cast<double>(e.w));
-      }
-      sum = block_sum(sum);
-    } else {
-      sum = static_cast<double>(v0) + static_cast<double>(at);  // a greedy sequence's slice: where its maximum is
-    }
-    uint32_t which = exchange(static_cast<double>(top), sum);
-
-    // ---- the children in turn: warp 0 of every CTA decides the same from the same numbers
-    if (rank == 0 && tid == 0) path[kept] = node;
-    ++kept;
-    // warp 0: lane r holds slice r's (maximum, sum of what is left), its e^((m_r - m) / T), and r's sum over it
-    double2 mine = make_double2(-INFINITY, 0.0);
-    double lift = 0.0, unit = 0.0, rest = 0.0, a = 0.0, z = 1.0;
-    int best = -1, tried = node + 1, rejected = 0;
-    if (warp == 0) {
-      if (lane < kCluster) mine = b.slice[which][lane];
-      double m = mine.x;
-#pragma unroll
-      for (int d = 4; d; d >>= 1) m = fmax(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-      m = __shfl_sync(0xFFFFFFFFu, m, 0);
-      if (warm) {
-        lift = static_cast<double>(power(static_cast<float>(mine.x), static_cast<float>(m), c));
-        if (lift < kNone) lift = 0.0;  // no token of the slice has a probability
-        unit = 1.0 / warp_sum(mine.y * lift);
-        rest = mine.y * lift * unit;
-      }
-      const uint32_t has = __ballot_sync(0xFFFFFFFFu, mine.x == m && m != -INFINITY);
-      const double where = __shfl_sync(0xFFFFFFFFu, mine.y, __ffs(has) - 1);
-      best = has ? (warm ? 0 : static_cast<int>(where)) : -1;  // -1: the row has no finite logit
-      tried = best < 0 || kept >= p.depth ? ntok : tried;
-    }
+  if (!decides) {
+    // ---------------------------------------------------------------- a slice of every row on the path
+    float* own = s_e + warp * p.slice;
+    auto send = [&](double x, double y) {
+      if (lane < kCluster) cluster_store(&b.slice[turn & 1u][mine], lane, x, y);
+      ++turn;
+      cluster_sync();
+    };
     for (;;) {
-      if (warp == 0) {
-        int command = kStop, child = 0;
-        for (; command == kStop && tried < ntok; tried += 32) {
-          const int i = tried + lane;
-          const bool is = i < ntok && (p.parent ? p.parent[row0 + i] == node : i == node + 1);
-          uint32_t left = __ballot_sync(0xFFFFFFFFu, is);
-          int tok = -1;
-          float x = 0.f, u = 0.f, q = 1.f;
-          if (is) {
-            tok = p.tokens[row0 + i];
-            if (tok >= 0 && tok < p.vocab) {
-              x = logit(widen<DT>(logits[tok]));
-              u = p.uniform[2 * (row0 + static_cast<int64_t>(i))];
-              if (has_q) q = draft_at(p.draft, p.draft_dtype, row * p.draft_stride + tok);
-            } else {
-              tok = -1;
-            }
-          }
-          while (left && command == kStop) {
-            const int l = __ffs(left) - 1;
-            left &= left - 1;
-            const int t = __shfl_sync(0xFFFFFFFFu, tok, l);
-            if (t < 0) continue;  // (a token outside the vocabulary is not tried)
-            child = tried + l;
-            if (!warm) {
-              if (t == best) command = kNext;
-              continue;
-            }
-            const int owner = t / p.slice;
-            const float e = power(__shfl_sync(0xFFFFFFFFu, x, l), static_cast<float>(__shfl_sync(0xFFFFFFFFu, mine.x, owner)), c);
-            const double le = static_cast<double>(e) * __shfl_sync(0xFFFFFFFFu, lift, owner);
-            const double qt = static_cast<double>(__shfl_sync(0xFFFFFFFFu, q, l));
-            double rt = le < kNone ? 0.0 : le * unit;
-            if (has_q) {
-              if (a > 0.0) rt = fmax(rt - a * qt, 0.0);
-            } else {
-              bool gone = false;
-              for (int j = lane; j < rejected; j += 32) gone |= s_out[j] == t;
-              if (__any_sync(0xFFFFFFFFu, gone)) continue;  // its sibling took it out of p
-            }
-            if (static_cast<double>(__shfl_sync(0xFFFFFFFFu, u, l)) * qt * z < rt) {
-              command = kNext;
-            } else if (has_q) {
-              a += z;
-              command = kCut;
-            } else {
-              if (lane == 0) {
-                s_out[rejected] = t;
-                if (owner == rank) s_e[pad + t - v0] = 0.f;
-              }
-              if (lane == owner) mine.y -= static_cast<double>(e), rest = fmax(mine.y, 0.0) * lift * unit;
-              ++rejected;
-              __syncwarp();
-              z = warp_sum(rest);
-              if (!(z > 0.0)) {  // nothing is left: p again
-                for (int j = 0; j < rejected; ++j) {
-                  const int g = s_out[j];
-                  const float ge = power(logit(widen<DT>(logits[g])), static_cast<float>(__shfl_sync(0xFFFFFFFFu, mine.x, g / p.slice)), c);
-                  if (lane == 0 && g / p.slice == rank) s_e[pad + g - v0] = ge;
-                }
-                if (lane < kCluster) mine.y = b.slice[which][lane].y;
-                rest = mine.y * lift * unit;
-                rejected = 0, z = 1.0;
-                __syncwarp();
-              }
-            }
-          }
-          if (command == kCut) {
-            tried = child + 1;
-            break;
-          }
-        }
-        if (command == kStop) {  // the slice that holds the next token, and what is left to pass in it
-          const float u = p.uniform[2 * row + 1];
-          const double goal = static_cast<double>(u) * z;
-          double upto = rest;
+      const Part<DT> part(row_of(node) + v0, n, lane);
+      const int pad = pad_of<DT>(part.src);
+      const bool whole = part.chunks <= kChunks * 32;
+      const float single = part.odd >= 0 ? logit(widen<DT>(odd)) : -INFINITY;
+      float top = single;
+      for (int from = 0; from < part.chunks; from += kChunks * 32) {
+        if (!whole) part.load(from, raw);
 #pragma unroll
-          for (int d = 1; d < kCluster; d <<= 1) {
-            const double o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-            if (lane >= d) upto += o;
+        for (int i = 0; i < kChunks; ++i)
+          if (from + i * 32 + lane < part.chunks)
+#pragma unroll
+            for (int k = 0; k < kVec; ++k) top = fmaxf(top, chunk_logit<DT>(raw[i], k));
+      }
+      top = unordered(__reduce_max_sync(0xFFFFFFFFu, ordered(top)));
+      double sum = 0.0;
+      if (warm) {
+        if (part.odd >= 0) {
+          const float e = power<DT>(single, top, c);
+          own[pad + part.odd] = e;
+          sum = static_cast<double>(e);
+        }
+        for (int from = 0; from < part.chunks; from += kChunks * 32) {
+          if (!whole) part.load(from, raw);
+#pragma unroll
+          for (int i = 0; i < kChunks; ++i) {
+            const int at = from + i * 32 + lane;
+            if (at >= part.chunks) continue;
+#pragma unroll
+            for (int k = 0; k < kVec; k += 4) {
+              float4 e;
+              e.x = power<DT>(chunk_logit<DT>(raw[i], k), top, c), e.y = power<DT>(chunk_logit<DT>(raw[i], k + 1), top, c);
+              e.z = power<DT>(chunk_logit<DT>(raw[i], k + 2), top, c), e.w = power<DT>(chunk_logit<DT>(raw[i], k + 3), top, c);
+              *reinterpret_cast<float4*>(own + pad + part.head + at * kVec + k) = e;
+              sum += (static_cast<double>(e.x) + static_cast<double>(e.y)) + (static_cast<double>(e.z) + static_cast<double>(e.w));
+            }
           }
-          const double before = __shfl_up_sync(0xFFFFFFFFu, upto, 1);
-          const uint32_t over = __ballot_sync(0xFFFFFFFFu, lane < kCluster && upto > goal && rest > 0.0);
-          const uint32_t some = __ballot_sync(0xFFFFFFFFu, lane < kCluster && rest > 0.0);
-          const int owner = over ? __ffs(over) - 1 : (some ? 31 - __clz(some) : 0);
-          if (lane == owner) b.target = goal - (lane ? before : 0.0);
-          if (lane == 0) b.owner = owner, b.token = best, b.found = b.last = -1;
         }
-        if (lane == rank) b.lift = lift;
-        if (lane == 0) b.command = command, b.node = child, b.a = a, b.unit = unit;
-      }
-      __syncthreads();
-      if (b.command != kCut) break;
-      double part = 0.0;  // r over this slice
-      const double la = b.a, lu = b.unit, ll = b.lift;
-      each_draft(p, row, v0, n, [&](int i, float q) {
-        const double e = static_cast<double>(s_e[pad + i]) * ll;
-        if (e >= kNone) part += fmax(e * lu - la * static_cast<double>(q), 0.0);
-      });
-      part = block_sum(part);
-      const uint32_t to = exchange(part, 0.0);
-      if (warp == 0) {
-        const double got = lane < kCluster ? b.slice[to][lane].x : 0.0;
-        z = warp_sum(got);
-        if (z > 0.0) {
-          rest = got;
-        } else {  // nothing is left: p again
-          a = 0.0, z = 1.0;
-          rest = mine.y * lift * unit;
+        sum = warp_sum(sum);
+      } else {  // a greedy sequence's slice: where its maximum is first
+        uint32_t at = single == top && part.odd >= 0 ? part.odd : 0x7FFFFFFFu;
+        for (int from = 0; from < part.chunks; from += kChunks * 32) {
+          if (!whole) part.load(from, raw);
+#pragma unroll
+          for (int i = 0; i < kChunks; ++i)
+            if (from + i * 32 + lane < part.chunks)
+#pragma unroll
+              for (int k = 0; k < kVec; ++k)
+                if (chunk_logit<DT>(raw[i], k) == top) at = min(at, static_cast<uint32_t>(part.head + (from + i * 32 + lane) * kVec + k));
         }
+        sum = static_cast<double>(v0) + static_cast<double>(__reduce_min_sync(0xFFFFFFFFu, at));
       }
+      // the first child's row, should it be the next
+      const int guess = kept + 1 < p.depth ? b.first[node] : kDraftMaxRows;
+      if (guess < kDraftMaxRows) fetch(guess);
+      send(static_cast<double>(top), sum);
+      ++kept;
+      for (;;) {
+        __syncthreads();  // the decision
+        if (b.command != kCut) break;
+        const float la = b.a, lu = static_cast<float>(b.lift[mine] * b.unit), cut = b.cut;
+        double r = 0.0;
+        each_draft(p, (row0 + static_cast<int64_t>(node)) * p.draft_stride + v0, own, pad, n, lane,
+                   [&](float e, float q) { r += static_cast<double>(rest_of(e, lu, la, q, cut)); });
+        send(warp_sum(r), 0.0);
+      }
+      if (b.command == kStop) break;
+      const int next = b.node;
+      if (next != guess) fetch(next);
+      node = next;
     }
-    if (b.command == kStop) break;
-    node = b.node;
-    __syncthreads();  // the walk's words are read
-  }
-
-  if (rank == 0) {
-    for (int d = kept + tid; d < p.depth; d += kThreads) path[d] = -1;
-    if (tid == 0) p.kept[s] = kept;
-  }
-  if (!warm || b.token < 0) {
-    if (rank == 0 && tid == 0) p.token[s] = b.token;
-    return;
-  }
-  // ---- the next token: the first of the slice whose cumulative sum passes the target
-  if (rank != b.owner) return;
-  const int64_t row = row0 + node;
-  const int pad = (4 - (head_of<DT>(static_cast<const T*>(p.logits) + row * p.logits_stride + v0, n) & 3)) & 3;
-  const double la = b.a, lu = b.unit, ll = b.lift, target = b.target;
-  auto at = [&](int i) {
-    const double e = static_cast<double>(s_e[pad + i]) * ll;
-    if (e < kNone) return 0.0;
-    if (!(has_q && la > 0.0)) return e * lu;
-    return fmax(e * lu - la * static_cast<double>(draft_at(p.draft, p.draft_dtype, row * p.draft_stride + v0 + i)), 0.0);
-  };
-  const int len = ((n + kThreads - 1) / kThreads) | 1;  // a run per thread; odd: no two lanes on one bank
-  const int lo = min(n, tid * len), hi = min(n, lo + len);
-  double own = 0.0;
-  int last = -1;
-  for (int i = lo; i < hi; ++i) {
-    const double r = at(i);
-    if (r > 0.0) last = i;
-    own += r;
-  }
-  double upto = own;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const double o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-    if (lane >= d) upto += o;
-  }
-  if (lane == 31) b.sum[warp] = upto;
-  const int top_last = __reduce_max_sync(0xFFFFFFFFu, last);
-  if (lane == 0) atomicMax(&b.last, top_last);
-  __syncthreads();
-  double off = 0.0;
-  for (int w = 0; w < warp; ++w) off += b.sum[w];
-  double before = __shfl_up_sync(0xFFFFFFFFu, upto, 1);
-  before = off + (lane ? before : 0.0);
-  upto += off;
-  if (before <= target && upto > target) {  // (one thread at most: before is the last one's upto)
-    double acc = before;
-    int found = last;  // rounding may leave none
+    if (!warm || b.token < 0 || mine != b.owner) return;
+    // ---- the next token: the first of the owner's slice whose cumulative sum passes the target, a run of places per lane
+    const int64_t q_at = (row0 + static_cast<int64_t>(node)) * p.draft_stride + v0;
+    const int pad = pad_of<DT>(row_of(node) + v0);
+    const double target = b.target, lift = b.lift[mine], unit = b.unit;
+    const float la = b.a, lu = static_cast<float>(lift * unit), cut = b.cut;
+    auto at = [&](int i) {
+      const float e = own[pad + i];
+      if (has_q && la > 0.f) return static_cast<double>(rest_of(e, lu, la, draft_at(p.draft, p.draft_dtype, q_at + i), cut));
+      const double le = static_cast<double>(e) * lift;
+      return le < kNone ? 0.0 : le * unit;
+    };
+    const int len = ((n + 31) / 32) | 1;  // odd: no two lanes on one bank
+    const int lo = min(n, lane * len), hi = min(n, lo + len);
+    double run = 0.0;
+    int last = -1;
     for (int i = lo; i < hi; ++i) {
       const double r = at(i);
-      acc += r;
-      if (r > 0.0 && acc > target) {
-        found = i;
-        break;
+      if (r > 0.0) last = i;
+      run += r;
+    }
+    double upto = run;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const double o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+      if (lane >= d) upto += o;
+    }
+    double before = __shfl_up_sync(0xFFFFFFFFu, upto, 1);
+    if (lane == 0) before = 0.0;
+    int found = -1;
+    if (before <= target && upto > target) {  // (one lane at most: before is the last one's upto)
+      found = last;                           // rounding may leave none
+      for (int i = lo; i < hi; ++i) {
+        const double r = at(i);
+        before += r;
+        if (r > 0.0 && before > target) {
+          found = i;
+          break;
+        }
       }
     }
-    b.found = found;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    int t = b.found;
-    if (t < 0) {  // before the first (a negative number) or past the last
-      t = target < 0.0 ? -1 : b.last;
-      if (t < 0)
-        for (t = 0; t < n - 1 && !(s_e[pad + t] > 0.f);) ++t;
+    found = __reduce_max_sync(0xFFFFFFFFu, found);
+    last = __reduce_max_sync(0xFFFFFFFFu, last);
+    if (lane == 0) {
+      if (found < 0 && !(target < 0.0)) found = last;  // past the last
+      if (found < 0)                                   // before the first (a negative number)
+        for (found = 0; found < n - 1 && !(own[pad + found] > 0.f);) ++found;
+      p.token[s] = v0 + found;
     }
-    p.token[s] = v0 + t;
+    return;
+  }
+
+  // ---------------------------------------------------------------- the decisions: the same in every CTA
+  for (;;) {
+    const int64_t row = row0 + static_cast<int64_t>(node);
+    const T* logits = row_of(node);
+    const int pad = pad_of<DT>(logits), base = rank * kWarps * p.slice;
+    // the children's numbers, of 32 rows at a time, one a lane
+    int tok = -1;
+    float x = 0.f, u = 0.f, q = 1.f;
+    auto look = [&](int i) {
+      tok = -1;
+      if (i >= ntok || b.parent[i] != node) return;
+      tok = b.tokens[i];
+      if (tok < 0 || tok >= p.vocab) {
+        tok = -1;  // (a token outside the vocabulary is not tried)
+        return;
+      }
+      x = logit(widen<DT>(logits[tok]));
+      u = p.uniform[2 * (row0 + static_cast<int64_t>(i))];
+      if (has_q) q = draft_at(p.draft, p.draft_dtype, row * p.draft_stride + tok);
+    };
+    const int guess = kept + 1 < p.depth ? b.first[node] : kDraftMaxRows;
+    if (guess < kDraftMaxRows) look(guess + lane);
+    const float u_next = p.uniform[2 * row + 1];
+    if (rank == 0 && lane == 0) path[kept] = node;
+    ++kept;
+    const double2* sent = b.slice[turn++ & 1u];
+    cluster_sync();
+
+    // a lane's slices: their sums of exponentials (of what is left of them) and e^((m_w - m) / T); r's sums
+    double sums[kOwn], rest[kOwn];
+    double a = 0.0, z = 1.0, unit = 0.0;
+    int best = -1, tried = guess, rejected = 0;
+    {
+      float m = -INFINITY, m_own[kOwn];
+#pragma unroll
+      for (int j = 0; j < kOwn; ++j) {
+        const double2 v = sent[lane * kOwn + j];
+        m_own[j] = static_cast<float>(v.x), sums[j] = v.y;
+        m = fmaxf(m, m_own[j]);
+      }
+      const float m_lane = m;
+      m = unordered(__reduce_max_sync(0xFFFFFFFFu, ordered(m)));
+      const uint32_t has = __ballot_sync(0xFFFFFFFFu, m_lane == m && m != -INFINITY);
+      if (warm) {
+        double total = 0.0;
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) {
+          double lift = static_cast<double>(power<EXL3_F32>(m_own[j], m, c));
+          if (lift < kNone) lift = 0.0;  // no token of the slice has a probability
+          rest[j] = sums[j] * lift;
+          total += rest[j];
+          b.top[lane * kOwn + j] = m_own[j], b.lift[lane * kOwn + j] = lift;
+        }
+        unit = 1.0 / warp_sum(total);
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) rest[j] *= unit;
+        best = has ? 0 : -1;
+        __syncwarp();
+      } else if (has) {  // the first slice with the maximum
+        double where = 0.0;
+#pragma unroll
+        for (int j = kOwn - 1; j >= 0; --j)
+          if (m_own[j] == m) where = sums[j];
+        best = static_cast<int>(__shfl_sync(0xFFFFFFFFu, where, __ffs(has) - 1));
+      }
+      if (best < 0) tried = kDraftMaxRows;  // the row has no finite logit
+    }
+    int command, child = 0;
+    for (;;) {
+      command = kStop;
+      for (; command == kStop && tried < ntok; tried += 32) {
+        if (tried != guess) look(tried + lane);
+        // every lane's token: its exponential and p, as the warp whose slice it is in computed them
+        float e = 0.f;
+        double le = 0.0;
+        if (tok >= 0 && warm) {
+          e = power<DT>(x, b.top[tok / p.slice], c);
+          le = static_cast<double>(e) * b.lift[tok / p.slice];
+          if (le < kNone) le = 0.0;
+        }
+        uint32_t left = __ballot_sync(0xFFFFFFFFu, tok >= 0);
+        while (left && command == kStop) {
+          const int l = __ffs(left) - 1;
+          left &= left - 1;
+          const int t = __shfl_sync(0xFFFFFFFFu, tok, l);
+          child = tried + l;
+          if (!warm) {
+            if (t == best) command = kNext;
+            continue;
+          }
+          const double qt = static_cast<double>(__shfl_sync(0xFFFFFFFFu, q, l));
+          double rt = __shfl_sync(0xFFFFFFFFu, le, l) * unit;
+          if (has_q) {
+            if (a > 0.0) rt = fmax(rt - a * qt, 0.0);
+          } else {
+            bool gone = false;
+            for (int j = lane; j < rejected; j += 32) gone |= b.out[j] == t;
+            if (__any_sync(0xFFFFFFFFu, gone)) continue;  // its sibling took it out of p
+          }
+          if (static_cast<double>(__shfl_sync(0xFFFFFFFFu, u, l)) * qt * z < rt) {
+            command = kNext;
+          } else if (has_q) {
+            a += z;
+            command = kCut;
+          } else {
+            const int slice = t / p.slice;
+            const double et = static_cast<double>(__shfl_sync(0xFFFFFFFFu, e, l));
+            if (lane == 0) {
+              b.out[rejected] = t;
+              if (slice / kWarps == rank) s_e[pad + t - base] = 0.f;
+            }
+            ++rejected;
+            z = 0.0;
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j) {
+              if (slice == lane * kOwn + j) sums[j] = fmax(sums[j] - et, 0.0), rest[j] = sums[j] * b.lift[slice] * unit;
+              z += rest[j];
+            }
+            __syncwarp();
+            z = warp_sum(z);
+            if (!(z > 0.0)) {  // nothing is left: p again
+              for (int j = lane; j < rejected; j += 32) {
+                const int g = b.out[j];
+                if (g / p.slice / kWarps == rank) s_e[pad + g - base] = power<DT>(logit(widen<DT>(logits[g])), b.top[g / p.slice], c);
+              }
+#pragma unroll
+              for (int j = 0; j < kOwn; ++j)
+                sums[j] = sent[lane * kOwn + j].y, rest[j] = sums[j] * b.lift[lane * kOwn + j] * unit;
+              rejected = 0, z = 1.0;
+              __syncwarp();
+            }
+          }
+        }
+        if (command == kCut) {
+          tried = child + 1;
+          break;
+        }
+      }
+      if (command == kStop) {  // the slice that holds the next token, and what is left to pass in it
+        const double goal = static_cast<double>(u_next) * z;
+        double upto = 0.0;
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) upto += rest[j];
+        const bool some = upto > 0.0;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const double o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+          if (lane >= d) upto += o;
+        }
+        const double before = __shfl_up_sync(0xFFFFFFFFu, upto, 1);
+        const uint32_t over = __ballot_sync(0xFFFFFFFFu, upto > goal && some);
+        const uint32_t any = __ballot_sync(0xFFFFFFFFu, some);
+        if (lane == (over ? __ffs(over) - 1 : (any ? 31 - __clz(any) : 0))) {
+          double acc = lane ? before : 0.0, target = 0.0;
+          int slice = -1;  // the last that begins at or before the goal
+#pragma unroll
+          for (int j = 0; j < kOwn; ++j) {
+            if (rest[j] > 0.0 && (slice < 0 || !(acc > goal))) slice = lane * kOwn + j, target = goal - acc;
+            acc += rest[j];
+          }
+          b.owner = slice, b.target = target, b.token = best;
+        }
+      }
+      if (lane == 0) {
+        b.command = command, b.node = child;
+        b.a = static_cast<float>(a), b.unit = unit, b.cut = static_cast<float>(kNone * unit);
+      }
+      __syncthreads();
+      if (command != kCut) break;
+      const double2* got = b.slice[turn++ & 1u];
+      cluster_sync();  // the slices' sums of r
+      z = 0.0;
+#pragma unroll
+      for (int j = 0; j < kOwn; ++j) rest[j] = got[lane * kOwn + j].x, z += rest[j];
+      z = warp_sum(z);
+      if (!(z > 0.0)) {  // nothing is left: p again
+        a = 0.0, z = 1.0;
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) rest[j] = sums[j] * b.lift[lane * kOwn + j] * unit;
+      }
+    }
+    if (command == kStop) break;
+    node = child;
+  }
+  if (rank == 0) {
+    for (int d = kept + lane; d < p.depth; d += 32) path[d] = -1;
+    if (lane == 0) {
+      p.kept[s] = kept;
+      if (!warm || b.token < 0) p.token[s] = b.token;
+    }
   }
 }
 
 template <int DT>
 cudaError_t launch_dtype(const DraftParams& p, int nseq, cudaStream_t st) {
   static KernelSetup setup;
-  const size_t smem = (static_cast<size_t>(p.slice) + 8) * sizeof(float);
+  const size_t smem = (static_cast<size_t>(p.slice) * kWarps + 8) * sizeof(float);
   cudaError_t e = kernel_setup(setup, verify_kernel<DT>, kThreads, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -486,7 +592,7 @@ cudaError_t launch_dtype(const DraftParams& p, int nseq, cudaStream_t st) {
 
 cudaError_t launch_draft_verify(const DraftParams& params, int nseq, cudaStream_t st) {
   DraftParams p = params;
-  p.slice = ((p.vocab + kCluster - 1) / kCluster + 7) & ~7;
+  p.slice = ((p.vocab + kSlices - 1) / kSlices + 7) & ~7;
   switch (p.logits_dtype) {
     case EXL3_F16: return launch_dtype<EXL3_F16>(p, nseq, st);
     case EXL3_BF16: return launch_dtype<EXL3_BF16>(p, nseq, st);
