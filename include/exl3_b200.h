@@ -655,7 +655,7 @@ typedef struct exl3_draft {
   const int32_t *tokens;    /* device, [rows] (row 0's is not read) */
   const int32_t *parent;    /* device, [rows], or null */
   const float *uniform;     /* device, [rows][2], in [0, 1): for the row's own token, for the token that follows the row */
-  const float *temperature; /* device, [nseq], 0 (greedy) or a positive number, or null: 1 */
+  const float *temperature; /* device, [nseq], 0 (greedy) or 2^-100 .. 2^100, or null: 1 */
 } exl3_draft;
 
 /* Verification of drafted tokens: the path of accepted rows from row 0 down, and the token that follows it, together
@@ -670,7 +670,8 @@ typedef struct exl3_draft {
  * sequence without rows), as exl3_cache_keep takes them; token [nseq] the token that follows (-1: no rows, or no logit above
  * -inf).  Logits: NaN counts as -inf, +inf as the largest finite number, and a token 2^-100 below the likeliest has no
  * probability; draft: NaN and negative numbers count as 0; a child whose token is outside the vocabulary is not tried.
- * Exponentials are f32 to a few ulp, their sums, r and Z f64.  At most 1024 rows a sequence.  The batch's context and table
+ * Exponentials are f32, within 2^-22 + 2^-24 |x - max| / temperature of themselves; their sums keep 2^-48, decisions are f64.
+ * Another temperature is taken as 0 (EXL3_ERR_BAD_SHAPE is recorded).  At most 1024 rows a sequence.  The batch's context and table
  * are not read. */
 exl3_verdict exl3_draft_verify(const exl3_kv_cache *cache, const exl3_tree_batch *batch, const exl3_draft *draft,
                                void *stream, int32_t *path, int32_t depth, int32_t *kept, int32_t *token);

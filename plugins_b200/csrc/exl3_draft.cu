@@ -58,14 +58,12 @@ __device__ __forceinline__ float widen(typename Elem<DT>::type v) {
   else if constexpr (DT == EXL3_BF16) return __uint_as_float(static_cast<uint32_t>(v) << 16);
   else return v;
 }
-// A logit as it counts: NaN as -inf, +inf as the largest finite number.
-__device__ __forceinline__ float logit(float x) { return x == x ? fminf(x, FLT_MAX) : -INFINITY; }
-// Element k of a chunk, as a logit.
+// Element k of a chunk.
 template <int DT>
-__device__ __forceinline__ float chunk_logit(const uint4& u, int k) {
+__device__ __forceinline__ float element(const uint4& u, int k) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-  if constexpr (DT == EXL3_F32) return logit(__uint_as_float(w[k]));
-  else return logit(widen<DT>(static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1)))));
+  if constexpr (DT == EXL3_F32) return __uint_as_float(w[k]);
+  else return widen<DT>(static_cast<uint16_t>(w[k / 2] >> (16 * (k & 1))));
 }
 // A drafter's probability: NaN and negative numbers as 0.
 template <int DT>
@@ -76,23 +74,77 @@ __device__ __forceinline__ float draft_at(const void* row, int dtype, int64_t i)
   return dtype == EXL3_F32 ? draft_p<EXL3_F32>(row, i) : dtype == EXL3_F16 ? draft_p<EXL3_F16>(row, i) : draft_p<EXL3_BF16>(row, i);
 }
 
-// 2^((x - m) c), c = c1 + c2 = log2(e) / T.  What the product and c's first part leave out, up to 2^-24 of an exponent of
-// 100, is carried along (and what the difference does, where x is f32: of 16-bit numbers it is exact): what is left is the
-// exponential's own error.
-struct Scale {
-  float c1, c2;
+// Two f32 in one 64-bit register pair: one issue slot for both.
+struct Two {
+  uint64_t v;
+  __device__ __forceinline__ Two() : v(0) {}
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void split(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
 };
-template <int DT>
-__device__ __forceinline__ float power(float x, float m, Scale c) {
-  const float d = x - m, z = d * c.c1;
-  float z2 = fmaf(d, c.c2, fmaf(d, c.c1, -z));
-  if constexpr (DT == EXL3_F32) {
-    const float b = d - x;
-    z2 = fmaf((x - (d - b)) + (-m - b), c.c1, z2);
-  }
-  const float e = exp2f(z);
-  return z > -150.f ? fmaf(e * 0.6931472f, z2, e) : 0.f;  // (x of -inf: z is -inf, or NaN beside m = -inf)
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
 }
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Two operator-(Two a, Two b) { return fma(b, Two(-1.f, -1.f), a); }
+__device__ __forceinline__ float ex2(float x) {  // 2^x
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 2^(d c), d = min(x - m, 0) and c = c1 + c2 = log2(e) / T.  What the product and c's first part leave out, up to 2^-24 of an
+// exponent of 100, is carried along: left are the exponential's own 2^-22 and the difference's rounding, 2^-24 |d| / T (none
+// for 16-bit logits near one another).  Nothing below 2^-200, which is zero: so x of -inf and NaN, and m of -inf; x of +inf
+// is m.
+struct Scale {
+  float c1, c2, least;
+};
+__device__ __forceinline__ Two power2(float x0, float x1, float m, Scale c) {
+  float d0, d1;
+  (Two(x0, x1) + Two(-m, -m)).split(d0, d1);
+  const Two d(fminf(fmaxf(d0, c.least), 0.f), fminf(fmaxf(d1, c.least), 0.f));
+  const Two c1(c.c1, c.c1), z = d * c1, none;
+  const Two z2 = fma(d, Two(c.c2, c.c2), fma(d, c1, none - z));
+  float z0, z1;
+  z.split(z0, z1);
+  const Two e(ex2(z0), ex2(z1));
+  return fma(e * Two(0.6931472f, 0.6931472f), z2, e);
+}
+__device__ __forceinline__ float power(float x, float m, Scale c) {  // (the same steps)
+  float a, b;
+  power2(x, x, m, c).split(a, b);
+  return a;
+}
+
+// A sum of f32 numbers with the rounding of every addition kept apart (Knuth's two-sum): good to 2^-48 of itself.  Of f64
+// arithmetic, the conversions alone would take as long as the exponentials.
+struct Sum {
+  Two s, c;
+  __device__ __forceinline__ void add(Two e) {
+    const Two t = s + e, b = t - s;
+    c = c + ((s - (t - b)) + (e - b));
+    s = t;
+  }
+  __device__ __forceinline__ double total() const {
+    float a, b, x, y;
+    s.split(a, b), c.split(x, y);
+    return (static_cast<double>(a) + static_cast<double>(b)) + (static_cast<double>(x) + static_cast<double>(y));
+  }
+};
+
+// Whether x counts as the maximum `top`.
+__device__ __forceinline__ bool is_top(float x, float top) { return x == x && fminf(x, FLT_MAX) == top; }
 
 __device__ __forceinline__ uint32_t ordered(float x) {  // whole numbers in the order of the floats
   const uint32_t u = __float_as_uint(x);
@@ -112,18 +164,18 @@ struct Block {
   double lift[kSlices];
   // the walk, as the deciding warp leaves it
   int command, node, owner, token;
-  float a, cut;               // A; what is none, in units of p
-  double unit, target;        // 1 / the row's sum; what is left to pass in the owner's slice
+  float a;                    // A, in units of the exponentials (as all of r)
+  double target;              // what is left to pass in the owner's slice
   // the sequence's rows
   int parent[kDraftMaxRows], tokens[kDraftMaxRows], first[kDraftMaxRows];  // first: a row's first child, or none
   int out[kDraftMaxRows];     // the node's rejected tokens, where there is no q
 };
 enum : int { kNext = 0, kStop = 1, kCut = 2 };  // on to a child; the path ends; r has to be summed
 
-// r of an element after rejections: e its exponential, lu what makes that p.
-__device__ __forceinline__ float rest_of(float e, float lu, float a, float q, float cut) {
-  const float v = e * lu;
-  return v < cut ? 0.f : fmaxf(fmaf(-a, q, v), 0.f);
+// r of an element after rejections: e its exponential in its slice, lift the slice's.
+__device__ __forceinline__ float rest_of(float e, float lift, float a, float q) {
+  const float v = e * lift;
+  return v < static_cast<float>(kNone) ? 0.f : fmaxf(fmaf(-a, q, v), 0.f);
 }
 
 // Where elements of a row lie in s_e: whole 16-byte chunks of the row on multiples of four.
@@ -158,7 +210,7 @@ struct Part {
   }
 };
 
-// f(e, q) for the elements of a warp's slice, four neighbours a lane.
+// f(e, q, e', q') for the elements of a warp's slice, four neighbours a lane (an element alone: beside zeros).
 template <int DT, typename F>
 __device__ __forceinline__ void each_draft_of(const void* draft, int64_t at, const float* own, int pad, int n, int lane, F&& f) {
   using T = typename Elem<DT>::type;
@@ -171,13 +223,13 @@ __device__ __forceinline__ void each_draft_of(const void* draft, int64_t at, con
       T v[4];
       if constexpr (DT == EXL3_F32) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(q + t);
       else *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(q + t);
-      f(e.x, fmaxf(widen<DT>(v[0]), 0.f)), f(e.y, fmaxf(widen<DT>(v[1]), 0.f));
-      f(e.z, fmaxf(widen<DT>(v[2]), 0.f)), f(e.w, fmaxf(widen<DT>(v[3]), 0.f));
+      f(e.x, fmaxf(widen<DT>(v[0]), 0.f), e.y, fmaxf(widen<DT>(v[1]), 0.f));
+      f(e.z, fmaxf(widen<DT>(v[2]), 0.f), e.w, fmaxf(widen<DT>(v[3]), 0.f));
     } else {
       const float es[4] = {e.x, e.y, e.z, e.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (t + k >= pad && t + k < pad + n) f(es[k], fmaxf(widen<DT>(q[t + k]), 0.f));
+        if (t + k >= pad && t + k < pad + n) f(es[k], fmaxf(widen<DT>(q[t + k]), 0.f), 0.f, 0.f);
     }
   }
 }
@@ -189,7 +241,7 @@ __device__ __forceinline__ void each_draft(const DraftParams& p, int64_t at, con
 }
 
 template <int DT>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) verify_kernel(const DraftParams p) {
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) verify_kernel(const DraftParams p) {
   using T = typename Elem<DT>::type;
   constexpr int kVec = Elem<DT>::kVec;
   extern __shared__ __align__(16) float s_e[];  // [slice + 8]
@@ -200,7 +252,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
   const int r0 = p.row_start[s], r1 = p.row_start[s + 1];
   const float temp = p.temperature ? p.temperature[s] : 1.f;
   const int row0 = max(0, min(r0, p.rows)), all = max(0, min(r1, p.rows) - row0), ntok = min(all, p.max_rows);
-  const bool warm = temp > 0.f && temp <= FLT_MAX;
+  const bool warm = temp >= 0x1p-100f && temp <= 0x1p100f;
   if (tid == 0 && rank == 0 && (r0 < 0 || r1 < r0 || r1 > p.rows || all > ntok || (!warm && temp != 0.f)))
     atomicOr(p.err, kErrBadShape);
   int32_t* path = p.path + static_cast<int64_t>(s) * p.depth;
@@ -229,11 +281,12 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
     b.tokens[i] = p.tokens[row0 + i];
     b.first[i] = kDraftMaxRows;
   }
-  Scale c{0.f, 0.f};
+  Scale c{0.f, 0.f, 0.f};
   if (warm) {
     const double cd = kLog2e / static_cast<double>(temp);
     c.c1 = static_cast<float>(fmin(cd, static_cast<double>(FLT_MAX)));
     c.c2 = cd < 1e30 ? static_cast<float>(cd - static_cast<double>(c.c1)) : 0.f;
+    c.least = fmaxf(-200.f / c.c1, -FLT_MAX);
   }
   __syncthreads();
   for (int i = tid; i < ntok; i += kThreads) {
@@ -257,23 +310,24 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
       const Part<DT> part(row_of(node) + v0, n, lane);
       const int pad = pad_of<DT>(part.src);
       const bool whole = part.chunks <= kChunks * 32;
-      const float single = part.odd >= 0 ? logit(widen<DT>(odd)) : -INFINITY;
-      float top = single;
+      const float single = part.odd >= 0 ? widen<DT>(odd) : -INFINITY;
+      float top = fmaxf(single, -INFINITY);  // (NaN is passed over)
       for (int from = 0; from < part.chunks; from += kChunks * 32) {
         if (!whole) part.load(from, raw);
 #pragma unroll
         for (int i = 0; i < kChunks; ++i)
           if (from + i * 32 + lane < part.chunks)
 #pragma unroll
-            for (int k = 0; k < kVec; ++k) top = fmaxf(top, chunk_logit<DT>(raw[i], k));
+            for (int k = 0; k < kVec; ++k) top = fmaxf(top, element<DT>(raw[i], k));
       }
-      top = unordered(__reduce_max_sync(0xFFFFFFFFu, ordered(top)));
+      top = fminf(unordered(__reduce_max_sync(0xFFFFFFFFu, ordered(top))), FLT_MAX);  // (+inf counts as the largest number)
       double sum = 0.0;
       if (warm) {
+        Sum parts;
         if (part.odd >= 0) {
-          const float e = power<DT>(single, top, c);
+          const float e = power(single, top, c);
           own[pad + part.odd] = e;
-          sum = static_cast<double>(e);
+          parts.s = Two(e, 0.f);
         }
         for (int from = 0; from < part.chunks; from += kChunks * 32) {
           if (!whole) part.load(from, raw);
@@ -283,17 +337,18 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
             if (at >= part.chunks) continue;
 #pragma unroll
             for (int k = 0; k < kVec; k += 4) {
+              const Two lo = power2(element<DT>(raw[i], k), element<DT>(raw[i], k + 1), top, c);
+              const Two hi = power2(element<DT>(raw[i], k + 2), element<DT>(raw[i], k + 3), top, c);
               float4 e;
-              e.x = power<DT>(chunk_logit<DT>(raw[i], k), top, c), e.y = power<DT>(chunk_logit<DT>(raw[i], k + 1), top, c);
-              e.z = power<DT>(chunk_logit<DT>(raw[i], k + 2), top, c), e.w = power<DT>(chunk_logit<DT>(raw[i], k + 3), top, c);
+              lo.split(e.x, e.y), hi.split(e.z, e.w);
               *reinterpret_cast<float4*>(own + pad + part.head + at * kVec + k) = e;
-              sum += (static_cast<double>(e.x) + static_cast<double>(e.y)) + (static_cast<double>(e.z) + static_cast<double>(e.w));
+              parts.add(lo), parts.add(hi);
             }
           }
         }
-        sum = warp_sum(sum);
+        sum = warp_sum(parts.total());
       } else {  // a greedy sequence's slice: where its maximum is first
-        uint32_t at = single == top && part.odd >= 0 ? part.odd : 0x7FFFFFFFu;
+        uint32_t at = part.odd >= 0 && is_top(single, top) ? part.odd : 0x7FFFFFFFu;
         for (int from = 0; from < part.chunks; from += kChunks * 32) {
           if (!whole) part.load(from, raw);
 #pragma unroll
@@ -301,7 +356,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
             if (from + i * 32 + lane < part.chunks)
 #pragma unroll
               for (int k = 0; k < kVec; ++k)
-                if (chunk_logit<DT>(raw[i], k) == top) at = min(at, static_cast<uint32_t>(part.head + (from + i * 32 + lane) * kVec + k));
+                if (is_top(element<DT>(raw[i], k), top)) at = min(at, static_cast<uint32_t>(part.head + (from + i * 32 + lane) * kVec + k));
         }
         sum = static_cast<double>(v0) + static_cast<double>(__reduce_min_sync(0xFFFFFFFFu, at));
       }
@@ -313,11 +368,11 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
       for (;;) {
         __syncthreads();  // the decision
         if (b.command != kCut) break;
-        const float la = b.a, lu = static_cast<float>(b.lift[mine] * b.unit), cut = b.cut;
-        double r = 0.0;
+        const float la = b.a, lu = static_cast<float>(b.lift[mine]);
+        Sum r;
         each_draft(p, (row0 + static_cast<int64_t>(node)) * p.draft_stride + v0, own, pad, n, lane,
-                   [&](float e, float q) { r += static_cast<double>(rest_of(e, lu, la, q, cut)); });
-        send(warp_sum(r), 0.0);
+                   [&](float e0, float q0, float e1, float q1) { r.add(Two(rest_of(e0, lu, la, q0), rest_of(e1, lu, la, q1))); });
+        send(warp_sum(r.total()), 0.0);
       }
       if (b.command == kStop) break;
       const int next = b.node;
@@ -328,13 +383,13 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
     // ---- the next token: the first of the owner's slice whose cumulative sum passes the target, a run of places per lane
     const int64_t q_at = (row0 + static_cast<int64_t>(node)) * p.draft_stride + v0;
     const int pad = pad_of<DT>(row_of(node) + v0);
-    const double target = b.target, lift = b.lift[mine], unit = b.unit;
-    const float la = b.a, lu = static_cast<float>(lift * unit), cut = b.cut;
+    const double target = b.target, lift = b.lift[mine];
+    const float la = b.a, lu = static_cast<float>(lift);
     auto at = [&](int i) {
       const float e = own[pad + i];
-      if (has_q && la > 0.f) return static_cast<double>(rest_of(e, lu, la, draft_at(p.draft, p.draft_dtype, q_at + i), cut));
+      if (has_q && la > 0.f) return static_cast<double>(rest_of(e, lu, la, draft_at(p.draft, p.draft_dtype, q_at + i)));
       const double le = static_cast<double>(e) * lift;
-      return le < kNone ? 0.0 : le * unit;
+      return le < kNone ? 0.0 : le;
     };
     const int len = ((n + 31) / 32) | 1;  // odd: no two lanes on one bank
     const int lo = min(n, lane * len), hi = min(n, lo + len);
@@ -392,7 +447,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
         tok = -1;  // (a token outside the vocabulary is not tried)
         return;
       }
-      x = logit(widen<DT>(logits[tok]));
+      x = widen<DT>(logits[tok]);
       u = p.uniform[2 * (row0 + static_cast<int64_t>(i))];
       if (has_q) q = draft_at(p.draft, p.draft_dtype, row * p.draft_stride + tok);
     };
@@ -406,7 +461,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
 
     // a lane's slices: their sums of exponentials (of what is left of them) and e^((m_w - m) / T); r's sums
     double sums[kOwn], rest[kOwn];
-    double a = 0.0, z = 1.0, unit = 0.0;
+    double a = 0.0, z = 0.0;
     int best = -1, tried = guess, rejected = 0;
     {
       float m = -INFINITY, m_own[kOwn];
@@ -420,18 +475,16 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
       m = unordered(__reduce_max_sync(0xFFFFFFFFu, ordered(m)));
       const uint32_t has = __ballot_sync(0xFFFFFFFFu, m_lane == m && m != -INFINITY);
       if (warm) {
-        double total = 0.0;
+        z = 0.0;
 #pragma unroll
         for (int j = 0; j < kOwn; ++j) {
-          double lift = static_cast<double>(power<EXL3_F32>(m_own[j], m, c));
+          double lift = static_cast<double>(power(m_own[j], m, c));
           if (lift < kNone) lift = 0.0;  // no token of the slice has a probability
           rest[j] = sums[j] * lift;
-          total += rest[j];
+          z += rest[j];
           b.top[lane * kOwn + j] = m_own[j], b.lift[lane * kOwn + j] = lift;
         }
-        unit = 1.0 / warp_sum(total);
-#pragma unroll
-        for (int j = 0; j < kOwn; ++j) rest[j] *= unit;
+        z = warp_sum(z);
         best = has ? 0 : -1;
         __syncwarp();
       } else if (has) {  // the first slice with the maximum
@@ -452,7 +505,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
         float e = 0.f;
         double le = 0.0;
         if (tok >= 0 && warm) {
-          e = power<DT>(x, b.top[tok / p.slice], c);
+          e = power(x, b.top[tok / p.slice], c);
           le = static_cast<double>(e) * b.lift[tok / p.slice];
           if (le < kNone) le = 0.0;
         }
@@ -467,7 +520,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
             continue;
           }
           const double qt = static_cast<double>(__shfl_sync(0xFFFFFFFFu, q, l));
-          double rt = __shfl_sync(0xFFFFFFFFu, le, l) * unit;
+          double rt = __shfl_sync(0xFFFFFFFFu, le, l);
           if (has_q) {
             if (a > 0.0) rt = fmax(rt - a * qt, 0.0);
           } else {
@@ -491,7 +544,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
             z = 0.0;
 #pragma unroll
             for (int j = 0; j < kOwn; ++j) {
-              if (slice == lane * kOwn + j) sums[j] = fmax(sums[j] - et, 0.0), rest[j] = sums[j] * b.lift[slice] * unit;
+              if (slice == lane * kOwn + j) sums[j] = fmax(sums[j] - et, 0.0), rest[j] = sums[j] * b.lift[slice];
               z += rest[j];
             }
             __syncwarp();
@@ -499,12 +552,14 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
             if (!(z > 0.0)) {  // nothing is left: p again
               for (int j = lane; j < rejected; j += 32) {
                 const int g = b.out[j];
-                if (g / p.slice / kWarps == rank) s_e[pad + g - base] = power<DT>(logit(widen<DT>(logits[g])), b.top[g / p.slice], c);
+                if (g / p.slice / kWarps == rank) s_e[pad + g - base] = power(widen<DT>(logits[g]), b.top[g / p.slice], c);
               }
+              z = 0.0;
 #pragma unroll
               for (int j = 0; j < kOwn; ++j)
-                sums[j] = sent[lane * kOwn + j].y, rest[j] = sums[j] * b.lift[lane * kOwn + j] * unit;
-              rejected = 0, z = 1.0;
+                sums[j] = sent[lane * kOwn + j].y, rest[j] = sums[j] * b.lift[lane * kOwn + j], z += rest[j];
+              z = warp_sum(z);
+              rejected = 0;
               __syncwarp();
             }
           }
@@ -541,7 +596,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
       }
       if (lane == 0) {
         b.command = command, b.node = child;
-        b.a = static_cast<float>(a), b.unit = unit, b.cut = static_cast<float>(kNone * unit);
+        b.a = static_cast<float>(a);
       }
       __syncthreads();
       if (command != kCut) break;
@@ -552,9 +607,10 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 2) 
       for (int j = 0; j < kOwn; ++j) rest[j] = got[lane * kOwn + j].x, z += rest[j];
       z = warp_sum(z);
       if (!(z > 0.0)) {  // nothing is left: p again
-        a = 0.0, z = 1.0;
+        a = z = 0.0;
 #pragma unroll
-        for (int j = 0; j < kOwn; ++j) rest[j] = sums[j] * b.lift[lane * kOwn + j] * unit;
+        for (int j = 0; j < kOwn; ++j) rest[j] = sums[j] * b.lift[lane * kOwn + j], z += rest[j];
+        z = warp_sum(z);
       }
     }
     if (command == kStop) break;

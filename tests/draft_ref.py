@@ -25,17 +25,19 @@ def verify_one(logits, tokens, parent, uniform, temperature, draft, depth):
     """One sequence's rows -> (path, token, near): near is the least distance of a decision (an acceptance, a place in the
     cumulative sums) from its border, in units of what f32 exponentials may move it by.
 
-    An exponential is within 2 ulp (2^-22 of itself) and a sum of them no further, so p is within 2^-21 of itself.  With k
-    rejections behind it, A_k = sum Z_i: each Z_i = sum max(p - A_i q, 0) is off by at most 2^-21 + err(A_i) (sum q = 1), so
-    err(A_k) <= (2^k - 1) 2^-21; u q Z - r and cumsum r - u Z are then within 2 (2^-21 + err(A_k)) = 2^(k - 20).  Without
-    draft nothing is subtracted but whole tokens, and it stays 2^-20."""
+    An exponential is within 2^-22 + 2^-24 |x - m| / T of itself, in its slice and the slice in the row together within twice
+    the first and once the second; weighted by p, |x - m| / T sums to at most ln(vocab) + 1 < 14.  So p's sums are within
+    2^-21 + 14 2^-24 of themselves, p (divided by one) within twice that, < 2^-18.6.  With k rejections behind it, A_k = sum
+    Z_i: each Z_i = sum max(p - A_i q, 0) is off by at most that + err(A_i) (sum q = 1), so err(A_k) <= (2^k - 1) 2^-18.6;
+    u q Z - r and cumsum r - u Z are then within 2 (2^-18.6 + err(A_k)) < 2^(k - 17).  Without draft nothing is subtracted
+    but whole tokens, and it stays 2^-17."""
     n, vocab = logits.shape
     path, at, near = [0], 0, math.inf
     while True:
         p = probabilities(logits[at], temperature)
         if p is None:
             return path, -1, near
-        r, z, child, unit = p, 1.0, None, 2.0 ** -20
+        r, z, child, unit = p, 1.0, None, 2.0 ** -17
         for c in range(at + 1, n) if len(path) < depth else ():
             x = int(tokens[c])
             if int(parent[c]) != at or not 0 <= x < vocab:
