@@ -93,6 +93,25 @@ class _Calls:
         cls.rope = proto(ctypes.cast(lib.exl3_qk_norm_rope, p).value)  # last: another thread takes it for all there
 
 
+class _StepCalls:
+    """Likewise the calls that end a step (exl3_kv_weight and exl3_draft as bytes)."""
+    weight = verify = None
+
+    @classmethod
+    def load(cls) -> None:
+        p, c, i, f = ctypes.c_void_p, ctypes.c_char_p, ctypes.c_int32, ctypes.c_float
+        lib = L.lib()
+        proto = ctypes.CFUNCTYPE(L.Verdict, p, i, p, c, f, p, f, p, c)
+        cls.weight = proto(ctypes.cast(lib.exl3_attention_weight, p).value)
+        proto = ctypes.CFUNCTYPE(L.Verdict, p, p, c, p, p, i, p, p)
+        cls.verify = proto(ctypes.cast(lib.exl3_draft_verify, p).value)  # last, as above
+
+
+_KV_WEIGHT = struct.Struct("@IiiiPqqq")
+_DRAFT = struct.Struct("@IiiiqqPPPPPP")
+assert _KV_WEIGHT.size == ctypes.sizeof(L.KvWeight) and _DRAFT.size == ctypes.sizeof(L.Draft)
+
+
 def _used_on(stream, *tensors) -> None:
     """Tensors the caching allocator must not hand out again before `stream` is done with them: all that a call reads or
     writes there.  (A stream given by its handle is the caller's to wait for.)"""
@@ -142,6 +161,8 @@ class KvCache:
         check(L.lib().exl3_kv_register(self.raw))
         if _Calls.rope is None:
             _Calls.load()
+        if _StepCalls.verify is None:
+            _StepCalls.load()
 
     @classmethod
     def empty(cls, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=torch.bfloat16,
@@ -275,15 +296,20 @@ def tree_attention(cache: KvCache, layer: int, batch: TreeBatch, q, scale: float
     return out if lse is None else (out, lse)
 
 
-def _kv_weight(t, layers: int, nseq: int, cache: KvCache) -> L.KvWeight:
-    """[layers, nseq, kv_heads, slots] f32 on the cache's GPU, a head's slots contiguous."""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != cache.device or t.dim() != 4:
-        _refuse("weights are f32 [layers, rows, kv_heads, slots] on the cache's GPU")
-    if tuple(t.shape[:3]) != (layers, nseq, cache.raw.kv_heads):
-        _refuse(f"the weights have shape {list(t.shape)}, not {[layers, nseq, cache.raw.kv_heads, 'any']}")
-    if t.stride(3) != 1 and t.shape[3] > 1:
+def _kv_weight(t, layers: int, nseq: int, cache: KvCache, dims: int = 4) -> tuple:
+    """The fields of exl3_kv_weight: f32 [layers,] rows, kv_heads, slots on the cache's GPU, a head's slots contiguous."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.get_device() != cache._index:
+        _refuse("weights are an f32 tensor on the cache's GPU")
+    shape, stride = t.shape, t.stride()
+    if len(shape) != dims:
+        _refuse("weights are [layers, rows, kv_heads, slots]" if dims == 4 else "a layer's weights are [rows, kv_heads, slots]")
+    if dims == 3:
+        shape, stride = (1, *shape), (0, *stride)
+    if shape[0] != layers or shape[1] != nseq or shape[2] != cache.raw.kv_heads:
+        _refuse(f"the weights have shape {list(shape)}, not {[layers, nseq, cache.raw.kv_heads, 'any']}")
+    if stride[3] != 1 and shape[3] > 1:
         _refuse("the weights of a head's slots must be contiguous")
-    return L.KvWeight(ctypes.sizeof(L.KvWeight), layers, nseq, t.shape[3], t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+    return _KV_WEIGHT.size, layers, nseq, shape[3], t.data_ptr(), stride[0], stride[1], stride[2]
 
 
 def attention_weight(cache: KvCache, layer: int, batch: TreeBatch, q, lse, weight, scale: float | None = None,
@@ -293,15 +319,12 @@ def attention_weight(cache: KvCache, layer: int, batch: TreeBatch, q, lse, weigh
     begin anew.  ``q``, ``scale`` and ``lse`` (f32 [rows, heads]) are :func:`tree_attention`'s, which comes first."""
     i = cache._index
     hq = _heads(q, i, "q")
-    _floats(lse, q.shape[:2], "lse", cache.device)
-    if not isinstance(weight, torch.Tensor) or weight.dim() != 3:
-        _refuse("a layer's weights are f32 [nseq, kv_heads, slots]")
-    raw = _kv_weight(weight[None], 1, batch.nseq, cache)
+    _floats(lse, q.shape[:2], "lse", i)
+    raw = _KV_WEIGHT.pack(*_kv_weight(weight, 1, batch.nseq, cache, 3))
     if stream is not None:
         _used_on(stream, q, lse, weight, cache.k, cache.v, *batch._keep)
-    batch._for(cache, q.shape[0])
-    check(L.lib().exl3_attention_weight(cache.raw, layer, batch.raw, hq, cache._scale if scale is None else scale,
-                                        lse.data_ptr(), decay, _on(stream, i), raw))
+    _check(_StepCalls.weight(cache._at, layer, batch._for(cache, q.shape[0]), hq, cache._scale if scale is None else scale,
+                             lse.data_ptr(), decay, _on(stream, i), raw))
     return weight
 
 
@@ -419,8 +442,8 @@ def cache_evict(cache: KvCache, state: PageState, weight, budget, sink: int = 0,
     from shared ones: then nothing changed).  The tokens' weights move with them, in place or to ``weight_out``."""
     n = state.raw.nseq
     _ints(budget, (n,), "budget", cache.device)
-    raw = _kv_weight(weight, cache.raw.layers, n, cache)
-    kept = raw if weight_out is None else _kv_weight(weight_out, cache.raw.layers, n, cache)
+    raw = L.KvWeight(*_kv_weight(weight, cache.raw.layers, n, cache))
+    kept = raw if weight_out is None else L.KvWeight(*_kv_weight(weight_out, cache.raw.layers, n, cache))
     out = _states(cache, state, out, stream)
     if missing is None:
         missing = _maker(stream, torch.empty)((), dtype=torch.int32, device=cache.device)
@@ -433,17 +456,17 @@ def cache_evict(cache: KvCache, state: PageState, weight, budget, sink: int = 0,
     return out, missing
 
 
-def _floats(t, shape, what: str, device):
-    """A contiguous f32 GPU tensor of this shape."""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != device or not t.is_contiguous():
+def _floats(t, shape, what: str, index: int):
+    """A contiguous f32 tensor of this shape on the cache's GPU."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.get_device() != index or not t.is_contiguous():
         _refuse(f"{what} is a contiguous f32 tensor on the cache's GPU")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         _refuse(f"{what} has shape {list(t.shape)}, not {list(shape)}")
 
 
-def _vocab_rows(t, rows: int, vocab, what: str, device):
+def _vocab_rows(t, rows: int, vocab, what: str, index: int):
     """[rows, vocab] with contiguous rows -> its dtype."""
-    if not isinstance(t, torch.Tensor) or t.device != device or t.dim() != 2 or t.shape[0] != rows or \
+    if not isinstance(t, torch.Tensor) or t.get_device() != index or t.dim() != 2 or t.shape[0] != rows or \
             (vocab is not None and t.shape[1] != vocab) or (t.stride(1) != 1 and t.shape[1] > 1):
         _refuse(f"{what} is [rows, vocab] on the cache's GPU, its rows contiguous")
     dt = _TORCH_DT.get(t.dtype)
@@ -463,16 +486,16 @@ def draft_verify(cache: KvCache, batch: TreeBatch, logits, tokens, parent, unifo
     any).  ``uniform`` (f32 [rows, 2], in [0, 1)): a number for the row's own token and one for the token that follows the
     row.  ``temperature`` (f32 [nseq], 0: greedy; None: 1).  The path and the token are distributed as tokens drawn one by one
     from softmax(logits / temperature).  ``depth``: the most rows of a path (max_rows, if not given)."""
-    dev, n = cache.device, batch.nseq
+    dev, n, i = cache.device, batch.nseq, cache._index
     rows = batch.rows if batch.rows is not None else logits.shape[0]
-    dt = _vocab_rows(logits, rows, None, "logits", dev)
+    dt = _vocab_rows(logits, rows, None, "logits", i)
     vocab = logits.shape[1]
-    qt = L.F32 if draft is None else _vocab_rows(draft, rows, vocab, "draft", dev)
+    qt = L.F32 if draft is None else _vocab_rows(draft, rows, vocab, "draft", i)
     _ints(tokens, (rows,), "tokens", dev)
     _ints(parent, (rows,), "parent", dev, optional=True)
-    _floats(uniform, (rows, 2), "uniform", dev)
+    _floats(uniform, (rows, 2), "uniform", i)
     if temperature is not None:
-        _floats(temperature, (n,), "temperature", dev)
+        _floats(temperature, (n,), "temperature", i)
     depth = max(1, batch.raw.max_rows if depth is None else int(depth))
     make = _maker(stream, torch.empty)
     if path is None and kept is None and token is None:  # one allocation
@@ -482,13 +505,11 @@ def draft_verify(cache: KvCache, batch: TreeBatch, logits, tokens, parent, unifo
         path = make((n, depth), dtype=torch.int32, device=dev) if path is None else _ints(path, (n, depth), "path", dev)
         kept = make(n, dtype=torch.int32, device=dev) if kept is None else _ints(kept, (n,), "kept", dev)
         token = make(n, dtype=torch.int32, device=dev) if token is None else _ints(token, (n,), "token", dev)
-    batch._for(cache, rows)
     if stream is not None:
         _used_on(stream, logits, tokens, parent, uniform, temperature, draft, path, kept, token, *batch._keep)
-    raw = L.Draft(ctypes.sizeof(L.Draft), vocab, dt, qt, logits.stride(0), 0 if draft is None else draft.stride(0),
-                  logits.data_ptr(), None if draft is None else draft.data_ptr(), tokens.data_ptr(),
-                  None if parent is None else parent.data_ptr(), uniform.data_ptr(),
-                  None if temperature is None else temperature.data_ptr())
-    check(L.lib().exl3_draft_verify(cache.raw, batch.raw, raw, _on(stream, cache._index), path.data_ptr(), depth,
-                                    kept.data_ptr(), token.data_ptr()))
+    raw = _DRAFT.pack(_DRAFT.size, vocab, dt, qt, logits.stride(0), 0 if draft is None else draft.stride(0), logits.data_ptr(),
+                      0 if draft is None else draft.data_ptr(), tokens.data_ptr(), 0 if parent is None else parent.data_ptr(),
+                      uniform.data_ptr(), 0 if temperature is None else temperature.data_ptr())
+    _check(_StepCalls.verify(cache._at, batch._for(cache, rows), raw, _on(stream, i), path.data_ptr(), depth, kept.data_ptr(),
+                             token.data_ptr()))
     return path, kept, token

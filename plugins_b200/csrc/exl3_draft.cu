@@ -16,6 +16,8 @@
 #include <cuda_runtime.h>
 #include <float.h>
 
+#include <type_traits>
+
 #include "exl3_attn.h"
 #include "exl3_common.cuh"
 #include "exl3_internal.h"
@@ -210,26 +212,39 @@ struct Part {
   }
 };
 
+__device__ __forceinline__ uint4 four(uint4 v) { return v; }
+__device__ __forceinline__ uint4 four(uint2 v) { return make_uint4(v.x, v.y, 0u, 0u); }
+
 // f(e, q, e', q') for the elements of a warp's slice, four neighbours a lane (an element alone: beside zeros).
 template <int DT, typename F>
 __device__ __forceinline__ void each_draft_of(const void* draft, int64_t at, const float* own, int pad, int n, int lane, F&& f) {
   using T = typename Elem<DT>::type;
   const T* q = static_cast<const T*>(draft) + at - pad;
   const bool vec = reinterpret_cast<uintptr_t>(q) % (4 * sizeof(T)) == 0;
-#pragma unroll 4
-  for (int t = lane * 4; t < pad + n; t += 128) {
-    const float4 e = *reinterpret_cast<const float4*>(own + t);
-    if (vec && t >= pad && t + 4 <= pad + n) {
-      T v[4];
-      if constexpr (DT == EXL3_F32) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(q + t);
-      else *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(q + t);
-      f(e.x, fmaxf(widen<DT>(v[0]), 0.f), e.y, fmaxf(widen<DT>(v[1]), 0.f));
-      f(e.z, fmaxf(widen<DT>(v[2]), 0.f), e.w, fmaxf(widen<DT>(v[3]), 0.f));
-    } else {
-      const float es[4] = {e.x, e.y, e.z, e.w};
+  constexpr int kBatch = 2;
+  using V = typename std::conditional<DT == EXL3_F32, uint4, uint2>::type;  // four elements
+  for (int t0 = lane * 4; t0 < pad + n; t0 += 128 * kBatch) {
+    V v[kBatch];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (t + k >= pad && t + k < pad + n) f(es[k], fmaxf(widen<DT>(q[t + k]), 0.f), 0.f, 0.f);
+    for (int i = 0; i < kBatch; ++i) {
+      const int t = t0 + i * 128;
+      if (vec && t >= pad && t + 4 <= pad + n) v[i] = *reinterpret_cast<const V*>(q + t);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int t = t0 + i * 128;
+      if (t >= pad + n) break;
+      const float4 e = *reinterpret_cast<const float4*>(own + t);
+      if (vec && t >= pad && t + 4 <= pad + n) {
+        const uint4 u = four(v[i]);
+        f(e.x, fmaxf(element<DT>(u, 0), 0.f), e.y, fmaxf(element<DT>(u, 1), 0.f));
+        f(e.z, fmaxf(element<DT>(u, 2), 0.f), e.w, fmaxf(element<DT>(u, 3), 0.f));
+      } else {
+        const float es[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (t + k >= pad && t + k < pad + n) f(es[k], fmaxf(widen<DT>(q[t + k]), 0.f), 0.f, 0.f);
+      }
     }
   }
 }
@@ -363,21 +378,26 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
       // the first child's row, should it be the next
       const int guess = kept + 1 < p.depth ? b.first[node] : kDraftMaxRows;
       if (guess < kDraftMaxRows) fetch(guess);
-      send(static_cast<double>(top), sum);
       ++kept;
-      for (;;) {
-        __syncthreads();  // the decision
-        if (b.command != kCut) break;
-        const float la = b.a, lu = static_cast<float>(b.lift[mine]);
-        Sum r;
-        each_draft(p, (row0 + static_cast<int64_t>(node)) * p.draft_stride + v0, own, pad, n, lane,
-                   [&](float e0, float q0, float e1, float q1) { r.add(Two(rest_of(e0, lu, la, q0), rest_of(e1, lu, la, q1))); });
-        send(warp_sum(r.total()), 0.0);
+      send(static_cast<double>(top), sum);
+      __syncthreads();  // the decision
+      if (b.command == kCut) {  // (the first child is rejected: what was fetched for it is not needed)
+        do {
+          const float la = b.a, lu = static_cast<float>(b.lift[mine]);
+          Sum r;
+          each_draft(p, (row0 + static_cast<int64_t>(node)) * p.draft_stride + v0, own, pad, n, lane,
+                     [&](float e0, float q0, float e1, float q1) { r.add(Two(rest_of(e0, lu, la, q0), rest_of(e1, lu, la, q1))); });
+          send(warp_sum(r.total()), 0.0);
+          __syncthreads();
+        } while (b.command == kCut);
+        if (b.command == kStop) break;
+        node = b.node;
+        fetch(node);
+      } else {
+        if (b.command == kStop) break;
+        node = b.node;
+        if (node != guess) fetch(node);
       }
-      if (b.command == kStop) break;
-      const int next = b.node;
-      if (next != guess) fetch(next);
-      node = next;
     }
     if (!warm || b.token < 0 || mine != b.owner) return;
     // ---- the next token: the first of the owner's slice whose cumulative sum passes the target, a run of places per lane
@@ -385,46 +405,53 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
     const int pad = pad_of<DT>(row_of(node) + v0);
     const double target = b.target, lift = b.lift[mine];
     const float la = b.a, lu = static_cast<float>(lift);
+    const float least = static_cast<float>(fmin(kNone / lift, 2.0));  // (lift is at least kNone)
+    const double scale = has_q && la > 0.f ? 1.0 : lift;              // of the numbers that at() gives
     auto at = [&](int i) {
       const float e = own[pad + i];
-      if (has_q && la > 0.f) return static_cast<double>(rest_of(e, lu, la, draft_at(p.draft, p.draft_dtype, q_at + i)));
-      const double le = static_cast<double>(e) * lift;
-      return le < kNone ? 0.0 : le;
+      if (has_q && la > 0.f) return rest_of(e, lu, la, draft_at(p.draft, p.draft_dtype, q_at + i));
+      return e < least ? 0.f : e;
     };
+    const double goal = target / scale;
     const int len = ((n + 31) / 32) | 1;  // odd: no two lanes on one bank
     const int lo = min(n, lane * len), hi = min(n, lo + len);
-    double run = 0.0;
+    Sum parts;
     int last = -1;
-    for (int i = lo; i < hi; ++i) {
-      const double r = at(i);
-      if (r > 0.0) last = i;
-      run += r;
+    for (int i = lo; i < hi; i += 2) {
+      const float x = at(i), y = i + 1 < hi ? at(i + 1) : 0.f;
+      if (x > 0.f) last = i;
+      if (y > 0.f) last = i + 1;
+      parts.add(Two(x, y));
     }
-    double upto = run;
+    auto scan = [&](double v) {  // inclusive
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const double o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-      if (lane >= d) upto += o;
-    }
-    double before = __shfl_up_sync(0xFFFFFFFFu, upto, 1);
-    if (lane == 0) before = 0.0;
-    int found = -1;
-    if (before <= target && upto > target) {  // (one lane at most: before is the last one's upto)
-      found = last;                           // rounding may leave none
-      for (int i = lo; i < hi; ++i) {
-        const double r = at(i);
-        before += r;
-        if (r > 0.0 && before > target) {
-          found = i;
-          break;
-        }
+      for (int d = 1; d < 32; d <<= 1) {
+        const double o = __shfl_up_sync(0xFFFFFFFFu, v, d);
+        if (lane >= d) v += o;
       }
+      return v;
+    };
+    const double upto = scan(parts.total());
+    const uint32_t over = __ballot_sync(0xFFFFFFFFu, upto > goal && last >= 0);
+    int found = -1;
+    if (over) {  // the run, a place per lane
+      const int l = __ffs(over) - 1;
+      double acc = __shfl_sync(0xFFFFFFFFu, upto, l > 0 ? l - 1 : 0);
+      if (l == 0) acc = 0.0;
+      const int end = min(n, (l + 1) * len);
+      for (int i0 = l * len; i0 < end && found < 0; i0 += 32) {
+        const float x = i0 + lane < end ? at(i0 + lane) : 0.f;
+        const double sum = acc + scan(static_cast<double>(x));
+        const uint32_t here = __ballot_sync(0xFFFFFFFFu, sum > goal && x > 0.f);
+        if (here) found = i0 + __ffs(here) - 1;
+        acc = __shfl_sync(0xFFFFFFFFu, sum, 31);
+      }
+      if (found < 0) found = __shfl_sync(0xFFFFFFFFu, last, l);  // rounding has left none
     }
-    found = __reduce_max_sync(0xFFFFFFFFu, found);
     last = __reduce_max_sync(0xFFFFFFFFu, last);
     if (lane == 0) {
-      if (found < 0 && !(target < 0.0)) found = last;  // past the last
-      if (found < 0)                                   // before the first (a negative number)
+      if (found < 0) found = last;  // past the last
+      if (found < 0)                // (what is left of the slice is none, token by token)
         for (found = 0; found < n - 1 && !(own[pad + found] > 0.f);) ++found;
       p.token[s] = v0 + found;
     }
