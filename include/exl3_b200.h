@@ -584,6 +584,11 @@ exl3_verdict exl3_attention_weight(const exl3_kv_cache *cache, int32_t layer, co
                                    const exl3_heads *q, float scale, const float *lse, float decay, void *stream,
                                    const exl3_kv_weight *weight);
 
+/* The weights' side of exl3_cache_keep (every layer; before it, where lens is the batch's context): the accepted rows' own
+ * weights move from slots context + path[d] to context + d.  Without a path there is nothing to move. */
+exl3_verdict exl3_weight_keep(const exl3_kv_cache *cache, const exl3_tree_batch *batch, const int32_t *path, int32_t depth,
+                              const int32_t *kept, void *stream, const exl3_kv_weight *weight);
+
 /* The host's page bookkeeping, on the device: how many rows refer to each page (none: free), each row's page ids (-1 past
  * its `held` pages), and its tokens. */
 typedef struct exl3_page_state {

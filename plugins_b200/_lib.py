@@ -43,7 +43,7 @@ EXPORTS = (
     "exl3_model_weight", "exl3_model_linear", "exl3_model_linears", "exl3_model_mlp", "exl3_model_experts", "exl3_resident", "exl3_resident_pending",
     "exl3_kv_register", "exl3_qk_norm_rope", "exl3_tree_attention", "exl3_cache_fork", "exl3_cache_grow",
     "exl3_cache_keep", "exl3_cache_compact", "exl3_draft_verify", "exl3_attention_weight",
-    "exl3_cache_evict",
+    "exl3_cache_evict", "exl3_weight_keep",
 )
 
 
@@ -353,6 +353,9 @@ def lib() -> ctypes.CDLL:
             L.exl3_cache_evict.restype = Verdict
             L.exl3_cache_evict.argtypes = [P(KvCache), P(PageState), P(KvWeight), ctypes.c_void_p, ctypes.c_int32,
                                            ctypes.c_int32, ctypes.c_void_p, P(PageState), P(KvWeight), ctypes.c_void_p]
+            L.exl3_weight_keep.restype = Verdict
+            L.exl3_weight_keep.argtypes = [P(KvCache), P(TreeBatch), ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p,
+                                           ctypes.c_void_p, P(KvWeight)]
             L.exl3_draft_verify.restype = Verdict
             L.exl3_draft_verify.argtypes = [P(KvCache), P(TreeBatch), P(Draft), ctypes.c_void_p, ctypes.c_void_p,
                                             ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p]

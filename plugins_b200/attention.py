@@ -1,14 +1,17 @@
-"""A layer's attention side over a paged key/value cache: what runs between its q|k|v linears and its o linear.
+"""A layer's attention side over a paged key/value cache: what runs between its q|k|v linears and its o linear, and what
+ends a step after the last layer.
 
     cache = A.KvCache.empty(layers=36, pages=4096, page_size=64, kv_heads=8, head_dim=128, dtype=torch.bfloat16)
     batch = A.TreeBatch(row_start, context, table, max_rows=..., tree=bits, position=pos)     # once per step
     for layer in ...:
         q = A.qk_norm_rope(cache, layer, batch, q, k, v, rope)      # norms, rotation, k and v into the cache
         o = A.tree_attention(cache, layer, batch, q)                # one token, a drafted tree, or a prompt chunk
+    path, kept, token = A.draft_verify(cache, batch, logits, tokens, parent, uniform, temperature)
     lens = A.cache_keep(cache, batch, path, kept)                   # the accepted path stays
 
-and the pages between steps: :func:`cache_fork` (fork, reorder, free), :func:`cache_grow` (new pages, copy on write) and
-:func:`cache_compact`.  Every call goes through the C ABI (include/exl3_b200.h says what each computes) on the current
+and the pages between steps: :func:`cache_fork` (fork, reorder, free), :func:`cache_grow` (new pages, copy on write),
+:func:`cache_compact`, and :func:`cache_evict`, which keeps a row's tokens inside a budget by how much they were attended to
+(:func:`attention_weight`, after each layer's attention).  Every call goes through the C ABI (include/exl3_b200.h says what each computes) on the current
 torch stream or ``stream``; refusals raise :class:`Exl3Error`.
 """
 from __future__ import annotations
@@ -404,10 +407,10 @@ def cache_grow(cache: KvCache, state: PageState, need, out: PageState | None = N
     return out, missing
 
 
-def cache_keep(cache: KvCache, batch: TreeBatch, path, kept, out=None, stream=None):
+def cache_keep(cache: KvCache, batch: TreeBatch, path, kept, out=None, stream=None, weight=None):
     """The accepted rows of each drafted tree, ``path[s][:kept[s]]`` (int32 [nseq, depth], ascending; None: the first
     kept rows), moved behind the context in every layer -> the sequences' new lengths, context + kept (``out`` may be the
-    batch's own context tensor)."""
+    batch's own context tensor).  ``weight`` ([layers, nseq, kv_heads, slots]): the rows' weights move likewise, first."""
     _ints(kept, (batch.nseq,), "kept", cache.device)
     _ints(path, (batch.nseq, None), "path", cache.device, optional=True)
     if out is None:
@@ -419,6 +422,12 @@ def cache_keep(cache: KvCache, batch: TreeBatch, path, kept, out=None, stream=No
     if stream is not None:
         _used_on(stream, path, kept, out, cache.k, cache.v, *batch._keep)
     batch._for(cache, batch.rows)
+    if weight is not None:
+        raw = L.KvWeight(*_kv_weight(weight, cache.raw.layers, batch.nseq, cache))
+        if stream is not None:
+            _used_on(stream, weight)
+        check(L.lib().exl3_weight_keep(cache.raw, batch.raw, None if path is None else path.data_ptr(),
+                                       0 if path is None else path.shape[1], kept.data_ptr(), _on(stream, cache._index), raw))
     check(L.lib().exl3_cache_keep(cache.raw, batch.raw, None if path is None else path.data_ptr(),
                                   0 if path is None else path.shape[1], kept.data_ptr(), _on(stream, cache._index),
                                   out.data_ptr()))

@@ -476,6 +476,32 @@ exl3_verdict exl3_cache_keep(const exl3_kv_cache* cache, const exl3_tree_batch* 
   return launched(exl3::launch_cache_keep(p, ws.counter_count, static_cast<cudaStream_t>(stream)));
 }
 
+exl3_verdict exl3_weight_keep(const exl3_kv_cache* cache, const exl3_tree_batch* batch, const int32_t* path, int32_t depth,
+                              const int32_t* kept, void* stream, const exl3_kv_weight* weight) {
+  exl3_verdict r = check_cache(cache);
+  if (r.code != EXL3_OK || (r = check_batch(batch)).code != EXL3_OK) return r;
+  int64_t bytes = 0;
+  if ((r = check_weight(weight, cache->layers, batch->nseq, cache->kv_heads, &bytes)).code != EXL3_OK) return r;
+  if (batch->nseq == 0) return kOk;
+  if (!kept) return refuse(EXL3_FAILED, "exl3_b200: keep without its arrays");
+  if (path && depth < 1) return refuse(EXL3_FAILED, "exl3_b200: a path without depth");
+  const int64_t n = batch->nseq * 4ll;
+  if (meet(weight->data, bytes, path, n * depth) || meet(weight->data, bytes, kept, n) || meet(weight->data, bytes, batch->context, n) ||
+      meet(weight->data, bytes, batch->row_start, n + 4))
+    return refuse(EXL3_FAILED, "exl3_b200: the weights lie over the call's arguments");
+  if (!path) return kOk;
+  exl3::Workspace ws;
+  if (!exl3::workspace_get(cache->device, ws)) return kNoWorkspace;
+  OnDevice guard(cache->device);
+  exl3::WeightKeepParams p{};
+  p.row_start = batch->row_start, p.context = batch->context, p.path = path, p.kept = kept;
+  p.rows = batch->rows, p.depth = depth, p.nseq = batch->nseq, p.layers = cache->layers, p.kv_heads = cache->kv_heads;
+  p.slots = weight->slots, p.w = weight->data;
+  p.w_layer = weight->layer_stride, p.w_row = weight->row_stride, p.w_head = weight->head_stride;
+  p.err = ws.err;
+  return launched(exl3::launch_weight_keep(p, static_cast<cudaStream_t>(stream)));
+}
+
 exl3_verdict exl3_cache_evict(const exl3_kv_cache* cache, const exl3_page_state* in, const exl3_kv_weight* weight,
                               const int32_t* budget, int32_t sink, int32_t recent, void* stream,
                               const exl3_page_state* out, const exl3_kv_weight* kept_weight, int32_t* missing) {

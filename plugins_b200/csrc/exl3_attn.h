@@ -132,6 +132,14 @@ struct EvictParams {
   int32_t sink, recent;
   uint32_t* err;
 };
+struct WeightKeepParams {
+  const int32_t *row_start, *context, *path, *kept;
+  int32_t rows, depth, nseq, layers, kv_heads, slots;
+  float* w;
+  int64_t w_layer, w_row, w_head;
+  uint32_t* err;
+};
+cudaError_t launch_weight_keep(const WeightKeepParams& p, cudaStream_t st);
 cudaError_t launch_evict_pages(const PageParams& p, cudaStream_t st);
 cudaError_t launch_evict_tokens(const EvictParams& p, cudaStream_t st);
 

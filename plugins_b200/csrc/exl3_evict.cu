@@ -216,6 +216,26 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const EvictParams p)
   while (done < found) move();
 }
 
+// A thread per layer and kv head of one sequence walks the path, which ascends: a weight is read before its slot is written.
+// A few hundred words in all; the launch is what it costs.
+__global__ void __launch_bounds__(256) weight_keep_kernel(const WeightKeepParams p) {
+  pdl_wait();
+  const int s = static_cast<int>(blockIdx.y), item = static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x);
+  const int ctx = p.context[s], kept = p.kept[s];
+  const int ntok = max(0, min(p.row_start[s + 1], p.rows) - max(p.row_start[s], 0));
+  const int32_t* path = p.path + static_cast<int64_t>(s) * p.depth;
+  bool ok = ctx >= 0 && kept >= 0 && kept <= min(ntok, p.depth) && static_cast<int64_t>(ctx) + ntok <= p.slots;
+  for (int d = 0; ok && d < kept; ++d) ok = path[d] < ntok && path[d] >= (d ? path[d - 1] + 1 : 0);
+  if (!ok) {
+    if (item == 0) atomicOr(p.err, kErrBadShape);
+    return;
+  }
+  if (item >= p.layers * p.kv_heads) return;
+  float* w = p.w + item / p.kv_heads * p.w_layer + s * p.w_row + item % p.kv_heads * p.w_head + ctx;
+  for (int d = 0; d < kept; ++d)
+    if (path[d] != d) w[d] = w[path[d]];
+}
+
 template <int D>
 cudaError_t launch_dim(const EvictParams& p, cudaStream_t st) {
   const int64_t units = static_cast<int64_t>(p.nseq) * p.pool.layers * p.pool.kv_heads;
@@ -223,6 +243,11 @@ cudaError_t launch_dim(const EvictParams& p, cudaStream_t st) {
 }
 
 }  // namespace
+
+cudaError_t launch_weight_keep(const WeightKeepParams& p, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(p.layers) * p.kv_heads + 255) / 256), static_cast<unsigned>(p.nseq));
+  return launch_pdl_k(weight_keep_kernel, grid, dim3(256), st, p);
+}
 
 cudaError_t launch_evict_tokens(const EvictParams& p, cudaStream_t st) {
   switch (p.pool.dim) {

@@ -55,6 +55,21 @@ def test_weights_over_the_page_state_are_refused():
         refused(evict(kept=weights(data=at)), L.EXL3_FAILED, "over the page state")
 
 
+def test_keeping_weights_is_refused_by_name():
+    from test_attention_cpu import batch
+    keep = (lambda c=None, b=None, path=40 * AT, depth=3, kept=41 * AT, w=None:
+            L.lib().exl3_weight_keep(c or cache(device=99), b or batch(nseq=2), path, depth, kept, None, w or weights()))
+    refused(keep(), L.EXL3_FAILED, "exl3_kv_register")
+    refused(keep(c=cache(size=1)), L.EXL3_FAILED, "not a key/value cache")
+    refused(keep(b=batch(size=1)), L.EXL3_FAILED, "not a batch")
+    refused(keep(w=weights(nseq=1)), L.EXL3_FAILED, "other layers or rows")
+    refused(keep(kept=None), L.EXL3_FAILED, "without its arrays")
+    refused(keep(depth=0), L.EXL3_FAILED, "without depth")
+    for at in (40 * AT, 41 * AT, AT):
+        refused(keep(w=weights(data=at)), L.EXL3_FAILED, "over the call's arguments")
+    assert keep(path=None).ok and keep(b=batch(nseq=0, rows=0, max_rows=0), w=weights(nseq=0)).ok
+
+
 def test_the_plain_eviction():
     w = [0.5, 3.0, math.nan, 0.0, 3.0, 1.0, 2.0, 0.0]
     assert E.kept_slots(w, 8, 3, 0, 0) == [1, 2, 4]
