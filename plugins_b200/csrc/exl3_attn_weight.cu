@@ -88,8 +88,18 @@ struct WtLine : WorkLine {
   }
   __device__ __forceinline__ static int64_t tiles_of_head(const WeightParams& p, const WtItem& it) {
     int64_t t = static_cast<int64_t>(it.nblocks) * it.row_tiles;
-    if (!p.a.b.tree && it.row_tiles > 1)
-      for (int b = it.s.context / S::KB; b < it.nblocks; ++b) t -= first_of(p, it, b);
+    if (p.a.b.tree || it.row_tiles == 1) return t;
+    // first_of for the blocks past the context, kept as quotient and remainder
+    int b = it.s.context / S::KB + 1;
+    const int64_t x = (static_cast<int64_t>(b) * S::KB - it.s.context) * p.a.group;
+    int64_t q = divide(x, p.row_tile);
+    int r = static_cast<int>(x - q * p.row_tile);
+    const int dq = S::KB * p.a.group / p.row_tile, dr = S::KB * p.a.group % p.row_tile;
+    for (; b < it.nblocks; ++b) {
+      t -= q;
+      q += dq, r += dr;
+      if (r >= p.row_tile) ++q, r -= p.row_tile;
+    }
     return t;
   }
   __device__ __forceinline__ int64_t seq_tiles(const WeightParams& p, int s) const {
