@@ -569,7 +569,7 @@ exl3_verdict exl3_tree_attention(const exl3_kv_cache *cache, int32_t layer, cons
 typedef struct exl3_kv_weight {
   uint32_t size;   /* sizeof(exl3_kv_weight) */
   int32_t layers, nseq;
-  int32_t slots;   /* >= 1 */
+  int32_t slots;   /* 1 .. 2^30 */
   float *data;     /* device, [layers][nseq][kv_heads][slots] */
   int64_t layer_stride, row_stride, head_stride;
 } exl3_kv_weight;

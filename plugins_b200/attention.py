@@ -450,6 +450,8 @@ def cache_evict(cache: KvCache, state: PageState, weight, budget, sink: int = 0,
     moved together in their order -> (the new state, ``missing``: an int32 scalar tensor, 0, or the free pages lacking to part
     from shared ones: then nothing changed).  The tokens' weights move with them, in place or to ``weight_out``."""
     n = state.raw.nseq
+    if not (0 <= sink < 1 << 31 and 0 <= recent < 1 << 31):
+        _refuse("counts of tokens that always stay are not negative")
     _ints(budget, (n,), "budget", cache.device)
     raw = L.KvWeight(*_kv_weight(weight, cache.raw.layers, n, cache))
     kept = raw if weight_out is None else L.KvWeight(*_kv_weight(weight_out, cache.raw.layers, n, cache))
@@ -505,7 +507,9 @@ def draft_verify(cache: KvCache, batch: TreeBatch, logits, tokens, parent, unifo
     _floats(uniform, (rows, 2), "uniform", i)
     if temperature is not None:
         _floats(temperature, (n,), "temperature", i)
-    depth = max(1, batch.raw.max_rows if depth is None else int(depth))
+    depth = max(1, batch.raw.max_rows) if depth is None else int(depth)
+    if depth < 1:
+        _refuse("a path without depth")
     make = _maker(stream, torch.empty)
     if path is None and kept is None and token is None:  # one allocation
         path, kept, token = make(n * (depth + 2), dtype=torch.int32, device=dev).split_with_sizes((n * depth, n, n))

@@ -249,6 +249,7 @@ exl3_verdict check_weight(const exl3_kv_weight* w, int32_t layers, int32_t nseq,
   if (!w || w->size != sizeof(exl3_kv_weight)) return refuse(EXL3_FAILED, "exl3_b200: not a cache's weights");
   if (w->layers != layers || w->nseq != nseq) return refuse(EXL3_FAILED, "exl3_b200: the weights have other layers or rows");
   if (w->slots < 1) return refuse(EXL3_FAILED, "exl3_b200: weights without slots");
+  if (w->slots > (1 << 30)) return refuse(EXL3_TOO_LARGE, "exl3_b200: weights of more than 2^30 slots");
   if (nseq > 0 && !w->data) return refuse(EXL3_FAILED, "exl3_b200: not a cache's weights");
   if (reinterpret_cast<uintptr_t>(w->data) % 4) return refuse(EXL3_UNSUPPORTED, "exl3_b200: weights lie on multiples of 4 bytes");
   std::pair<int64_t, int64_t> dims[3] = {{w->head_stride, kv_heads}, {w->row_stride, nseq}, {w->layer_stride, layers}};

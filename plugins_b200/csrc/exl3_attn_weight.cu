@@ -697,7 +697,7 @@ cudaError_t launch_dim(const WeightParams& params, int sms, size_t partial_float
   p.row_tile = p.a.group <= S::RT ? S::RT / p.a.group * p.a.group : S::RT;
   CUtensorMap qmap = kmap;
   if (p.a.q.vec && p.a.group <= S::RT) {
-    const int tokens = S::RT / p.a.group < p.a.max_rows ? S::RT / p.a.group : p.a.max_rows;
+    const int tokens = S::RT / p.a.group;
     if (q_tensor_map(qmap, p.a, D, tokens)) p.box_tokens = tokens;
   }
   const int64_t tiles = static_cast<int64_t>(p.a.b.nseq) * p.a.b.kv_heads * ((p.a.max_context + S::KB - 1) / S::KB) *

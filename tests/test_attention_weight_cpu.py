@@ -38,7 +38,7 @@ def test_what_is_served_fails_for_want_of_a_workspace_alone():
     (dict(size=0), L.EXL3_FAILED, "not a cache's weights"), (dict(data=None), L.EXL3_FAILED, "not a cache's weights"),
     (dict(layers=2), L.EXL3_FAILED, "other layers or rows"), (dict(nseq=2), L.EXL3_FAILED, "other layers or rows"),
     (dict(slots=0), L.EXL3_FAILED, "without slots"), (dict(data=500 * AT + 2), L.EXL3_UNSUPPORTED, "multiples of 4"),
-    (dict(head_stride=99), L.EXL3_FAILED, "overlap"), (dict(head_stride=0), L.EXL3_FAILED, "overlap"),
+    (dict(slots=(1 << 30) + 1), L.EXL3_TOO_LARGE, "2^30"), (dict(head_stride=99), L.EXL3_FAILED, "overlap"), (dict(head_stride=0), L.EXL3_FAILED, "overlap"),
     (dict(head_stride=-100), L.EXL3_FAILED, "overlap"),
 ])
 def test_weights_are_refused_by_name(kw, code, text):

@@ -190,6 +190,20 @@ def test_the_bits_do_not_depend_on_the_bounds_and_captures_replay(A):
     assert torch.equal(w, fresh) and bool((w[1] == 1).all()) and bool((w[0, :, 502:] == 1).all())
 
 
+@pytest.mark.parametrize("rows", [(9, 3), (40, 130)])
+def test_a_bound_on_the_rows_that_is_too_low_costs_time_alone(A, rows):
+    step = Step(list(rows), [100, 300], 2, 128, 16, "bf16")
+    cache, batch = step.device(A, rows=sum(rows))
+    q = queries(step, 8, 128)
+    _, lse = A.tree_attention(cache, step.layer, batch, q, lse=True)
+    old = old_weights(step, 2, 440)
+    want, off = E.weights(step.k[step.layer], q.cpu(), lse.cpu(), step.row_start, step.lens, step.table, 128 ** -0.5, 1.0, old)
+    for most in (1, 2, 5):
+        batch.raw.max_rows = most
+        w = A.attention_weight(cache, step.layer, batch, q, lse, old.cuda())
+        assert bool(((w.cpu().double() - want).abs() <= off).all())
+
+
 def test_another_stream_and_padding_rows(A):
     step = Step([3, 2], [200, 40], 2, 128, 16, "bf16")
     cache, batch = step.device(A, rows=5)

@@ -278,3 +278,20 @@ def test_values_out_of_range_are_recorded_and_not_followed():
     batch._keep[0].copy_(torch.tensor([-3, 5, 400], dtype=torch.int32))
     A.draft_verify(cache, batch, *args, **kw)
     assert Q.device_error(0, clear=True) != 0
+
+
+def test_arguments_the_wrappers_refuse():
+    from plugins_b200 import attention as A
+    i = setup([3, 2], 2, 300, "f32", "f16", [0.9], seed=14)
+    cache, batch, args, kw = make(i)
+    logits, tokens, parent, uniform = args
+    bad = [dict(logits=logits[:, ::2]), dict(logits=logits.cpu()), dict(logits=logits[:3]), dict(logits=logits.double()),
+           dict(logits=logits.int()), dict(tokens=tokens.long()), dict(tokens=tokens[:2]), dict(parent=parent.float()),
+           dict(uniform=uniform[:, :1]), dict(uniform=uniform.double()), dict(uniform=uniform.t().contiguous().t()),
+           dict(temperature=kw["temperature"][:1]), dict(temperature=kw["temperature"].half()),
+           dict(draft=kw["draft"][:, :200]), dict(draft=kw["draft"].long()), dict(depth=0), dict(depth=-3),
+           dict(path=torch.zeros((2, 4), dtype=torch.int32, device="cuda"), depth=3), dict(kept=torch.zeros(2, device="cuda"))]
+    for change in bad:
+        call = dict(logits=logits, tokens=tokens, parent=parent, uniform=uniform) | kw | change
+        with pytest.raises(A.Exl3Error):
+            A.draft_verify(cache, batch, **call)

@@ -257,3 +257,25 @@ def test_slots_past_two_to_the_31_elements(A):
     for t, old in zip((k, v), was):
         assert torch.equal(t[0, new.table[0].long()[at // page], 0, at % page], old[keep])
     assert new.held.tolist() == [2] and int(missing) == 0
+
+
+def test_arguments_the_wrappers_refuse(A):
+    c = Case([100, 40], [50, 20])
+    cache, st, w = c.cache(A), c.state(A), c.w.cuda()
+    budget = torch.tensor(c.budget, dtype=torch.int32).cuda()
+    k0 = cache.k.clone()
+    for change in (dict(weight=w[:1]), dict(weight=w[:, :1]), dict(weight=w.double()), dict(weight=w.cpu()), dict(weight=w[0]),
+                   dict(weight=w[..., ::2]), dict(weight_out=w[..., :50]), dict(budget=budget.long()), dict(budget=budget[:1]),
+                   dict(sink=-1), dict(recent=-5), dict(recent=2 ** 32 + 5), dict(sink=2 ** 31),
+                   dict(weight_out=w.flatten()[:w[..., 1:].numel()].view_as(w[..., 1:])), dict(out=st)):
+        call = dict(weight=w, budget=budget) | change
+        with pytest.raises(A.Exl3Error):
+            A.cache_evict(cache, st, **call)
+    lse, q = torch.zeros((2, 4), device="cuda"), torch.zeros((2, 4, 64), dtype=torch.float16, device="cuda")
+    batch = A.TreeBatch(*(torch.tensor(x, dtype=torch.int32).cuda() for x in ([0, 1, 2], [100, 40], c.state(A).table.tolist())), max_rows=1, rows=2)
+    for change in (dict(weight=w), dict(weight=w[0, :1]), dict(weight=w[0].half()), dict(lse=lse[:1]), dict(lse=lse.double()),
+                   dict(lse=lse.t().contiguous().t()), dict(decay=1.5), dict(decay=-0.5), dict(scale=-1.0), dict(q=q.float()), dict(layer=2)):
+        call = dict(layer=0, q=q, lse=lse, weight=w[0]) | change
+        with pytest.raises(A.Exl3Error):
+            A.attention_weight(cache, batch=batch, **call)
+    assert torch.equal(cache.k, k0)
