@@ -98,7 +98,7 @@ class _Calls:
 
 class _StepCalls:
     """Likewise the calls that end a step (exl3_kv_weight and exl3_draft as bytes)."""
-    weight = verify = None
+    weight = evict = verify = None
 
     @classmethod
     def load(cls) -> None:
@@ -106,6 +106,8 @@ class _StepCalls:
         lib = L.lib()
         proto = ctypes.CFUNCTYPE(L.Verdict, p, i, p, c, f, p, f, p, c)
         cls.weight = proto(ctypes.cast(lib.exl3_attention_weight, p).value)
+        proto = ctypes.CFUNCTYPE(L.Verdict, p, p, c, p, i, i, p, p, c, p)
+        cls.evict = proto(ctypes.cast(lib.exl3_cache_evict, p).value)
         proto = ctypes.CFUNCTYPE(L.Verdict, p, p, c, p, p, i, p, p)
         cls.verify = proto(ctypes.cast(lib.exl3_draft_verify, p).value)  # last, as above
 
@@ -453,8 +455,8 @@ def cache_evict(cache: KvCache, state: PageState, weight, budget, sink: int = 0,
     if not (0 <= sink < 1 << 31 and 0 <= recent < 1 << 31):
         _refuse("counts of tokens that always stay are not negative")
     _ints(budget, (n,), "budget", cache.device)
-    raw = L.KvWeight(*_kv_weight(weight, cache.raw.layers, n, cache))
-    kept = raw if weight_out is None else L.KvWeight(*_kv_weight(weight_out, cache.raw.layers, n, cache))
+    raw = _KV_WEIGHT.pack(*_kv_weight(weight, cache.raw.layers, n, cache))
+    kept = raw if weight_out is None else _KV_WEIGHT.pack(*_kv_weight(weight_out, cache.raw.layers, n, cache))
     out = _states(cache, state, out, stream)
     if missing is None:
         missing = _maker(stream, torch.empty)((), dtype=torch.int32, device=cache.device)
@@ -462,8 +464,8 @@ def cache_evict(cache: KvCache, state: PageState, weight, budget, sink: int = 0,
         _ints(missing, (), "missing", cache.device)
     if stream is not None:
         _used_on(stream, budget, missing, weight, weight_out, cache.k, cache.v, *state._tensors(), *out._tensors())
-    check(L.lib().exl3_cache_evict(cache.raw, state.raw, raw, budget.data_ptr(), sink, recent, _on(stream, cache._index),
-                                   out.raw, kept, missing.data_ptr()))
+    _check(_StepCalls.evict(cache._at, ctypes.addressof(state.raw), raw, budget.data_ptr(), sink, recent,
+                            _on(stream, cache._index), ctypes.addressof(out.raw), kept, missing.data_ptr()))
     return out, missing
 
 
@@ -502,8 +504,10 @@ def draft_verify(cache: KvCache, batch: TreeBatch, logits, tokens, parent, unifo
     dt = _vocab_rows(logits, rows, None, "logits", i)
     vocab = logits.shape[1]
     qt = L.F32 if draft is None else _vocab_rows(draft, rows, vocab, "draft", i)
-    _ints(tokens, (rows,), "tokens", dev)
-    _ints(parent, (rows,), "parent", dev, optional=True)
+    for t, what in ((tokens, "tokens"), (parent, "parent")):
+        # (the common case at a glance; the other says what is wrong, or that there are no parents)
+        if t is None or t.dtype != torch.int32 or t.shape != (rows,) or t.get_device() != i or not t.is_contiguous():
+            _ints(t, (rows,), what, dev, optional=what == "parent")
     _floats(uniform, (rows, 2), "uniform", i)
     if temperature is not None:
         _floats(temperature, (n,), "temperature", i)
