@@ -553,7 +553,7 @@ exl3_verdict exl3_cache_evict(const exl3_kv_cache* cache, const exl3_page_state*
   e.w_out = kept_weight->data;
   e.out_layer = kept_weight->layer_stride, e.out_row = kept_weight->row_stride, e.out_head = kept_weight->head_stride;
   e.sink = sink, e.recent = recent, e.err = ws.err;
-  return launched(exl3::launch_evict_tokens(e, st));
+  return launched(exl3::launch_evict_tokens(e, ws.sms, st));
 }
 
 exl3_verdict exl3_draft_verify(const exl3_kv_cache* cache, const exl3_tree_batch* batch, const exl3_draft* draft,

@@ -141,7 +141,7 @@ struct WeightKeepParams {
 };
 cudaError_t launch_weight_keep(const WeightKeepParams& p, cudaStream_t st);
 cudaError_t launch_evict_pages(const PageParams& p, cudaStream_t st);
-cudaError_t launch_evict_tokens(const EvictParams& p, cudaStream_t st);
+cudaError_t launch_evict_tokens(const EvictParams& p, int sms, cudaStream_t st);
 
 constexpr int kDraftMaxRows = 1024;     // rows of one sequence
 constexpr int kDraftMaxVocab = 393216;  // a slice of an eighth, as f32, fits in shared memory

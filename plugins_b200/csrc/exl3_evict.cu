@@ -18,10 +18,7 @@ namespace exl3 {
 
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
 constexpr int kPer = 4;                    // slots of a thread in a run
-constexpr int kRun = kThreads * kPer;
 constexpr int kBins = 2048;
 constexpr int kAhead = 4;                  // tokens of a thread in flight
 
@@ -33,6 +30,7 @@ __device__ __forceinline__ uint32_t key_of(float w) {
 }
 
 // Exclusive scan of a pair of 16-bit counts over the CTA; *total receives the sum.
+template <int kWarps>
 __device__ __forceinline__ uint32_t scan_pair(uint32_t v, uint32_t* s_warp, uint32_t* total) {
   const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
   uint32_t x = v;
@@ -54,17 +52,19 @@ __device__ __forceinline__ uint32_t scan_pair(uint32_t v, uint32_t* s_warp, uint
   return before + x - v;
 }
 
+template <int kThreads>
 struct Shared {
+  static constexpr int kRing = kThreads * kPer + 512;
   uint32_t hist[kBins];
-  uint32_t warp[2][kWarps];
-  uint32_t digit, above;
-  int slot[kRun + 1024], page[kRun + 1024];  // tokens that stay and have not moved: old slots and their pages, a ring
+  uint32_t warp[2][kThreads / 32];
+  uint32_t digit, above, inside;
+  int slot[kRing], page[kRing];  // tokens that stay and have not moved: old slots and their pages, a ring
 };
-constexpr int kRing = kRun + 1024;
 
 // The key of the n-th heaviest of the slots [lo, hi) (n of at least 1 and fewer than there are), and how many of its equals
 // stay.
-__device__ void select_key(const float* w, int lo, int hi, int n, Shared& s, uint32_t& key, int& equals) {
+template <int kThreads>
+__device__ void select_key(const float* w, int lo, int hi, int n, Shared<kThreads>& s, uint32_t& key, int& equals) {
   uint32_t prefix = 0, mask = 0;
   int left = n;
 #pragma unroll 1
@@ -98,20 +98,25 @@ __device__ void select_key(const float* w, int lo, int hi, int n, Shared& s, uin
     if (before < static_cast<uint32_t>(left) && upto >= static_cast<uint32_t>(left)) {
       int i = 0;
       while (before + s.hist[top - i] < static_cast<uint32_t>(left)) before += s.hist[top - i], ++i;
-      s.digit = top - i, s.above = before;
+      s.digit = top - i, s.above = before, s.inside = s.hist[top - i];
     }
     __syncthreads();
     left -= static_cast<int>(s.above);
     prefix |= s.digit << shift;
     mask |= static_cast<uint32_t>(bins - 1) << shift;
+    if (static_cast<int>(s.inside) == left && prefix != 0u) {  // the whole digit stays
+      key = prefix - 1u, equals = 0;
+      return;
+    }
   }
   key = prefix;
   equals = left;
 }
 
-template <int D>
-__global__ void __launch_bounds__(kThreads, 2) evict_kernel(const EvictParams p) {
-  __shared__ Shared s;
+template <int D, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) evict_kernel(const EvictParams p) {
+  constexpr int kRun = kThreads * kPer, kRing = Shared<kThreads>::kRing;
+  __shared__ Shared<kThreads> s;
   pdl_wait();
   const int tid = static_cast<int>(threadIdx.x);
   const int head = static_cast<int>(blockIdx.x) % p.pool.kv_heads;
@@ -132,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const EvictParams p)
   if (want > 0) select_key(w, lo, hi, want, s, key, equals);
 
   constexpr int kLanes = D / 8, kTokens = kThreads / kLanes, kGroup = kTokens * kAhead;
-  static_assert(kGroup <= 1024, "what is left in the ring");
+  static_assert(kGroup <= 512, "what is left in the ring");
   const int c = tid % kLanes, g = tid / kLanes;
   const int64_t base = layer * p.pool.layer_stride + head * p.pool.head_stride + c * 8;
   const int32_t* from = p.table_in + static_cast<int64_t>(row) * p.width;
@@ -192,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const EvictParams p)
       mine += pair[i];
     }
     uint32_t total;
-    uint32_t before = scan_pair(mine, s.warp[turn++ & 1u], &total);
+    uint32_t before = scan_pair<kThreads / 32>(mine, s.warp[turn++ & 1u], &total);
     // (its barrier: all of the run's weights are read)
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -237,9 +242,14 @@ __global__ void __launch_bounds__(256) weight_keep_kernel(const WeightKeepParams
 }
 
 template <int D>
-cudaError_t launch_dim(const EvictParams& p, cudaStream_t st) {
+cudaError_t launch_dim(const EvictParams& p, int sms, cudaStream_t st) {
   const int64_t units = static_cast<int64_t>(p.nseq) * p.pool.layers * p.pool.kv_heads;
-  return launch_pdl_k(evict_kernel<D>, dim3(static_cast<unsigned>(units)), dim3(kThreads), st, p);
+  // Smaller CTAs where there are many: more of them hide one another's selections (4608 rows of 300-1300 slots: 512 threads
+  // 335 us, 256 threads 307); larger ones where a few have to move much each (960 rows of 0.9-4k slots: 262 / 272; 192 rows of
+  // 30-40k: 216 / 292).
+  const auto grid = dim3(static_cast<unsigned>(units));
+  return units >= 16 * static_cast<int64_t>(sms) ? launch_pdl_k(evict_kernel<D, 256>, grid, dim3(256), st, p)
+                                                 : launch_pdl_k(evict_kernel<D, 512>, grid, dim3(512), st, p);
 }
 
 }  // namespace
@@ -249,11 +259,11 @@ cudaError_t launch_weight_keep(const WeightKeepParams& p, cudaStream_t st) {
   return launch_pdl_k(weight_keep_kernel, grid, dim3(256), st, p);
 }
 
-cudaError_t launch_evict_tokens(const EvictParams& p, cudaStream_t st) {
+cudaError_t launch_evict_tokens(const EvictParams& p, int sms, cudaStream_t st) {
   switch (p.pool.dim) {
-    case 64: return launch_dim<64>(p, st);
-    case 128: return launch_dim<128>(p, st);
-    default: return launch_dim<256>(p, st);
+    case 64: return launch_dim<64>(p, sms, st);
+    case 128: return launch_dim<128>(p, sms, st);
+    default: return launch_dim<256>(p, sms, st);
   }
 }
 

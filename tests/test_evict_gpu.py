@@ -69,10 +69,9 @@ class Case:
         assert new.lens.tolist() == lens and new.held.tolist() == held and new.refs.tolist() == refs
         for got, row in zip(new.table.tolist(), table):
             assert got == [p for p in row if p >= 0] + [-1] * (self.width - sum(p >= 0 for p in row))
+        bits = (lambda t: t.cpu().contiguous().view({2: torch.int16, 4: torch.int32}[t.element_size()]))  # (NaN compares too)
         if not in_place:
-            assert torch.equal(w.cpu(), self.w)
-        # as bits, so that NaN compares too; a cut row's own slots past its new length are free to hold anything
-        bits = (lambda t: t.cpu().contiguous().view({2: torch.int16, 4: torch.int32}[t.element_size()]))
+            assert torch.equal(bits(w), bits(self.w))
         assert torch.equal(bits(w if in_place else out), bits(w2))
         assert torch.equal(bits(cache.k), bits(k)) and torch.equal(bits(cache.v), bits(v))
         # what was read stays as it was
@@ -144,6 +143,18 @@ def test_page_bookkeeping_of_many_rows(A):
     r = random.Random(1)
     lens = [r.randrange(0, 60) for _ in range(1500)]
     Case(lens, [r.randrange(0, 50) for _ in lens], sink=1, recent=2, layers=1, kv_heads=1, seed=1).check(A)
+
+
+@pytest.mark.parametrize("dim,in_place", [(64, True), (128, False), (256, True)])
+def test_many_rows_of_layers_and_heads(A, dim, in_place):
+    """2560 of them, which take smaller blocks: two rows of several runs among many short ones."""
+    r = random.Random(dim)
+    lens = [1500, 1030, 1024, 1025] + [r.randrange(0, 60) for _ in range(36)]
+    odd = (lambda w: torch.where(w > 20, torch.nan, (w * 4).floor() / 4))  # many equals
+    c = Case(lens, [700, 40, 500, 1024] + [r.randrange(0, 50) for _ in range(36)], sink=2, recent=3, layers=8, kv_heads=8, dim=dim,
+             weight=odd if dim == 128 else None, seed=dim)
+    assert 8 * 8 * len(c.lens) >= 16 * torch.cuda.get_device_properties(0).multi_processor_count
+    c.check(A, in_place)
 
 
 def test_tokens_can_be_evicted_again_and_grown(A):
