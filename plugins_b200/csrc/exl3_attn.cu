@@ -552,7 +552,7 @@ exl3_verdict exl3_cache_evict(const exl3_kv_cache* cache, const exl3_page_state*
   e.w = weight->data, e.w_layer = weight->layer_stride, e.w_row = weight->row_stride, e.w_head = weight->head_stride;
   e.w_out = kept_weight->data;
   e.out_layer = kept_weight->layer_stride, e.out_row = kept_weight->row_stride, e.out_head = kept_weight->head_stride;
-  e.sink = sink, e.recent = recent, e.err = ws.err;
+  e.sink = sink, e.recent = recent, e.slots = weight->slots, e.err = ws.err;
   return launched(exl3::launch_evict_tokens(e, ws.sms, st));
 }
 

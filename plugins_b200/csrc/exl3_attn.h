@@ -129,7 +129,7 @@ struct EvictParams {
   const float* w;               // [layers][nseq][kv_heads][slots]
   float* w_out;                 // may be w
   int64_t w_layer, w_row, w_head, out_layer, out_row, out_head;
-  int32_t sink, recent;
+  int32_t sink, recent, slots;
   uint32_t* err;
 };
 struct WeightKeepParams {

@@ -242,6 +242,23 @@ def test_rows_that_make_no_sense_are_recorded_and_left():
     assert torch.equal(cache.k[:, used], k0[:, used])
 
 
+def test_a_length_past_the_weights_slots_copies_what_there_is(A):
+    from plugins_b200 import quant as Q
+    c = Case([300, 90, 250], [100, 50, 100], seed=8, slots=260)
+    for far in (300, 2 ** 31 - 1, -5):
+        cache, st, w = c.cache(A), c.state(A), c.w.cuda()
+        st.lens[0] = far
+        whole = torch.full((2, 4, 2, 262), -7.0, device="cuda")  # the result lies inside
+        out = whole[:, :3, :, 1:261]
+        Q.device_error(0, clear=True)
+        new, missing = A.cache_evict(cache, st, w, torch.tensor(c.budget, dtype=torch.int32).cuda(), weight_out=out)
+        assert Q.device_error(0, clear=True) != 0
+        assert int(missing) == 0 and new.lens.tolist() == [far, 50, 100]
+        want = w[:, 0] if far > 0 else torch.full_like(w[:, 0], -7.0)
+        assert torch.equal(out[:, 0], want)
+        assert (whole[:, 3] == -7).all() and (whole[..., [0, 261]] == -7).all()
+
+
 def test_slots_past_two_to_the_31_elements(A):
     """A pool whose last pages lie beyond 2^31 elements; only what is used is looked at."""
     page, dim = 256, 256
