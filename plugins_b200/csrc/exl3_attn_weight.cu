@@ -18,6 +18,15 @@
 // per kv head than a tile has rows, are brought by two warps instead.  Heads up to 128 wide: an item is 256 keys, two groups per half
 // that take its row tiles by turns.  256 wide: 128 keys, all four by turns.
 //
+// A quarter of the exponentials are polynomials on the FMA pipe, beside the special-function unit (4096 rows on 4096 slots, an
+// eighth / a quarter / half of them: 245 / 235 / 271 us; a step earlier none took 265 where a quarter took 256).
+//
+// What bounds it: few rows, HBM (32 sequences' tokens over 1.5-9k slots 64 us in a graph, 5.5 TB/s; nine trees of 5-17 rows over
+// 6-16k 256-wide slots 73 us, 5.8 TB/s), the rest being the start and the line's cut; many rows, the summing warps' issue and
+// their special-function unit (a 4096-row chunk on 4096 slots 232 us, 0.89 PFLOP/s, against 127 us of products and 179 us of
+// exponentials at one unit's rate).  Two groups of summing warps took
+// 256 us there where four took 253; fetching the log-sum-exps a tile ahead then brought 233.
+//
 // Every mbarrier wait is bounded (wait_bar): one that gives up raises an abort flag that all roles poll.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -723,7 +732,7 @@ cudaError_t launch_dim(const WeightParams& params, int sms, size_t partial_float
 }  // namespace
 
 cudaError_t launch_attn_weight(const WeightParams& p, int dim, int sms, size_t partial_floats, cudaStream_t st) {
-  // blocks with room for 32 query rows leave it to the keys
+  // blocks with room for 32 query rows leave the rest to the keys (32 sequences' tokens: 66.3 us with room for 128, 64.5 us)
   const bool few = static_cast<int64_t>(p.a.max_rows) * p.a.group <= 32;
   switch (dim) {
     case 64: return (few ? launch_dim<64, true> : launch_dim<64, false>)(p, sms, partial_floats, st);
