@@ -10,8 +10,8 @@
 // later group's old ones: in place, nothing is overwritten before it is read.
 //
 // What bounds it: HBM while tokens move, every moved byte read and written once (16 rows of 300-1300 slots cut to 400-517 in 36
-// layers: 303 us, 1.69 GB, 5.6 TB/s; 20 forked rows in 12 layers: 262 us, 1.53 GB, 5.8 TB/s); with few long rows the chain of
-// one CTA (four rows of 30-40k slots cut to 4096 in 6 layers: 215 us, 0.84 GB, 3.9 TB/s; all but the moves 119 us of it).
+// layers: 297 us, 1.69 GB, 5.7 TB/s; 20 forked rows in 12 layers: 261 us, 1.53 GB, 5.9 TB/s); with few long rows the chain of
+// one CTA (four rows of 30-40k slots cut to 4096 in 6 layers: 195 us, 0.84 GB, 4.3 TB/s).
 #include <cuda_runtime.h>
 
 #include "exl3_attn.h"
@@ -24,7 +24,7 @@ namespace {
 
 constexpr int kPer = 4;                    // slots of a thread in a run
 constexpr int kBins = 2048;
-constexpr int kAhead = 4;                  // tokens of a thread in flight
+constexpr int kAhead = 4;                  // tokens of a thread in flight (two: 327 us where four take 297)
 
 // Weights as whole numbers of their order: -NaN .. NaN all at the top, -0 as 0.
 __device__ __forceinline__ uint32_t key_of(float w) {
@@ -76,7 +76,7 @@ __device__ void select_key(const float* w, int lo, int hi, int n, Shared<kThread
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : kBins;
     for (int i = static_cast<int>(threadIdx.x); i < bins; i += kThreads) s.hist[i] = 0u;
     __syncthreads();
-#pragma unroll 4
+#pragma unroll kThreads / 64  // (512 threads, long rows: 8 at a time 195 us, 4 199, 16 194; 256 threads: 4 297 us, 8 305)
     for (int j = lo + static_cast<int>(threadIdx.x); j < hi; j += kThreads) {
       const uint32_t k = key_of(w[j]);
       if ((k & mask) == prefix) atomicAdd(&s.hist[(k >> shift) & (bins - 1)], 1u);
@@ -148,8 +148,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) evict_kernel(const 
   const int32_t* from = p.table_in + static_cast<int64_t>(row) * p.width;
   const int32_t* to = p.table + static_cast<int64_t>(row) * p.width;
   const int page_mask = (1 << p.page_shift) - 1;
-  auto page_of = [&](const int32_t* table, int slot) {
-    const int id = table[slot >> p.page_shift];
+  auto page_of = [&](int id) {  // of a table's entry
     if (id >= 0 && id < p.pages) return id;
     atomicOr(p.err, kErrBadShape);
     return -1;
@@ -165,7 +164,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) evict_kernel(const 
       const int d = done + i * kTokens + g;
       dst[i] = -1;
       if (d < found) {
-        const int slot = s.slot[d % kRing], page = s.page[d % kRing], page2 = page_of(to, d);
+        const int slot = s.slot[d % kRing], page = s.page[d % kRing], page2 = page_of(to[d >> p.page_shift]);
         if (page >= 0 && page2 >= 0 && (slot != d || page != page2)) {
           const int64_t at = base + page * p.pool.page_stride + (slot & page_mask) * p.pool.token_stride;
           k[i] = *reinterpret_cast<const uint4*>(p.pool.k + at);
@@ -184,13 +183,27 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) evict_kernel(const 
     done += kGroup;
   };
   uint32_t turn = 0;
+  // A run's weights and pages, fetched a run ahead (what this run writes lies before the next: 4 rows of 30-40k slots 213 us,
+  // 198 so; 16 rows in 36 layers 301 / 292).  A thread's slots lie in one page.
+  float next[kPer];
+  int next_id;
+  auto fetch = [&](int j0) {
+    const int j = j0 + tid * kPer;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) next[i] = j + i < len ? w[j + i] : 0.f;
+    next_id = j < len ? from[j >> p.page_shift] : 0;
+  };
+  fetch(0);
   for (int j0 = 0; j0 < len; j0 += kRun) {
     float x[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) x[i] = next[i];
+    const int id = next_id;
+    fetch(j0 + kRun);
     uint32_t pair[kPer], mine = 0;  // low half: stays whatever its equals; high half: equals the key
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int j = j0 + tid * kPer + i;
-      x[i] = j < len ? w[j] : 0.f;
       pair[i] = 0u;
       if (j < len) {
         if (j < lo || j >= hi) pair[i] = 1u;
@@ -212,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) evict_kernel(const 
       if (stays) {
         const int d = found + static_cast<int>(before & 0xFFFFu) + min(tie, equals) - min(ties, equals);
         s.slot[d % kRing] = j;
-        s.page[d % kRing] = page_of(from, j);
+        s.page[d % kRing] = page_of(id);
         if (out != w || d != j) out[d] = x[i];
       }
       before += pair[i];
