@@ -579,7 +579,8 @@ typedef struct exl3_kv_weight {
  * r that see slot j and the query heads h of the kv head.  q, scale and lse are exl3_tree_attention's (call it first); a row
  * whose lse is -inf saw nothing and adds nothing, decay 0 does not read w.  0 <= decay <= 1.  What lies in other slots, or in
  * rows that do not see a slot, does not reach its weight; other sequences' and slots' weights stay.  Products and sums are
- * f32, in an order that does not vary.  Slots from `slots` on have no weight (EXL3_ERR_BAD_SHAPE is recorded). */
+ * f32, in an order that does not vary; no term may reach e^88 (with the attention's own lse none is above 1).  Slots from
+ * `slots` on have no weight (EXL3_ERR_BAD_SHAPE is recorded). */
 exl3_verdict exl3_attention_weight(const exl3_kv_cache *cache, int32_t layer, const exl3_tree_batch *batch,
                                    const exl3_heads *q, float scale, const float *lse, float decay, void *stream,
                                    const exl3_kv_weight *weight);
