@@ -211,7 +211,7 @@ __device__ __forceinline__ uint32_t seeing32(const WeightParams& p, const Item& 
 }
 
 // 2^x of two numbers at most about 0 on the FMA pipe: x = n + f with |f| <= 1/2, a polynomial of degree 5 for 2^f (the
-// minimax of its relative error, 7.5e-8, by Remez' exchange) and n into the exponent.  Below -125 exactly zero, NaN stays.
+// minimax of its relative error, 7.5e-8, by Remez' exchange), times 2^n.  Below -125 exactly zero, NaN stays.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -227,12 +227,12 @@ __device__ __forceinline__ uint64_t exp2_fma(float a, float b) {
   y = fma2(y, f, f2(0.240221197f, 0.240221197f));
   y = fma2(y, f, f2(0.693146967f, 0.693146967f));
   y = fma2(y, f, f2(1.00000007f, 1.00000007f));
-  float t0, t1, y0, y1;
-  f2_split(t, t0, t1), f2_split(y, y0, y1);
-  y0 = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23));
-  y1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23));
-  constexpr float kLeast = 2.35098887e-38f * 1.00000007f;  // what x = -125 comes to
-  return add2(f2(y0, y1), f2(-kLeast, -kLeast));
+  float t0, t1;
+  f2_split(t, t0, t1);
+  const float n0 = __uint_as_float((__float_as_uint(t0) << 23) + 0x3F800000u);  // 2^n (a NaN's is whatever it is)
+  const float n1 = __uint_as_float((__float_as_uint(t1) << 23) + 0x3F800000u);
+  constexpr float kLeast = 0x1p-125f * 1.00000007f;  // what x = -125 comes to
+  return fma2(y, f2(n0, n1), f2(-kLeast, -kLeast));
 }
 
 // The sum of 2^(scale x - lse) over 32 accumulators; lse in shared memory, in units of log 2.

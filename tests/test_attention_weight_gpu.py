@@ -106,6 +106,31 @@ def test_a_bad_row_reaches_the_slots_it_sees_alone(A, rows):
     assert torch.isnan(w).nonzero().tolist() == [[0, 1, 3 * 16 + 5]]
 
 
+@pytest.mark.parametrize("heads,dim", [(2, 128), (8, 64), (4, 256)])
+def test_a_bad_row_of_a_full_tile_wherever_it_lies(A, heads, dim):
+    step = Step([256], [300], 2, dim, 64, "f16")
+    cache, batch = step.device(A, rows=256)
+    old = old_weights(step, 2, 560)
+    for at in (0, 1, 2, 3, 4, 5, 6, 7, 130, 255):
+        for head in range(heads // 2):
+            q = queries(step, heads, dim)
+            q[at, head] = math.nan
+            _, lse = A.tree_attention(cache, step.layer, batch, q, lse=True)
+            w = A.attention_weight(cache, step.layer, batch, q, lse, old.cuda())[0].isnan().cpu()
+            assert bool(w[0, :300 + at + 1].all()) and not bool(w[0, 300 + at + 1:].any()) and not bool(w[1].any())
+
+
+def test_probabilities_next_to_nothing_stay_above_zero(A):
+    """Scores hundreds apart: what is below 2^-125 adds nothing, and no weight ends below zero."""
+    for dim in (64, 128, 256):
+        step = Step([256, 1, 40], [300, 500, 5], 2, dim, 64, "bf16")
+        q = queries(step, 8, dim) * 40
+        cache, batch = step.device(A, rows=step.row_start[-1])
+        _, lse = A.tree_attention(cache, step.layer, batch, q, lse=True)
+        w = A.attention_weight(cache, step.layer, batch, q, lse, torch.zeros((3, 2, 560), device="cuda"))
+        assert bool((w >= 0).all()) and bool((w == 0).any()) and not bool(torch.signbit(w).any())
+
+
 @pytest.mark.parametrize("pad", [1, 4, 8])
 def test_queries_of_any_stride(A, pad):
     for rows, lens in (([1, 2], [40, 300]), ([90], [50])):
