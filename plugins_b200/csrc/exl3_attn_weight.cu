@@ -62,7 +62,7 @@ struct WtShape {
   static constexpr int kLoad = 64;                  // threads that bring the queries
   static constexpr int kThreads = kEpi + 64 + kLoad;
   static constexpr int kTmem = D == 256 ? 256 : 512;
-  static constexpr int kBars = 2 * KS + 2 * QS + LS + 2 * HB * kBufs + 2;
+  static constexpr int kBars = 2 * KS + 2 * QS + 2 * LS + 2 * HB * kBufs + 2;
   static constexpr int kSmem = KS * kKTile + QS * kQTile + LS * RT * 4 + 2 * 3 * 128 * 4 + kBars * 8 + 64;
   static_assert(HB * kBufs * RT <= kTmem && kSmem <= 232448 - 2048, "shared memory or TMEM");
 };
@@ -262,8 +262,8 @@ __global__ void __launch_bounds__(WtShape<D, FEW>::kThreads, 1)
   float* s_lse = reinterpret_cast<float*>(s_q + QS * S::kQTile);  // [slot][RT], negated, in units of log 2
   float* s_sums = s_lse + LS * RT;               // [2][3][128]: the other groups' sums, by turns
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_sums + 768);
-  uint64_t *kfull = bars, *kempty = kfull + KS, *qfull = kempty + KS, *qempty = qfull + QS, *lempty = qempty + QS;
-  uint64_t *afull = lempty + LS, *aempty = afull + HB * kBufs, *xsync = aempty + HB * kBufs, *fin = xsync + 1;
+  uint64_t *kfull = bars, *kempty = kfull + KS, *qfull = kempty + KS, *qempty = qfull + QS, *lfull = qempty + QS;
+  uint64_t *lempty = lfull + LS, *afull = lempty + LS, *aempty = afull + HB * kBufs, *xsync = aempty + HB * kBufs, *fin = xsync + 1;
   uint32_t* words = reinterpret_cast<uint32_t*>(bars + S::kBars);
   uint32_t* s_tmem = words;
   volatile uint32_t* abort_flag = words + 1;
@@ -282,7 +282,11 @@ __global__ void __launch_bounds__(WtShape<D, FEW>::kThreads, 1)
   if (tid == 0) {
     for (int i = 0; i < KS; ++i) mbar_init(&kfull[i], 1), mbar_init(&kempty[i], 1);
     for (int i = 0; i < QS; ++i) mbar_init(&qfull[i], p.box_tokens ? 1 + 32 : S::kLoad), mbar_init(&qempty[i], 1);
-    for (int i = 0; i < LS; ++i) mbar_init(&lempty[i], 16);
+    // The log-sum-exps' ring: every summing warp has seen a tile published before it releases it (lempty), by lfull, or by the
+    // accumulators of a tile that it reads itself (their MMA waits for the same loader).  So a warp arrives once in a phase:
+    // it cannot release tile n + LS before that is published, which the loader does not do before all sixteen have released
+    // tile n; and neither side can be two phases ahead of the other, which a parity does not tell apart.
+    for (int i = 0; i < LS; ++i) mbar_init(&lfull[i], p.box_tokens ? 32 : S::kLoad), mbar_init(&lempty[i], 16);
     for (int i = 0; i < HB * kBufs; ++i) mbar_init(&afull[i], 1), mbar_init(&aempty[i], 4);
     mbar_init(xsync, 16), mbar_init(fin, 1);
     fence_barrier_init();
@@ -365,6 +369,9 @@ __global__ void __launch_bounds__(WtShape<D, FEW>::kThreads, 1)
         const int rows = min(p.row_tile, nrows - row0);
         if (bring) {
           if (brought && lane == 0) mbar_arrive(&lempty[(brought - 1) % LS]);
+          // (a tile of its own: its accumulators say so.  With the whole wait there too 240 us for the 4096-row chunk, 237 so)
+          if (!(mine && served % GH == g % GH) && !__all_sync(0xFFFFFFFFu, mbar_try_wait(&lfull[brought % LS], brought / LS & 1u)))
+            ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(&lfull[brought % LS], brought / LS & 1u, abort_flag, b.err));
           ++brought;
         }
         bring = true;
@@ -600,7 +607,7 @@ __global__ void __launch_bounds__(WtShape<D, FEW>::kThreads, 1)
           // a row that saw nothing (or is not there) adds nothing: 2^(x - inf)
 #pragma unroll
           for (int j = 0; j < RT / 32; ++j) s_lse[n % LS * RT + j * 32 + lane] = l[j] == -INFINITY ? -INFINITY : -l[j] * kLog2e;
-          mbar_arrive(&qfull[slot]);
+          mbar_arrive(&qfull[slot]), mbar_arrive(&lfull[n % LS]);
           ++n;
         }
         advance(tiles);
@@ -622,7 +629,7 @@ __global__ void __launch_bounds__(WtShape<D, FEW>::kThreads, 1)
     bool ok = true, pending = false;  // the last one's copies are on their way: not published yet
     auto publish = [&](uint32_t which) {
       fence_proxy_async_smem();
-      mbar_arrive(&qfull[which % QS]);
+      mbar_arrive(&qfull[which % QS]), mbar_arrive(&lfull[which % LS]);
     };
     auto flush = [&]() {
       if (!pending) return;
