@@ -44,6 +44,9 @@ constexpr double kNone = 0x1p-100;  // a token this far below the likeliest has 
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
+// The first barrier in two halves: a CTA's shared memory may be written by others once it is known to have started.
+__device__ __forceinline__ void cluster_started() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_store(void* p, int rank, double a, double b) {
   uint32_t at;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
@@ -284,6 +287,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
     }
     return;
   }
+  cluster_started();
   const bool decides = warp == kWarps;
   // this warp's slice, of p.slice elements but for the last
   const int mine = rank * kWarps + warp;
@@ -323,6 +327,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
     // ---------------------------------------------------------------- a slice of every row on the path
     float* own = s_e + warp * p.slice;
     auto send = [&](double x, double y) {
+      if (turn == 0) cluster_wait();  // every CTA of the cluster has started
       if (lane < kCluster) cluster_store(&b.slice[turn & 1u][mine], lane, x, y);
       ++turn;
       cluster_sync();
@@ -489,6 +494,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
     const float u_next = p.uniform[2 * row + 1];
     if (rank == 0 && lane == 0) path[kept] = node;
     ++kept;
+    if (turn == 0) cluster_wait();  // (the first of two)
     const double2* sent = b.slice[turn++ & 1u];
     cluster_sync();
 
