@@ -270,6 +270,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
   constexpr int kVec = Elem<DT>::kVec;
   extern __shared__ __align__(16) float s_e[];  // [slice + 8]
   __shared__ Block b;
+  cluster_started();
   pdl_wait();
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int rank = static_cast<int>(blockIdx.x) % kCluster, s = static_cast<int>(blockIdx.x) / kCluster;
@@ -285,9 +286,9 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 1) 
       for (int d = tid; d < p.depth; d += kThreads) path[d] = -1;
       if (tid == 0) p.kept[s] = 0, p.token[s] = -1;
     }
+    cluster_wait();
     return;
   }
-  cluster_started();
   const bool decides = warp == kWarps;
   // this warp's slice, of p.slice elements but for the last
   const int mine = rank * kWarps + warp;
