@@ -580,7 +580,8 @@ typedef struct exl3_kv_weight {
  * whose lse is -inf saw nothing and adds nothing, decay 0 does not read w.  0 <= decay <= 1.  What lies in other slots, or in
  * rows that do not see a slot, does not reach its weight; other sequences' and slots' weights stay.  Products and sums are
  * f32, in an order that does not vary; no term may reach e^88 (with the attention's own lse none is above 1).  Slots from
- * `slots` on have no weight (EXL3_ERR_BAD_SHAPE is recorded). */
+ * `slots` on have no weight (EXL3_ERR_BAD_SHAPE is recorded).  Should a wait give up (EXL3_ERR_WAIT_TIMEOUT), a slot has its
+ * new weight or the one it had. */
 exl3_verdict exl3_attention_weight(const exl3_kv_cache *cache, int32_t layer, const exl3_tree_batch *batch,
                                    const exl3_heads *q, float scale, const float *lse, float decay, void *stream,
                                    const exl3_kv_weight *weight);

@@ -27,7 +27,8 @@
 // exponentials at one unit's rate).  Two groups of summing warps took
 // 256 us there where four took 253; fetching the log-sum-exps a tile ahead then brought 233.
 //
-// Every mbarrier wait is bounded (wait_bar): one that gives up raises an abort flag that all roles poll.
+// Every mbarrier wait is bounded (wait_bar): one that gives up raises an abort flag that all roles poll.  A weight is then
+// written whole or not at all, and the counters of the items that the CTA shares return to zero (exl3_parts.h).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -36,6 +37,7 @@
 #include "exl3_attn_tc.cuh"
 #include "exl3_common.cuh"
 #include "exl3_internal.h"
+#include "exl3_parts.h"
 
 namespace exl3 {
 
@@ -248,6 +250,26 @@ __device__ __forceinline__ void add32(const uint32_t (&x)[32], const float* lse,
   }
 }
 
+// Counts a part of an item that is cut between CTAs c0 .. c1 -> whether it is the item's last and all have brought theirs.
+__device__ __forceinline__ bool arrive_part(const WeightParams& p, int c0, int c1, bool brought) {
+  const uint32_t n = atomicAdd(p.a.counters + c0, part_arrival(brought)) + part_arrival(brought);
+  if (!parts_arrived(n, c1 - c0 + 1)) return false;
+  p.a.counters[c0] = 0u;
+  return parts_whole(n);
+}
+
+// A CTA that gave up still counts itself into the items it shares from tile `at` on, as one that brings nothing: their counters
+// return to zero, and none of them is written.
+template <int D, bool FEW>
+__device__ __noinline__ void give_up(const WeightParams& p, const WtLine<D, FEW>& line, WtItem& it, int64_t at) {
+  while (at < line.end) {
+    while (at >= it.first + it.tiles) WtLine<D, FEW>::step(p, it);
+    const int64_t to = min(line.end, it.first + it.tiles);
+    if (to - at != it.tiles) arrive_part(p, line.part_of(it.first), line.part_of(it.first + it.tiles - 1), false);
+    at = to;
+  }
+}
+
 template <int D, bool FEW, bool BF16>
 __global__ void __launch_bounds__(WtShape<D, FEW>::kThreads, 1)
     weight_kernel(const __grid_constant__ WeightParams p, const __grid_constant__ CUtensorMap kmap,
@@ -268,6 +290,7 @@ __global__ void __launch_bounds__(WtShape<D, FEW>::kThreads, 1)
   uint32_t* s_tmem = words;
   volatile uint32_t* abort_flag = words + 1;
   int* s_last = reinterpret_cast<int*>(words + 2);
+  int64_t* s_counted = reinterpret_cast<int64_t*>(words + 4);  // the end of the last item this CTA has counted itself into
   const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
   const PagedBatch& b = p.a.b;
 
@@ -291,6 +314,7 @@ __global__ void __launch_bounds__(WtShape<D, FEW>::kThreads, 1)
     mbar_init(xsync, 16), mbar_init(fin, 1);
     fence_barrier_init();
     *abort_flag = 0u;
+    *s_counted = 0;
   }
   if (tid == 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
   if (tid == 64 && p.box_tokens) asm volatile("prefetch.tensormap [%0];" ::"l"(&qmap) : "memory");
@@ -338,9 +362,9 @@ __global__ void __launch_bounds__(WtShape<D, FEW>::kThreads, 1)
     const uint64_t scale2 = f2(p.a.scale_log2, p.a.scale_log2);
     uint32_t brought = 0, served = 0, x_phase = 0, turn = 0;  // query tiles so far; the half's tiles so far
     bool ok = true;
-    auto group_sync = [&]() {  // all groups
+    auto group_sync = [&]() {  // all groups, none of which has given up
       __syncwarp();
-      if (lane == 0) mbar_arrive(xsync);
+      if (ok && lane == 0) mbar_arrive(xsync);
       ok = __all_sync(0xFFFFFFFFu, ok && wait_bar(xsync, x_phase, abort_flag, b.err));
       x_phase ^= 1u;
     };
@@ -433,6 +457,7 @@ __global__ void __launch_bounds__(WtShape<D, FEW>::kThreads, 1)
 #pragma unroll
           for (uint32_t o = 1; o < GH; ++o) total += there[(g + o - 1) * 128 + r128];
       }
+      if (!ok) break;
       if (tiles == it.tiles) {
         if (writes) *w = keeps ? fmaf(p.decay, old, total) : total;
       } else {
@@ -441,11 +466,8 @@ __global__ void __launch_bounds__(WtShape<D, FEW>::kThreads, 1)
         const int c0 = line.part_of(it.first), c1 = line.part_of(it.first + it.tiles - 1);
         __threadfence();
         group_sync();
-        if (tid == 0) {
-          const bool last = atomicAdd(p.a.counters + c0, 1u) + 1u == static_cast<uint32_t>(c1 - c0 + 1);
-          if (last) p.a.counters[c0] = 0u;
-          *s_last = last;
-        }
+        if (!ok) break;
+        if (tid == 0) *s_last = arrive_part(p, c0, c1, true), *s_counted = at + tiles;
         group_sync();
         if (ok && *s_last) {
           __threadfence();
@@ -461,6 +483,7 @@ __global__ void __launch_bounds__(WtShape<D, FEW>::kThreads, 1)
       }
       advance(tiles);
     }
+    if (tid == 0 && at < end) give_up(p, line, it, max(at, *s_counted));
   } else if (warp == 16) {
     // ---------------------------------------------------------------- MMA issuer: converged, one elected lane issues
     const uint32_t on = elect_one();
@@ -722,6 +745,7 @@ cudaError_t launch_dim(const WeightParams& params, int sms, size_t partial_float
   if (grid > tiles) grid = tiles;
   const int64_t fit = static_cast<int64_t>(partial_floats / (2 * S::KB));
   if (grid > fit) grid = fit;
+  if (grid > kMaxParts) grid = kMaxParts;
   if (grid < 1) grid = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
