@@ -96,12 +96,36 @@ class TreeDecoder:
         return A.TreeBatch(self._ints(start), self.state.lens, self.state.table, max_rows=max(counts), rows=start[-1],
                            max_context=max(need), tree=tree, position=depth)
 
+    def _logits(self, x: torch.Tensor) -> torch.Tensor:
+        return x.float() @ self.embed.float().T
+
     def _verify(self, x: torch.Tensor, batch: A.TreeBatch, tokens: torch.Tensor, parent, depth: int, draft=None):
-        """Which of the rows stay, by their hidden states, and each sequence's token after them."""
+        """Which of the rows stay, by their hidden states, and each sequence's token after them (on the device and here)."""
         n, dev = batch.nseq, self.embed.device
         uniform = torch.rand((x.shape[0], 2), generator=self.random, device=dev)
-        return A.draft_verify(self.cache, batch, x.float() @ self.embed.float().T, tokens, parent, uniform,
-                              torch.full((n,), self.temperature, device=dev), draft, depth=depth)
+        path, kept, token = A.draft_verify(self.cache, batch, self._logits(x), tokens, parent, uniform,
+                                           torch.full((n,), self.temperature, device=dev), draft, depth=depth)
+        after = token.tolist()
+        return path, kept, after
+
+    def _choices(self, x: torch.Tensor) -> list[int]:
+        return self._logits(x).argmax(-1).tolist()
+
+    def _follow(self, choice: list[int], tokens: list[int], parents: list[list], counts: list[int]):
+        """The model's own choices down each tree -> its path, and the choice after it (trees and vocabularies of any size)."""
+        paths, after, row0 = [], [], 0
+        for par, count in zip(parents, counts):
+            path, at = [0], 0
+            while True:  # the drafted child the model would have chosen
+                nxt = next((i for i in range(at + 1, count) if par[i] == at and tokens[row0 + i] == choice[row0 + at]), None)
+                if nxt is None:
+                    break
+                path.append(nxt)
+                at = nxt
+            paths.append(path)
+            after.append(choice[row0 + at])
+            row0 += count
+        return paths, after
 
     def _commit(self, batch: A.TreeBatch, path, kept: torch.Tensor, counts: list[int]) -> None:
         A.cache_keep(self.cache, batch, path, kept, out=self.state.lens, weight=self.weight)
@@ -131,8 +155,11 @@ class TreeDecoder:
         for c in counts:
             ends.append(ends[-1] + c)
         rows = [e - 1 for e in ends[1:]]
-        last = A.TreeBatch(self._ints(list(range(len(rows) + 1))), self.state.lens, self.state.table, max_rows=1, rows=len(rows))
-        self.last = self._verify(x[rows], last, tokens[rows], None, 1)[2].tolist()
+        if self.temperature == 0:
+            self.last = self._choices(x[rows])
+        else:
+            last = A.TreeBatch(self._ints(list(range(len(rows) + 1))), self.state.lens, self.state.table, max_rows=1, rows=len(rows))
+            self.last = self._verify(x[rows], last, tokens[rows], None, 1)[2]
         self._commit(batch, None, self._ints(counts), counts)
         return list(self.last)
 
@@ -159,10 +186,16 @@ class TreeDecoder:
                 place.append(n + d)
         batch = self._batch(counts, self._ints(bits), self._ints(place))
         rows = self._ints(tokens)
-        parent = self._ints([-1 if p is None else p for par in parents for p in par])
-        deep = max(p - n for n, c, at in zip(self.seen, counts, self._starts(counts)) for p in place[at:at + c]) + 1
-        path, kept, token = self._verify(self.forward(rows, batch), batch, rows, parent, deep, draft)
-        paths, stay, self.last = path.tolist(), kept.tolist(), token.tolist()
+        x = self.forward(rows, batch)
+        if self.temperature == 0:
+            paths, self.last = self._follow(self._choices(x), tokens, parents, counts)
+            stay = [len(p) for p in paths]
+            path, kept = self._ints([p + [-1] * (max(stay) - len(p)) for p in paths]), self._ints(stay)
+        else:
+            parent = self._ints([-1 if p is None else p for par in parents for p in par])
+            deep = max(p - n for n, c, at in zip(self.seen, counts, self._starts(counts)) for p in place[at:at + c]) + 1
+            path, kept, self.last = self._verify(x, batch, rows, parent, deep, draft)
+            paths, stay = path.tolist(), kept.tolist()
         self._commit(batch, path, kept, stay)
         return [[tokens[at + i] for i in p[1:k]] + [t] for at, p, k, t in zip(self._starts(counts), paths, stay, self.last)]
 
