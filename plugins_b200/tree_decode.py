@@ -106,6 +106,8 @@ class TreeDecoder:
         path, kept, token = A.draft_verify(self.cache, batch, self._logits(x), tokens, parent, uniform,
                                            torch.full((n,), self.temperature, device=dev), draft, depth=depth)
         after = token.tolist()
+        if min(after) < 0:
+            raise RuntimeError(f"no token has a probability in sequence {after.index(-1)}: its logits are NaN or -inf")
         return path, kept, after
 
     def _choices(self, x: torch.Tensor) -> list[int]:
