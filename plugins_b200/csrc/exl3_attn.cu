@@ -585,8 +585,9 @@ exl3_verdict exl3_draft_verify(const exl3_kv_cache* cache, const exl3_tree_batch
                        runs_of(draft->temperature, draft->temperature ? n * 4 : 0), runs_of(batch->row_start, (n + 1) * 4)};
   const Runs made[] = {runs_of(path, n * depth * 4), runs_of(kept, n * 4), runs_of(token, n * 4)};
   for (int i = 0; i < 3; ++i) {
-    for (const Runs& o : read)
-      if (rows > 0 && meet(made[i], o)) return refuse(EXL3_FAILED, "exl3_b200: verify's results lie over its arguments");
+    for (const Runs& o : read)  // (without rows, temperature and row_start alone are read)
+      if ((rows > 0 || &o >= read + 5) && meet(made[i], o))
+        return refuse(EXL3_FAILED, "exl3_b200: verify's results lie over its arguments");
     for (int j = 0; j < i; ++j)
       if (meet(made[i], made[j])) return refuse(EXL3_FAILED, "exl3_b200: verify's results lie over one another");
   }
