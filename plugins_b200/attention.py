@@ -140,6 +140,11 @@ def _maker(stream, make):
     return functools.partial(_made_on, stream, make) if isinstance(stream, torch.cuda.Stream) else make
 
 
+def _overlap(a, b) -> bool:
+    """Whether two contiguous tensors of one device share memory (None has none)."""
+    return b is not None and a.data_ptr() < b.data_ptr() + b.nbytes and b.data_ptr() < a.data_ptr() + a.nbytes
+
+
 class KvCache:
     """The paged cache of every layer: ``k`` and ``v`` [layers, pages, kv_heads, page_size, head_dim], f16 or bf16, of
     any strides (the same for both) with contiguous head vectors -- so also the transposed view of a pool stored
@@ -426,6 +431,11 @@ def cache_keep(cache: KvCache, batch: TreeBatch, path, kept, out=None, stream=No
     batch._for(cache, batch.rows)
     if weight is not None:
         raw = L.KvWeight(*_kv_weight(weight, cache.raw.layers, batch.nseq, cache))
+        # what exl3_cache_keep refuses, before the weights move (a second call would move them again)
+        row_start, context, table = batch._keep[:3]
+        if any(_overlap(out, t) for t in (row_start, table, path)) or \
+                any(_overlap(out, t) and out.data_ptr() != t.data_ptr() for t in (context, kept)):
+            _refuse("exl3_b200: lens lies over the call's arguments")
         if stream is not None:
             _used_on(stream, weight)
         check(L.lib().exl3_weight_keep(cache.raw, batch.raw, None if path is None else path.data_ptr(),
