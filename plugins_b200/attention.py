@@ -521,7 +521,7 @@ def draft_verify(cache: KvCache, batch: TreeBatch, logits, tokens, parent, unifo
     _floats(uniform, (rows, 2), "uniform", i)
     if temperature is not None:
         _floats(temperature, (n,), "temperature", i)
-    depth = max(1, batch.raw.max_rows) if depth is None else int(depth)
+    depth = max(1, batch.raw.max_rows or rows) if depth is None else int(depth)  # (max_rows 0: no bound is given)
     if depth < 1:
         _refuse("a path without depth")
     make = _maker(stream, torch.empty)

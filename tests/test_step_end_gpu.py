@@ -48,3 +48,20 @@ def test_kept_weights_stay_inside_their_slots(A):
     want[:, :, 2, 9:13] = pool[:, :, 2, [9, 10, 12, 15]]
     A.cache_keep(cache, batch, path, kept, weight=pool.permute(1, 2, 0, 3)[:, :3, :, 9:49])
     assert torch.equal(pool, want)
+
+
+def test_paths_are_as_deep_as_the_rows_where_no_bound_is_given(A):
+    cache = A.KvCache.empty(1, 4, 16, 1, 64)
+    n, vocab = 6, 50
+    tokens = ints([3, 8, 1, 30, 7, 2, 40, 41])  # a chain that the model agrees with, then another sequence's one draft
+    logits = torch.zeros((n + 2, vocab), device="cuda")
+    logits[torch.arange(n - 1), tokens[1:n].long()] = 5.0
+    logits[n - 1, 11], logits[n, 41], logits[n + 1, 9] = 5.0, 5.0, 5.0
+    uniform = torch.full((n + 2, 2), 0.5, device="cuda")
+    got = []
+    for most in (n, 0):
+        batch = A.TreeBatch(ints([0, n, n + 2]), ints([0, 0]), ints([[0], [1]]), max_rows=most, rows=n + 2)
+        got.append(A.draft_verify(cache, batch, logits, tokens, None, uniform, torch.zeros(2, device="cuda")))
+    for path, kept, token in got:
+        assert kept.tolist() == [n, 2] and token.tolist() == [11, 9]
+        assert path[0, :n].tolist() == list(range(n)) and path[1, :2].tolist() == [0, 1] and path[1, 2] == -1
