@@ -134,15 +134,32 @@ class TreeDecoder:
         self.lens = [n + k for n, k in zip(self.lens, counts)]
         self.seen = [n + k for n, k in zip(self.seen, counts)]
         if self.budget is not None and max(self.lens) > self.budget + self.recent:
-            self.evict()
+            self._cut()  # (rows that cannot be cut yet are left to the next step: this one's tokens are not lost)
 
     def evict(self) -> None:
         """Cuts every row to the budget."""
-        budget = self._ints([self.budget] * len(self.lens))
-        self.state, missing = A.cache_evict(self.cache, self.state, self.weight, budget, self.sink, self.recent)
-        if int(missing):
-            raise RuntimeError(f"the cache lacks {int(missing)} pages")
-        self.lens = [min(n, self.budget) for n in self.lens]
+        missing = self._cut()
+        if missing:
+            raise RuntimeError(f"the cache lacks {missing} pages")
+
+    def _cut(self) -> int:
+        """Cuts the rows to the budget, together, or, where the free pages do not suffice for all that share some, one after the
+        other: a row that is cut gives pages back, and those it shared may be another's alone by then -> the pages lacking for
+        the rows that had to be left."""
+        def cut(rows) -> int:
+            budget = self._ints([self.budget if i in rows else 0x7FFFFFFF for i in range(len(self.lens))])
+            self.state, missing = A.cache_evict(self.cache, self.state, self.weight, budget, self.sink, self.recent)
+            lacking = int(missing)
+            if not lacking:
+                self.lens = [min(n, self.budget) if i in rows else n for i, n in enumerate(self.lens)]
+            return lacking
+
+        lacking = cut(range(len(self.lens)))
+        left, before = [i for i, n in enumerate(self.lens) if lacking and n > self.budget], None
+        while left and left != before:
+            before = left
+            left = [i for i in left if cut((i,))]
+        return cut(left) if left else 0
 
     def prompt(self, prompts: list[list[int]]) -> list[int]:
         """Every sequence's prompt in one pass -> its next token."""
