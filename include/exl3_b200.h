@@ -677,7 +677,9 @@ typedef struct exl3_draft {
  * sequence without rows), as exl3_cache_keep takes them; token [nseq] the token that follows (-1: no rows, or no logit above
  * -inf).  Logits: NaN counts as -inf, +inf as the largest finite number, and a token 2^-100 below the likeliest has no
  * probability; draft: NaN and negative numbers count as 0; a child whose token is outside the vocabulary is not tried.
- * Exponentials are f32, within 2^-22 + 2^-24 |x - max| / temperature of themselves; their sums keep 2^-48, decisions are f64.
+ * Exponentials are f32: within 2^-22 of themselves in their part of the row and as much again in the part's own factor, and
+ * 2^-24 |x - max| / temperature.  Their sums keep 2^-48, decisions are f64; in r after a rejection the sum of the Z so far is
+ * rounded to f32.
  * Another temperature is taken as 0 (EXL3_ERR_BAD_SHAPE is recorded).  At most 1024 rows a sequence.  The batch's context and table
  * are not read. */
 exl3_verdict exl3_draft_verify(const exl3_kv_cache *cache, const exl3_tree_batch *batch, const exl3_draft *draft,

@@ -508,7 +508,8 @@ def draft_verify(cache: KvCache, batch: TreeBatch, logits, tokens, parent, unifo
     or f32; ``draft`` [rows, vocab]: the probabilities that the children of each row were drawn from (None: a drafter without
     any).  ``uniform`` (f32 [rows, 2], in [0, 1)): a number for the row's own token and one for the token that follows the
     row.  ``temperature`` (f32 [nseq], 0: greedy; None: 1).  The path and the token are distributed as tokens drawn one by one
-    from softmax(logits / temperature).  ``depth``: the most rows of a path (max_rows, if not given)."""
+    from softmax(logits / temperature).  ``depth``: the most rows of a path (if not given max_rows, or all rows without such a
+    bound)."""
     dev, n, i = cache.device, batch.nseq, cache._index
     rows = batch.rows if batch.rows is not None else logits.shape[0]
     dt = _vocab_rows(logits, rows, None, "logits", i)

@@ -21,11 +21,14 @@
 // A quarter of the exponentials are polynomials on the FMA pipe, beside the special-function unit (4096 rows on 4096 slots, an
 // eighth / a quarter / half of them: 245 / 235 / 271 us; a step earlier none took 265 where a quarter took 256).
 //
-// What bounds it: few rows, HBM (32 sequences' tokens over 1.5-9k slots 64 us in a graph, 5.5 TB/s; nine trees of 5-17 rows over
-// 6-16k 256-wide slots 73 us, 5.8 TB/s), the rest being the start and the line's cut; many rows, the summing warps' issue and
-// their special-function unit (a 4096-row chunk on 4096 slots 232 us, 0.89 PFLOP/s, against 127 us of products and 179 us of
-// exponentials at one unit's rate).  Two groups of summing warps took
-// 256 us there where four took 253; fetching the log-sum-exps a tile ahead then brought 233.
+// What bounds it: few rows, HBM (32 sequences' tokens over 1.5-9k slots 65 us in a graph, 5.4 TB/s; nine trees of 5-17 rows over
+// 6-16k 256-wide slots 72 us, 5.8 TB/s), the rest being the start and the line's cut.  Many rows, no one unit: a 4096-row chunk
+// on 4096 slots takes 238 us at 1965 MHz (0.87 PFLOP/s, against 127 us of products), its schedulers issue in 62 % of the active
+// cycles, the special-function unit is busy for 64 % and the tensor pipe for 43 %, and of a warp's 8.1 cycles an instruction
+// 2.0 are on the long scoreboard, 1.3 a fixed latency, 0.9 another warp's issue and 0.8 at barriers; the SMs are active for
+// 88 % of it.  Called for longer than a few hundred milliseconds it draws the card's 1000 W, which clocks it
+// at about 1790 MHz: 263 us.  Two groups of summing warps took 256 us (of 232 then) where four took 253; fetching the
+// log-sum-exps a tile ahead then brought 233; passing every tile's publication (lfull), which order needs, costs 2 %.
 //
 // Every mbarrier wait is bounded (wait_bar): one that gives up raises an abort flag that all roles poll.  A weight is then
 // written whole or not at all, and the counters of the items that the CTA shares return to zero (exl3_parts.h).

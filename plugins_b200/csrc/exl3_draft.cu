@@ -14,10 +14,11 @@
 // which can be a small rest of p, keeps what the exponentials have (an f32 sum would leave 2^-24 of all of p in it).  Only rows
 // on the path are read, and each node's first child, whose slice is on its way to registers while the node is decided.
 //
-// The chain of a node bounds the call: in a 17-token tree of 128000 about 0.9k clocks for its row, 2.4k for the exponentials,
-// 0.7k to start the next row, 1.5k for the barrier, 1.9k for the decision, and 5k more where a child is rejected against q.  In
-// a graph: one token of 32000 5.8 us, 8 chains of 65537 22 us, 32 16-token trees of 131072 28 us, 64 17-token trees of 128000
-// with the drafter's probabilities 84 us.  Eight CTAs to a cluster: four take 36 us for the 32 trees, sixteen 50 (fewer clusters
+// What bounds it is this walk, a row at a time: in a 17-token tree of 128000 a node takes about 0.9k clocks for its row, 2.4k
+// for the exponentials, 0.7k to start the next row, 1.5k for the barrier, 1.9k for the decision, and 5k more where a child is
+// rejected against q.  (A row's maxima and sums depend on the row alone: taken for all rows at once they would not wait.)  In
+// a graph: one token of 32000 5.9 us, 8 chains of 65537 21 us, 32 16-token trees of 131072 28 us, 64 17-token trees of 128000
+// with the drafter's probabilities 85 us.  Eight CTAs to a cluster: four take 36 us for the 32 trees, sixteen 50 (fewer clusters
 // fit).  Sixteen warps with a slice each: eight took 122 us for the 64 trees where sixteen took 96.
 #include <cuda_runtime.h>
 #include <float.h>
